@@ -347,6 +347,77 @@ W4A16_API int w4a16_fused_moe_prepared(void* stream, const void* x, const float*
                                        int32_t block_m, void* workspace, size_t workspace_bytes,
                                        void* out);
 
+/* ------------------------------------------------------------------ key/value cache in 4 bits
+ * Not in the reference (it has neither cache nor attention): what a program whose linear layers
+ * run here needs between its q, k, v projection and its output projection. `elem` is 0 (fp16) or
+ * W4A16_BF16, the type of q, k, v, out and of the cache's scales.
+ *
+ * A cache holds num_pages pages of page_size tokens (a power of two, 16..1024) of Hkv heads of D
+ * dimensions (64, 128, 192 or 256): [num_pages][Hkv][page_size / 16] blocks of 16 D + 128 bytes,
+ * 16-byte aligned. A block holds 16 tokens of one head: keys (token t's row at t D / 2, dimension
+ * d in nibble d, lowest first); from 8 D values (token t = 4 u + 2 p + i, dimension d =
+ * c D / 16 + 4 h + e in nibble e of the 16 bits at u 2 D + c D / 8 + p D / 16 + 4 h + 2 i); from
+ * 16 D one 32-bit word a token for keys and, 64 bytes on, for values: scale in bits 0..15, zero
+ * point in bits 16..31. A nibble n holds (n - zero) * scale. Token `slot % page_size` of page
+ * `slot / page_size` is slot `slot`.
+ *
+ * A row x[0, D) is quantised over the range that it and 0 span: scale = (max - min) / 15 rounded
+ * to fp32, then to the element type; zero = rint(-min / scale); n = clamp(rint(x / scale) + zero,
+ * 0, 15), ties to even. A scale of 0 holds zeros; a row with an infinity or NaN is NaN throughout. */
+
+/* Bytes of a cache (0: not supported). A cache needs no initialisation. */
+W4A16_API size_t w4a16_kv4_cache_bytes(int32_t num_pages, int32_t Hkv, int32_t D, int32_t page_size);
+
+/* Quantises rows k, v [T, Hkv, D] (strides in elements, multiples of 8; 16-byte aligned) into the
+ * slots [T] of the cache. A row whose slot is negative or beyond the cache is passed over. Slots of
+ * one call must differ: of two rows with one slot, either may remain, or parts of both. */
+W4A16_API int w4a16_kv4_write(void* stream, int elem, const void* k, const void* v,
+                              int32_t k_stride_t, int32_t k_stride_h, int32_t v_stride_t,
+                              int32_t v_stride_h, const int32_t* slots, void* cache,
+                              int32_t num_pages, int32_t T, int32_t Hkv, int32_t D,
+                              int32_t page_size);
+
+/* The rows that the slots hold, rounded to the element type (to its largest finite value beyond
+ * that), into k_out, v_out [T, Hkv, D] (strides as above, rows not over each other). Rows whose
+ * slot is negative or beyond the cache are left as they were. A slot may be named more than once. */
+W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const int32_t* slots,
+                             void* k_out, void* v_out, int32_t k_stride_t, int32_t k_stride_h,
+                             int32_t v_stride_t, int32_t v_stride_h, int32_t num_pages, int32_t T,
+                             int32_t Hkv, int32_t D, int32_t page_size);
+
+/* Attention of queries q [T, Hq, D] over the cache, query head a on key/value head
+ * a / (Hq / Hkv). Sequence b's keys are tokens 0 .. kv_lens[b] - 1, token j in page
+ * page_table[b * pages_per_seq + j / page_size]; its queries are rows cu_q[b] .. cu_q[b + 1] - 1
+ * (cu_q null: row b, T = B), the last of them at token kv_lens[b] - 1. A query at token i sees key
+ * j < kv_lens[b] where (causal != 0) j <= i and (window > 0) j > i - window:
+ *   out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j), lse = ln sum_j p_j (nullable, fp32
+ *   [T, Hq]), both over the unrounded values that the nibbles hold, in fp32 with p_j |v_j| rounded
+ *   to fp16 before the product with v_j, out rounded once (to its type's largest finite value).
+ * A query that sees no key: out 0, lse -infinity. Keys in a page whose number is outside
+ * [0, num_pages) are not seen. Rows of q outside every sequence are left as they were in out and
+ * lse. max_q_len and max_kv_len bound the sequences of the call (they choose the split of the work);
+ * a kv_lens entry beyond max_kv_len or the table's width counts as that, a negative one as 0, and
+ * queries of a sequence beyond max_q_len are left as they were. The new tokens' rows are written
+ * before the call, on the same stream.
+ *
+ * workspace (256-byte aligned, w4a16_kv4_attention_workspace_size bytes) is caller-owned, its
+ * first W4A16_KV4_COUNTER_BYTES zero at its first use; every call leaves them zero, so one workspace
+ * serves any number of calls, of any sizes that fit, one after another. Calls (or replays of captured
+ * graphs) that may overlap in time need workspaces of their own. Nothing is allocated. The
+ * workspace's size does not depend on the lengths on the device, only on the arguments. */
+#define W4A16_KV4_COUNTER_BYTES 65536
+W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv,
+                                                    int32_t D, int32_t max_q_len,
+                                                    int32_t max_kv_len);
+W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t q_stride_t,
+                                  int32_t q_stride_h, const void* cache, const int32_t* page_table,
+                                  const int32_t* kv_lens, const int32_t* cu_q, void* out,
+                                  int32_t out_stride_t, int32_t out_stride_h, float* lse, int32_t T,
+                                  int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t num_pages,
+                                  int32_t page_size, int32_t pages_per_seq, int32_t max_q_len,
+                                  int32_t max_kv_len, float scale, int32_t causal, int32_t window,
+                                  void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ runtime
  * A HIP backend for the reference's DeviceRuntime trait (crates/triton-runtime/src/
  * lib.rs:64-85): load a code object, launch a kernel by name with KernelArg-style

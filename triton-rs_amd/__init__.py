@@ -78,6 +78,8 @@ EXPORTED = (
     "w4a16_moe_gemm", "fused_silu_mul_interleaved_f16", "fused_silu_mul_interleaved_f32",
     "w4a16_moe_sum",
     "w4a16_fused_moe_workspace_size", "w4a16_fused_moe", "w4a16_fused_moe_prepared",
+    "w4a16_kv4_cache_bytes", "w4a16_kv4_write", "w4a16_kv4_read",
+    "w4a16_kv4_attention_workspace_size", "w4a16_kv4_attention",
     "hiprt_create", "hiprt_destroy", "hiprt_module_load", "hiprt_module_unload", "hiprt_launch",
     "hiprt_stream_create", "hiprt_stream_destroy", "hiprt_stream_synchronize", "hiprt_malloc",
     "hiprt_free", "hiprt_memcpy_htod_async", "hiprt_memcpy_dtoh_async", "hiprt_memset_async",
@@ -134,6 +136,14 @@ def lib() -> ctypes.CDLL:
                                       _P, _I, _I, _I, _P, _Z, _P]
         L.w4a16_fused_moe_prepared.argtypes = [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I,
                                                _P, _Z, _P]
+        L.w4a16_kv4_cache_bytes.restype = ctypes.c_size_t
+        L.w4a16_kv4_cache_bytes.argtypes = [_I] * 4
+        L.w4a16_kv4_write.argtypes = [_P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I]
+        L.w4a16_kv4_read.argtypes = [_P, _I, _P, _P, _P, _P] + [_I] * 9
+        L.w4a16_kv4_attention_workspace_size.restype = ctypes.c_size_t
+        L.w4a16_kv4_attention_workspace_size.argtypes = [_I] * 7
+        L.w4a16_kv4_attention.argtypes = [_P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P] + \
+            [_I] * 10 + [ctypes.c_float, _I, _I, _P, _Z]
         L.hiprt_create.argtypes = [_I, ctypes.POINTER(_P)]
         L.hiprt_destroy.argtypes = [_P]
         L.hiprt_module_load.argtypes = [_P, _P, _Z, ctypes.POINTER(_P)]
@@ -560,6 +570,171 @@ def fused_moe_prepared(x, router_logits, w13: PreparedWeights, w2: PreparedWeigh
                                          K, I, E, topk, int(renormalize), _ptr(w13.buffer),
                                          _ptr(w2.buffer), G, block_m, _ptr(workspace),
                                          workspace.numel(), _ptr(out)))
+    return out
+
+
+# ------------------------------------------------------------------ key/value cache in 4 bits
+
+KV4_COUNTER_BYTES = 65536
+
+
+def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
+              device="cuda") -> torch.Tensor:
+    """An empty 4-bit key/value cache: uint8 [num_pages, num_kv_heads, page_size / 16,
+    16 head_dim + 128] (the layout is in include/w4a16.h). head_dim 64, 128, 192 or 256, page_size
+    a power of two from 16 to 1024."""
+    if lib().w4a16_kv4_cache_bytes(num_pages, num_kv_heads, head_dim, page_size) == 0:
+        raise Unsupported(f"no 4-bit cache of {num_pages} pages of {page_size} tokens, "
+                          f"{num_kv_heads} heads of {head_dim}")
+    return torch.zeros((num_pages, num_kv_heads, page_size // 16, 16 * head_dim + 128),
+                       dtype=torch.uint8, device=device)
+
+
+def _kv4_cache_shape(cache: torch.Tensor):
+    """(pages, kv heads, page size, head dim) of a cache tensor."""
+    _require(cache, "cache", (torch.uint8,))
+    if cache.dim() != 4 or not cache.is_contiguous():
+        raise InvalidArgument("cache must be a contiguous [pages, kv heads, page_size / 16, 16 D + 128] tensor")
+    pages, Hkv, blocks, width = cache.shape
+    D = (width - 128) // 16
+    if D < 1 or width != 16 * D + 128:
+        raise InvalidArgument(f"cache has blocks of {width} bytes, not 16 D + 128")
+    return pages, Hkv, blocks * 16, D
+
+
+def _kv4_rows(t, name: str, dtypes, dev, shape=None):
+    """(token stride, head stride) of rows [T, H, D] with contiguous D."""
+    _require(t, name, dtypes, dev)
+    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
+        raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
+    st, sh, sd = t.stride()
+    if sd != 1 and t.shape[2] != 1:
+        raise InvalidArgument(f"{name} must be contiguous along its last dimension")
+    return st, sh
+
+
+def _kv4_index(t, name: str, dev, numel=None):
+    _require(t, name, _INT32, dev)
+    if not t.is_contiguous() or (numel is not None and (t.dim() != 1 or t.numel() != numel)):
+        raise InvalidArgument(f"{name} must be a contiguous int32 tensor"
+                              + ("" if numel is None else f" of {numel} entries"))
+
+
+def _on(dev: torch.device):
+    """The device as the current one: kernels are launched on the current device's code object."""
+    return torch.cuda.device(dev)
+
+
+def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """Quantises rows k, v [T, kv heads, D] (fp16 or bfloat16; any token and head strides that are
+    multiples of 8) to 4 bits into the slots (int32 [T], page * page_size + offset) of the cache,
+    which it returns. A row whose slot is negative or beyond the cache is passed over; slots of one
+    call must differ from each other."""
+    pages, Hkv, page, D = _kv4_cache_shape(cache)
+    dev = cache.device
+    _require(k, "k", _ELEM, dev)
+    shape = (k.shape[0], Hkv, D)
+    kst, ksh = _kv4_rows(k, "k", _ELEM, dev, shape)
+    vst, vsh = _kv4_rows(v, "v", (k.dtype,), dev, shape)
+    _kv4_index(slots, "slots", dev, shape[0])
+    with _on(dev):
+        check(lib().w4a16_kv4_write(_stream(cache), _elem_flag(k), _ptr(k), _ptr(v), kst, ksh, vst, vsh,
+                                    _ptr(slots), _ptr(cache), pages, shape[0], Hkv, D, page))
+    return cache
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_out=None, v_out=None):
+    """(k, v) [T, kv heads, D]: the rows that the slots of the cache hold, rounded to the element
+    type that they were written in (`dtype`, or that of k_out and v_out). Rows whose slot is negative
+    or beyond the cache are left as they were in k_out and v_out (0 where these are not given)."""
+    pages, Hkv, page, D = _kv4_cache_shape(cache)
+    dev = cache.device
+    _kv4_index(slots, "slots", dev)
+    T = slots.numel()
+    if slots.dim() != 1:
+        raise InvalidArgument("slots must be 1-D")
+    if (k_out is None) != (v_out is None):
+        raise InvalidArgument("give both k_out and v_out, or neither")
+    if k_out is None:
+        k_out, v_out = torch.zeros((2, T, Hkv, D), dtype=dtype, device=dev)
+    kst, ksh = _kv4_rows(k_out, "k_out", _ELEM, dev, (T, Hkv, D))
+    vst, vsh = _kv4_rows(v_out, "v_out", (k_out.dtype,), dev, (T, Hkv, D))
+    with _on(dev):
+        check(lib().w4a16_kv4_read(_stream(cache), _elem_flag(k_out), _ptr(cache), _ptr(slots), _ptr(k_out),
+                                   _ptr(v_out), kst, ksh, vst, vsh, pages, T, Hkv, D, page))
+    return k_out, v_out
+
+
+def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int, max_q_len: int,
+                            max_kv_len: int) -> torch.Tensor:
+    """A workspace for kv4_attention calls with queries of q's shape: enough for any batch within
+    these bounds. Calls that may overlap in time need one each."""
+    _, Hkv, _, D = _kv4_cache_shape(cache)
+    T, Hq = q.shape[:2]
+    need = lib().w4a16_kv4_attention_workspace_size(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
+    if need == 0:
+        check(ERR_INVALID_ARG)
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
+    ws[:KV4_COUNTER_BYTES].zero_()
+    return ws
+
+
+def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                  cu_q: torch.Tensor | None = None, max_q_len: int | None = None,
+                  max_kv_len: int | None = None, scale: float | None = None, causal: bool = True,
+                  window: int = 0, out=None, lse=None, workspace=None) -> torch.Tensor:
+    """softmax(scale q k^T) v over the keys and values of a 4-bit cache; returns out [T, heads, D].
+
+    q [T, heads, D] (fp16 or bfloat16, the type the cache was written in), sequence b's queries in
+    rows cu_q[b] .. cu_q[b + 1] (int32 [B + 1]; None: one row each, T = B), the last of them at token
+    kv_lens[b] - 1 (int32 [B]) of pages page_table[b] (int32 [B, pages per sequence]). The new tokens'
+    keys and values are in the cache already (kv4_write). causal: a query sees no later token; window:
+    and only the last `window` up to its own (0: all). Query heads h G .. h G + G - 1 read key/value
+    head h, G = heads / kv heads. scale: 1 / sqrt(D) unless given. lse (fp32 [T, heads]) takes the
+    logarithm of each row's sum of exponentials. A row that sees no key is 0, its lse -infinity; rows
+    of q behind the last sequence are left as they were in out and lse (0 in an out made here).
+    max_q_len, max_kv_len: bounds on the batch (T, or 1 without cu_q, and the table's width unless
+    given). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
+    given."""
+    pages, Hkv, page, D = _kv4_cache_shape(cache)
+    dev = cache.device
+    qst, qsh = _kv4_rows(q, "q", _ELEM, dev)
+    T, Hq = q.shape[:2]
+    if q.shape[2] != D:
+        raise InvalidArgument(f"q has heads of {q.shape[2]} dimensions, the cache {D}")
+    _kv4_index(page_table, "page_table", dev)
+    if page_table.dim() != 2:
+        raise InvalidArgument("page_table must be [sequences, pages per sequence]")
+    B, per = page_table.shape
+    _kv4_index(kv_lens, "kv_lens", dev, B)
+    if cu_q is not None:
+        _kv4_index(cu_q, "cu_q", dev, B + 1)
+    if max_q_len is None:
+        max_q_len = 1 if cu_q is None else max(1, T)
+    if max_kv_len is None:
+        max_kv_len = per * page
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev) if cu_q is None else \
+            torch.zeros((T, Hq, D), dtype=q.dtype, device=dev)
+    ost, osh = _kv4_rows(out, "out", (q.dtype,), dev, (T, Hq, D))
+    if lse is not None:
+        _require(lse, "lse", (torch.float32,), dev)
+        if tuple(lse.shape) != (T, Hq) or not lse.is_contiguous():
+            raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
+    if T == 0 or B == 0:
+        return out
+    with _on(dev):
+        if workspace is None:
+            workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
+        else:
+            _require(workspace, "workspace", (torch.uint8,), dev)
+            if not workspace.is_contiguous():
+                raise InvalidArgument("workspace must be contiguous")
+        check(lib().w4a16_kv4_attention(
+            _stream(cache), _elem_flag(q), _ptr(q), qst, qsh, _ptr(cache), _ptr(page_table), _ptr(kv_lens),
+            _ptr(cu_q), _ptr(out), ost, osh, _ptr(lse), T, B, Hq, Hkv, D, pages, page, per, max_q_len,
+            max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window, _ptr(workspace),
+            workspace.numel()))
     return out
 
 

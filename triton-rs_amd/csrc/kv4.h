@@ -1,0 +1,55 @@
+// Key/value cache in 4 bits: layout, launch parameters and the launchers of kv4_cache.hip and
+// kv4_attention.hip.
+//
+// A cache is num_pages pages of [Hkv][page_size / 16] blocks; a block holds 16 tokens of one head in
+// 16 D + 128 bytes:
+//   [0, 8 D)        keys: row `tok` at tok D / 2, dimension d in nibble d of the row (lowest first)
+//   [8 D, 16 D)     values: token tok = 4 quad + 2 pair + i, dimension d = column D / 16 + 4 h + e in
+//                   nibble e of the 16-bit word at quad 2 D + column D / 8 + pair D / 16 + 4 h + 2 i
+//   [16 D, +64)     keys' parameters, one 32-bit word a token: scale (bits 0..15, the element
+//                   type's bits), zero point 0..15 (bits 16..31), as in the prepared weights' table
+//   [16 D + 64, +64) values' parameters
+// A nibble n stands for (n - zero) * scale, exact in fp32.
+// The order serves the matrix cores: a lane of an MFMA operand takes consecutive k of one row. With
+// keys the k are dimensions, so a row's nibbles lie together; with values they are tokens, so two
+// tokens share a 32-bit word, in its two halves, where one mask turns them into a pair of operands.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace w4a16 {
+
+constexpr int KV4_BLOCK = 16;   // tokens of a block
+__host__ __device__ constexpr int kv4_block_bytes(int D) { return 16 * D + 128; }
+constexpr bool kv4_head_dim_ok(int D) { return D == 64 || D == 128 || D == 192 || D == 256; }
+constexpr bool kv4_page_ok(int P) { return P >= 16 && P <= 1024 && (P & (P - 1)) == 0; }
+
+struct Kv4RowParams {
+    const void *k, *v;                // write: rows [T, Hkv, D], strides in elements
+    void *k_out, *v_out;              // read
+    int k_st, k_sh, v_st, v_sh;
+    const int32_t* slots;             // [T]; outside [0, num_pages * page_size): the row is passed over
+    unsigned char* cache;
+    int num_pages, T, Hkv, page_shift;   // page_size = 1 << page_shift
+};
+hipError_t launch_kv4_write(bool bf16, int D, const Kv4RowParams& p, hipStream_t st);
+hipError_t launch_kv4_read(bool bf16, int D, const Kv4RowParams& p, hipStream_t st);
+
+struct Kv4AttnParams {
+    const void* q;                    // [T, Hq, D]
+    void* out;                        // [T, Hq, D]
+    float* lse;                       // [T, Hq] or null
+    const unsigned char* cache;
+    const int32_t* table;             // [B, pages_per_seq]
+    const int32_t* kv_lens;           // [B]
+    const int32_t* cu_q;              // [B + 1], or null: one query a sequence
+    int q_st, q_sh, o_st, o_sh;
+    int num_pages, pages_per_seq, T, B, Hq, Hkv, page_shift, max_q, max_kv;
+    float scale_log2;                 // scale * log2(e)
+    int causal, window;
+};
+hipError_t launch_kv4_attention(bool bf16, int D, const Kv4AttnParams& p, hipStream_t st);
+
+}  // namespace w4a16

@@ -1,0 +1,157 @@
+// C-ABI entry points of the 4-bit key/value cache: argument checks (before any HIP call), then
+// the launchers of kv4_cache.hip and kv4_attention.hip.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "../../include/w4a16.h"
+#include "kv4.h"
+#include "launch.h"
+
+namespace w4a16 {
+
+static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+
+constexpr int KV4_MAX_HEADS = 1024;
+constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
+
+static int check_elem(int elem) {
+    if (elem != 0 && elem != W4A16_BF16) return fail(W4A16_ERR_INVALID_ARG, "unknown element type %d", elem);
+    return W4A16_OK;
+}
+
+static int check_geometry(int32_t num_pages, int32_t Hkv, int32_t D, int32_t page_size) {
+    if (num_pages < 1 || Hkv < 1 || D < 1 || page_size < 1)
+        return fail(W4A16_ERR_INVALID_ARG, "sizes must be positive (num_pages=%d Hkv=%d D=%d page_size=%d)", num_pages,
+                    Hkv, D, page_size);
+    if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
+    if (!kv4_page_ok(page_size)) return fail(W4A16_ERR_UNSUPPORTED, "page_size %d: a power of two from 16 to 1024", page_size);
+    if (Hkv > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hkv, KV4_MAX_HEADS);
+    if ((int64_t)num_pages * page_size > INT32_MAX)
+        return fail(W4A16_ERR_UNSUPPORTED, "%d pages of %d tokens: slots are int32", num_pages, page_size);
+    return W4A16_OK;
+}
+
+// Rows [T, H, D] at these strides (elements), D contiguous: 16-byte rows, and for an output no two
+// rows over each other.
+static int check_rows(const char* what, const void* p, int32_t st, int32_t sh, int32_t T, int32_t H, int32_t D, bool out) {
+    if (!p) return fail(W4A16_ERR_INVALID_ARG, "null pointer argument (%s)", what);
+    if (!aligned(p, 16)) return fail(W4A16_ERR_INVALID_ARG, "%s must be 16-byte aligned", what);
+    if (st < 0 || sh < 0 || st % 8 || sh % 8)
+        return fail(W4A16_ERR_INVALID_ARG, "%s: strides (%d, %d) must be non-negative multiples of 8 elements", what, st, sh);
+    if (out) {
+        const bool token_major = (H == 1 || sh >= D) && (T == 1 || st >= (int64_t)(H - 1) * sh + D);
+        const bool head_major = (T == 1 || st >= D) && (H == 1 || sh >= (int64_t)(T - 1) * st + D);
+        if (!token_major && !head_major)
+            return fail(W4A16_ERR_INVALID_ARG, "%s: rows at strides (%d, %d) lie over each other", what, st, sh);
+    }
+    return W4A16_OK;
+}
+
+static int kv4_rows(bool write, void* stream, int elem, void* k, void* v, int32_t k_st, int32_t k_sh, int32_t v_st,
+                    int32_t v_sh, const int32_t* slots, void* cache, int32_t num_pages, int32_t T, int32_t Hkv,
+                    int32_t D, int32_t page_size) {
+    if (int rc = check_elem(elem)) return rc;
+    if (int rc = check_geometry(num_pages, Hkv, D, page_size)) return rc;
+    if (T < 0) return fail(W4A16_ERR_INVALID_ARG, "T (%d) must not be negative", T);
+    if (T > KV4_MAX_ROWS) return fail(W4A16_ERR_UNSUPPORTED, "%d rows: at most %d in a call", T, KV4_MAX_ROWS);
+    if (T == 0) return W4A16_OK;
+    if (!slots || !cache) return fail(W4A16_ERR_INVALID_ARG, "null pointer argument (slots or cache)");
+    if (!aligned(cache, 16) || !aligned(slots, 4)) return fail(W4A16_ERR_INVALID_ARG, "cache must be 16-byte aligned, slots 4-byte");
+    if (int rc = check_rows(write ? "k" : "k_out", k, k_st, k_sh, T, Hkv, D, !write)) return rc;
+    if (int rc = check_rows(write ? "v" : "v_out", v, v_st, v_sh, T, Hkv, D, !write)) return rc;
+    Kv4RowParams p{};
+    p.k = p.k_out = k; p.v = p.v_out = v;
+    p.k_st = k_st; p.k_sh = k_sh; p.v_st = v_st; p.v_sh = v_sh;
+    p.slots = slots; p.cache = static_cast<unsigned char*>(cache);
+    p.num_pages = num_pages; p.T = T; p.Hkv = Hkv; p.page_shift = __builtin_ctz((unsigned)page_size);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    const hipError_t e = write ? launch_kv4_write(elem == W4A16_BF16, D, p, st) : launch_kv4_read(elem == W4A16_BF16, D, p, st);
+    return e == hipSuccess ? W4A16_OK : hip_fail(e, write ? "kv4 write launch" : "kv4 read launch");
+}
+
+}  // namespace w4a16
+
+using namespace w4a16;
+
+extern "C" {
+
+W4A16_API size_t w4a16_kv4_cache_bytes(int32_t num_pages, int32_t Hkv, int32_t D, int32_t page_size) {
+    if (num_pages < 1 || Hkv < 1 || Hkv > KV4_MAX_HEADS || !kv4_head_dim_ok(D) || !kv4_page_ok(page_size) ||
+        (int64_t)num_pages * page_size > INT32_MAX)
+        return 0;
+    return (size_t)num_pages * Hkv * (page_size / KV4_BLOCK) * kv4_block_bytes(D);
+}
+
+W4A16_API int w4a16_kv4_write(void* stream, int elem, const void* k, const void* v, int32_t k_stride_t,
+                              int32_t k_stride_h, int32_t v_stride_t, int32_t v_stride_h, const int32_t* slots,
+                              void* cache, int32_t num_pages, int32_t T, int32_t Hkv, int32_t D, int32_t page_size) {
+    return kv4_rows(true, stream, elem, const_cast<void*>(k), const_cast<void*>(v), k_stride_t, k_stride_h, v_stride_t,
+                    v_stride_h, slots, cache, num_pages, T, Hkv, D, page_size);
+}
+
+W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const int32_t* slots, void* k_out, void* v_out,
+                             int32_t k_stride_t, int32_t k_stride_h, int32_t v_stride_t, int32_t v_stride_h,
+                             int32_t num_pages, int32_t T, int32_t Hkv, int32_t D, int32_t page_size) {
+    return kv4_rows(false, stream, elem, k_out, v_out, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots,
+                    const_cast<void*>(cache), num_pages, T, Hkv, D, page_size);
+}
+
+static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q, int32_t max_kv) {
+    if (T < 0 || B < 0 || max_q < 1 || max_kv < 0)
+        return fail(W4A16_ERR_INVALID_ARG, "bad sizes (T=%d B=%d max_q_len=%d max_kv_len=%d)", T, B, max_q, max_kv);
+    if (Hq < 1 || Hkv < 1 || Hq % Hkv)
+        return fail(W4A16_ERR_INVALID_ARG, "%d query heads must be a multiple of %d key/value heads", Hq, Hkv);
+    if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
+    if (Hq > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hq, KV4_MAX_HEADS);
+    if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
+    if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
+    return W4A16_OK;
+}
+
+W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D,
+                                                    int32_t max_q_len, int32_t max_kv_len) {
+    if (check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return 0;
+    return 256;
+}
+
+W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t q_stride_t, int32_t q_stride_h,
+                                  const void* cache, const int32_t* page_table, const int32_t* kv_lens,
+                                  const int32_t* cu_q, void* out, int32_t out_stride_t, int32_t out_stride_h, float* lse,
+                                  int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t num_pages,
+                                  int32_t page_size, int32_t pages_per_seq, int32_t max_q_len, int32_t max_kv_len,
+                                  float scale, int32_t causal, int32_t window, void* workspace, size_t workspace_bytes) {
+    if (int rc = check_elem(elem)) return rc;
+    if (int rc = check_geometry(num_pages, Hkv, D, page_size)) return rc;
+    if (int rc = check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return rc;
+    if (pages_per_seq < 1) return fail(W4A16_ERR_INVALID_ARG, "pages_per_seq (%d) must be positive", pages_per_seq);
+    if (window < 0) return fail(W4A16_ERR_INVALID_ARG, "window (%d) must not be negative", window);
+    if (!std::isfinite(scale)) return fail(W4A16_ERR_INVALID_ARG, "scale must be finite");
+    if (!cu_q && T != B) return fail(W4A16_ERR_INVALID_ARG, "without cu_q every sequence has one query (T=%d B=%d)", T, B);
+    if (!cu_q && max_q_len != 1) return fail(W4A16_ERR_INVALID_ARG, "without cu_q max_q_len is 1, not %d", max_q_len);
+    if (T == 0 || B == 0) return W4A16_OK;
+    if (!cache || !page_table || !kv_lens) return fail(W4A16_ERR_INVALID_ARG, "null pointer argument (cache, page_table or kv_lens)");
+    if (!aligned(cache, 16)) return fail(W4A16_ERR_INVALID_ARG, "cache must be 16-byte aligned");
+    if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(cu_q, 4) || !aligned(lse, 4))
+        return fail(W4A16_ERR_INVALID_ARG, "page_table, kv_lens, cu_q and lse must be 4-byte aligned");
+    if (int rc = check_rows("q", q, q_stride_t, q_stride_h, T, Hq, D, false)) return rc;
+    if (int rc = check_rows("out", out, out_stride_t, out_stride_h, T, Hq, D, true)) return rc;
+    const size_t need = w4a16_kv4_attention_workspace_size(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
+    if (!workspace || workspace_bytes < need)
+        return fail(W4A16_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace ? workspace_bytes : (size_t)0, need);
+    if (!aligned(workspace, 256)) return fail(W4A16_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
+    Kv4AttnParams p{};
+    p.q = q; p.out = out; p.lse = lse; p.cache = static_cast<const unsigned char*>(cache);
+    p.table = page_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
+    p.q_st = q_stride_t; p.q_sh = q_stride_h; p.o_st = out_stride_t; p.o_sh = out_stride_h;
+    p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
+    p.page_shift = __builtin_ctz((unsigned)page_size);
+    p.max_q = max_q_len < T ? max_q_len : T; p.max_kv = max_kv_len;
+    p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window;
+    (void)hipGetLastError();
+    const hipError_t e = launch_kv4_attention(elem == W4A16_BF16, D, p, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? W4A16_OK : hip_fail(e, "kv4 attention launch");
+}
+
+}  // extern "C"

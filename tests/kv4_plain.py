@@ -50,13 +50,14 @@ def pack(cache: np.ndarray, slot: int, h: int, which: int, n, s16: torch.Tensor,
 
 
 def attention(q, k, v, nq, lens, causal=True, window=0, scale=None, seen=None):
-    """(out, lse, spread, reach) in 64 bits: q [T, Hq, D] rows of sequence after sequence, k and v
+    """(out, lse, spread, reach, vtop) in 64 bits: q [T, Hq, D] rows of sequence after sequence, k and v
     lists of [len, Hkv, D] arrays. spread: sum p |v| / sum p; reach: the largest sum of |q k| scale of
-    a row, both for error bounds. seen: per sequence a mask [len] of keys that exist at all."""
+    a row, vtop: the largest |v| of its sequence and head, all for error bounds. seen: per sequence a mask [len] of keys that exist at all."""
     T, Hq, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     out, spread = np.zeros((T, Hq, D)), np.zeros((T, Hq, D))
     lse, reach = np.full((T, Hq), -np.inf), np.zeros((T, Hq))
+    vtop = np.zeros((T, Hq))
     at = 0
     for b, (n, L) in enumerate(zip(nq, lens)):
         G = Hq // k[b].shape[1]
@@ -71,6 +72,7 @@ def attention(q, k, v, nq, lens, causal=True, window=0, scale=None, seen=None):
             if not see.any():
                 continue
             for a in range(Hq):
+                vtop[at + i, a] = np.abs(v[b][:, a // G]).max()
                 kk, vv = k[b][see, a // G], v[b][see, a // G]
                 with np.errstate(all="ignore"):
                     w = kk @ q[at + i, a] * scale
@@ -81,4 +83,4 @@ def attention(q, k, v, nq, lens, causal=True, window=0, scale=None, seen=None):
                     lse[at + i, a] = m + np.log(p.sum())
                     reach[at + i, a] = (np.abs(kk) @ np.abs(q[at + i, a])).max() * abs(scale)
         at += n
-    return out, lse, spread, reach
+    return out, lse, spread, reach, vtop

@@ -150,16 +150,18 @@ class Batch:
     def check(self, out, lse, causal=True, window=0, scale=None, seen=None, what=""):
         """Bounds: the weights p_j, rounded to fp16 (2^-11), times values; the logits, whose products
         (sum of |q k| at most `reach`) are summed in fp32 over D terms, an error in the exponent of p;
-        sums over the keys in fp32; one rounding of the result."""
+        sums over the keys in fp32; one rounding of the result. Weights below fp16's normal range move
+        by half of 2^-24: they are p_j s_j 2^7 / r with r at most 4 times the largest scale s, so a key's
+        share of the sum by 2^-25 2^-7 4 s |n - z| <= 2^-30 15 s <= 2^-29 max|v|, the sum of all p_j
+        being 1 or more."""
         q = self.q.double().numpy()
-        o, l, spread, reach = plain.attention(q, self.k, self.v, self.nq, self.lens, causal, window, scale, seen)
+        o, l, spread, reach, vtop = plain.attention(q, self.k, self.v, self.nq, self.lens, causal, window, scale, seen)
         keys = max(self.lens) + 8
-        # a nibble's product is bounded by 15 / 7.5 of the largest value's: n and z are summed apart
         logit = (self.D + 8) * 2.0 ** -23 * (4 * reach + 1)
         eps = torch.finfo(self.dtype).eps / 2
         tiny = 2.0 ** -25 if self.dtype == F16 else 2.0 ** -134
         part = (2.0 ** -11 + 2 * logit + keys * 2.0 ** -23 + 2.0 ** -16)[..., None]
-        tol = eps * np.abs(o) + part * (1 + eps) * 2 * spread + tiny
+        tol = eps * np.abs(o) + part * (1 + eps) * 2 * spread + tiny + keys * 2.0 ** -29 * vtop[..., None]
         got = out.double().cpu().numpy()
         bad = ~(np.abs(got - o) <= tol)
         assert not bad.any(), (what, np.argwhere(bad)[:5], got[bad][:5], o[bad][:5], tol[bad][:5])

@@ -49,7 +49,23 @@ struct Kv4AttnParams {
     int num_pages, pages_per_seq, T, B, Hq, Hkv, page_shift, max_q, max_kv;
     float scale_log2;                 // scale * log2(e)
     int causal, window;
+    uint32_t* counters;               // one a tile of columns, zero between calls
+    float* partials;                  // [tile][B][Hkv][splits] of slot_cols (D + 2) floats
+    // set by the launcher from the shape
+    int G, tiles, splits, chunk_thin, chunk_full, slot_cols;
 };
-hipError_t launch_kv4_attention(bool bf16, int D, const Kv4AttnParams& p, hipStream_t st);
+constexpr size_t KV4_MAX_COUNTERS = 16384;
+struct Kv4AttnShape {
+    bool ok;
+    int nt;            // columns of a wave / 16
+    int tiles;         // tiles of 64 nt columns of a sequence and key/value head
+    int splits;        // chunks of the keys, at most
+    int chunk_thin;    // keys of a chunk where waves share columns (at most half a tile's)
+    int chunk_full;    // where each wave has columns of its own
+    int slot_cols;     // columns of a chunk's partial results
+    size_t partial_bytes;
+};
+Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv, int num_cus);
+hipError_t launch_kv4_attention(bool bf16, int D, Kv4AttnParams p, const Kv4AttnShape& s, hipStream_t st);
 
 }  // namespace w4a16

@@ -13,6 +13,9 @@ namespace w4a16 {
 static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 constexpr int KV4_MAX_HEADS = 1024;
+// Compute units that the split of the keys is planned for: MI355X's, so that a workspace's size is the same wherever it is asked for.
+constexpr int KV4_CUS = 256;
+static_assert(KV4_MAX_COUNTERS * sizeof(uint32_t) == W4A16_KV4_COUNTER_BYTES, "counters fill their area");
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
 static int check_elem(int elem) {
@@ -106,6 +109,8 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
     if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
     if (Hq > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hq, KV4_MAX_HEADS);
     if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
+    if (!kv4_attention_shape(T < 1 ? 1 : T, B < 1 ? 1 : B, Hq, Hkv, D, max_q, max_kv, KV4_CUS).ok)
+        return fail(W4A16_ERR_UNSUPPORTED, "max_q_len %d with max_kv_len %d: too long for one call", max_q, max_kv);
     if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
     return W4A16_OK;
 }
@@ -113,7 +118,7 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
 W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D,
                                                     int32_t max_q_len, int32_t max_kv_len) {
     if (check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return 0;
-    return 256;
+    return W4A16_KV4_COUNTER_BYTES + kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len, KV4_CUS).partial_bytes;
 }
 
 W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t q_stride_t, int32_t q_stride_h,
@@ -137,7 +142,8 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
         return fail(W4A16_ERR_INVALID_ARG, "page_table, kv_lens, cu_q and lse must be 4-byte aligned");
     if (int rc = check_rows("q", q, q_stride_t, q_stride_h, T, Hq, D, false)) return rc;
     if (int rc = check_rows("out", out, out_stride_t, out_stride_h, T, Hq, D, true)) return rc;
-    const size_t need = w4a16_kv4_attention_workspace_size(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
+    const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len, KV4_CUS);
+    const size_t need = W4A16_KV4_COUNTER_BYTES + s.partial_bytes;
     if (!workspace || workspace_bytes < need)
         return fail(W4A16_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace ? workspace_bytes : (size_t)0, need);
     if (!aligned(workspace, 256)) return fail(W4A16_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
@@ -148,9 +154,11 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
     p.page_shift = __builtin_ctz((unsigned)page_size);
     p.max_q = max_q_len < T ? max_q_len : T; p.max_kv = max_kv_len;
-    p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window;
+    p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
+    p.counters = static_cast<uint32_t*>(workspace);
+    p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
     (void)hipGetLastError();
-    const hipError_t e = launch_kv4_attention(elem == W4A16_BF16, D, p, static_cast<hipStream_t>(stream));
+    const hipError_t e = launch_kv4_attention(elem == W4A16_BF16, D, p, s, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? W4A16_OK : hip_fail(e, "kv4 attention launch");
 }
 

@@ -608,7 +608,7 @@ def _kv4_rows(t, name: str, dtypes, dev, shape=None):
     if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
         raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
     st, sh, sd = t.stride()
-    if sd != 1 and t.shape[2] != 1:
+    if sd != 1:
         raise InvalidArgument(f"{name} must be contiguous along its last dimension")
     return st, sh
 
@@ -620,9 +620,18 @@ def _kv4_index(t, name: str, dev, numel=None):
                               + ("" if numel is None else f" of {numel} entries"))
 
 
-def _on(dev: torch.device):
-    """The device as the current one: kernels are launched on the current device's code object."""
-    return torch.cuda.device(dev)
+def _call_on(dev: torch.device, fn, *args) -> None:
+    """fn(stream, *args) on the device's current stream, with the device as the current one (kernels
+    are launched on the current device). Pointers go as plain integers: a decode step makes many of
+    these calls and each is a few microseconds of host time."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(torch.cuda.current_stream(index).cuda_stream, *args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(torch.cuda.current_stream(index).cuda_stream, *args)
+    if rc != OK:
+        check(rc)
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
@@ -637,9 +646,8 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torc
     kst, ksh = _kv4_rows(k, "k", _ELEM, dev, shape)
     vst, vsh = _kv4_rows(v, "v", (k.dtype,), dev, shape)
     _kv4_index(slots, "slots", dev, shape[0])
-    with _on(dev):
-        check(lib().w4a16_kv4_write(_stream(cache), _elem_flag(k), _ptr(k), _ptr(v), kst, ksh, vst, vsh,
-                                    _ptr(slots), _ptr(cache), pages, shape[0], Hkv, D, page))
+    _call_on(dev, lib().w4a16_kv4_write, _elem_flag(k), k.data_ptr(), v.data_ptr(), kst, ksh, vst, vsh,
+             slots.data_ptr(), cache.data_ptr(), pages, shape[0], Hkv, D, page)
     return cache
 
 
@@ -650,18 +658,17 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
     pages, Hkv, page, D = _kv4_cache_shape(cache)
     dev = cache.device
     _kv4_index(slots, "slots", dev)
-    T = slots.numel()
     if slots.dim() != 1:
         raise InvalidArgument("slots must be 1-D")
+    T = slots.shape[0]
     if (k_out is None) != (v_out is None):
         raise InvalidArgument("give both k_out and v_out, or neither")
     if k_out is None:
         k_out, v_out = torch.zeros((2, T, Hkv, D), dtype=dtype, device=dev)
     kst, ksh = _kv4_rows(k_out, "k_out", _ELEM, dev, (T, Hkv, D))
     vst, vsh = _kv4_rows(v_out, "v_out", (k_out.dtype,), dev, (T, Hkv, D))
-    with _on(dev):
-        check(lib().w4a16_kv4_read(_stream(cache), _elem_flag(k_out), _ptr(cache), _ptr(slots), _ptr(k_out),
-                                   _ptr(v_out), kst, ksh, vst, vsh, pages, T, Hkv, D, page))
+    _call_on(dev, lib().w4a16_kv4_read, _elem_flag(k_out), cache.data_ptr(), slots.data_ptr(),
+             k_out.data_ptr(), v_out.data_ptr(), kst, ksh, vst, vsh, pages, T, Hkv, D, page)
     return k_out, v_out
 
 
@@ -723,18 +730,17 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
             raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
     if T == 0 or B == 0:
         return out
-    with _on(dev):
-        if workspace is None:
-            workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
-        else:
-            _require(workspace, "workspace", (torch.uint8,), dev)
-            if not workspace.is_contiguous():
-                raise InvalidArgument("workspace must be contiguous")
-        check(lib().w4a16_kv4_attention(
-            _stream(cache), _elem_flag(q), _ptr(q), qst, qsh, _ptr(cache), _ptr(page_table), _ptr(kv_lens),
-            _ptr(cu_q), _ptr(out), ost, osh, _ptr(lse), T, B, Hq, Hkv, D, pages, page, per, max_q_len,
-            max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window, _ptr(workspace),
-            workspace.numel()))
+    if workspace is None:
+        workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
+    else:
+        _require(workspace, "workspace", (torch.uint8,), dev)
+        if not workspace.is_contiguous():
+            raise InvalidArgument("workspace must be contiguous")
+    _call_on(dev, lib().w4a16_kv4_attention, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),
+             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
+             out.data_ptr(), ost, osh, None if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, pages, page,
+             per, max_q_len, max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window,
+             workspace.data_ptr(), workspace.numel())
     return out
 
 

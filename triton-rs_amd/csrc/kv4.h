@@ -1,5 +1,5 @@
-// Key/value cache in 4 bits: layout, launch parameters and the launchers of kv4_cache.hip and
-// kv4_attention.hip.
+// Key/value cache in 4 bits: layout, launch parameters and the launchers of kv4_cache.hip,
+// kv4_few.hip and kv4_many.hip.
 //
 // A cache is num_pages pages of [Hkv][page_size / 16] blocks; a block holds 16 tokens of one head in
 // 16 D + 128 bytes:
@@ -51,21 +51,21 @@ struct Kv4AttnParams {
     int causal, window;
     uint32_t* counters;               // one a tile of columns, zero between calls
     float* partials;                  // [tile][B][Hkv][splits] of slot_cols (D + 2) floats
-    // set by the launcher from the shape
-    int G, tiles, splits, chunk_thin, chunk_full, slot_cols;
+    // from the shape
+    int G, tiles, splits, chunk, slot_cols, pair_tiles;
 };
 constexpr size_t KV4_MAX_COUNTERS = 16384;
 struct Kv4AttnShape {
-    bool ok;
+    bool many;         // kv4_many.hip, else kv4_few.hip
     int nt;            // columns of a wave / 16
-    int tiles;         // tiles of 64 nt columns of a sequence and key/value head
+    int tiles;         // tiles of columns of a sequence and key/value head
     int splits;        // chunks of the keys, at most
-    int chunk_thin;    // keys of a chunk where waves share columns (at most half a tile's)
-    int chunk_full;    // where each wave has columns of its own
+    int chunk;         // keys of a chunk
     int slot_cols;     // columns of a chunk's partial results
+    bool pair_tiles;   // long and short tiles of columns by turns
     size_t partial_bytes;
 };
-Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv, int num_cus);
-hipError_t launch_kv4_attention(bool bf16, int D, Kv4AttnParams p, const Kv4AttnShape& s, hipStream_t st);
+hipError_t launch_kv4_few(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
+hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
 
 }  // namespace w4a16

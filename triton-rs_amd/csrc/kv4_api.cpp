@@ -1,7 +1,9 @@
 // C-ABI entry points of the 4-bit key/value cache: argument checks (before any HIP call), then
-// the launchers of kv4_cache.hip and kv4_attention.hip.
+// the choice of an attention kernel, then the launchers of
+// kv4_cache.hip, kv4_few.hip and kv4_many.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/w4a16.h"
@@ -74,6 +76,30 @@ static int kv4_rows(bool write, void* stream, int elem, void* k, void* v, int32_
     return e == hipSuccess ? W4A16_OK : hip_fail(e, write ? "kv4 write launch" : "kv4 read launch");
 }
 
+// Which kernel, and how the keys are split. Few columns (up to 64) go to the kernel whose waves share them. The
+// keys are split as far as it takes to fill the places of workgroups that run at once (`slots`), no further:
+// each chunk costs its partial results a round trip through memory.
+static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv) {
+    Kv4AttnShape s{};
+    const int64_t G = Hq / Hkv, C = (int64_t)(max_q < T ? max_q : T) * G;
+    s.many = C > 64;
+    s.nt = s.many || C > 16 ? 2 : 1;
+    const int wg_cols = s.many ? 128 : 32 * s.nt;
+    const int64_t tiles = std::max<int64_t>(1, (C + wg_cols - 1) / wg_cols), items = std::max<int64_t>(1, tiles * B * Hkv);
+    const int per_cu = s.many ? (D <= 128 ? 2 : 1) : D * s.nt >= 512 ? 1 : D * s.nt > 128 ? 2 : 3;
+    const int64_t slots = (int64_t)KV4_CUS * per_cu, least = s.many ? 512 : 128;
+    int64_t want = s.many ? (slots + items - 1) / items : slots / items;
+    if (items > (int64_t)KV4_MAX_COUNTERS) want = 1;
+    want = std::max<int64_t>(1, std::min(want, (max_kv + least - 1) / least));
+    s.chunk = (int)((((int64_t)max_kv + want - 1) / want + 127) / 128 * 128);
+    s.splits = s.chunk > 0 ? (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk) : 1;
+    s.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
+    s.pair_tiles = s.many && items * s.splits <= slots;
+    s.slot_cols = s.many ? wg_cols : (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
+    if (s.splits > 1) s.partial_bytes = (size_t)items * s.splits * s.slot_cols * (D + 2) * sizeof(float);
+    return s;
+}
+
 }  // namespace w4a16
 
 using namespace w4a16;
@@ -109,16 +135,17 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
     if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
     if (Hq > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hq, KV4_MAX_HEADS);
     if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
-    if (!kv4_attention_shape(T < 1 ? 1 : T, B < 1 ? 1 : B, Hq, Hkv, D, max_q, max_kv, KV4_CUS).ok)
-        return fail(W4A16_ERR_UNSUPPORTED, "max_q_len %d with max_kv_len %d: too long for one call", max_q, max_kv);
     if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
+    const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q, max_kv);
+    if ((int64_t)s.tiles * s.splits > 65535)
+        return fail(W4A16_ERR_UNSUPPORTED, "max_q_len %d with max_kv_len %d: too many tiles for one call", max_q, max_kv);
     return W4A16_OK;
 }
 
 W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D,
                                                     int32_t max_q_len, int32_t max_kv_len) {
     if (check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return 0;
-    return W4A16_KV4_COUNTER_BYTES + kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len, KV4_CUS).partial_bytes;
+    return W4A16_KV4_COUNTER_BYTES + kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len).partial_bytes;
 }
 
 W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t q_stride_t, int32_t q_stride_h,
@@ -142,7 +169,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
         return fail(W4A16_ERR_INVALID_ARG, "page_table, kv_lens, cu_q and lse must be 4-byte aligned");
     if (int rc = check_rows("q", q, q_stride_t, q_stride_h, T, Hq, D, false)) return rc;
     if (int rc = check_rows("out", out, out_stride_t, out_stride_h, T, Hq, D, true)) return rc;
-    const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len, KV4_CUS);
+    const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
     const size_t need = W4A16_KV4_COUNTER_BYTES + s.partial_bytes;
     if (!workspace || workspace_bytes < need)
         return fail(W4A16_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace ? workspace_bytes : (size_t)0, need);
@@ -157,8 +184,12 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
     p.counters = static_cast<uint32_t*>(workspace);
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
+    p.G = Hq / Hkv; p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.slot_cols = s.slot_cols;
+    p.pair_tiles = s.pair_tiles;
     (void)hipGetLastError();
-    const hipError_t e = launch_kv4_attention(elem == W4A16_BF16, D, p, s, static_cast<hipStream_t>(stream));
+    const bool bf16 = elem == W4A16_BF16;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const hipError_t e = s.many ? launch_kv4_many(bf16, D, p, s, st) : launch_kv4_few(bf16, D, p, s, st);
     return e == hipSuccess ? W4A16_OK : hip_fail(e, "kv4 attention launch");
 }
 

@@ -1,0 +1,508 @@
+// Attention over the 4-bit key/value cache (kv4.h): what its two kernels share.
+//
+// Query row i of sequence b stands at position kv_len - q_len + i and sees key j < kv_len where
+// (causal) j <= its position and (window) j > its position - window:
+//   w_j = scale q . k_j,  out = sum_j p_j v_j / sum_j p_j,  p_j = exp(w_j - m),  lse = m + ln sum
+// in one pass over the keys with a running reference m (no visible key: out = 0, lse = -infinity).
+//
+// A row of keys is s (n - z), so q . k = s (q . (n - z)), and sum_j p_j v_j is sum_j (p_j s_j) (n_j - z_j):
+// the matrix cores (v_mfma_f32_16x16x32_f16) take the integers n - z and a scale acts on one logit or
+// weight a token. Masked out of its word into 0x6400 a nibble is the fp16 number 1024 + n (1024 + 16 n
+// from bits 4..7 of a half); one packed subtraction of 1024 + z, or fma with 1/16 and 64 + z, gives
+// n - z exactly: nine instructions for eight operands. (A nibble left as the fp16 subnormal that it is
+// without the 0x6400 needs five, but the matrix cores align a sum's terms by the exponents that their
+// operands show, and a subnormal shows 2^-14: errors of 2^-12 of the largest term.)
+//
+// A wave holds 16 NT columns (query rows times the G query heads of one key/value head) and walks the
+// keys 32 at a time. With S^T = K Q^T a lane has the logits of one column at tokens 4 (lane / 16) + i of
+// either block of 16, which is how the second product takes them as its operand (the sum over the
+// tokens may run in any order as long as the values follow), so no logit or weight passes between lanes
+// or through LDS. q is scaled by a power of two (wave-wide) into fp16's range, exactly for fp16 and bf16
+// alike but for what lies 2^27 below the largest. A weight p_j s_j is rounded to fp16; the reference m is
+// such that all of them are below 2^16, and raised (with the sums scaled down) only where a logit or a
+// value scale passes what it leaves room for, 8 in base 2, so maxima pass between lanes only then. Sums
+// are fp32.
+#pragma once
+#include <cfloat>
+
+#include "device_common.h"
+#include "kv4.h"
+#include "splitk.h"
+
+namespace w4a16 {
+
+constexpr int KV4_WEIGHT_LOG2 = 15;   // p_j s_j <= 2^15
+constexpr float KV4_ROOM = 8.0f;      // a raise leaves the largest p_j at 2^-8 of what it may be
+
+template <typename E>
+__device__ __forceinline__ float param_scale(uint32_t w) {
+    if constexpr (__is_same(E, half_t)) return (float)__builtin_bit_cast(half_t, (uint16_t)w);
+    else return bf16_bits_to_f32(w);   // the shift drops the upper half
+}
+
+__device__ __forceinline__ half8_t as_h8(half2_t a, half2_t b, half2_t c, half2_t d) {
+    const u32x4 t = {as_u32(a), as_u32(b), as_u32(c), as_u32(d)};
+    return __builtin_bit_cast(half8_t, t);
+}
+
+// n - z of the nibbles at bits 0 and 16 of x, z1 = 1024 + z; of those at bits 4 and 20, z16 = 64 + z
+__device__ __forceinline__ half2_t centred(uint32_t x, half2_t z1) { return nib_pair(x) - z1; }
+__device__ __forceinline__ half2_t centred16(uint32_t x, half2_t z16) {
+    return __builtin_elementwise_fma(nib_pair16(x), half2_t{(half_t)0.0625f, (half_t)0.0625f}, -z16);
+}
+// a pair of zero points (one in each half) as 1024 + z and 64 + z
+__device__ __forceinline__ half2_t zero1024(uint32_t z) { return as_h2(z | 0x64006400u); }
+__device__ __forceinline__ half2_t zero64(uint32_t z) { return as_h2((z << 4) | 0x54005400u); }
+// zero points out of parameter words: of one, twice; of two
+__device__ __forceinline__ uint32_t zeros_of(uint32_t w) { return perm(0u, w, 0x03020302u); }
+__device__ __forceinline__ uint32_t zeros_of(uint32_t lo, uint32_t hi) { return perm(hi, lo, 0x07060302u); }
+
+// the operand of a word of keys: dimensions 8 w + (0, 4, 1, 5, 2, 6, 3, 7) of the lane's quarter row
+__device__ __forceinline__ half8_t key_operand(uint32_t x, half2_t z1, half2_t z16) {
+    const uint32_t y = x >> 8;
+    return as_h8(centred(x, z1), centred16(x, z16), centred(y, z1), centred16(y, z16));
+}
+// a pair of tokens' values at nibble e (0..3) of their halves of x
+template <int EI>
+__device__ __forceinline__ half2_t value_pair(uint32_t x, half2_t z1, half2_t z16) {
+    const uint32_t y = EI & 2 ? x >> 8 : x;
+    return EI & 1 ? centred16(y, z16) : centred(y, z1);
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+
+template <typename E>
+__device__ __forceinline__ float saturate(float v) {
+    constexpr float most = __is_same(E, half_t) ? 65504.f : 0x1.fep127f;
+    return v > most ? most : v < -most ? -most : v;   // (NaN stays)
+}
+
+__device__ __forceinline__ float kb_sum(float v) {   // over the four lanes of a column
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float kb_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
+
+// A scale of NaN (a row that held an infinity or NaN, n = z = 0) as the largest number: the weight of a column that
+// does not see the token is then 0, of one that does it is infinity, and its product with n - z NaN.
+__device__ __forceinline__ float seen_scale(float s) { return fminf(s, FLT_MAX); }
+
+// What a workgroup takes of sequence b, key/value head h: columns from c0 on, of keys [k0, k1) of this chunk.
+struct Kv4Item {
+    int h, b, q0, n, len, first;   // first row of q, queries, keys, position of query 0
+    int c0, cols;                  // first column, columns from there to the sequence's end
+    int split, chunks, k0, k1;
+    size_t at;                     // number of (tile, b, h)
+    __device__ __forceinline__ int see_hi(const Kv4AttnParams& p, int i) const { return p.causal ? max(0, min(len, first + i + 1)) : len; }
+    __device__ __forceinline__ int see_lo(const Kv4AttnParams& p, int i) const { return p.window ? max(0, first + i - p.window + 1) : 0; }
+};
+
+// wg_cols columns a workgroup; chunks start at multiples of `step`. false: nothing to do.
+template <int WG_COLS, int STEP>
+__device__ __forceinline__ bool kv4_item(const Kv4AttnParams& p, Kv4Item& w) {
+    w.h = blockIdx.x;
+    w.b = blockIdx.y;
+    const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
+    w.split = p.splits == 1 ? 0 : blockIdx.z - z * p.splits;
+    // columns of long rows first, or (where all workgroups run at once) long and short by turns
+    const int tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
+    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
+    int q1 = w.b + 1;
+    w.q0 = w.b;
+    if (p.cu_q) {
+        w.q0 = min(max(p.cu_q[w.b], 0), p.T);
+        q1 = min(max(p.cu_q[w.b + 1], 0), p.T);
+    }
+    w.n = min(q1 - w.q0, p.max_q);
+    w.c0 = tile * WG_COLS;
+    w.cols = w.n * p.G - w.c0;
+    if (w.cols <= 0) return false;
+    const long long cap = (long long)p.pages_per_seq << p.page_shift;
+    w.len = (int)max(0ll, min((long long)min(p.kv_lens[w.b], p.max_kv), cap));
+    w.first = w.len - (q1 - w.q0);
+    const int i0 = w.n == 1 ? 0 : w.c0 / p.G, i1 = w.n == 1 ? 0 : (min(w.c0 + WG_COLS, w.n * p.G) - 1) / p.G;
+    const int hi = w.see_hi(p, i1), lo = min(w.see_lo(p, i0), hi) & ~(STEP - 1);
+    w.chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
+    if (w.split >= w.chunks) return false;
+    w.k0 = p.splits == 1 ? lo : lo + w.split * p.chunk;
+    w.k1 = p.splits == 1 ? hi : min(hi, w.k0 + p.chunk);
+    return true;
+}
+
+// A wave's 16 NT columns.
+template <typename E, int D, int NT>
+struct Kv4Cols {
+    static constexpr int KW = D / 32;   // words of a lane's quarter row of keys: MFMAs of a block
+    static constexpr int VT = D / 16;   // 16-row tiles of the result
+    int c, n;              // first column, columns (0 or less: none)
+    int lo[NT], hi[NT];    // keys that this lane's columns see
+    int jlo, jhi;          // keys that some column sees, of the chunk
+    int all_lo, all_hi;    // keys that every column sees
+    half8_t qf[NT][KW];
+    float kscale;          // logits in base 2 are kscale s (q . (n - z))
+    float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
+    float most[NT];        // logits less m may be this; -infinity until a column has seen a key
+    float vtop;            // a power of two, 2^vlog2, above the largest value scale so far
+    int vlog2;
+    float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
+
+    // the rows of q, as they are
+    __device__ __forceinline__ void load(const Kv4AttnParams& p, const Kv4Item& w, int first_col, int lane) {
+        c = first_col;
+        n = min(16 * NT, w.n * p.G - c);
+        const int col = lane & 15, kb = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = c + 16 * t + col, i = w.n == 1 ? 0 : r / p.G;
+            const bool in = 16 * t + col < n;
+            hi[t] = in ? w.see_hi(p, i) : 0;
+            lo[t] = in ? w.see_lo(p, i) : 0;
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + (size_t)(w.q0 + i) * p.q_st + (size_t)(w.h * p.G + r - i * p.G) * p.q_sh + kb * (D / 4);
+#pragma unroll
+            for (int x = 0; x < KW; ++x) {
+                u32x4 v = {0, 0, 0, 0};
+                if (in) v = *reinterpret_cast<const u32x4*>(src + 8 * x);
+                qf[t][x] = __builtin_bit_cast(half8_t, v);
+            }
+        }
+        const int i0 = w.n == 1 ? 0 : c / p.G, i1 = w.n == 1 ? 0 : (c + max(n, 1) - 1) / p.G;
+        jlo = max(w.k0, w.see_lo(p, i0));
+        jhi = n > 0 ? min(w.k1, w.see_hi(p, i1)) : 0;
+        all_lo = w.see_lo(p, i1);
+        all_hi = w.see_hi(p, i0);
+    }
+
+    // the largest |q| of the wave's rows, infinities and NaN aside
+    __device__ __forceinline__ float largest() const {
+        float top = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < KW; ++x) {
+                const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float a = fabsf(param_scale<E>(v[e >> 1] >> (16 * (e & 1))));
+                    top = fmaxf(top, a < INFINITY ? a : 0.f);
+                }
+            }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        return top;
+    }
+
+    // q in operand order under the power of two that `top`, the largest of the rows, gives
+    __device__ __forceinline__ void start(const Kv4AttnParams& p, float top) {
+        // q 2^e has its largest value in [2^13, 2^14) (or all of it is zero)
+        const int e2 = top > 0.f ? min(100, max(-100, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
+        const float up = pow2(e2);
+        kscale = p.scale_log2 * pow2(-e2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int x = 0; x < KW; ++x) {
+                const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
+                half8_t f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)   // dimension e meets the nibble at bits 4 e: operand slot 2 (e % 4) + e / 4
+                    f[2 * (e & 3) + (e >> 2)] = (half_t)(param_scale<E>(v[e >> 1] >> (16 * (e & 1))) * up);
+                qf[t][x] = f;
+            }
+            m[t] = l[t] = 0.f;
+            most[t] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < VT; ++x) o[t][x] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        vtop = 0.f;
+        vlog2 = 0;
+    }
+
+    // The largest value scale of a step, vmax, of all lanes: room made for it.
+    __device__ __forceinline__ void value_top(float vmax) {
+        // 2 to 4 times the largest; value scales below 2^-60 share one
+        const int e = min(126, max(-60, (int)(__float_as_uint(vmax) >> 23) - 127 + 2));
+        const float by = (float)(e - vlog2), fall = __builtin_amdgcn_exp2f(-by);
+        vtop = pow2(e);
+        vlog2 = e;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const bool set = most[t] != -INFINITY;   // (else nothing is summed yet)
+            m[t] += set ? by : 0.f;
+            l[t] *= fall;
+            if (set) most[t] = (float)(KV4_WEIGHT_LOG2 - e);
+#pragma unroll
+            for (int x = 0; x < VT; ++x) o[t][x] *= fall;
+        }
+    }
+
+    // Logits less m of 32 tokens from j on for columns t: acc = q . (n - z), ks = key scale times kscale, of the
+    // lane's tokens j + 16 s + 4 kb + i. whole: every column sees all 32; else tokens from `end` on and those
+    // of blocks in `bad` are not seen. Raises m where they pass it by too much.
+    __device__ __forceinline__ void logits(int t, float (&x)[2][4], const float4_t (&acc)[2], const float (&ks)[2][4], bool whole,
+                                           int j, int end, int bad, int kb) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[s][i] = __builtin_fmaf(acc[s][i], ks[s][i], -m[t]);
+        if (!whole) {
+            const int from = lo[t], to = min(hi[t], end);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = j + 16 * s + 4 * kb + i;
+                    if (at < from || at >= to || ((bad >> s) & 1)) x[s][i] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[s][i]);
+        if (__any(top > most[t])) {
+            top = kb_max(top);
+            const bool up = top > most[t];
+            const float room = (float)(KV4_WEIGHT_LOG2 - vlog2), by = up ? top - (room - KV4_ROOM) : 0.f;
+            // (a column's first keys: nothing summed yet)
+            const float fall = most[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-by);
+            m[t] += by;
+            l[t] *= fall;
+#pragma unroll
+            for (int y = 0; y < VT; ++y) o[t][y] *= fall;
+            if (up) most[t] = room;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[s][i] -= by;
+        }
+    }
+
+    // Their weights p_j s_j as operand, vs = value scales (seen_scale of them where `whole` is not); the sum of p_j.
+    __device__ __forceinline__ half8_t weights(int t, const float (&x)[2][4], const float (&vs)[2][4]) {
+        half8_t w;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pj = __builtin_amdgcn_exp2f(x[s][i]);
+                l[t] += pj;
+                w[4 * s + i] = (half_t)(pj * vs[s][i]);
+            }
+        return w;
+    }
+
+    // sums over the lanes of a column
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            l[t] = kb_sum(l[t]);
+            if (most[t] == -INFINITY && l[t] == 0.f) m[t] = -FLT_MAX;
+        }
+    }
+};
+
+// Where a workgroup's results go: out and lse, or (more than one chunk) its slot of fp32 partials.
+template <typename E, int D>
+struct Kv4Sink {
+    const Kv4AttnParams& p;
+    const Kv4Item& w;
+    float *item, *part, *part_ml;
+    size_t slot_floats;
+    __device__ __forceinline__ Kv4Sink(const Kv4AttnParams& p_, const Kv4Item& w_) : p(p_), w(w_) {
+        slot_floats = (size_t)p.slot_cols * (D + 2);
+        item = p.partials + w.at * p.splits * slot_floats;
+        part = item + w.split * slot_floats;
+        part_ml = part + (size_t)p.slot_cols * D;
+    }
+    // column r (of the sequence): row of q and head
+    __device__ __forceinline__ void place(int r, int& row, int& head) const {
+        const int i = w.n == 1 ? 0 : r / p.G;
+        row = w.q0 + i;
+        head = w.h * p.G + r - i * p.G;
+    }
+    __device__ __forceinline__ void out(int r, int d, float4_t v, float inv) const {
+        int row, head;
+        place(r, row, head);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (size_t)row * p.o_st + (size_t)head * p.o_sh + d;
+        *reinterpret_cast<u32x2*>(dst) = u32x2{pack2(E{}, saturate<E>(v[0] * inv), saturate<E>(v[1] * inv)),
+                                               pack2(E{}, saturate<E>(v[2] * inv), saturate<E>(v[3] * inv))};
+    }
+    __device__ __forceinline__ void lse(int r, float m, float l) const {
+        if (!p.lse) return;
+        int row, head;
+        place(r, row, head);
+        p.lse[(size_t)row * p.Hq + head] = lse_of(m, l);
+    }
+    // four values of column r from dimension d on, unnormalised; its reference and sum
+    __device__ __forceinline__ void put(int r, int d, float4_t v, float inv) const {
+        if (w.chunks > 1) st_partial4<SCOPE_DEVICE>(part + (size_t)(r - w.c0) * D + d, v);
+        else out(r, d, v, inv);
+    }
+    __device__ __forceinline__ void put_ml(int r, float m, float l) const {
+        if (w.chunks > 1) {
+            st_partial<SCOPE_DEVICE>(part_ml + 2 * (r - w.c0), m);
+            st_partial<SCOPE_DEVICE>(part_ml + 2 * (r - w.c0) + 1, l);
+        } else {
+            lse(r, m, l);
+        }
+    }
+    // The last of the chunks to arrive (splitk.h) joins them: per column (m, 1 / l) over all chunks, then the
+    // results, chunks in order within a share and shares in order (a share of the chunks a group of
+    // threads where there are fewer values than threads). 256 threads; ml: two floats a column, sums:
+    // 256 float4 of LDS. LANES: of 128 columns, in the order in which lanes have them.
+    template <bool LANES>
+    __device__ __forceinline__ void join(int live, float* ml, float4_t* sums, int* last) const {
+        if (!splitk_arrive(p.counters + w.at, w.chunks, last)) return;
+        const int chunks = w.chunks;
+        const float* heads = item + (size_t)p.slot_cols * D;
+        for (int c = threadIdx.x >> 2; c < ((live + 15) & ~15); c += 64) {   // (whole waves)
+            float mm = -FLT_MAX, ll = 0.f;
+            for (int s0 = threadIdx.x & 3; s0 < chunks; s0 += 32) {
+                uint64_t x[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    x[y] = c < live && s0 + 4 * y < chunks
+                               ? __hip_atomic_load(reinterpret_cast<const uint64_t*>(heads + (s0 + 4 * y) * slot_floats + 2 * c), __ATOMIC_RELAXED, SCOPE_DEVICE)
+                               : (uint64_t)__float_as_uint(-FLT_MAX);
+                float mn = mm;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) mn = fmaxf(mn, __uint_as_float((uint32_t)x[y]));
+                ll *= __builtin_amdgcn_exp2f(mm - mn);
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    ll += __uint_as_float((uint32_t)(x[y] >> 32)) * __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)x[y]) - mn);
+                mm = mn;
+            }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                const float om = __shfl_xor(mm, x), ol = __shfl_xor(ll, x), mn = fmaxf(mm, om);
+                ll = ll * __builtin_amdgcn_exp2f(mm - mn) + ol * __builtin_amdgcn_exp2f(om - mn);
+                mm = mn;
+            }
+            if ((threadIdx.x & 3) == 0 && c < live) {
+                ml[2 * c] = mm;
+                ml[2 * c + 1] = ll == 0.f ? 0.f : 1.f / ll;
+                lse(w.c0 + c, mm, ll);
+            }
+        }
+        __syncthreads();
+        if constexpr (LANES) {
+            // many values: four at a time, two chunks of each in flight
+            constexpr int U = 4, QUADS = 32 * D;   // 128 columns
+#pragma unroll 1
+            for (int e0 = threadIdx.x; e0 < QUADS; e0 += 256 * U) {
+                float4_t v[U];
+                float mm[U];
+                int c[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    int d;
+                    lane_place(e0 + 256 * u, c[u], d);
+                    c[u] = min(c[u], live - 1);
+                    mm[u] = ml[2 * c[u]];
+                    v[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+                }
+                for (int s0 = 0; s0 < chunks; s0 += 2) {
+                    float4_t x[U][2];
+                    float f[U][2];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const size_t s = min(s0 + y, chunks - 1);
+                            f[u][y] = __hip_atomic_load(heads + s * slot_floats + 2 * c[u], __ATOMIC_RELAXED, SCOPE_DEVICE);
+                            x[u][y] = ld_partial4<SCOPE_DEVICE>(item + s * slot_floats + 4 * (e0 + 256 * u));
+                        }
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            if (s0 + y < chunks) v[u] += x[u][y] * __builtin_amdgcn_exp2f(f[u][y] - mm[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    int cc, d;
+                    lane_place(e0 + 256 * u, cc, d);
+                    if (cc < live) out(w.c0 + cc, d, v[u], ml[2 * cc + 1]);
+                }
+            }
+            return;
+        }
+        const int quads = live * (D / 4);
+        const int shares = quads >= 256 ? 1 : min(256 / quads, 8), per = (chunks + shares - 1) / shares;
+        const int span = shares == 1 ? 256 : quads;
+        for (int e0 = 0; e0 < quads; e0 += span) {
+            const int share = threadIdx.x / span, e = e0 + threadIdx.x - share * span;
+            const bool on = e < quads && share < shares;
+            const int c = on ? e / (D / 4) : 0, d = 4 * (e - c * (D / 4));
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
+            if (on) {
+                const float mm = ml[2 * c];
+                const float* at = item + (size_t)c * D + d;
+                const int end = min(chunks, (share + 1) * per);
+                for (int s0 = share * per; s0 < end; s0 += 8) {
+                    float4_t x[8];
+                    float f[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const int s = min(s0 + y, end - 1);
+                        f[y] = __hip_atomic_load(heads + s * slot_floats + 2 * c, __ATOMIC_RELAXED, SCOPE_DEVICE);
+                        x[y] = ld_partial4<SCOPE_DEVICE>(at + s * slot_floats);
+                    }
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        if (s0 + y < end) v += x[y] * __builtin_amdgcn_exp2f(f[y] - mm);
+                }
+            }
+            if (shares > 1) {
+                sums[threadIdx.x] = v;
+                __syncthreads();
+                if (share == 0)
+                    for (int x = 1; x < shares; ++x) v += sums[x * span + threadIdx.x];
+            }
+            if (on && share == 0) out(w.c0 + c, d, v, ml[2 * c + 1]);
+        }
+    }
+    // Partial results in the order in which lanes have them (LANES): place of quad e
+    static constexpr int VT = D / 16;
+    __device__ __forceinline__ static int lane_quad(int wave, int t, int i, int x, int lane) {
+        return (((wave * 2 + t) * 4 + i) * (VT / 4) + x / 4) * 64 + lane;
+    }
+    __device__ __forceinline__ static void lane_place(int e, int& c, int& d) {
+        const int lane = e & 63, q = e >> 6, x = q % (VT / 4), r = q / (VT / 4);
+        c = 16 * (r >> 2) + (lane & 15);
+        d = (4 * (lane >> 4) + (r & 3)) * VT + 4 * x;
+    }
+};
+
+// Pages of a sequence, clamped to its keys (len > 0).
+struct Kv4Pages {
+    const int32_t* table;
+    const unsigned char* heads;   // head h of page 0
+    size_t page_bytes;
+    int bshift, last, num_pages, block_bytes;
+    __device__ __forceinline__ Kv4Pages(const Kv4AttnParams& p, const Kv4Item& w, int block) {
+        table = p.table + (size_t)w.b * p.pages_per_seq;
+        bshift = p.page_shift - 4;
+        last = (w.len - 1) >> 4;
+        num_pages = p.num_pages;
+        block_bytes = block;
+        page_bytes = ((size_t)p.Hkv * block) << bshift;
+        heads = p.cache + (((size_t)w.h * block) << bshift);
+    }
+    // (constant address space: a scalar load, also behind LDS loads written in asm, that is not counted with them)
+    __device__ __forceinline__ int page(int blk) const {
+        return ((const __attribute__((address_space(4))) int32_t*)table)[min(blk, last) >> bshift];
+    }
+    __device__ __forceinline__ bool ok(int page) const { return (unsigned)page < (unsigned)num_pages; }
+    __device__ __forceinline__ const unsigned char* block(int page, int blk) const {
+        return heads + (ok(page) ? (size_t)page * page_bytes : 0) + (size_t)(min(blk, last) & ((1 << bshift) - 1)) * block_bytes;
+    }
+};
+
+}  // namespace w4a16

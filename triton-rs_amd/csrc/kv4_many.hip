@@ -1,0 +1,235 @@
+// Attention over the 4-bit cache for many columns (prompts, chunks of them): bound by the matrix and
+// vector instructions. The mathematics is in kv4_attn_body.h.
+//
+// A workgroup of four waves takes 128 columns, 32 a wave, and walks the keys 64 at a time: each wave turns
+// a block of 16 tokens into the operands n - z once for all four, in LDS and in the order in which lanes
+// take them (16 bytes a lane, no bank conflicts), while the step before is computed from the other half
+// of the LDS: one barrier a step. The packed words come two steps ahead into registers.
+#include "kv4_attn_body.h"
+
+namespace w4a16 {
+
+template <int D>
+struct ManyLds {
+    static constexpr int KW = D / 32, VT = D / 16;
+    half8_t k[4][KW][64];      // block, word of the quarter row, lane
+    half8_t v[2][VT][64];      // pair of blocks, tile of the result, lane (first block's two pairs, second's)
+    float ks[64], vs[64];      // scales of the tokens, those of keys times kscale
+    float vtop[4];             // the largest of a block's value scales
+    int live[4];               // tokens of a block that there are (0 or less: none)
+};
+
+// A lane's words of a block (of this wave): keys of token lane % 16, values of tokens 4 (lane / 16)..+3, and
+// the parameters of these.
+template <int D>
+struct Packed {
+    uint32_t k[D / 32], v[D / 32], kc;
+    u32x4 vp;
+};
+
+template <int D>
+__device__ __forceinline__ void load_packed(Packed<D>& t, const unsigned char* b, int lane) {
+    const uint32_t ko = (lane & 15) * (D / 2) + (lane >> 4) * (D / 8), vo = 8 * D + lane * (D / 8);
+    if constexpr (D % 128 == 0) {
+#pragma unroll
+        for (int x = 0; x < D / 128; ++x) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(at_bytes(b, ko + 16 * x)), c = *reinterpret_cast<const u32x4*>(at_bytes(b, vo + 16 * x));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                t.k[4 * x + e] = a[e];
+                t.v[4 * x + e] = c[e];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+            const u32x2 a = *reinterpret_cast<const u32x2*>(at_bytes(b, ko + 8 * x)), c = *reinterpret_cast<const u32x2*>(at_bytes(b, vo + 8 * x));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                t.k[2 * x + e] = a[e];
+                t.v[2 * x + e] = c[e];
+            }
+        }
+    }
+    t.kc = *reinterpret_cast<const uint32_t*>(at_bytes(b, 16 * D + (lane & 15) * 4));
+    t.vp = *reinterpret_cast<const u32x4*>(at_bytes(b, 16 * D + 64 + (lane >> 4) * 16));
+}
+
+// Block `wave` of a step into LDS; its first `live` tokens (16 or more: all; the others' parameters may be anything)
+template <typename E, int D>
+__device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int live, float kscale, int wave, int lane) {
+    const int col = lane & 15, kb = lane >> 4;
+    t.kc = col < live ? t.kc : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.vp[i] = 4 * kb + i < live ? t.vp[i] : 0u;
+    const uint32_t zk = zeros_of(t.kc);
+    const half2_t kz1 = zero1024(zk), kz16 = zero64(zk);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) s.k[wave][x][lane] = key_operand(t.k[x], kz1, kz16);
+    half2_t vz1[2], vz16[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        const uint32_t z = zeros_of(t.vp[2 * y], t.vp[2 * y + 1]);
+        vz1[y] = zero1024(z);
+        vz16[y] = zero64(z);
+    }
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) {
+        auto put = [&](auto ei) {
+            constexpr int e = decltype(ei)::value;
+            u32x2* dst = reinterpret_cast<u32x2*>(&s.v[wave >> 1][4 * g + e][lane]) + (wave & 1);
+            *dst = u32x2{as_u32(value_pair<e>(t.v[g], vz1[0], vz16[0])), as_u32(value_pair<e>(t.v[D / 64 + g], vz1[1], vz16[1]))};
+        };
+        put(std::integral_constant<int, 0>{});
+        put(std::integral_constant<int, 1>{});
+        put(std::integral_constant<int, 2>{});
+        put(std::integral_constant<int, 3>{});
+    }
+    if (kb == 0) s.ks[16 * wave + col] = param_scale<E>(t.kc) * kscale;
+    float4_t f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = param_scale<E>(t.vp[i]);
+    const float top = kb_max(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = seen_scale(f[i]);
+    if (col == 0) *reinterpret_cast<float4_t*>(&s.vs[16 * wave + 4 * kb]) = f;
+    if (lane == 0) {
+        s.vtop[wave] = top;
+        s.live[wave] = live;
+    }
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4AttnParams p) {
+    constexpr int NT = 2, COLS = 16 * NT, STEP = 64;
+    typedef Kv4Cols<E, D, NT> C;
+    __shared__ ManyLds<D> lds[2];
+    __shared__ float ml[4 * COLS][2];
+    __shared__ int last;
+    Kv4Item w;
+    if (!kv4_item<4 * COLS, STEP>(p, w)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, kb = lane >> 4;
+    C a;
+    a.load(p, w, w.c0 + wave * COLS, lane);
+
+    const Kv4Pages pages(p, w, kv4_block_bytes(D));
+    Packed<D> t;
+    int live = 0;   // tokens of this wave's block of the step in t
+    // (beyond the keys: their last block again, none of it alive)
+    auto fetch = [&](int j) {
+        const int blk = (j >> 4) + wave, page = pages.page(blk);
+        live = pages.ok(page) ? w.k1 - 16 * blk : 0;
+        load_packed<D>(t, pages.block(page, blk), lane);
+    };
+    const bool any = w.k0 < w.k1;
+    if (any) fetch(w.k0);
+    // one power of two for the workgroup's rows of q
+    float top = a.largest();
+    if (lane == 0) ml[wave][0] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
+    a.start(p, top);
+    __syncthreads();
+
+    if (any) {
+        unpack<E, D>(lds[0], t, live, a.kscale, wave, lane);
+        fetch(w.k0 + STEP);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int j = w.k0; j < w.k1; j += STEP, buf ^= 1) {
+        if (j + STEP < w.k1) {
+            unpack<E, D>(lds[buf ^ 1], t, live, a.kscale, wave, lane);
+            fetch(j + 2 * STEP);
+        }
+        const ManyLds<D>& s = lds[buf];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int jh = j + 32 * half;
+            if (jh >= a.jhi || jh + 32 <= a.jlo) continue;   // none of this wave's columns sees these
+            float4_t acc[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+            float ks[2][4], vs[2][4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float4_t fk = *reinterpret_cast<const float4_t*>(&s.ks[32 * half + 16 * b + 4 * kb]);
+                const float4_t fv = *reinterpret_cast<const float4_t*>(&s.vs[32 * half + 16 * b + 4 * kb]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ks[b][i] = fk[i];
+                    vs[b][i] = fv[i];
+                }
+            }
+            int bad = 0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) bad |= (s.live[2 * half + b] <= 0 ? 1 : 0) << b;
+            bad = __builtin_amdgcn_readfirstlane(bad);
+            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad;
+            const float vmax = fmaxf(s.vtop[2 * half], s.vtop[2 * half + 1]);
+            // operands from LDS all at once, ahead of the products that take them: one wait instead of eight
+            half8_t kf[2][C::KW], vf[C::VT];
+#pragma unroll
+            for (int x = 0; x < C::KW; ++x)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) kf[b][x] = s.k[2 * half + b][x][lane];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < C::KW; ++x)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
+            if (__any(vmax > a.vtop)) a.value_top(vmax);   // rare after the first steps
+            float x[NT][2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, whole, jh, a.jhi, bad, kb);
+#pragma unroll
+            for (int x = 0; x < C::VT; ++x) vf[x] = s.v[half][x][lane];
+            __builtin_amdgcn_sched_barrier(0);
+            half8_t pw[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) pw[n] = a.weights(n, x[n], vs);
+#pragma unroll
+            for (int x = 0; x < C::VT; ++x)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) a.o[n][x] = mfma16x16x32(vf[x], pw[n], a.o[n][x]);
+        }
+        __syncthreads();
+    }
+    a.finish();
+
+    const Kv4Sink<E, D> sink(p, w);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = 16 * n + col;
+        const float inv = a.l[n] == 0.f ? 0.f : 1.f / a.l[n];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < C::VT; x += 4) {
+                const float4_t v = {a.o[n][x][i], a.o[n][x + 1][i], a.o[n][x + 2][i], a.o[n][x + 3][i]};
+                // (chunks of partial results as they lie: 1 KiB a store and wave)
+                if (w.chunks > 1) st_partial4<SCOPE_DEVICE>(sink.part + 4 * sink.lane_quad(wave, n, i, x, lane), v);
+                else if (c < a.n) sink.out(a.c + c, (4 * kb + i) * C::VT + x, v, inv);
+            }
+        if (kb == 0 && c < a.n) sink.put_ml(a.c + c, a.m[n], a.l[n]);
+    }
+    if (w.chunks == 1) return;
+    sink.template join<true>(min(4 * COLS, w.cols), &ml[0][0], reinterpret_cast<float4_t*>(&lds[0]), &last);
+}
+
+hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {
+    const dim3 grid(p.Hkv, p.B, s.tiles * s.splits);
+    switch (D) {
+        case 64: bf16 ? kv4_many_kernel<bf16_t, 64><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 64><<<grid, 256, 0, st>>>(p); break;
+        case 128: bf16 ? kv4_many_kernel<bf16_t, 128><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 128><<<grid, 256, 0, st>>>(p); break;
+        case 192: bf16 ? kv4_many_kernel<bf16_t, 192><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 192><<<grid, 256, 0, st>>>(p); break;
+        case 256: bf16 ? kv4_many_kernel<bf16_t, 256><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 256><<<grid, 256, 0, st>>>(p); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace w4a16

@@ -591,21 +591,30 @@ def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int =
 
 
 def _kv4_cache_shape(cache: torch.Tensor):
-    """(pages, kv heads, page size, head dim) of a cache tensor."""
-    _require(cache, "cache", (torch.uint8,))
-    if cache.dim() != 4 or not cache.is_contiguous():
+    """(pages, kv heads, page size, head dim, device index) of a cache tensor."""
+    index = cache.get_device() if isinstance(cache, torch.Tensor) else -1
+    if index < 0 or cache.dtype is not torch.uint8:
+        _require(cache, "cache", (torch.uint8,))
+    shape = cache.shape
+    if len(shape) != 4 or not cache.is_contiguous():
         raise InvalidArgument("cache must be a contiguous [pages, kv heads, page_size / 16, 16 D + 128] tensor")
-    pages, Hkv, blocks, width = cache.shape
+    pages, Hkv, blocks, width = shape
     D = (width - 128) // 16
     if D < 1 or width != 16 * D + 128:
         raise InvalidArgument(f"cache has blocks of {width} bytes, not 16 D + 128")
-    return pages, Hkv, blocks * 16, D
+    return pages, Hkv, blocks * 16, D, index
 
 
-def _kv4_rows(t, name: str, dtypes, dev, shape=None):
+def _kv4_tensor(t, name: str, dtypes, index: int):
+    # (the one test that a good call pays; _require says what is wrong with a bad one)
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != index:
+        _require(t, name, dtypes, torch.device("cuda", index))
+
+
+def _kv4_rows(t, name: str, dtypes, index: int, shape=None):
     """(token stride, head stride) of rows [T, H, D] with contiguous D."""
-    _require(t, name, dtypes, dev)
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
+    _kv4_tensor(t, name, dtypes, index)
+    if t.shape != shape if shape is not None else t.dim() != 3:
         raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
     st, sh, sd = t.stride()
     if sd != 1:
@@ -613,23 +622,22 @@ def _kv4_rows(t, name: str, dtypes, dev, shape=None):
     return st, sh
 
 
-def _kv4_index(t, name: str, dev, numel=None):
-    _require(t, name, _INT32, dev)
-    if not t.is_contiguous() or (numel is not None and (t.dim() != 1 or t.numel() != numel)):
-        raise InvalidArgument(f"{name} must be a contiguous int32 tensor"
-                              + ("" if numel is None else f" of {numel} entries"))
+def _kv4_index(t, name: str, index: int, shape=None):
+    _kv4_tensor(t, name, _INT32, index)
+    if not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise InvalidArgument(f"{name} must be a contiguous int32 tensor" + ("" if shape is None else f" {list(shape)}"))
 
 
-def _call_on(dev: torch.device, fn, *args) -> None:
+def _call_on(index: int, fn, *args) -> None:
     """fn(stream, *args) on the device's current stream, with the device as the current one (kernels
-    are launched on the current device). Pointers go as plain integers: a decode step makes many of
-    these calls and each is a few microseconds of host time."""
-    index = dev.index
+    are launched on the current device). Pointers go as plain integers and the stream without an
+    object around it: a decode step makes many of these calls, each a few microseconds of host time."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
     if torch.cuda.current_device() == index:
-        rc = fn(torch.cuda.current_stream(index).cuda_stream, *args)
+        rc = fn(stream, *args)
     else:
         with torch.cuda.device(index):
-            rc = fn(torch.cuda.current_stream(index).cuda_stream, *args)
+            rc = fn(stream, *args)
     if rc != OK:
         check(rc)
 
@@ -639,13 +647,12 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torc
     multiples of 8) to 4 bits into the slots (int32 [T], page * page_size + offset) of the cache,
     which it returns. A row whose slot is negative or beyond the cache is passed over; slots of one
     call must differ from each other."""
-    pages, Hkv, page, D = _kv4_cache_shape(cache)
-    dev = cache.device
-    _require(k, "k", _ELEM, dev)
-    shape = (k.shape[0], Hkv, D)
+    pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
+    _kv4_tensor(k, "k", _ELEM, dev)
+    shape = (k.shape[0] if k.dim() else 0, Hkv, D)
     kst, ksh = _kv4_rows(k, "k", _ELEM, dev, shape)
     vst, vsh = _kv4_rows(v, "v", (k.dtype,), dev, shape)
-    _kv4_index(slots, "slots", dev, shape[0])
+    _kv4_index(slots, "slots", dev, shape[:1])
     _call_on(dev, lib().w4a16_kv4_write, _elem_flag(k), k.data_ptr(), v.data_ptr(), kst, ksh, vst, vsh,
              slots.data_ptr(), cache.data_ptr(), pages, shape[0], Hkv, D, page)
     return cache
@@ -655,20 +662,19 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
     """(k, v) [T, kv heads, D]: the rows that the slots of the cache hold, rounded to the element
     type that they were written in (`dtype`, or that of k_out and v_out). Rows whose slot is negative
     or beyond the cache are left as they were in k_out and v_out (0 where these are not given)."""
-    pages, Hkv, page, D = _kv4_cache_shape(cache)
-    dev = cache.device
+    pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
     _kv4_index(slots, "slots", dev)
     if slots.dim() != 1:
         raise InvalidArgument("slots must be 1-D")
-    T = slots.shape[0]
+    shape = (slots.shape[0], Hkv, D)
     if (k_out is None) != (v_out is None):
         raise InvalidArgument("give both k_out and v_out, or neither")
     if k_out is None:
-        k_out, v_out = torch.zeros((2, T, Hkv, D), dtype=dtype, device=dev)
-    kst, ksh = _kv4_rows(k_out, "k_out", _ELEM, dev, (T, Hkv, D))
-    vst, vsh = _kv4_rows(v_out, "v_out", (k_out.dtype,), dev, (T, Hkv, D))
+        k_out, v_out = torch.zeros((2, *shape), dtype=dtype, device=cache.device)
+    kst, ksh = _kv4_rows(k_out, "k_out", _ELEM, dev, shape)
+    vst, vsh = _kv4_rows(v_out, "v_out", (k_out.dtype,), dev, shape)
     _call_on(dev, lib().w4a16_kv4_read, _elem_flag(k_out), cache.data_ptr(), slots.data_ptr(),
-             k_out.data_ptr(), v_out.data_ptr(), kst, ksh, vst, vsh, pages, T, Hkv, D, page)
+             k_out.data_ptr(), v_out.data_ptr(), kst, ksh, vst, vsh, pages, shape[0], Hkv, D, page)
     return k_out, v_out
 
 
@@ -676,7 +682,7 @@ def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int,
                             max_kv_len: int) -> torch.Tensor:
     """A workspace for kv4_attention calls with queries of q's shape: enough for any batch within
     these bounds. Calls that may overlap in time need one each."""
-    _, Hkv, _, D = _kv4_cache_shape(cache)
+    _, Hkv, _, D, _ = _kv4_cache_shape(cache)
     T, Hq = q.shape[:2]
     need = lib().w4a16_kv4_attention_workspace_size(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
     if need == 0:
@@ -703,37 +709,35 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     max_q_len, max_kv_len: bounds on the batch (T, or 1 without cu_q, and the table's width unless
     given). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
     given."""
-    pages, Hkv, page, D = _kv4_cache_shape(cache)
-    dev = cache.device
+    pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
     qst, qsh = _kv4_rows(q, "q", _ELEM, dev)
-    T, Hq = q.shape[:2]
-    if q.shape[2] != D:
-        raise InvalidArgument(f"q has heads of {q.shape[2]} dimensions, the cache {D}")
+    T, Hq, Dq = shape = q.shape
+    if Dq != D:
+        raise InvalidArgument(f"q has heads of {Dq} dimensions, the cache {D}")
     _kv4_index(page_table, "page_table", dev)
     if page_table.dim() != 2:
         raise InvalidArgument("page_table must be [sequences, pages per sequence]")
     B, per = page_table.shape
-    _kv4_index(kv_lens, "kv_lens", dev, B)
+    _kv4_index(kv_lens, "kv_lens", dev, (B,))
     if cu_q is not None:
-        _kv4_index(cu_q, "cu_q", dev, B + 1)
+        _kv4_index(cu_q, "cu_q", dev, (B + 1,))
     if max_q_len is None:
         max_q_len = 1 if cu_q is None else max(1, T)
     if max_kv_len is None:
         max_kv_len = per * page
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev) if cu_q is None else \
-            torch.zeros((T, Hq, D), dtype=q.dtype, device=dev)
-    ost, osh = _kv4_rows(out, "out", (q.dtype,), dev, (T, Hq, D))
+        out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
+    ost, osh = _kv4_rows(out, "out", (q.dtype,), dev, shape)
     if lse is not None:
-        _require(lse, "lse", (torch.float32,), dev)
-        if tuple(lse.shape) != (T, Hq) or not lse.is_contiguous():
+        _kv4_tensor(lse, "lse", (torch.float32,), dev)
+        if lse.shape != (T, Hq) or not lse.is_contiguous():
             raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
     if T == 0 or B == 0:
         return out
     if workspace is None:
         workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
     else:
-        _require(workspace, "workspace", (torch.uint8,), dev)
+        _kv4_tensor(workspace, "workspace", (torch.uint8,), dev)
         if not workspace.is_contiguous():
             raise InvalidArgument("workspace must be contiguous")
     _call_on(dev, lib().w4a16_kv4_attention, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),

@@ -52,20 +52,32 @@ struct Kv4AttnParams {
     uint32_t* counters;               // one a tile of columns, zero between calls
     float* partials;                  // [tile][B][Hkv][splits] of slot_cols (D + 2) floats
     // from the shape
-    int G, tiles, splits, chunk, slot_cols, pair_tiles;
+    int G, slot_cols;
+    int tiles, splits, chunk, pair_tiles;        // kv4_many.hip
+    int places, budget, whole, join_apart;       // kv4_few.hip
 };
 constexpr size_t KV4_MAX_COUNTERS = 16384;
 struct Kv4AttnShape {
     bool many;         // kv4_many.hip, else kv4_few.hip
     int nt;            // columns of a wave / 16
     int tiles;         // tiles of columns of a sequence and key/value head
-    int splits;        // chunks of the keys, at most
-    int chunk;         // keys of a chunk
     int slot_cols;     // columns of a chunk's partial results
-    bool pair_tiles;   // long and short tiles of columns by turns
+    // many: groups of four waves a workgroup; chunks of the keys, at most, and their length; long and short tiles of
+    // columns by turns
+    int groups, splits, chunk;
+    bool pair_tiles;
+    // few: chunks of all sequences of a head, at most, and about how many are wanted; whole: one a sequence;
+    // join_apart: chunks are joined by a kernel of their own
+    int places, budget;
+    bool whole, join_apart;
     size_t partial_bytes;
 };
+// Workgroups of kv4_few.hip that a compute unit holds, by registers (95, 149; 127, 204; 163; 196 of D = 64, 128, 192, 256
+// with one and, up to 128, two column tiles a wave) and LDS.
+constexpr int kv4_few_per_cu(int D, int nt) { return nt == 2 ? (D == 64 ? 3 : 2) : D <= 128 ? 4 : D == 192 ? 3 : 2; }
 hipError_t launch_kv4_few(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
+// Waves of kv4_many.hip a SIMD, by registers (some 144, 212, 386 and 490 of D = 64, 128, 192 and 256).
+constexpr int kv4_many_simd_waves(int D, int groups) { return D == 64 && groups == 1 ? 3 : D <= 128 ? 2 : 1; }
 hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
 
 }  // namespace w4a16

@@ -20,6 +20,8 @@ constexpr int KV4_CUS = 256;
 static_assert(KV4_MAX_COUNTERS * sizeof(uint32_t) == W4A16_KV4_COUNTER_BYTES, "counters fill their area");
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
+constexpr int64_t KV4_JOIN_BYTES = 40 << 10;   // partial results of a sequence and head that its last workgroup joins itself
+
 static int check_elem(int elem) {
     if (elem != 0 && elem != W4A16_BF16) return fail(W4A16_ERR_INVALID_ARG, "unknown element type %d", elem);
     return W4A16_OK;
@@ -77,26 +79,46 @@ static int kv4_rows(bool write, void* stream, int elem, void* k, void* v, int32_
 }
 
 // Which kernel, and how the keys are split. Few columns (up to 64) go to the kernel whose waves share them. The
-// keys are split as far as it takes to fill the places of workgroups that run at once (`slots`), no further:
-// each chunk costs its partial results a round trip through memory.
+// keys are split as far as it takes to fill the places of workgroups that run at once, no further: each chunk
+// costs its partial results a round trip through memory.
 static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv) {
     Kv4AttnShape s{};
-    const int64_t G = Hq / Hkv, C = (int64_t)(max_q < T ? max_q : T) * G;
+    const int64_t G = Hq / Hkv, C = (int64_t)(max_q < T ? max_q : T) * G, slots_of_cu = KV4_CUS;
     s.many = C > 64;
-    s.nt = s.many || C > 16 ? 2 : 1;
+    s.nt = s.many || (C > 16 && D <= 128) ? 2 : 1;
     const int wg_cols = s.many ? 128 : 32 * s.nt;
-    const int64_t tiles = std::max<int64_t>(1, (C + wg_cols - 1) / wg_cols), items = std::max<int64_t>(1, tiles * B * Hkv);
-    const int per_cu = s.many ? (D <= 128 ? 2 : 1) : D * s.nt >= 512 ? 1 : D * s.nt > 128 ? 2 : 3;
-    const int64_t slots = (int64_t)KV4_CUS * per_cu, least = s.many ? 512 : 128;
-    int64_t want = s.many ? (slots + items - 1) / items : slots / items;
-    if (items > (int64_t)KV4_MAX_COUNTERS) want = 1;
-    want = std::max<int64_t>(1, std::min(want, (max_kv + least - 1) / least));
-    s.chunk = (int)((((int64_t)max_kv + want - 1) / want + 127) / 128 * 128);
-    s.splits = s.chunk > 0 ? (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk) : 1;
+    const int64_t tiles = std::max<int64_t>(1, (C + wg_cols - 1) / wg_cols);
+    const int64_t items = std::max<int64_t>(1, tiles * B * Hkv);
     s.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
-    s.pair_tiles = s.many && items * s.splits <= slots;
-    s.slot_cols = s.many ? wg_cols : (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
-    if (s.splits > 1) s.partial_bytes = (size_t)items * s.splits * s.slot_cols * (D + 2) * sizeof(float);
+    size_t slots = 0;
+    if (s.many) {
+        // Up to two tiles a compute unit, the longest one sets the time: two groups of waves share its keys. Not where
+        // the tiles are of one length (a chunk behind a long context) and fill the device by themselves.
+        s.groups = D <= 128 && items <= 2 * KV4_CUS && !(items >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
+        const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
+        int64_t want = std::min((at_once + items - 1) / items, ((int64_t)max_kv + 511) / 512);
+        if (items > (int64_t)KV4_MAX_COUNTERS) want = 1;
+        want = std::max<int64_t>(1, want);
+        s.chunk = (int)std::max<int64_t>(128, (((int64_t)max_kv + want - 1) / want + 127) / 128 * 128);
+        s.splits = std::max(1, (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk));
+        s.pair_tiles = items * s.splits <= at_once;
+        s.slot_cols = wg_cols;
+        if (s.splits > 1) slots = (size_t)items * s.splits;
+    } else {
+        // chunks of a head and tile: what runs at once, or several rounds of it; B sequences have one each at least,
+        // and a remainder
+        const int64_t at_once = std::max<int64_t>(1, slots_of_cu * kv4_few_per_cu(D, s.nt) / (Hkv * tiles));
+        const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
+        s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= 128;
+        s.budget = (int)std::max<int64_t>(2 * (int64_t)B, rounds * at_once);
+        s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
+        s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
+        if (!s.whole) slots = (size_t)tiles * Hkv * s.places;
+        // one workgroup reads partial results at some 32 KB a microsecond; the chunks of a sequence, in a batch of like ones
+        const int64_t chunks = std::min<int64_t>(s.budget / std::max(B, 1), ((int64_t)max_kv + 127) / 128);
+        s.join_apart = !s.whole && C * D * 4 * chunks > KV4_JOIN_BYTES;
+    }
+    s.partial_bytes = slots * s.slot_cols * (D + 2) * sizeof(float);
     return s;
 }
 
@@ -137,7 +159,7 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
     if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
     if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
     const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q, max_kv);
-    if ((int64_t)s.tiles * s.splits > 65535)
+    if (s.many ? (int64_t)s.tiles * s.splits > 65535 : s.places > 65535)
         return fail(W4A16_ERR_UNSUPPORTED, "max_q_len %d with max_kv_len %d: too many tiles for one call", max_q, max_kv);
     return W4A16_OK;
 }
@@ -184,8 +206,9 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
     p.counters = static_cast<uint32_t*>(workspace);
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
-    p.G = Hq / Hkv; p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.slot_cols = s.slot_cols;
-    p.pair_tiles = s.pair_tiles;
+    p.G = Hq / Hkv; p.slot_cols = s.slot_cols;
+    p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
+    p.places = s.places; p.budget = s.budget; p.whole = s.whole; p.join_apart = s.join_apart;
     (void)hipGetLastError();
     const bool bf16 = elem == W4A16_BF16;
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -77,14 +77,17 @@ __device__ __forceinline__ float saturate(float v) {
     return v > most ? most : v < -most ? -most : v;   // (NaN stays)
 }
 
-__device__ __forceinline__ float kb_sum(float v) {   // over the four lanes of a column
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+// over the four lanes of a column, 16 apart: each swap of rows or halves with itself leaves a lane's own value and
+// its partner's in the two results
+template <typename F>
+__device__ __forceinline__ float kb_all(float v, F f) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float kb_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
+__device__ __forceinline__ float kb_sum(float v) { return kb_all(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float kb_max(float v) { return kb_all(v, [](float a, float b) { return fmaxf(a, b); }); }
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
 
@@ -98,41 +101,37 @@ struct Kv4Item {
     int c0, cols;                  // first column, columns from there to the sequence's end
     int split, chunks, k0, k1;
     size_t at;                     // number of (tile, b, h)
+    size_t slot;                   // of its first chunk's partial results
     __device__ __forceinline__ int see_hi(const Kv4AttnParams& p, int i) const { return p.causal ? max(0, min(len, first + i + 1)) : len; }
     __device__ __forceinline__ int see_lo(const Kv4AttnParams& p, int i) const { return p.window ? max(0, first + i - p.window + 1) : 0; }
-};
 
-// wg_cols columns a workgroup; chunks start at multiples of `step`. false: nothing to do.
-template <int WG_COLS, int STEP>
-__device__ __forceinline__ bool kv4_item(const Kv4AttnParams& p, Kv4Item& w) {
-    w.h = blockIdx.x;
-    w.b = blockIdx.y;
-    const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
-    w.split = p.splits == 1 ? 0 : blockIdx.z - z * p.splits;
-    // columns of long rows first, or (where all workgroups run at once) long and short by turns
-    const int tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
-    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
-    int q1 = w.b + 1;
-    w.q0 = w.b;
-    if (p.cu_q) {
-        w.q0 = min(max(p.cu_q[w.b], 0), p.T);
-        q1 = min(max(p.cu_q[w.b + 1], 0), p.T);
+    // Sequence b and its columns from c0 on; keys [lo, hi) that they see, lo a multiple of STEP.
+    template <int WG_COLS, int STEP>
+    __device__ __forceinline__ void sequence(const Kv4AttnParams& p, int b_, int c0_, int& lo, int& hi) {
+        b = b_;
+        c0 = c0_;
+        // (the loads go out together; without cu_q its place is not looked at)
+        const int32_t* cu = p.cu_q ? p.cu_q + b : p.kv_lens;
+        const int kv = p.kv_lens[b], cu0 = cu[0], cu1 = p.cu_q ? cu[1] : 0;
+        q0 = p.cu_q ? min(max(cu0, 0), p.T) : b;
+        const int q1 = p.cu_q ? min(max(cu1, 0), p.T) : b + 1;
+        n = min(q1 - q0, p.max_q);
+        cols = n * p.G - c0;
+        const long long cap = (long long)p.pages_per_seq << p.page_shift;
+        len = (int)max(0ll, min((long long)min(kv, p.max_kv), cap));
+        first = len - (q1 - q0);
+        const int i0 = n <= 1 ? 0 : c0 / p.G, i1 = n <= 1 ? 0 : (min(c0 + WG_COLS, n * p.G) - 1) / p.G;
+        hi = see_hi(p, i1);
+        lo = min(see_lo(p, i0), hi) & ~(STEP - 1);
     }
-    w.n = min(q1 - w.q0, p.max_q);
-    w.c0 = tile * WG_COLS;
-    w.cols = w.n * p.G - w.c0;
-    if (w.cols <= 0) return false;
-    const long long cap = (long long)p.pages_per_seq << p.page_shift;
-    w.len = (int)max(0ll, min((long long)min(p.kv_lens[w.b], p.max_kv), cap));
-    w.first = w.len - (q1 - w.q0);
-    const int i0 = w.n == 1 ? 0 : w.c0 / p.G, i1 = w.n == 1 ? 0 : (min(w.c0 + WG_COLS, w.n * p.G) - 1) / p.G;
-    const int hi = w.see_hi(p, i1), lo = min(w.see_lo(p, i0), hi) & ~(STEP - 1);
-    w.chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
-    if (w.split >= w.chunks) return false;
-    w.k0 = p.splits == 1 ? lo : lo + w.split * p.chunk;
-    w.k1 = p.splits == 1 ? hi : min(hi, w.k0 + p.chunk);
-    return true;
-}
+    // Chunk split_ of chunks_ of `chunk` keys in [lo, hi).
+    __device__ __forceinline__ void take(int split_, int chunks_, int chunk, int lo, int hi) {
+        split = split_;
+        chunks = chunks_;
+        k0 = lo + split * chunk;
+        k1 = chunks == 1 ? hi : min(hi, k0 + chunk);
+    }
+};
 
 // A wave's 16 NT columns.
 template <typename E, int D, int NT>
@@ -179,27 +178,42 @@ struct Kv4Cols {
 
     // the largest |q| of the wave's rows, infinities and NaN aside
     __device__ __forceinline__ float largest() const {
-        float top = 0.f;
+        typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+        constexpr uint32_t inf = __is_same(E, half_t) ? 0x7C00u : 0x7F80u;
+        ushort2_t top = {0, 0};   // (bits of non-negative numbers are ordered)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int x = 0; x < KW; ++x) {
                 const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = fabsf(param_scale<E>(v[e >> 1] >> (16 * (e & 1))));
-                    top = fmaxf(top, a < INFINITY ? a : 0.f);
-                }
+                for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, v[e] & 0x7FFF7FFFu));
             }
+        uint32_t most = max((uint32_t)top[0], (uint32_t)top[1]);
+        if (__any(most >= inf)) {
+            most = 0;
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-        return top;
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int x = 0; x < KW; ++x) {
+                    const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t a = (v[e >> 1] >> (16 * (e & 1))) & 0x7FFFu;
+                        most = max(most, a < inf ? a : 0u);
+                    }
+                }
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, x));
+        return kb_max(param_scale<E>(most));
     }
 
-    // q in operand order under the power of two that `top`, the largest of the rows, gives
+    // q in operand order under the power of two that `top`, the largest of the rows, gives: 2^13 to 2^14, or (fp16,
+    // whose own range is enough) less where q is small
     __device__ __forceinline__ void start(const Kv4AttnParams& p, float top) {
-        // q 2^e has its largest value in [2^13, 2^14) (or all of it is zero)
-        const int e2 = top > 0.f ? min(100, max(-100, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
+        constexpr bool F16 = __is_same(E, half_t);
+        const int e2 = top > 0.f ? min(F16 ? 15 : 100, max(F16 ? -14 : -100, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
         const float up = pow2(e2);
         kscale = p.scale_log2 * pow2(-e2);
 #pragma unroll
@@ -207,11 +221,16 @@ struct Kv4Cols {
 #pragma unroll
             for (int x = 0; x < KW; ++x) {
                 const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
-                half8_t f;
+                half2_t a[4];   // dimensions (0, 1), (2, 3), (4, 5), (6, 7)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)   // dimension e meets the nibble at bits 4 e: operand slot 2 (e % 4) + e / 4
-                    f[2 * (e & 3) + (e >> 2)] = (half_t)(param_scale<E>(v[e >> 1] >> (16 * (e & 1))) * up);
-                qf[t][x] = f;
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (F16) a[e] = as_h2(v[e]) * half2_t{(half_t)up, (half_t)up};
+                    else a[e] = half2_t{(half_t)(param_scale<E>(v[e]) * up), (half_t)(param_scale<E>(v[e] >> 16) * up)};
+                }
+                // dimension e meets the nibble at bits 4 e: operand slot 2 (e % 4) + e / 4
+                const uint32_t w01 = as_u32(a[0]), w23 = as_u32(a[1]), w45 = as_u32(a[2]), w67 = as_u32(a[3]);
+                qf[t][x] = as_h8(as_h2(perm(w45, w01, 0x05040100u)), as_h2(perm(w45, w01, 0x07060302u)),
+                                 as_h2(perm(w67, w23, 0x05040100u)), as_h2(perm(w67, w23, 0x07060302u)));
             }
             m[t] = l[t] = 0.f;
             most[t] = -INFINITY;
@@ -315,7 +334,7 @@ struct Kv4Sink {
     size_t slot_floats;
     __device__ __forceinline__ Kv4Sink(const Kv4AttnParams& p_, const Kv4Item& w_) : p(p_), w(w_) {
         slot_floats = (size_t)p.slot_cols * (D + 2);
-        item = p.partials + w.at * p.splits * slot_floats;
+        item = p.partials + w.slot * slot_floats;
         part = item + w.split * slot_floats;
         part_ml = part + (size_t)p.slot_cols * D;
     }
@@ -331,6 +350,15 @@ struct Kv4Sink {
         uint16_t* dst = static_cast<uint16_t*>(p.out) + (size_t)row * p.o_st + (size_t)head * p.o_sh + d;
         *reinterpret_cast<u32x2*>(dst) = u32x2{pack2(E{}, saturate<E>(v[0] * inv), saturate<E>(v[1] * inv)),
                                                pack2(E{}, saturate<E>(v[2] * inv), saturate<E>(v[3] * inv))};
+    }
+    __device__ __forceinline__ void out8(int r, int d, float4_t v, float4_t u, float inv) const {
+        int row, head;
+        place(r, row, head);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (size_t)row * p.o_st + (size_t)head * p.o_sh + d;
+        *reinterpret_cast<u32x4*>(dst) = u32x4{pack2(E{}, saturate<E>(v[0] * inv), saturate<E>(v[1] * inv)),
+                                               pack2(E{}, saturate<E>(v[2] * inv), saturate<E>(v[3] * inv)),
+                                               pack2(E{}, saturate<E>(u[0] * inv), saturate<E>(u[1] * inv)),
+                                               pack2(E{}, saturate<E>(u[2] * inv), saturate<E>(u[3] * inv))};
     }
     __device__ __forceinline__ void lse(int r, float m, float l) const {
         if (!p.lse) return;
@@ -351,124 +379,129 @@ struct Kv4Sink {
             lse(r, m, l);
         }
     }
-    // The last of the chunks to arrive (splitk.h) joins them: per column (m, 1 / l) over all chunks, then the
-    // results, chunks in order within a share and shares in order (a share of the chunks a group of
-    // threads where there are fewer values than threads). 256 threads; ml: two floats a column, sums:
-    // 256 float4 of LDS. LANES: of 128 columns, in the order in which lanes have them.
-    template <bool LANES>
-    __device__ __forceinline__ void join(int live, float* ml, float4_t* sums, int* last) const {
+    // Quad e of values (column e / (D / 4)) over chunks share, share + shares, ...; then over the shares, `span` threads
+    // apart, through LDS (256 entries each). on: there is such a quad and share. In order of the chunks within a
+    // share, then of the shares. For kv4_few.hip: partial results by column.
+    __device__ __forceinline__ void join_quads(int e, int share, int shares, int span, bool on, float4_t* vals, float (*ml)[2]) const {
+        const int c = on ? e / (D / 4) : 0, d = 4 * (e - c * (D / 4)), chunks = w.chunks;
+        const float* at = item + (size_t)c * D + d;
+        const float* heads = item + (size_t)p.slot_cols * D + 2 * c;
+        float m = -FLT_MAX, l = 0.f;
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (on)
+            for (int s0 = share; s0 < chunks; s0 += 8 * shares) {
+                float4_t x[8];
+                uint64_t h[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const size_t s = min(s0 + shares * y, chunks - 1);
+                    h[y] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(heads + s * slot_floats), __ATOMIC_RELAXED, SCOPE_DEVICE);
+                    x[y] = ld_partial4<SCOPE_DEVICE>(at + s * slot_floats);
+                }
+                float mn = m;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) mn = fmaxf(mn, __uint_as_float((uint32_t)h[y]));
+                const float f = __builtin_amdgcn_exp2f(m - mn);
+                v *= f;
+                l *= f;
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    if (s0 + shares * y < chunks) {
+                        const float g = __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)h[y]) - mn);
+                        v += x[y] * g;
+                        l += __uint_as_float((uint32_t)(h[y] >> 32)) * g;
+                    }
+                m = mn;
+            }
+        if (shares > 1) {
+            vals[threadIdx.x] = v;
+            ml[threadIdx.x][0] = m;
+            ml[threadIdx.x][1] = l;
+            __syncthreads();
+            if (on && share == 0) {
+                float mm = m;
+                for (int x = 1; x < shares; ++x) mm = fmaxf(mm, ml[threadIdx.x + x * span][0]);
+                const float f = __builtin_amdgcn_exp2f(m - mm);
+                v *= f;
+                l *= f;
+                for (int x = 1; x < shares; ++x) {
+                    const float g = __builtin_amdgcn_exp2f(ml[threadIdx.x + x * span][0] - mm);
+                    v += vals[threadIdx.x + x * span] * g;
+                    l += ml[threadIdx.x + x * span][1] * g;
+                }
+                m = mm;
+            }
+        }
+        if (on && share == 0) {
+            out(w.c0 + c, d, v, l == 0.f ? 0.f : 1.f / l);
+            if (d == 0) lse(w.c0 + c, m, l);
+        }
+    }
+    // The last of the chunks to arrive (splitk.h) joins them: 256 threads, `live` columns.
+    __device__ __forceinline__ void join(int live, float4_t* vals, float (*ml)[2], int* last) const {
+        if (!splitk_arrive(p.counters + w.at, w.chunks, last)) return;
+        const int quads = live * (D / 4), shares = quads >= 256 ? 1 : min(256 / quads, 8), span = shares == 1 ? 256 : quads;
+        const int share = threadIdx.x / span;
+        for (int e0 = 0; e0 < quads; e0 += span) {
+            const int e = e0 + threadIdx.x - share * span;
+            join_quads(e, share, shares, span, e < quads && share < shares, vals, ml);
+        }
+    }
+    // The same for kv4_many.hip, 128 columns of partial results as lanes have them: per column (m, 1 / l) over all
+    // chunks, then the values, four quads a thread and two chunks of each in flight.
+    template <int THREADS>
+    __device__ __forceinline__ void join_lanes(int live, float* ml, int* last) const {
         if (!splitk_arrive(p.counters + w.at, w.chunks, last)) return;
         const int chunks = w.chunks;
         const float* heads = item + (size_t)p.slot_cols * D;
-        for (int c = threadIdx.x >> 2; c < ((live + 15) & ~15); c += 64) {   // (whole waves)
+        if ((int)threadIdx.x < live) {
             float mm = -FLT_MAX, ll = 0.f;
-            for (int s0 = threadIdx.x & 3; s0 < chunks; s0 += 32) {
-                uint64_t x[8];
-#pragma unroll
-                for (int y = 0; y < 8; ++y)
-                    x[y] = c < live && s0 + 4 * y < chunks
-                               ? __hip_atomic_load(reinterpret_cast<const uint64_t*>(heads + (s0 + 4 * y) * slot_floats + 2 * c), __ATOMIC_RELAXED, SCOPE_DEVICE)
-                               : (uint64_t)__float_as_uint(-FLT_MAX);
-                float mn = mm;
-#pragma unroll
-                for (int y = 0; y < 8; ++y) mn = fmaxf(mn, __uint_as_float((uint32_t)x[y]));
-                ll *= __builtin_amdgcn_exp2f(mm - mn);
-#pragma unroll
-                for (int y = 0; y < 8; ++y)
-                    ll += __uint_as_float((uint32_t)(x[y] >> 32)) * __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)x[y]) - mn);
+            for (int s = 0; s < chunks; ++s) {
+                const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(heads + s * slot_floats + 2 * threadIdx.x), __ATOMIC_RELAXED, SCOPE_DEVICE);
+                const float mx = __uint_as_float((uint32_t)x), mn = fmaxf(mm, mx);
+                ll = ll * __builtin_amdgcn_exp2f(mm - mn) + __uint_as_float((uint32_t)(x >> 32)) * __builtin_amdgcn_exp2f(mx - mn);
                 mm = mn;
             }
-#pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
-                const float om = __shfl_xor(mm, x), ol = __shfl_xor(ll, x), mn = fmaxf(mm, om);
-                ll = ll * __builtin_amdgcn_exp2f(mm - mn) + ol * __builtin_amdgcn_exp2f(om - mn);
-                mm = mn;
-            }
-            if ((threadIdx.x & 3) == 0 && c < live) {
-                ml[2 * c] = mm;
-                ml[2 * c + 1] = ll == 0.f ? 0.f : 1.f / ll;
-                lse(w.c0 + c, mm, ll);
-            }
+            ml[2 * threadIdx.x] = mm;
+            ml[2 * threadIdx.x + 1] = ll == 0.f ? 0.f : 1.f / ll;
+            lse(w.c0 + threadIdx.x, mm, ll);
         }
         __syncthreads();
-        if constexpr (LANES) {
-            // many values: four at a time, two chunks of each in flight
-            constexpr int U = 4, QUADS = 32 * D;   // 128 columns
+        constexpr int U = 4, QUADS = 32 * D;   // of 128 columns
 #pragma unroll 1
-            for (int e0 = threadIdx.x; e0 < QUADS; e0 += 256 * U) {
-                float4_t v[U];
-                float mm[U];
-                int c[U];
+        for (int e0 = threadIdx.x; e0 < QUADS; e0 += THREADS * U) {
+            float4_t v[U];
+            float mm[U];
+            int c[U], d[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    int d;
-                    lane_place(e0 + 256 * u, c[u], d);
-                    c[u] = min(c[u], live - 1);
-                    mm[u] = ml[2 * c[u]];
-                    v[u] = float4_t{0.f, 0.f, 0.f, 0.f};
-                }
-                for (int s0 = 0; s0 < chunks; s0 += 2) {
-                    float4_t x[U][2];
-                    float f[U][2];
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const size_t s = min(s0 + y, chunks - 1);
-                            f[u][y] = __hip_atomic_load(heads + s * slot_floats + 2 * c[u], __ATOMIC_RELAXED, SCOPE_DEVICE);
-                            x[u][y] = ld_partial4<SCOPE_DEVICE>(item + s * slot_floats + 4 * (e0 + 256 * u));
-                        }
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            if (s0 + y < chunks) v[u] += x[u][y] * __builtin_amdgcn_exp2f(f[u][y] - mm[u]);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    int cc, d;
-                    lane_place(e0 + 256 * u, cc, d);
-                    if (cc < live) out(w.c0 + cc, d, v[u], ml[2 * cc + 1]);
-                }
+            for (int u = 0; u < U; ++u) {
+                lane_place(e0 + THREADS * u, c[u], d[u]);
+                mm[u] = ml[2 * min(c[u], live - 1)];
+                v[u] = float4_t{0.f, 0.f, 0.f, 0.f};
             }
-            return;
-        }
-        const int quads = live * (D / 4);
-        const int shares = quads >= 256 ? 1 : min(256 / quads, 8), per = (chunks + shares - 1) / shares;
-        const int span = shares == 1 ? 256 : quads;
-        for (int e0 = 0; e0 < quads; e0 += span) {
-            const int share = threadIdx.x / span, e = e0 + threadIdx.x - share * span;
-            const bool on = e < quads && share < shares;
-            const int c = on ? e / (D / 4) : 0, d = 4 * (e - c * (D / 4));
-            float4_t v = {0.f, 0.f, 0.f, 0.f};
-            if (on) {
-                const float mm = ml[2 * c];
-                const float* at = item + (size_t)c * D + d;
-                const int end = min(chunks, (share + 1) * per);
-                for (int s0 = share * per; s0 < end; s0 += 8) {
-                    float4_t x[8];
-                    float f[8];
+            for (int s0 = 0; s0 < chunks; s0 += 2) {
+                float4_t x[U][2];
+                float f[U][2];
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        const int s = min(s0 + y, end - 1);
-                        f[y] = __hip_atomic_load(heads + s * slot_floats + 2 * c, __ATOMIC_RELAXED, SCOPE_DEVICE);
-                        x[y] = ld_partial4<SCOPE_DEVICE>(at + s * slot_floats);
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const size_t s = min(s0 + y, chunks - 1);
+                        f[u][y] = __hip_atomic_load(heads + s * slot_floats + 2 * min(c[u], live - 1), __ATOMIC_RELAXED, SCOPE_DEVICE);
+                        x[u][y] = ld_partial4<SCOPE_DEVICE>(item + s * slot_floats + 4 * (e0 + THREADS * u));
                     }
 #pragma unroll
-                    for (int y = 0; y < 8; ++y)
-                        if (s0 + y < end) v += x[y] * __builtin_amdgcn_exp2f(f[y] - mm);
-                }
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        if (s0 + y < chunks) v[u] += x[u][y] * __builtin_amdgcn_exp2f(f[u][y] - mm[u]);
             }
-            if (shares > 1) {
-                sums[threadIdx.x] = v;
-                __syncthreads();
-                if (share == 0)
-                    for (int x = 1; x < shares; ++x) v += sums[x * span + threadIdx.x];
-            }
-            if (on && share == 0) out(w.c0 + c, d, v, ml[2 * c + 1]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c[u] < live) out(w.c0 + c[u], d[u], v[u], ml[2 * c[u] + 1]);
         }
     }
-    // Partial results in the order in which lanes have them (LANES): place of quad e
+    // Partial results as lanes have them: number of a quad, and place of quad e
     static constexpr int VT = D / 16;
     __device__ __forceinline__ static int lane_quad(int wave, int t, int i, int x, int lane) {
         return (((wave * 2 + t) * 4 + i) * (VT / 4) + x / 4) * 64 + lane;

@@ -15,12 +15,12 @@ constexpr int STEP = 32;   // keys of a step
 template <int D>
 struct FewShape {
     static constexpr int BLOCK = kv4_block_bytes(D);
-    static constexpr int SLOTS = D <= 128 ? 3 : 2;
+    static constexpr int SLOTS = 2;
     static constexpr int RING = SLOTS * 2 * BLOCK;   // bytes of a wave
     // 16-byte loads of a block: whole waves of it, then the parameters
     static constexpr int FULL = D / 64, LOADS = FULL + 1;
     static constexpr int ROW = D + 4;                // LDS row of a column's result, in the ring's place
-    static_assert(16 * ROW * 4 <= RING, "a wave's results fit its ring");
+    static_assert(16 * ROW * 4 <= RING && 4096 + 2048 <= 4 * RING, "results of a wave, and what joins chunks, fit the rings");
 };
 
 // A block into LDS at dst: keys and values of D = 128 and 256 in the order in which lanes take them (16 bytes
@@ -64,8 +64,90 @@ __device__ __forceinline__ void take(uint32_t (&dst)[D / 32], const unsigned cha
     }
 }
 
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ int wave_sums(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // one lane up the row, two, four, eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last of a row to the next
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // the last of the lower half to the upper
+    return v;
+}
+
+// Chunks of `steps` steps of keys in chunks of c 128 (4 c steps). Up to 768 keys stay whole: a chunk more costs some 3 us
+// (its partial results' way to the last one and back), 128 keys 0.5.
+__device__ __forceinline__ int few_chunks(int steps, int c) {
+    return steps <= max(24, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
+}
+
+// The chunks of all sequences for one head and tile of columns stand in a row; workgroup u takes the u-th. Their
+// length is such that there are at most p.budget of them, whatever the lengths of the sequences: keys / budget or
+// keys / (budget - B / 2) where that is enough, else keys / (budget - B) (the budget is twice B or more). With by_seq,
+// sequence u's first chunk instead. A lane a sequence.
+template <int WG_COLS>
+__device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w) {
+    const int lane = threadIdx.x & 63;
+    Kv4Item mine;
+    int lo = 0, hi = 0, steps = 0;
+    auto look = [&](int base) {   // this lane's sequence of 64 from base on; whether it has columns here
+        const int b = base + lane;
+        steps = 0;
+        if (b >= p.B) return false;
+        mine.sequence<WG_COLS, STEP>(p, b, tile * WG_COLS, lo, hi);
+        steps = (hi - lo + STEP - 1) / STEP;
+        return mine.cols > 0;
+    };
+    bool has = look(0);
+    // sum over all sequences of f(); the first 64 stay in registers
+    auto all = [&](auto f) {
+        unsigned sum = 0;
+        for (int base = 0; base < p.B; base += 64) {
+            if (p.B > 64) has = look(base);
+            sum += (unsigned)__builtin_amdgcn_readlane(wave_sums(has ? f() : 0), 63);
+        }
+        return sum;
+    };
+    int c = 1 << 23;   // in 128 keys
+    if (!p.whole) {
+        const unsigned sum = all([&] { return steps; });
+        // with no remainders, half a chunk a sequence, one a sequence
+        for (int rest = 0; rest <= 4; rest += 2) {
+            const unsigned room = 4 * p.budget - rest * p.B;
+            c = (int)max(1u, (sum + room - 1) / room);
+            if (rest == 4 || all([&] { return few_chunks(steps, c); }) <= (unsigned)p.budget) break;
+        }
+    }
+    for (int base = 0, before = 0; base < p.B; base += 64) {
+        if (p.B > 64) has = look(base);
+        const int n = has ? few_chunks(steps, c) : 0, upto = wave_sums(n);
+        const bool hit = by_seq ? base + lane == u && has : before + upto - n <= u && u < before + upto;
+        const uint64_t who = __ballot(hit);
+        if (who) {
+            const int l = __builtin_ctzll(who);
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            w.h = blockIdx.x;
+            w.b = base + l;
+            w.q0 = of(mine.q0);
+            w.n = of(mine.n);
+            w.len = of(mine.len);
+            w.first = of(mine.first);
+            w.c0 = tile * WG_COLS;
+            w.cols = of(mine.cols);
+            const int at = before + of(upto - n);   // its first chunk's number
+            w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
+            w.slot = ((size_t)tile * p.Hkv + w.h) * p.places + at;
+            w.take(by_seq ? 0 : u - at, of(n), 128 * c, of(lo), of(hi));
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+        if (!by_seq && before > u) return false;
+    }
+    return false;
+}
+
 template <typename E, int D, int NT>
-__global__ __launch_bounds__(256, D * NT >= 512 ? 1 : D * NT > 128 ? 2 : 3) void kv4_few_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4AttnParams p) {
     typedef FewShape<D> S;
     typedef Kv4Cols<E, D, NT> C;
     constexpr int COLS = 16 * NT;
@@ -73,7 +155,7 @@ __global__ __launch_bounds__(256, D * NT >= 512 ? 1 : D * NT > 128 ? 2 : 3) void
     __shared__ float ml[4][COLS][2];
     __shared__ int last;
     Kv4Item w;
-    if (!kv4_item<2 * COLS, STEP>(p, w)) return;
+    if (!few_item<2 * COLS>(p, blockIdx.y, blockIdx.z, false, w)) return;
     // one group of columns, its keys over four waves, or two over two
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kshift = w.cols <= COLS ? 2 : 1, kspl = 1 << kshift, g0 = wave & ~(kspl - 1);
@@ -170,9 +252,7 @@ __global__ __launch_bounds__(256, D * NT >= 512 ? 1 : D * NT > 128 ? 2 : 3) void
                 vmax = fmaxf(vmax, vs[s][i]);
             }
         if (__any(vmax > a.vtop)) {   // rare after the first steps
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, x));
-            a.value_top(vmax);
+            a.value_top(kb_max(vmax));   // (the lanes of a row have the same tokens)
         }
         if (!whole) {
 #pragma unroll
@@ -252,23 +332,43 @@ __global__ __launch_bounds__(256, D * NT >= 512 ? 1 : D * NT > 128 ? 2 : 3) void
             if (d == 0) sink.put_ml(a.c + 16 * t + c, mm, ll);
         }
     }
-    if (w.chunks == 1) return;
-    sink.template join<false>(min(2 * COLS, w.cols), &ml[0][0][0], reinterpret_cast<float4_t*>(&ring[0][0]), &last);
+    if (w.chunks == 1 || p.join_apart) return;
+    sink.join(min(2 * COLS, w.cols), reinterpret_cast<float4_t*>(&ring[0][0]), reinterpret_cast<float(*)[2]>(&ring[0][4096]), &last);
 }
 
+// Joins the chunks of one sequence and head where that is more than one workgroup does in passing: 64 quads of
+// values a workgroup, a quarter of the chunks a wave.
+template <typename E, int D, int NT>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnParams p) {
+    __shared__ float4_t vals[256];
+    __shared__ float ml[256][2];
+    constexpr int COLS = 32 * NT, PARTS = COLS * (D / 4) / 64;
+    Kv4Item w;
+    const int tile = blockIdx.z / PARTS;
+    if (!few_item<COLS>(p, tile, blockIdx.y, true, w) || w.chunks == 1) return;
+    const Kv4Sink<E, D> sink(p, w);
+    const int e = (blockIdx.z - tile * PARTS) * 64 + (threadIdx.x & 63);
+    sink.join_quads(e, threadIdx.x >> 6, 4, 64, e < w.cols * (D / 4), vals, ml);
+}
+
+template <typename E, int D, int NT>
+static void run(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+    kv4_few_kernel<E, D, NT><<<dim3(p.Hkv, s.tiles, s.places), 256, 0, st>>>(p);
+    if (p.join_apart) kv4_join_kernel<E, D, NT><<<dim3(p.Hkv, p.B, s.tiles * 32 * NT * (D / 4) / 64), 256, 0, st>>>(p);
+}
 template <typename E, int D>
-static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, dim3 grid, hipStream_t st) {
-    if (s.nt == 2) kv4_few_kernel<E, D, 2><<<grid, 256, 0, st>>>(p);
-    else kv4_few_kernel<E, D, 1><<<grid, 256, 0, st>>>(p);
+static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+    if constexpr (D <= 128)
+        if (s.nt == 2) return run<E, D, 2>(s, p, st);
+    run<E, D, 1>(s, p, st);
 }
 
 hipError_t launch_kv4_few(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {
-    const dim3 grid(p.Hkv, p.B, s.tiles * s.splits);
     switch (D) {
-        case 64: bf16 ? go<bf16_t, 64>(s, p, grid, st) : go<half_t, 64>(s, p, grid, st); break;
-        case 128: bf16 ? go<bf16_t, 128>(s, p, grid, st) : go<half_t, 128>(s, p, grid, st); break;
-        case 192: bf16 ? go<bf16_t, 192>(s, p, grid, st) : go<half_t, 192>(s, p, grid, st); break;
-        case 256: bf16 ? go<bf16_t, 256>(s, p, grid, st) : go<half_t, 256>(s, p, grid, st); break;
+        case 64: bf16 ? go<bf16_t, 64>(s, p, st) : go<half_t, 64>(s, p, st); break;
+        case 128: bf16 ? go<bf16_t, 128>(s, p, st) : go<half_t, 128>(s, p, st); break;
+        case 192: bf16 ? go<bf16_t, 192>(s, p, st) : go<half_t, 192>(s, p, st); break;
+        case 256: bf16 ? go<bf16_t, 256>(s, p, st) : go<half_t, 256>(s, p, st); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

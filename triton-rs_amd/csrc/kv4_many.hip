@@ -99,16 +99,27 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int live, flo
     }
 }
 
-template <typename E, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4AttnParams p) {
-    constexpr int NT = 2, COLS = 16 * NT, STEP = 64;
+template <typename E, int D, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void kv4_many_kernel(Kv4AttnParams p) {
+    constexpr int NT = 2, COLS = 16 * NT, STEP = 64, ALL = STEP * GROUPS;
     typedef Kv4Cols<E, D, NT> C;
-    __shared__ ManyLds<D> lds[2];
+    __shared__ ManyLds<D> lds[2][GROUPS];
     __shared__ float ml[4 * COLS][2];
     __shared__ int last;
     Kv4Item w;
-    if (!kv4_item<4 * COLS, STEP>(p, w)) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // columns of long rows first, or (where all workgroups run at once) long and short by turns
+    const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
+    const int tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
+    int lo, hi;
+    w.h = blockIdx.x;
+    w.sequence<4 * COLS, STEP>(p, blockIdx.y, tile * 4 * COLS, lo, hi);
+    const int chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
+    w.take(p.splits == 1 ? 0 : blockIdx.z - z * p.splits, chunks, p.chunk, lo, hi);
+    if (w.cols <= 0 || w.split >= chunks) return;
+    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
+    w.slot = w.at * p.splits;
+    // wave `wave` of group `group`: the group takes every GROUPS-th step of the keys
+    const int lane = threadIdx.x & 63, number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3, group = number >> 2;
     const int col = lane & 15, kb = lane >> 4;
     C a;
     a.load(p, w, w.c0 + wave * COLS, lane);
@@ -118,7 +129,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4Attn
     int live = 0;   // tokens of this wave's block of the step in t
     // (beyond the keys: their last block again, none of it alive)
     auto fetch = [&](int j) {
-        const int blk = (j >> 4) + wave, page = pages.page(blk);
+        const int blk = ((j + STEP * group) >> 4) + wave, page = pages.page(blk);
         live = pages.ok(page) ? w.k1 - 16 * blk : 0;
         load_packed<D>(t, pages.block(page, blk), lane);
     };
@@ -126,27 +137,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4Attn
     if (any) fetch(w.k0);
     // one power of two for the workgroup's rows of q
     float top = a.largest();
-    if (lane == 0) ml[wave][0] = top;
+    if (lane == 0 && group == 0) ml[wave][0] = top;   // (the groups have the same rows)
     __syncthreads();
     top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
     a.start(p, top);
     __syncthreads();
 
     if (any) {
-        unpack<E, D>(lds[0], t, live, a.kscale, wave, lane);
-        fetch(w.k0 + STEP);
+        unpack<E, D>(lds[0][group], t, live, a.kscale, wave, lane);
+        fetch(w.k0 + ALL);
     }
     __syncthreads();
     int buf = 0;
-    for (int j = w.k0; j < w.k1; j += STEP, buf ^= 1) {
-        if (j + STEP < w.k1) {
-            unpack<E, D>(lds[buf ^ 1], t, live, a.kscale, wave, lane);
-            fetch(j + 2 * STEP);
+    for (int j = w.k0; j < w.k1; j += ALL, buf ^= 1) {
+        if (j + ALL < w.k1) {
+            unpack<E, D>(lds[buf ^ 1][group], t, live, a.kscale, wave, lane);
+            fetch(j + 2 * ALL);
         }
-        const ManyLds<D>& s = lds[buf];
+        const ManyLds<D>& s = lds[buf][group];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int jh = j + 32 * half;
+            const int jh = j + STEP * group + 32 * half;
             if (jh >= a.jhi || jh + 32 <= a.jlo) continue;   // none of this wave's columns sees these
             float4_t acc[NT][2];
 #pragma unroll
@@ -200,9 +211,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4Attn
     }
     a.finish();
 
+    if constexpr (GROUPS == 2) {   // the second group's share of the keys to the first
+        float4_t* const o = reinterpret_cast<float4_t*>(&lds[0][0]) + wave * (NT * C::VT) * 64;
+        float* const mls = reinterpret_cast<float*>(reinterpret_cast<float4_t*>(&lds[0][0]) + 4 * (NT * C::VT) * 64) + wave * NT * 128;
+        static_assert(4 * NT * C::VT * 64 * 16 + 4 * NT * 128 * 4 <= sizeof(lds), "results of four waves fit");
+        if (group) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mls[128 * n + lane] = a.m[n];
+                mls[128 * n + 64 + lane] = a.l[n];
+#pragma unroll
+                for (int x = 0; x < C::VT; ++x) o[(n * C::VT + x) * 64 + lane] = a.o[n][x];
+            }
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m1 = mls[128 * n + lane], mm = fmaxf(a.m[n], m1);
+                const float f0 = __builtin_amdgcn_exp2f(a.m[n] - mm), f1 = __builtin_amdgcn_exp2f(m1 - mm);
+                a.m[n] = mm;
+                a.l[n] = a.l[n] * f0 + mls[128 * n + 64 + lane] * f1;
+#pragma unroll
+                for (int x = 0; x < C::VT; ++x) a.o[n][x] = a.o[n][x] * f0 + o[(n * C::VT + x) * 64 + lane] * f1;
+            }
+        }
+    }
     const Kv4Sink<E, D> sink(p, w);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+        if (group) break;
         const int c = 16 * n + col;
         const float inv = a.l[n] == 0.f ? 0.f : 1.f / a.l[n];
 #pragma unroll
@@ -211,22 +249,39 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv4_many_kernel(Kv4Attn
             for (int x = 0; x < C::VT; x += 4) {
                 const float4_t v = {a.o[n][x][i], a.o[n][x + 1][i], a.o[n][x + 2][i], a.o[n][x + 3][i]};
                 // (chunks of partial results as they lie: 1 KiB a store and wave)
-                if (w.chunks > 1) st_partial4<SCOPE_DEVICE>(sink.part + 4 * sink.lane_quad(wave, n, i, x, lane), v);
-                else if (c < a.n) sink.out(a.c + c, (4 * kb + i) * C::VT + x, v, inv);
+                if (w.chunks > 1) {
+                    st_partial4<SCOPE_DEVICE>(sink.part + 4 * sink.lane_quad(wave, n, i, x, lane), v);
+                } else if (c < a.n) {
+                    if constexpr (C::VT % 8 == 0) {   // 16 bytes a store
+                        if (x % 8 == 4) sink.out8(a.c + c, (4 * kb + i) * C::VT + x - 4, float4_t{a.o[n][x - 4][i], a.o[n][x - 3][i], a.o[n][x - 2][i], a.o[n][x - 1][i]}, v, inv);
+                    } else {
+                        sink.out(a.c + c, (4 * kb + i) * C::VT + x, v, inv);
+                    }
+                }
             }
         if (kb == 0 && c < a.n) sink.put_ml(a.c + c, a.m[n], a.l[n]);
     }
     if (w.chunks == 1) return;
-    sink.template join<true>(min(4 * COLS, w.cols), &ml[0][0], reinterpret_cast<float4_t*>(&lds[0]), &last);
+    sink.template join_lanes<256 * GROUPS>(min(4 * COLS, w.cols), &ml[0][0], &last);
+}
+
+template <typename E, int D>
+static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+    const dim3 grid(p.Hkv, p.B, s.tiles * s.splits);
+    if constexpr (D <= 128)
+        if (s.groups == 2) {
+            kv4_many_kernel<E, D, 2><<<grid, 512, 0, st>>>(p);
+            return;
+        }
+    kv4_many_kernel<E, D, 1><<<grid, 256, 0, st>>>(p);
 }
 
 hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {
-    const dim3 grid(p.Hkv, p.B, s.tiles * s.splits);
     switch (D) {
-        case 64: bf16 ? kv4_many_kernel<bf16_t, 64><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 64><<<grid, 256, 0, st>>>(p); break;
-        case 128: bf16 ? kv4_many_kernel<bf16_t, 128><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 128><<<grid, 256, 0, st>>>(p); break;
-        case 192: bf16 ? kv4_many_kernel<bf16_t, 192><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 192><<<grid, 256, 0, st>>>(p); break;
-        case 256: bf16 ? kv4_many_kernel<bf16_t, 256><<<grid, 256, 0, st>>>(p) : kv4_many_kernel<half_t, 256><<<grid, 256, 0, st>>>(p); break;
+        case 64: bf16 ? go<bf16_t, 64>(s, p, st) : go<half_t, 64>(s, p, st); break;
+        case 128: bf16 ? go<bf16_t, 128>(s, p, st) : go<half_t, 128>(s, p, st); break;
+        case 192: bf16 ? go<bf16_t, 192>(s, p, st) : go<half_t, 192>(s, p, st); break;
+        case 256: bf16 ? go<bf16_t, 256>(s, p, st) : go<half_t, 256>(s, p, st); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -200,3 +200,319 @@ def test_several_queries(dtype, Hq, Hkv, D, nq, lens, causal, window):
     P = need_gpu()
     b = Batch(P, nq, lens, Hq, Hkv, D, 16, dtype)
     b.check(*b.gpu(P, causal=causal, window=window), causal=causal, window=window)
+
+
+def attention_path(P, T, B, Hq, Hkv, D, max_q, max_kv):
+    """What kv4_attention runs: ("few", column tiles a wave, chunks a head at most, joined apart) or
+    ("many", wave groups, chunks)."""
+    import ctypes
+    out = (ctypes.c_int32 * 4)()
+    P.lib().w4a16_internal_kv4_path(T, B, Hq, Hkv, D, max_q, max_kv, out)
+    return ("few", *out[1:]) if out[0] == 1 else ("many", *out[1:3])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,lens,Hq,Hkv,D,page,window,path", [
+    # few columns: one and two column tiles a wave, one chunk a sequence and several, joined by the last
+    # workgroup and by a kernel of their own, more sequences than a wave has lanes
+    ([1] * 3, [100, 128, 7], 8, 2, 128, 16, 0, ("few", 1, 3, 0)),
+    ([1] * 2, [1500, 900], 8, 8, 64, 32, 0, ("few", 1, 24, 0)),
+    ([1], [3000], 4, 1, 128, 64, 0, ("few", 1, 24, 1)),
+    ([1] * 5, [2100, 1, 850, 0, 1300], 24, 1, 128, 16, 0, ("few", 2, 85, 1)),
+    ([5, 5, 3], [1100, 9, 1400], 16, 2, 64, 16, 300, ("few", 2, 36, 1)),
+    ([5], [1000], 4, 1, 64, 16, 0, ("few", 2, 9, 0)),
+    ([8, 2, 8], [1700, 800, 33], 8, 1, 256, 64, 0, ("few", 1, 42, 1)),
+    ([4, 9], [900, 1000], 10, 2, 192, 32, 0, ("few", 1, 18, 1)),
+    ([1] * 130, [(37 * i) % 331 for i in range(130)], 2, 1, 64, 16, 0, ("few", 1, 390, 0)),
+    # many: two groups of waves on a tile, one of them, keys in one chunk and in several
+    ([300, 70], [300, 500], 2, 1, 128, 32, 0, ("many", 2, 1)),
+    ([90], [2500], 4, 2, 64, 16, 0, ("many", 2, 5)),
+    ([70, 66], [1500, 1030], 1, 1, 256, 64, 700, ("many", 1, 3)),
+    ([65, 2], [600, 1200], 3, 3, 192, 16, 0, ("many", 1, 3)),
+    ([129] * 172, [129 + i for i in range(172)], 3, 3, 64, 16, 33, ("many", 1, 1)),
+])
+def test_every_path(dtype, nq, lens, Hq, Hkv, D, page, window, path):
+    P = need_gpu()
+    assert attention_path(P, sum(nq), len(nq), Hq, Hkv, D, max(nq), max(lens)) == path
+    b = Batch(P, nq, lens, Hq, Hkv, D, page, dtype)
+    out, lse = b.gpu(P, window=window)
+    b.check(out, lse, window=window)
+    again, _ = b.gpu(P, window=window)
+    assert torch.equal(out, again), "the same call twice"
+
+
+def test_long_sequence_and_workspace_of_many_calls():
+    """70,000 keys; one workspace through calls of other shapes, back and forth."""
+    P = need_gpu()
+    a = Batch(P, [1, 1], [70000, 300], 8, 2, 64, 128, F16, seed=4)
+    b = Batch(P, [40, 7], [600, 50], 8, 2, 64, 16, F16, seed=5)
+    ws = P.kv4_attention_workspace(a.q.cuda(), a.cache, 2, 1, 70000)
+    need = P.kv4_attention_workspace(b.q.cuda(), b.cache, 2, 40, 600).numel()
+    if ws.numel() < need:
+        ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        a.check(*a.gpu(P, cu_q=None, workspace=ws))
+        b.check(*b.gpu(P, workspace=ws))
+    assert int(ws[:P.KV4_COUNTER_BYTES].sum()) == 0
+
+
+def test_beyond_32_bit_offsets():
+    """Rows, and attention, in the pages past 4 GiB of a cache."""
+    P = need_gpu()
+    Hkv, D, page = 2, 128, 64
+    per = P.lib().w4a16_kv4_cache_bytes(1, Hkv, D, page)
+    pages = 5 * 2 ** 30 // per
+    cache = torch.empty((pages, Hkv, page // 16, 16 * D + 128), dtype=torch.uint8, device="cuda")
+    gen = torch.Generator().manual_seed(9)
+    L = 150
+    k, v = rows(gen, L, Hkv, D, F16), rows(gen, L, Hkv, D, F16)
+    table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32)
+    t = torch.arange(L)
+    slots = (table[0, t // page].long() * page + t % page).int()
+    assert pages * page < 2 ** 31 and (pages - 2) * per > 2 ** 32
+    P.kv4_write(k.cuda(), v.cuda(), cache, slots.cuda())
+    ko, vo = P.kv4_read(cache, slots.cuda())
+    held = [plain.quantise(x)[3] for x in (k, v)]
+    assert same(ko, plain.rounded(held[0], F16)) and same(vo, plain.rounded(held[1], F16))
+    q = torch.randn((1, 4, D), generator=gen).half()
+    out = P.kv4_attention(q.cuda(), cache, table.cuda(), torch.tensor([L], dtype=torch.int32, device="cuda"))
+    o = plain.attention(q.double().numpy(), [held[0]], [held[1]], [1], [L])[0]
+    assert np.abs(out.double().cpu().numpy() - o).max() <= 2.0 ** -9 * np.abs(o).max()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,lens", [([1, 1], [70, 200]), ([80, 90], [100, 95])])
+def test_rows_that_are_not_finite(dtype, nq, lens):
+    """A key or value row of NaN reaches the queries that see it, whole rows of them, and no other; a query
+    with an infinity or NaN itself alone."""
+    P = need_gpu()
+    b = Batch(P, nq, lens, 4, 2, 64, 16, dtype)
+    gen = torch.Generator().manual_seed(3)
+    k, v = rows(gen, 2, 2, 64, dtype), rows(gen, 2, 2, 64, dtype)
+    k[0, 1, 5], v[1, 0, 7] = float("nan"), float("inf")
+    # the key at token len - 1 of sequence 0 (head 1), the value at token len - 1 of sequence 1 (head 0)
+    last = torch.tensor([int(b.table[s, (lens[s] - 1) // 16]) * 16 + (lens[s] - 1) % 16 for s in (0, 1)], dtype=torch.int32)
+    P.kv4_write(k.cuda(), v.cuda(), b.cache, last.cuda())
+    for s in (0, 1):
+        b.k[s][lens[s] - 1], b.v[s][lens[s] - 1] = plain.quantise(k)[3][s], plain.quantise(v)[3][s]
+    b.q[0, 0, 3] = float("inf")
+    if nq[0] > 1:
+        b.q[0, 3, 3], b.q[1, 1, 0] = float("nan"), -float("inf")
+    out, lse = (x.cpu().double().numpy() for x in b.gpu(P))
+    want, wl, *_ = plain.attention(b.q.double().numpy(), b.k, b.v, nq, lens)
+    assert (np.isnan(out) == np.isnan(want)).all()
+    assert np.isnan(want).any() and not np.isnan(want).all()
+    fine = ~np.isnan(want)
+    assert np.abs(out[fine] - want[fine]).max() < 0.05
+
+
+@pytest.mark.parametrize("dtype,q,k,v", [(F16, 4.0, 40.0, 1.0), (F16, 1e-3, 1e-2, 1e-4), (F16, 1.0, 1.0, 6e4 / 5), (F16, 0.0, 1.0, 1.0),
+                                         (BF16, 1e4, 1e-4, 1e20), (BF16, 1e-20, 1e18, 1e-12), (BF16, 1e15, 1e-15, 1.0)])
+def test_magnitudes(dtype, q, k, v):
+    """Keys, values and queries far from 1; all weight on one key; none of it anywhere."""
+    P = need_gpu()
+    for nq, lens in (([1, 1], [400, 33]), ([70], [130])):
+        b = Batch(P, nq, lens, 4, 1, 128, 16, dtype, kscale=k, vscale=v)
+        b.q = (b.q.float() * q).to(dtype)
+        b.check(*b.gpu(P), what=(q, k, v))
+
+
+def test_scales_and_no_lse():
+    P = need_gpu()
+    for scale in (0.0, -0.3, 1.7):
+        b = Batch(P, [1, 4], [50, 300], 4, 4, 64, 32, F16)
+        b.check(*b.gpu(P, scale=scale), scale=scale)
+    out = b.gpu(P, scale=1.7)[0]
+    assert torch.equal(out, b.gpu(P, scale=1.7, lse=None)[0])
+
+
+@pytest.mark.parametrize("nq,lens", [([1, 1, 1], [100, 260, 64]), ([40, 100, 3], [100, 260, 64])])
+def test_pages_that_do_not_exist(nq, lens):
+    """Keys in a page whose number is outside the cache are not seen."""
+    P = need_gpu()
+    b = Batch(P, nq, lens, 8, 2, 64, 16, F16)
+    seen = [np.ones(L, bool) for L in lens]
+    for s, at, number in ((0, 2, -1), (1, 0, len(b.cache)), (1, 9, -2 ** 31), (1, 16, 2 ** 31 - 1), (2, 3, -5)):
+        b.table[s, at] = number
+        seen[s][16 * at:16 * at + 16] = False
+    b.check(*b.gpu(P), seen=seen)
+
+
+@pytest.mark.parametrize("nq,lens,small", [([2, 3], [40, 20], True), ([70, 80], [90, 100], False)])
+def test_rows_and_lengths_out_of_bounds(nq, lens, small):
+    """Rows outside every sequence stay as they were; lengths are cut to the table and to max_kv_len, negative
+    ones to 0; queries beyond max_q_len stay; what the arrays say beyond T is cut."""
+    P = need_gpu()
+    b = Batch(P, nq, lens, 4, 2, 64, 16, F16)
+    T = sum(nq)
+    q = torch.randn((T + 5, 4, 64)).half()
+    q[2:2 + T] = b.q
+    for cu, kv, want_lens in (([2, 2 + nq[0], 2 + T], lens, lens),
+                              ([2, 2 + nq[0], 2 + T], [10 ** 9, -7], [lens[0], 0])):
+        out = torch.full((T + 5, 4, 64), 3.0, dtype=F16, device="cuda")
+        lse = torch.full((T + 5, 4), 3.0, device="cuda")
+        # (10^9 is cut to max_kv_len)
+        P.kv4_attention(q.cuda(), b.cache, b.table.cuda(), torch.tensor(kv, dtype=torch.int32, device="cuda"),
+                        cu_q=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_q_len=max(nq),
+                        max_kv_len=lens[0] if want_lens[1] == 0 else max(lens), out=out, lse=lse)
+        assert (out[:2] == 3).all() and (out[2 + T:] == 3).all() and (lse[:2] == 3).all() and (lse[2 + T:] == 3).all()
+        keep = b.lens
+        b.lens = want_lens
+        b.k, b.v = ([x[:L] for x, L in zip(y, want_lens)] for y in (b.k, b.v))
+        b.check(out[2:2 + T], lse[2:2 + T])
+        b.lens = keep
+    # two queries of each sequence only
+    b = Batch(P, nq, lens, 4, 2, 64, 16, F16)
+    out = torch.full((T, 4, 64), 3.0, dtype=F16, device="cuda")
+    full, _ = b.gpu(P)
+    b.gpu(P, out=out, max_q_len=2)
+    for s in (0, 1):
+        a = int(b.cu[s])
+        assert (out[a + 2:int(b.cu[s + 1])] == 3).all()
+        torch.testing.assert_close(out[a:a + 2], full[a:a + 2], rtol=2e-3, atol=2e-3)
+    # sequences that overlap, run backwards or leave the rows: memory stays intact, the others' rows right
+    out = b.gpu(P, cu_q=torch.tensor([0, nq[0], 10 ** 6], dtype=torch.int32, device="cuda"), max_q_len=T)[0]
+    assert out.shape == (T, 4, 64)
+    torch.testing.assert_close(out[:nq[0]], full[:nq[0]], rtol=2e-3, atol=2e-3)
+    b.gpu(P, cu_q=torch.tensor([T, 3, -9], dtype=torch.int32, device="cuda"), max_q_len=T)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("nq", [1, 90])
+def test_strided_queries_and_outputs(nq):
+    """Queries out of a fused projection, results into head-major rows."""
+    P = need_gpu()
+    Hq, Hkv, D = 8, 2, 128
+    b = Batch(P, [nq, nq], [100, 130], Hq, Hkv, D, 16, F16)
+    qkv = torch.zeros((2 * nq, Hq + 2 * Hkv, D), dtype=F16, device="cuda")
+    qkv[:, :Hq] = b.q.cuda()
+    out = torch.zeros((Hq, 2 * nq, D), dtype=F16, device="cuda").transpose(0, 1)
+    _, lse = b.gpu(P, q=qkv[:, :Hq], out=out)
+    b.check(out, lse)
+
+
+def test_no_work():
+    P = need_gpu()
+    cache = P.kv4_cache(2, 2, 64, 16)
+    empty = torch.zeros((0, 2, 64), dtype=F16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    P.kv4_write(empty, empty, cache, none)
+    assert P.kv4_read(cache, none)[0].shape == (0, 2, 64)
+    assert P.kv4_attention(torch.zeros((0, 4, 64), dtype=F16, device="cuda"), cache,
+                           torch.zeros((0, 1), dtype=torch.int32, device="cuda"), none).shape == (0, 4, 64)
+
+
+# ------------------------------------------------------------------ as a program uses them
+
+def test_steps_of_a_program():
+    """A prompt, then token by token: written, attended over, on a captured graph that is replayed with new
+    slots, lengths and rows; every step against 64 bits, and the eager call between them."""
+    P = need_gpu()
+    B, Hq, Hkv, D, page, dtype = 3, 8, 2, 128, 16, F16
+    gen = torch.Generator().manual_seed(2)
+    first, steps = [40, 15, 700], 5
+    per = 46
+    table = torch.randperm(B * per, generator=gen).view(B, per).int()
+    cache = P.kv4_cache(B * per, Hkv, D, page)
+    k = [rows(gen, n + steps, Hkv, D, dtype) for n in first]
+    v = [rows(gen, n + steps, Hkv, D, dtype) for n in first]
+    held_k, held_v = [plain.quantise(x)[3] for x in k], [plain.quantise(x)[3] for x in v]
+
+    def slot(b, t):
+        return int(table[b, t // page]) * page + t % page
+
+    # the prompts
+    slots = torch.tensor([slot(b, t) for b in range(B) for t in range(first[b])], dtype=torch.int32)
+    P.kv4_write(torch.cat([x[:n] for x, n in zip(k, first)]).cuda(), torch.cat([x[:n] for x, n in zip(v, first)]).cuda(), cache, slots.cuda())
+    # one step, captured
+    d = {"k": torch.zeros((B, Hkv, D), dtype=dtype, device="cuda"), "v": torch.zeros((B, Hkv, D), dtype=dtype, device="cuda"),
+         "q": torch.zeros((B, Hq, D), dtype=dtype, device="cuda"), "slots": torch.full((B,), -1, dtype=torch.int32, device="cuda"),
+         "lens": torch.zeros(B, dtype=torch.int32, device="cuda"), "out": torch.zeros((B, Hq, D), dtype=dtype, device="cuda"),
+         "lse": torch.zeros((B, Hq), device="cuda"), "table": table.cuda()}
+    ws = P.kv4_attention_workspace(d["q"], cache, B, 1, per * page)
+
+    def step(out, lse, ws):
+        P.kv4_write(d["k"], d["v"], cache, d["slots"])
+        P.kv4_attention(d["q"], cache, d["table"], d["lens"], out=out, lse=lse, workspace=ws)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(d["out"], d["lse"], ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(d["out"], d["lse"], ws)
+    for i in range(steps):
+        q = torch.randn((B, Hq, D), generator=gen).to(dtype)
+        lens = [n + i + 1 for n in first]
+        d["q"].copy_(q)
+        d["k"].copy_(torch.stack([x[n + i] for x, n in zip(k, first)]))
+        d["v"].copy_(torch.stack([x[n + i] for x, n in zip(v, first)]))
+        d["slots"].copy_(torch.tensor([slot(b, first[b] + i) for b in range(B)], dtype=torch.int32))
+        d["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        b = Batch.__new__(Batch)
+        b.nq, b.lens, b.dtype, b.D, b.Hq, b.q = [1] * B, lens, dtype, D, Hq, q
+        b.k, b.v = [x[:L] for x, L in zip(held_k, lens)], [x[:L] for x, L in zip(held_v, lens)]
+        b.check(d["out"], d["lse"], what=f"step {i}")
+        eager, lse = torch.zeros_like(d["out"]), torch.zeros_like(d["lse"])
+        step(eager, lse, None)
+        assert torch.equal(eager, d["out"]) and torch.equal(lse, d["lse"])
+
+
+def test_two_streams_with_a_workspace_each():
+    P = need_gpu()
+    bs = [Batch(P, [1, 1], [3000, 2000], 8, 2, 128, 64, F16, seed=s) for s in (1, 2)]
+    args = [(b.q.cuda(), b.table.cuda(), torch.tensor(b.lens, dtype=torch.int32, device="cuda")) for b in bs]
+    ws = [P.kv4_attention_workspace(a[0], b.cache, 2, 1, 3000) for a, b in zip(args, bs)]
+    outs = [[torch.zeros_like(a[0]) for _ in range(10)] for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(10):
+        for s in (0, 1):
+            with torch.cuda.stream(streams[s]):
+                P.kv4_attention(args[s][0], bs[s].cache, args[s][1], args[s][2], max_kv_len=3000, out=outs[s][i], workspace=ws[s])
+    torch.cuda.synchronize()
+    for s in (0, 1):
+        want = bs[s].gpu(P, cu_q=None)
+        bs[s].check(*want)
+        assert all(torch.equal(o, want[0]) for o in outs[s])
+
+
+def test_attention_block_on_int4_weights():
+    """An attention block as a decode step runs it: fused q, k, v projection with int4 weights, the new rows into the
+    cache, attention, output projection; the chain against 64 bits on the same weights and cache."""
+    P = need_gpu()
+    Hq, Hkv, D, B, G = 8, 2, 64, 2, 64
+    hidden = Hq * D
+    gen = torch.Generator("cuda").manual_seed(11)
+
+    def layer(K, N):
+        qw = torch.randint(-2 ** 31, 2 ** 31 - 1, (K // 8, N), generator=gen, device="cuda", dtype=torch.int64).int()
+        sc = (torch.rand((K // G, N), generator=gen, device="cuda") * 0.004 + 0.002).half()
+        return qw, sc
+
+    wqkv, wo = layer(hidden, (Hq + 2 * Hkv) * D), layer(hidden, hidden)
+    dense = [P.dequant(q, s, None, fmt="gptq_sym", group_size=G).double() for q, s in (wqkv, wo)]
+    cache = P.kv4_cache(8, Hkv, D, 16)
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(B, 4)
+    keys, vals = [[], []], [[], []]
+    for i in range(20):
+        x = torch.randn((B, hidden), generator=gen, device="cuda").half()
+        qkv = P.gemm(x, wqkv[0], wqkv[1], None, fmt="gptq_sym", group_size=G).view(B, Hq + 2 * Hkv, D)
+        slots = (table[:, i // 16] * 16 + i % 16).int()
+        P.kv4_write(qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:], cache, slots)
+        lens = torch.full((B,), i + 1, dtype=torch.int32, device="cuda")
+        att = P.kv4_attention(qkv[:, :Hq], cache, table, lens)
+        y = P.gemm(att.view(B, hidden), wo[0], wo[1], None, fmt="gptq_sym", group_size=G)
+        for b in range(B):
+            keys[b].append(plain.quantise(qkv[b:b + 1, Hq:Hq + Hkv].cpu())[3])
+            vals[b].append(plain.quantise(qkv[b:b + 1, Hq + Hkv:].cpu())[3])
+    o = plain.attention(qkv[:, :Hq].double().cpu().numpy(), [np.concatenate(a) for a in keys], [np.concatenate(a) for a in vals],
+                        [1] * B, [20] * B)[0]
+    want = torch.from_numpy(o).view(B, hidden).cuda() @ dense[1]
+    err = (y.double() - want).norm() / want.norm()
+    assert err < 2e-3, float(err)
+    torch.testing.assert_close(qkv.reshape(B, -1).double(), x.double() @ dense[0], rtol=1e-2, atol=1e-2)

@@ -170,6 +170,16 @@ W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_
     return W4A16_KV4_COUNTER_BYTES + kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len).partial_bytes;
 }
 
+// Which kernel a call runs, so that tests can hold a case to the path it is for; not part of the public header.
+// out: {1, column tiles a wave, chunks a head at most, joined by a kernel of their own} few columns; {2, wave
+// groups, chunks, 0} many.
+W4A16_API void w4a16_internal_kv4_path(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q_len,
+                                       int32_t max_kv_len, int32_t* out) {
+    const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
+    const int32_t few[4] = {1, s.nt, s.places, s.join_apart}, many[4] = {2, s.groups, s.splits, 0};
+    for (int i = 0; i < 4; ++i) out[i] = s.many ? many[i] : few[i];
+}
+
 W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t q_stride_t, int32_t q_stride_h,
                                   const void* cache, const int32_t* page_table, const int32_t* kv_lens,
                                   const int32_t* cu_q, void* out, int32_t out_stride_t, int32_t out_stride_h, float* lse,

@@ -114,6 +114,7 @@ def _attention(P, **over):
     (dict(page=40), "page_size 40", True),
     (dict(Hq=2048, Hkv=4), "2048 heads", True),
     (dict(B=70000), "sequences", True),
+    (dict(mkv=2 ** 30 + 1), "max_kv_len", True),
     (dict(T=2 ** 27, mq=2 ** 27, qst=512), "at most", True),
 ])
 def test_attention_refusals(over, needle, unsupported):
@@ -149,7 +150,7 @@ def test_workspace_covers_every_split():
             assert out[2] == 1 or -(-C // 128) * B * Hkv <= 16384
         else:
             tiles = -(-C // (32 * out[1]))
-            whole = mkv <= 128 or tiles * B * Hkv > 16384
+            whole = mkv <= 768 or tiles * B * Hkv > 16384
             slots = 0 if whole else tiles * Hkv * out[2] * (-(-min(C, 32 * out[1]) // 16) * 16)
             assert out[2] >= B
             # the rule of the kernel: chunks of c 128 keys, at most `places` of them for any lengths

@@ -576,6 +576,7 @@ def fused_moe_prepared(x, router_logits, w13: PreparedWeights, w2: PreparedWeigh
 # ------------------------------------------------------------------ key/value cache in 4 bits
 
 KV4_COUNTER_BYTES = 65536
+_Tensor = torch.Tensor
 
 
 def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -592,7 +593,7 @@ def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int =
 
 def _kv4_cache_shape(cache: torch.Tensor):
     """(pages, kv heads, page size, head dim, device index) of a cache tensor."""
-    index = cache.get_device() if isinstance(cache, torch.Tensor) else -1
+    index = cache.get_device() if isinstance(cache, _Tensor) else -1
     if index < 0 or cache.dtype is not torch.uint8:
         _require(cache, "cache", (torch.uint8,))
     shape = cache.shape
@@ -605,15 +606,17 @@ def _kv4_cache_shape(cache: torch.Tensor):
     return pages, Hkv, blocks * 16, D, index
 
 
+# (each check of a tensor is the one test that a good call pays; _require says what is wrong with a bad one)
+
 def _kv4_tensor(t, name: str, dtypes, index: int):
-    # (the one test that a good call pays; _require says what is wrong with a bad one)
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != index:
+    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
         _require(t, name, dtypes, torch.device("cuda", index))
 
 
 def _kv4_rows(t, name: str, dtypes, index: int, shape=None):
     """(token stride, head stride) of rows [T, H, D] with contiguous D."""
-    _kv4_tensor(t, name, dtypes, index)
+    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
+        _require(t, name, dtypes, torch.device("cuda", index))
     if t.shape != shape if shape is not None else t.dim() != 3:
         raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
     st, sh, sd = t.stride()
@@ -623,7 +626,8 @@ def _kv4_rows(t, name: str, dtypes, index: int, shape=None):
 
 
 def _kv4_index(t, name: str, index: int, shape=None):
-    _kv4_tensor(t, name, _INT32, index)
+    if not isinstance(t, _Tensor) or t.dtype is not torch.int32 or t.get_device() != index:
+        _require(t, name, _INT32, torch.device("cuda", index))
     if not t.is_contiguous() or (shape is not None and t.shape != shape):
         raise InvalidArgument(f"{name} must be a contiguous int32 tensor" + ("" if shape is None else f" {list(shape)}"))
 
@@ -633,7 +637,7 @@ def _call_on(index: int, fn, *args) -> None:
     are launched on the current device). Pointers go as plain integers and the stream without an
     object around it: a decode step makes many of these calls, each a few microseconds of host time."""
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(stream, *args)
     else:
         with torch.cuda.device(index):

@@ -18,6 +18,7 @@ constexpr int KV4_MAX_HEADS = 1024;
 // Compute units that the split of the keys is planned for: MI355X's, so that a workspace's size is the same wherever it is asked for.
 constexpr int KV4_CUS = 256;
 static_assert(KV4_MAX_COUNTERS * sizeof(uint32_t) == W4A16_KV4_COUNTER_BYTES, "counters fill their area");
+constexpr int KV4_MAX_KEYS = 1 << 30;   // of a sequence: positions a few steps further still are int32
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
 constexpr int64_t KV4_JOIN_BYTES = 40 << 10;   // partial results of a sequence and head that its last workgroup joins itself
@@ -108,8 +109,8 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         // chunks of a head and tile: what runs at once, or several rounds of it; B sequences have one each at least,
         // and a remainder
         const int64_t at_once = std::max<int64_t>(1, slots_of_cu * kv4_few_per_cu(D, s.nt) / (Hkv * tiles));
-        const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
-        s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= 128;
+        const int64_t rounds = more * (2 * (int64_t)B + at_once - 1) / at_once;
+        s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= KV4_WHOLE_KEYS;
         s.budget = (int)std::max<int64_t>(2 * (int64_t)B, rounds * at_once);
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
         s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
@@ -156,6 +157,7 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
         return fail(W4A16_ERR_INVALID_ARG, "%d query heads must be a multiple of %d key/value heads", Hq, Hkv);
     if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
     if (Hq > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hq, KV4_MAX_HEADS);
+    if (max_kv > KV4_MAX_KEYS) return fail(W4A16_ERR_UNSUPPORTED, "max_kv_len %d: at most %d", max_kv, KV4_MAX_KEYS);
     if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
     if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
     const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q, max_kv);

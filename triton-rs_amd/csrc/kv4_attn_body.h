@@ -129,7 +129,7 @@ struct Kv4Item {
         split = split_;
         chunks = chunks_;
         k0 = lo + split * chunk;
-        k1 = chunks == 1 ? hi : min(hi, k0 + chunk);
+        k1 = chunks == 1 ? hi : k0 + min(hi - k0, chunk);
     }
 };
 

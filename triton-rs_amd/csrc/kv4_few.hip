@@ -78,7 +78,7 @@ __device__ __forceinline__ int wave_sums(int v) {
 // Chunks of `steps` steps of keys in chunks of c 128 (4 c steps). Up to 768 keys stay whole: a chunk more costs some 3 us
 // (its partial results' way to the last one and back), 128 keys 0.5.
 __device__ __forceinline__ int few_chunks(int steps, int c) {
-    return steps <= max(24, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
+    return steps <= max(KV4_WHOLE_KEYS / STEP, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
 }
 
 // The chunks of all sequences for one head and tile of columns stand in a row; workgroup u takes the u-th. Their
@@ -87,6 +87,13 @@ __device__ __forceinline__ int few_chunks(int steps, int c) {
 // sequence u's first chunk instead. A lane a sequence.
 template <int WG_COLS>
 __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w) {
+    w.h = blockIdx.x;
+    if (p.whole) {   // sequence u, in one chunk
+        int lo, hi;
+        w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
+        w.take(0, 1, 0, lo, hi);
+        return w.cols > 0;
+    }
     const int lane = threadIdx.x & 63;
     Kv4Item mine;
     int lo = 0, hi = 0, steps = 0;
@@ -108,15 +115,12 @@ __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u
         }
         return sum;
     };
-    int c = 1 << 23;   // in 128 keys
-    if (!p.whole) {
-        const unsigned sum = all([&] { return steps; });
-        // with no remainders, half a chunk a sequence, one a sequence
-        for (int rest = 0; rest <= 4; rest += 2) {
-            const unsigned room = 4 * p.budget - rest * p.B;
-            c = (int)max(1u, (sum + room - 1) / room);
-            if (rest == 4 || all([&] { return few_chunks(steps, c); }) <= (unsigned)p.budget) break;
-        }
+    const unsigned sum = all([&] { return steps; });
+    int c = 1;   // in 128 keys: with no remainders, half a chunk a sequence, one a sequence
+    for (int rest = 0; rest <= 4; rest += 2) {
+        const unsigned room = 4 * p.budget - rest * p.B;
+        c = (int)max(1u, (sum + room - 1) / room);
+        if (rest == 4 || all([&] { return few_chunks(steps, c); }) <= (unsigned)p.budget) break;
     }
     for (int base = 0, before = 0; base < p.B; base += 64) {
         if (p.B > 64) has = look(base);
@@ -126,7 +130,6 @@ __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u
         if (who) {
             const int l = __builtin_ctzll(who);
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            w.h = blockIdx.x;
             w.b = base + l;
             w.q0 = of(mine.q0);
             w.n = of(mine.n);

@@ -109,7 +109,7 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         // chunks of a head and tile: what runs at once, or several rounds of it; B sequences have one each at least,
         // and a remainder
         const int64_t at_once = std::max<int64_t>(1, slots_of_cu * kv4_few_per_cu(D, s.nt) / (Hkv * tiles));
-        const int64_t rounds = more * (2 * (int64_t)B + at_once - 1) / at_once;
+        const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
         s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= KV4_WHOLE_KEYS;
         s.budget = (int)std::max<int64_t>(2 * (int64_t)B, rounds * at_once);
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));

@@ -306,6 +306,30 @@ def test_rows_that_are_not_finite(dtype, nq, lens):
     assert np.abs(out[fine] - want[fine]).max() < 0.05
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,L,window", [(1, 90, 50), (5, 300, 0), (5, 300, 77), (150, 200, 0), (150, 400, 70)])
+def test_rows_that_a_query_does_not_see(dtype, nq, L, window):
+    """What masked tokens hold moves no bit of a query's result: any bytes before the window and behind the
+    keys, and, for queries that do not see them, keys and values at the type's end, NaN and infinities."""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, dtype, seed=6)
+    out, lse = b.gpu(P, window=window)
+    b.check(out, lse, window=window)
+    blocks = b.cache[b.table[0].long()].cpu().numpy()          # pages of 16 tokens
+    before = max(0, L - nq + 1 - window) if window else 0     # tokens that no query sees
+    for t in [*range(before), *range(L, 16 * b.table.shape[1])]:
+        for at in (16 * 64 + 4 * (t % 16), 16 * 64 + 64 + 4 * (t % 16)):   # scales of NaN and near the type's end
+            blocks[t // 16, :, 0, at:at + 4] = np.frombuffer(np.uint32(0x7FFF if t % 3 else 0x7BFF).tobytes(), np.uint8)
+    b.cache[b.table[0].long()] = torch.from_numpy(blocks).cuda()
+    out2, lse2 = b.gpu(P, window=window)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    for x in (torch.finfo(dtype).max, float("nan"), float("inf")):   # the last token: the last query's alone
+        far = torch.full((1, 2, 64), x, dtype=dtype, device="cuda")
+        P.kv4_write(far, far, b.cache, (b.table[0, (L - 1) // 16:(L - 1) // 16 + 1] * 16 + (L - 1) % 16).cuda())
+        out2, lse2 = b.gpu(P, window=window)
+        assert torch.equal(out[:-1], out2[:-1]) and torch.equal(lse[:-1], lse2[:-1]), x
+
+
 @pytest.mark.parametrize("dtype,q,k,v", [(F16, 4.0, 40.0, 1.0), (F16, 1e-3, 1e-2, 1e-4), (F16, 1.0, 1.0, 6e4 / 5), (F16, 0.0, 1.0, 1.0),
                                          (BF16, 1e4, 1e-4, 1e20), (BF16, 1e-20, 1e18, 1e-12), (BF16, 1e15, 1e-15, 1.0)])
 def test_magnitudes(dtype, q, k, v):

@@ -99,6 +99,7 @@ def _attention(P, **over):
     (dict(window=-1), "window", False),
     (dict(scale=float("nan")), "finite", False),
     (dict(scale=float("inf")), "finite", False),
+    (dict(scale=3e38), "finite", False),      # (times log2 e it is not)
     (dict(cu=None), "one query", False),
     (dict(cu=None, T=2), "max_q_len is 1", False),
     (dict(q=P16 + 2), "16-byte aligned", False),
@@ -115,6 +116,7 @@ def _attention(P, **over):
     (dict(Hq=2048, Hkv=4), "2048 heads", True),
     (dict(B=70000), "sequences", True),
     (dict(mkv=2 ** 30 + 1), "max_kv_len", True),
+    (dict(B=65, mkv=2 ** 30), "2^36 keys", True),
     (dict(T=2 ** 27, mq=2 ** 27, qst=512), "at most", True),
 ])
 def test_attention_refusals(over, needle, unsupported):

@@ -19,6 +19,7 @@ constexpr int KV4_MAX_HEADS = 1024;
 constexpr int KV4_CUS = 256;
 static_assert(KV4_MAX_COUNTERS * sizeof(uint32_t) == W4A16_KV4_COUNTER_BYTES, "counters fill their area");
 constexpr int KV4_MAX_KEYS = 1 << 30;   // of a sequence: positions a few steps further still are int32
+constexpr int64_t KV4_MAX_ALL_KEYS = 1ll << 36;   // of all sequences: their steps of 32 are summed in 32 bits
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
 constexpr int64_t KV4_JOIN_BYTES = 40 << 10;   // partial results of a sequence and head that its last workgroup joins itself
@@ -158,6 +159,8 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
     if (!kv4_head_dim_ok(D)) return fail(W4A16_ERR_UNSUPPORTED, "head dimension %d: 64, 128, 192 or 256", D);
     if (Hq > KV4_MAX_HEADS) return fail(W4A16_ERR_UNSUPPORTED, "%d heads: at most %d", Hq, KV4_MAX_HEADS);
     if (max_kv > KV4_MAX_KEYS) return fail(W4A16_ERR_UNSUPPORTED, "max_kv_len %d: at most %d", max_kv, KV4_MAX_KEYS);
+    if ((int64_t)B * max_kv > KV4_MAX_ALL_KEYS)
+        return fail(W4A16_ERR_UNSUPPORTED, "%d sequences with max_kv_len %d: at most 2^36 keys in a call", B, max_kv);
     if (B > 65535) return fail(W4A16_ERR_UNSUPPORTED, "%d sequences: at most 65535 in a call", B);
     if (T > KV4_MAX_ROWS / Hq) return fail(W4A16_ERR_UNSUPPORTED, "%d queries of %d heads: at most %d in a call", T, Hq, KV4_MAX_ROWS);
     const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q, max_kv);
@@ -193,7 +196,8 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     if (int rc = check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return rc;
     if (pages_per_seq < 1) return fail(W4A16_ERR_INVALID_ARG, "pages_per_seq (%d) must be positive", pages_per_seq);
     if (window < 0) return fail(W4A16_ERR_INVALID_ARG, "window (%d) must not be negative", window);
-    if (!std::isfinite(scale)) return fail(W4A16_ERR_INVALID_ARG, "scale must be finite");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return fail(W4A16_ERR_INVALID_ARG, "scale must be finite, and below 2e38");
     if (!cu_q && T != B) return fail(W4A16_ERR_INVALID_ARG, "without cu_q every sequence has one query (T=%d B=%d)", T, B);
     if (!cu_q && max_q_len != 1) return fail(W4A16_ERR_INVALID_ARG, "without cu_q max_q_len is 1, not %d", max_q_len);
     if (T == 0 || B == 0) return W4A16_OK;
@@ -215,7 +219,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
     p.page_shift = __builtin_ctz((unsigned)page_size);
     p.max_q = max_q_len < T ? max_q_len : T; p.max_kv = max_kv_len;
-    p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
+    p.scale_log2 = scale_log2; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
     p.counters = static_cast<uint32_t*>(workspace);
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
     p.G = Hq / Hkv; p.slot_cols = s.slot_cols;

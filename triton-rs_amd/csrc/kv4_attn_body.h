@@ -19,9 +19,9 @@
 // tokens may run in any order as long as the values follow), so no logit or weight passes between lanes
 // or through LDS. q is scaled by a power of two (wave-wide) into fp16's range, exactly for fp16 and bf16
 // alike but for what lies 2^27 below the largest. A weight p_j s_j is rounded to fp16; the reference m is
-// such that all of them are below 2^16, and raised (with the sums scaled down) only where a logit or a
-// value scale passes what it leaves room for, 8 in base 2, so maxima pass between lanes only then. Sums
-// are fp32.
+// such that all of them are below 2^16, and raised (with the sums scaled down) only where a logit passes
+// the room that it and the value scales leave, 8 in base 2, so maxima pass between lanes only then. A
+// column's reference follows what the column sees, nothing else. Sums are fp32.
 #pragma once
 #include <cfloat>
 
@@ -89,6 +89,18 @@ __device__ __forceinline__ float kb_all(float v, F f) {
 __device__ __forceinline__ float kb_sum(float v) { return kb_all(v, [](float a, float b) { return a + b; }); }
 __device__ __forceinline__ float kb_max(float v) { return kb_all(v, [](float a, float b) { return fmaxf(a, b); }); }
 
+// over the 16 lanes of a row: neighbours, pairs, halves mirrored, the row mirrored
+__device__ __forceinline__ float row_min(float v) {
+    auto step = [&](auto ctrl) {
+        v = fminf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true)));
+    };
+    step(std::integral_constant<int, 0xB1>{});
+    step(std::integral_constant<int, 0x4E>{});
+    step(std::integral_constant<int, 0x141>{});
+    step(std::integral_constant<int, 0x140>{});
+    return v;
+}
+
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
 
 // A scale of NaN (a row that held an infinity or NaN, n = z = 0) as the largest number: the weight of a column that
@@ -145,9 +157,10 @@ struct Kv4Cols {
     half8_t qf[NT][KW];
     float kscale;          // logits in base 2 are kscale s (q . (n - z))
     float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
-    float most[NT];        // logits less m may be this; -infinity until a column has seen a key
-    float vtop;            // a power of two, 2^vlog2, above the largest value scale so far
-    int vlog2;
+    float most[NT];        // the same, -infinity until a column has seen a key
+    float room[NT];        // what logits less m may be: p_j s_j <= 2^KV4_WEIGHT_LOG2
+    float vtop[NT];        // a power of two above the largest value scale that a column has seen; 0 before it
+    float vleast;          // the least of them of all columns
     float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
 
     // the rows of q, as they are
@@ -234,29 +247,46 @@ struct Kv4Cols {
             }
             m[t] = l[t] = 0.f;
             most[t] = -INFINITY;
+            vleast = 0.f;
+            room[t] = (float)KV4_WEIGHT_LOG2;
+            vtop[t] = hi[t] > lo[t] ? 0.f : INFINITY;   // (one that sees nothing asks for no room)
 #pragma unroll
             for (int x = 0; x < VT; ++x) o[t][x] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        vtop = 0.f;
-        vlog2 = 0;
     }
 
-    // The largest value scale of a step, vmax, of all lanes: room made for it.
-    __device__ __forceinline__ void value_top(float vmax) {
-        // 2 to 4 times the largest; value scales below 2^-60 share one
-        const int e = min(126, max(-60, (int)(__float_as_uint(vmax) >> 23) - 127 + 2));
-        const float by = (float)(e - vlog2), fall = __builtin_amdgcn_exp2f(-by);
-        vtop = pow2(e);
-        vlog2 = e;
+    // The lane's tokens j + 4 kb + (0..3, 16..19) that columns t see: those at [from, to) from the first on, not in
+    // a block in `bad`.
+    struct Seen {
+        int from, to, bad;
+        __device__ __forceinline__ bool operator()(int s, int i) const { return (16 * s + i >= from) & (16 * s + i < to) & !((bad >> s) & 1); }
+    };
+    __device__ __forceinline__ Seen seen(int t, int j, int end, int bad, int kb) const {
+        int at = j + 4 * kb;
+        asm volatile("" : "+v"(at), "+s"(bad));   // (else kept over the loop: every token's distances, in registers)
+        return Seen{lo[t] - at, min(hi[t], end) - at, bad};
+    }
+
+    // Room for the value scales of a step, those that a column sees: what others see does not move its reference.
+    // vmax: the largest of them all, of this lane or more; of(t): of this lane's, the largest that columns t see.
+    template <typename F>
+    __device__ __forceinline__ void value_room(float vmax, F of) {
+        if (!__any(vmax > vleast)) return;   // rare after the first steps
+        vleast = INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const bool set = most[t] != -INFINITY;   // (else nothing is summed yet)
-            m[t] += set ? by : 0.f;
-            l[t] *= fall;
-            if (set) most[t] = (float)(KV4_WEIGHT_LOG2 - e);
-#pragma unroll
-            for (int x = 0; x < VT; ++x) o[t][x] *= fall;
+            const float top = kb_max(of(t));
+            // 2 to 4 times the largest; value scales below 2^-60 share one
+            const int e = min(126, max(-60, (int)(__float_as_uint(top) >> 23) - 127 + 2));
+            const bool up = top > vtop[t];
+            float fresh = pow2(e), left = (float)(KV4_WEIGHT_LOG2 - e);
+            asm("" : "+v"(fresh), "+v"(left));   // (selects, not a branch)
+            vtop[t] = up ? fresh : vtop[t];
+            room[t] = up ? left : room[t];
+            most[t] = most[t] == -INFINITY ? most[t] : room[t];   // (the next logits raise m where that is too little)
+            vleast = fminf(vleast, vtop[t]);
         }
+        vleast = row_min(vleast);
     }
 
     // Logits less m of 32 tokens from j on for columns t: acc = q . (n - z), ks = key scale times kscale, of the
@@ -270,14 +300,12 @@ struct Kv4Cols {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[s][i] = __builtin_fmaf(acc[s][i], ks[s][i], -m[t]);
         if (!whole) {
-            const int from = lo[t], to = min(hi[t], end);
+            const Seen in = seen(t, j, end, bad, kb);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = j + 16 * s + 4 * kb + i;
-                    if (at < from || at >= to || ((bad >> s) & 1)) x[s][i] = -INFINITY;
-                }
+                for (int i = 0; i < 4; ++i)
+                    if (!in(s, i)) x[s][i] = -INFINITY;
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -286,14 +314,14 @@ struct Kv4Cols {
         if (__any(top > most[t])) {
             top = kb_max(top);
             const bool up = top > most[t];
-            const float room = (float)(KV4_WEIGHT_LOG2 - vlog2), by = up ? top - (room - KV4_ROOM) : 0.f;
+            const float by = up ? top - (room[t] - KV4_ROOM) : 0.f;
             // (a column's first keys: nothing summed yet)
             const float fall = most[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-by);
             m[t] += by;
             l[t] *= fall;
 #pragma unroll
             for (int y = 0; y < VT; ++y) o[t][y] *= fall;
-            if (up) most[t] = room;
+            most[t] = up ? room[t] : most[t];
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll

@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (((here >> s) & 1) || j + 16 * s + 4 * kb + i >= end) kp[s][i] = vp[s][i] = 0u;
+                    if (((here >> s) & 1) || j + 16 * s + 4 * kb + i >= end || j + 16 * s + 4 * kb + i < a.jlo) kp[s][i] = vp[s][i] = 0u;
         }
         float4_t acc[NT][2];
 #pragma unroll
@@ -254,9 +254,16 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
                 vs[s][i] = param_scale<E>(vp[s][i]);
                 vmax = fmaxf(vmax, vs[s][i]);
             }
-        if (__any(vmax > a.vtop)) {   // rare after the first steps
-            a.value_top(kb_max(vmax));   // (the lanes of a row have the same tokens)
-        }
+        a.value_room(vmax, [&](int t) {
+            if (whole) return vmax;
+            const auto in = a.seen(t, j, end, here, kb);
+            float top = 0.f;   // (fmaxf: NaN aside)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, in(s, i) ? vs[s][i] : 0.f);
+            return top;
+        });
         if (!whole) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)

@@ -55,13 +55,13 @@ __device__ __forceinline__ void load_packed(Packed<D>& t, const unsigned char* b
     t.vp = *reinterpret_cast<const u32x4*>(at_bytes(b, 16 * D + 64 + (lane >> 4) * 16));
 }
 
-// Block `wave` of a step into LDS; its first `live` tokens (16 or more: all; the others' parameters may be anything)
+// Block `wave` of a step into LDS; its tokens [dead, live) (the others' parameters may be anything)
 template <typename E, int D>
-__device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int live, float kscale, int wave, int lane) {
+__device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int live, float kscale, int wave, int lane) {
     const int col = lane & 15, kb = lane >> 4;
-    t.kc = col < live ? t.kc : 0u;
+    t.kc = col >= dead && col < live ? t.kc : 0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.vp[i] = 4 * kb + i < live ? t.vp[i] : 0u;
+    for (int i = 0; i < 4; ++i) t.vp[i] = 4 * kb + i >= dead && 4 * kb + i < live ? t.vp[i] : 0u;
     const uint32_t zk = zeros_of(t.kc);
     const half2_t kz1 = zero1024(zk), kz16 = zero64(zk);
 #pragma unroll
@@ -143,15 +143,15 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     a.start(p, top);
     __syncthreads();
 
-    if (any) {
-        unpack<E, D>(lds[0][group], t, live, a.kscale, wave, lane);
+    if (any) {   // (only a first step holds tokens before what its columns see)
+        unpack<E, D>(lds[0][group], t, w.see_lo(p, w.n <= 1 ? 0 : w.c0 / p.G) - (w.k0 + STEP * group + 16 * wave), live, a.kscale, wave, lane);
         fetch(w.k0 + ALL);
     }
     __syncthreads();
     int buf = 0;
     for (int j = w.k0; j < w.k1; j += ALL, buf ^= 1) {
         if (j + ALL < w.k1) {
-            unpack<E, D>(lds[buf ^ 1][group], t, live, a.kscale, wave, lane);
+            unpack<E, D>(lds[buf ^ 1][group], t, 0, live, a.kscale, wave, lane);
             fetch(j + 2 * ALL);
         }
         const ManyLds<D>& s = lds[buf][group];
@@ -192,7 +192,15 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            if (__any(vmax > a.vtop)) a.value_top(vmax);   // rare after the first steps
+            a.value_room(vmax, [&](int n) {
+                const auto in = a.seen(n, jh, a.jhi, bad, kb);
+                float top = 0.f;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, (vs[b][i] < FLT_MAX && in(b, i)) ? vs[b][i] : 0.f);
+                return top;
+            });
             float x[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, whole, jh, a.jhi, bad, kb);

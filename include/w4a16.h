@@ -391,20 +391,27 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  * (cu_q null: row b, T = B), the last of them at token kv_lens[b] - 1. A query at token i sees key
  * j < kv_lens[b] where (causal != 0) j <= i and (window > 0) j > i - window:
  *   out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j), lse = ln sum_j p_j (nullable, fp32
- *   [T, Hq]), both over the unrounded values that the nibbles hold, in fp32 with p_j |v_j| rounded
- *   to fp16 before the product with v_j, out rounded once (to its type's largest finite value).
- * A query that sees no key: out 0, lse -infinity. Keys in a page whose number is outside
- * [0, num_pages) are not seen. Rows of q outside every sequence are left as they were in out and
- * lse. max_q_len and max_kv_len bound the sequences of the call (they choose the split of the work);
+ *   [T, Hq]), both over the unrounded values (n - zero) scale that the cache holds. Sums are fp32;
+ *   p_j times the value row's scale is rounded to fp16 before its product with n - zero (scales
+ *   below 2^-60 count as 2^-60 in how p_j is scaled for that), bf16 queries are taken in fp16 under
+ *   a power of two that the queries of up to 128 (query, head) pairs share (what lies 2^27 below
+ *   their largest loses bits), and out is rounded once (to its type's largest finite value).
+ * A query that sees no key: out 0, lse -infinity. What a query does not see moves no bit of its
+ * result, whatever the cache holds there; a key or value row of NaN that it does see makes it NaN.
+ * Keys in a page whose number is outside [0, num_pages) are not seen. Rows of q outside every
+ * sequence are left as they were in out and lse. max_q_len and max_kv_len bound the sequences of the call (they choose the split of the work);
  * a kv_lens entry beyond max_kv_len or the table's width counts as that, a negative one as 0, and
- * queries of a sequence beyond max_q_len are left as they were. The new tokens' rows are written
- * before the call, on the same stream.
+ * queries of a sequence beyond max_q_len are left as they were. Sequences must not share rows of q.
+ * The new tokens' rows are written before the call, on the same stream. At most 2^30 keys a
+ * sequence, 2^36 in all (B max_kv_len), 65535 sequences and 2^27 query rows T Hq.
  *
  * workspace (256-byte aligned, w4a16_kv4_attention_workspace_size bytes) is caller-owned, its
  * first W4A16_KV4_COUNTER_BYTES zero at its first use; every call leaves them zero, so one workspace
  * serves any number of calls, of any sizes that fit, one after another. Calls (or replays of captured
  * graphs) that may overlap in time need workspaces of their own. Nothing is allocated. The
- * workspace's size does not depend on the lengths on the device, only on the arguments. */
+ * workspace's size does not depend on the lengths on the device, only on the arguments, and
+ * never shrinks with max_kv_len; fewer queries or sequences may need more (their keys are split
+ * further), so a workspace for several shapes is as large as the largest of their sizes. */
 #define W4A16_KV4_COUNTER_BYTES 65536
 W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv,
                                                     int32_t D, int32_t max_q_len,

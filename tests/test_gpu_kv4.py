@@ -426,6 +426,20 @@ def test_no_work():
                            torch.zeros((0, 1), dtype=torch.int32, device="cuda"), none).shape == (0, 4, 64)
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """(The C entry takes 32-bit sizes, and the upper bits of a Python integer would be dropped on the way.)"""
+    P = need_gpu()
+    b = Batch(P, [1], [20], 4, 2, 64, 16, F16)
+    for over in (dict(max_kv_len=2 ** 32 + 20), dict(window=2 ** 32 + 1), dict(cu_q=b.cu.cuda(), max_q_len=2 ** 32 + 1)):
+        with pytest.raises(P.InvalidArgument, match="32-bit"):
+            b.gpu(P, **over)
+    with pytest.raises(P.InvalidArgument, match="32-bit"):
+        P.kv4_attention_workspace(b.q.cuda(), b.cache, 1, 1, 2 ** 32 + 20)
+    k = torch.zeros((1, 2, 64), dtype=F16, device="cuda").as_strided((1, 2, 64), (2 ** 32, 64, 1))
+    with pytest.raises(P.InvalidArgument, match="32-bit"):
+        P.kv4_write(k, k, b.cache, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
 # ------------------------------------------------------------------ as a program uses them
 
 def test_steps_of_a_program():

@@ -606,6 +606,9 @@ def _kv4_cache_shape(cache: torch.Tensor):
     return pages, Hkv, blocks * 16, D, index
 
 
+_INT32_MAX = 2 ** 31 - 1   # (ctypes drops what lies above, silently)
+
+
 # (each check of a tensor is the one test that a good call pays; _require says what is wrong with a bad one)
 
 def _kv4_tensor(t, name: str, dtypes, index: int):
@@ -622,6 +625,8 @@ def _kv4_rows(t, name: str, dtypes, index: int, shape=None):
     st, sh, sd = t.stride()
     if sd != 1:
         raise InvalidArgument(f"{name} must be contiguous along its last dimension")
+    if st > _INT32_MAX or sh > _INT32_MAX or t.shape[0] > _INT32_MAX:
+        raise InvalidArgument(f"{name}: rows and strides are 32-bit ({t.shape[0]} rows at {st}, {sh})")
     return st, sh
 
 
@@ -684,10 +689,14 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
 
 def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int, max_q_len: int,
                             max_kv_len: int) -> torch.Tensor:
-    """A workspace for kv4_attention calls with queries of q's shape: enough for any batch within
-    these bounds. Calls that may overlap in time need one each."""
+    """A workspace for kv4_attention calls of num_seqs sequences with queries of q's shape, at this
+    max_q_len and this max_kv_len or a smaller one. A call of another shape may need more, a smaller
+    one too: a workspace for several is as large as the largest of theirs. Calls that may overlap in
+    time need one each."""
     _, Hkv, _, D, _ = _kv4_cache_shape(cache)
     T, Hq = q.shape[:2]
+    if max(T, num_seqs, max_q_len, max_kv_len) > _INT32_MAX:
+        raise InvalidArgument(f"sizes are 32-bit ({T}, {num_seqs}, {max_q_len}, {max_kv_len})")
     need = lib().w4a16_kv4_attention_workspace_size(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
     if need == 0:
         check(ERR_INVALID_ARG)
@@ -729,6 +738,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         max_q_len = 1 if cu_q is None else max(1, T)
     if max_kv_len is None:
         max_kv_len = per * page
+    if max_q_len > _INT32_MAX or max_kv_len > _INT32_MAX or window > _INT32_MAX:
+        raise InvalidArgument(f"max_q_len, max_kv_len and window are 32-bit ({max_q_len}, {max_kv_len}, {window})")
     if out is None:
         out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
     ost, osh = _kv4_rows(out, "out", (q.dtype,), dev, shape)

@@ -54,7 +54,7 @@ struct Kv4AttnParams {
     // from the shape
     int G, slot_cols;
     int tiles, splits, chunk, pair_tiles;        // kv4_many.hip
-    int places, budget, whole, join_apart;       // kv4_few.hip
+    int places, budget, whole, join_apart, join_parts;   // kv4_few.hip
 };
 constexpr size_t KV4_MAX_COUNTERS = 16384;
 struct Kv4AttnShape {

@@ -22,7 +22,11 @@ constexpr int KV4_MAX_KEYS = 1 << 30;   // of a sequence: positions a few steps 
 constexpr int64_t KV4_MAX_ALL_KEYS = 1ll << 36;   // of all sequences: their steps of 32 are summed in 32 bits
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
-constexpr int64_t KV4_JOIN_BYTES = 40 << 10;   // partial results of a sequence and head that its last workgroup joins itself
+// Up to this much a sequence's and head's last workgroup joins itself; more is a kernel's, which costs its launch
+// but waits for no counter. 32 queries' heads of 4096 keys, in us (itself, kernel): D = 128, 16 chunks 31.1, 20.1;
+// 8 of 128 KB 28.3, 26.5; 5 of 84 KB 32.6, 33.1. 8 heads: 16 chunks 22.6, 19.1; 10 chunks 21.4, 23.3; 4 35.2, 38.4.
+constexpr int KV4_JOIN_CHUNKS = 12;
+constexpr int64_t KV4_JOIN_BYTES = 96 << 10;
 
 static int check_elem(int elem) {
     if (elem != 0 && elem != W4A16_BF16) return fail(W4A16_ERR_INVALID_ARG, "unknown element type %d", elem);
@@ -105,7 +109,7 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         s.splits = std::max(1, (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk));
         s.pair_tiles = items * s.splits <= at_once;
         s.slot_cols = wg_cols;
-        if (s.splits > 1) slots = (size_t)items * s.splits;
+        if (want > 1) slots = (size_t)items * want;   // (splits or more: enough for a smaller max_kv, too)
     } else {
         // chunks of a head and tile: what runs at once, or several rounds of it; B sequences have one each at least,
         // and a remainder
@@ -116,9 +120,9 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
         s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
         if (!s.whole) slots = (size_t)tiles * Hkv * s.places;
-        // one workgroup reads partial results at some 32 KB a microsecond; the chunks of a sequence, in a batch of like ones
+        // the chunks of a sequence, in a batch of like ones
         const int64_t chunks = std::min<int64_t>(s.budget / std::max(B, 1), ((int64_t)max_kv + 127) / 128);
-        s.join_apart = !s.whole && C * D * 4 * chunks > KV4_JOIN_BYTES;
+        s.join_apart = !s.whole && (chunks > KV4_JOIN_CHUNKS || C * D * 4 * chunks >= KV4_JOIN_BYTES);
     }
     s.partial_bytes = slots * s.slot_cols * (D + 2) * sizeof(float);
     return s;
@@ -225,6 +229,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.G = Hq / Hkv; p.slot_cols = s.slot_cols;
     p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
     p.places = s.places; p.budget = s.budget; p.whole = s.whole; p.join_apart = s.join_apart;
+    p.join_parts = (int)((std::min<int64_t>((int64_t)p.max_q * p.G, 32 * s.nt) * (D / 4) + 63) / 64);
     (void)hipGetLastError();
     const bool bf16 = elem == W4A16_BF16;
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -352,19 +352,19 @@ template <typename E, int D, int NT>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnParams p) {
     __shared__ float4_t vals[256];
     __shared__ float ml[256][2];
-    constexpr int COLS = 32 * NT, PARTS = COLS * (D / 4) / 64;
+    constexpr int COLS = 32 * NT;
     Kv4Item w;
-    const int tile = blockIdx.z / PARTS;
+    const int tile = p.tiles == 1 ? 0 : blockIdx.z / p.join_parts;
     if (!few_item<COLS>(p, tile, blockIdx.y, true, w) || w.chunks == 1) return;
     const Kv4Sink<E, D> sink(p, w);
-    const int e = (blockIdx.z - tile * PARTS) * 64 + (threadIdx.x & 63);
+    const int e = (blockIdx.z - tile * p.join_parts) * 64 + (threadIdx.x & 63);
     sink.join_quads(e, threadIdx.x >> 6, 4, 64, e < w.cols * (D / 4), vals, ml);
 }
 
 template <typename E, int D, int NT>
 static void run(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
     kv4_few_kernel<E, D, NT><<<dim3(p.Hkv, s.tiles, s.places), 256, 0, st>>>(p);
-    if (p.join_apart) kv4_join_kernel<E, D, NT><<<dim3(p.Hkv, p.B, s.tiles * 32 * NT * (D / 4) / 64), 256, 0, st>>>(p);
+    if (p.join_apart) kv4_join_kernel<E, D, NT><<<dim3(p.Hkv, p.B, s.tiles * p.join_parts), 256, 0, st>>>(p);
 }
 template <typename E, int D>
 static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {

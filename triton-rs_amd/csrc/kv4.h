@@ -54,7 +54,7 @@ struct Kv4AttnParams {
     // from the shape
     int G, slot_cols;
     int tiles, splits, chunk, pair_tiles;        // kv4_many.hip
-    int places, budget, whole, join_apart, join_parts;   // kv4_few.hip
+    int places, budget, at_once, whole, join_apart, join_parts;   // kv4_few.hip
 };
 constexpr size_t KV4_MAX_COUNTERS = 16384;
 struct Kv4AttnShape {
@@ -66,9 +66,9 @@ struct Kv4AttnShape {
     // columns by turns
     int groups, splits, chunk;
     bool pair_tiles;
-    // few: chunks of all sequences of a head, at most, and about how many are wanted; whole: one a sequence;
+    // few: chunks of all sequences of a head, at most, about how many are wanted, and how many run at once; whole: one a sequence;
     // join_apart: chunks are joined by a kernel of their own
-    int places, budget;
+    int places, budget, at_once;
     bool whole, join_apart;
     size_t partial_bytes;
 };

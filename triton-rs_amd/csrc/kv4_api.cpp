@@ -117,6 +117,7 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
         s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= KV4_WHOLE_KEYS;
         s.budget = (int)std::max<int64_t>(2 * (int64_t)B, rounds * at_once);
+        s.at_once = (int)at_once;
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
         s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
         if (!s.whole) slots = (size_t)tiles * Hkv * s.places;
@@ -228,7 +229,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
     p.G = Hq / Hkv; p.slot_cols = s.slot_cols;
     p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
-    p.places = s.places; p.budget = s.budget; p.whole = s.whole; p.join_apart = s.join_apart;
+    p.places = s.places; p.budget = s.budget; p.at_once = s.at_once; p.whole = s.whole; p.join_apart = s.join_apart;
     p.join_parts = (int)((std::min<int64_t>((int64_t)p.max_q * p.G, 32 * s.nt) * (D / 4) + 63) / 64);
     (void)hipGetLastError();
     const bool bf16 = elem == W4A16_BF16;

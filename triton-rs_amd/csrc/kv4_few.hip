@@ -64,71 +64,106 @@ __device__ __forceinline__ void take(uint32_t (&dst)[D / 32], const unsigned cha
     }
 }
 
-// inclusive sums over the lanes of a wave
-__device__ __forceinline__ int wave_sums(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // one lane up the row, two, four, eight
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last of a row to the next
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // the last of the lower half to the upper
+// over the lanes of a wave: inclusive f-sums (f(0, v) = v)
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));   // one lane up the row, two, four, eight
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));   // the last of a row to the next
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // the last of the lower half to the upper
     return v;
 }
+__device__ __forceinline__ int wave_sums(int v) { return wave_scan(v, [](int a, int b) { return a + b; }); }
+__device__ __forceinline__ unsigned wave_sum(int v) { return (unsigned)__builtin_amdgcn_readlane(wave_sums(v), 63); }
+__device__ __forceinline__ int wave_max(int v) { return __builtin_amdgcn_readlane(wave_scan(v, [](int a, int b) { return max(a, b); }), 63); }
 
-// Chunks of `steps` steps of keys in chunks of c 128 (4 c steps). Up to 768 keys stay whole: a chunk more costs some 3 us
-// (its partial results' way to the last one and back), 128 keys 0.5.
+// Chunks of `steps` steps of keys in chunks of c 128 (4 c steps); -1: no columns here. Up to 768 keys stay whole: a chunk
+// more costs some 3 us (its partial results' way to the last one and back), 128 keys 0.5.
 __device__ __forceinline__ int few_chunks(int steps, int c) {
-    return steps <= max(KV4_WHOLE_KEYS / STEP, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
+    return steps < 0 ? 0 : steps <= max(KV4_WHOLE_KEYS / STEP, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
 }
 
 // The chunks of all sequences for one head and tile of columns stand in a row; workgroup u takes the u-th. Their
 // length is such that there are at most p.budget of them, whatever the lengths of the sequences: keys / budget or
-// keys / (budget - B / 2) where that is enough, else keys / (budget - B) (the budget is twice B or more). With by_seq,
-// sequence u's first chunk instead. A lane a sequence.
+// keys / (budget - B / 2) where that is enough, else keys / (budget - B) (the budget is twice B or more). Sequences stay
+// whole where that is estimated to take no longer. With by_seq, sequence u's first chunk instead. A lane a sequence.
 template <int WG_COLS>
 __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w) {
     w.h = blockIdx.x;
+    int lo = 0, hi = 0;
     if (p.whole) {   // sequence u, in one chunk
-        int lo, hi;
         w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
         w.take(0, 1, 0, lo, hi);
         return w.cols > 0;
     }
     const int lane = threadIdx.x & 63;
     Kv4Item mine;
-    int lo = 0, hi = 0, steps = 0;
-    auto look = [&](int base) {   // this lane's sequence of 64 from base on; whether it has columns here
-        const int b = base + lane;
-        steps = 0;
-        if (b >= p.B) return false;
-        mine.sequence<WG_COLS, STEP>(p, b, tile * WG_COLS, lo, hi);
-        steps = (hi - lo + STEP - 1) / STEP;
-        return mine.cols > 0;
+    auto look = [&](int base) {   // steps of this lane's sequence of 64 from base on, -1 without columns
+        mine.sequence<WG_COLS, STEP>(p, min(base + lane, p.B - 1), tile * WG_COLS, lo, hi);
+        return base + lane < p.B && mine.cols > 0 ? (hi - lo + STEP - 1) / STEP : -1;
     };
-    bool has = look(0);
-    // sum over all sequences of f(); the first 64 stay in registers
-    auto all = [&](auto f) {
-        unsigned sum = 0;
-        for (int base = 0; base < p.B; base += 64) {
-            if (p.B > 64) has = look(base);
-            sum += (unsigned)__builtin_amdgcn_readlane(wave_sums(has ? f() : 0), 63);
+    // the first 256 sequences' steps stay in registers, their loads in flight together
+    constexpr int HELD = 4;
+    int held[HELD];
+    if (p.B > 64) {
+#pragma unroll
+        for (int g = HELD - 1; g > 0; --g) held[g] = look(64 * g);
+    }
+    held[0] = look(0);
+    auto each = [&](auto f) {   // f(base, steps) until it says so
+        if (f(0, held[0])) return;
+        if (p.B > 64) {
+#pragma unroll
+            for (int g = 1; g < HELD; ++g)
+                if (f(64 * g, held[g])) return;
+            for (int base = 64 * HELD; base < p.B; base += 64)
+                if (f(base, look(base))) return;
         }
-        return sum;
     };
-    const unsigned sum = all([&] { return steps; });
+    unsigned sum = 0;
+    int most = 0;
+    each([&](int, int steps) {
+        sum += wave_sum(max(steps, 0));
+        most = max(most, wave_max(max(steps, 0)));
+        return false;
+    });
     int c = 1;   // in 128 keys: with no remainders, half a chunk a sequence, one a sequence
+    unsigned n = p.budget;
     for (int rest = 0; rest <= 4; rest += 2) {
         const unsigned room = 4 * p.budget - rest * p.B;
         c = (int)max(1u, (sum + room - 1) / room);
-        if (rest == 4 || all([&] { return few_chunks(steps, c); }) <= (unsigned)p.budget) break;
+        if (rest == 4) break;
+        unsigned total = 0;
+        each([&](int, int steps) {
+            total += wave_sum(few_chunks(steps, c));
+            return false;
+        });
+        if (total <= (unsigned)p.budget) {
+            n = total;
+            break;
+        }
     }
-    for (int base = 0, before = 0; base < p.B; base += 64) {
-        if (p.B > 64) has = look(base);
-        const int n = has ? few_chunks(steps, c) : 0, upto = wave_sums(n);
-        const bool hit = by_seq ? base + lane == u && has : before + upto - n <= u && u < before + upto;
+    // In steps of a full device (0.85 us at D = 128): a round of workgroups costs 6 besides its steps, a step of one
+    // workgroup alone 0.45, joining 7. Whole and in two, 8 heads of D = 128: 128 sequences of 1000 keys 35, 49 us, 256
+    // of 900 60, 103; 48 of 4096 56, 54.
+    auto cost = [&](unsigned chunks, int steps) {
+        const float rounds = (float)((chunks + p.at_once - 1) / p.at_once);
+        return 6.f * rounds + fmaxf(0.45f * rounds * (float)steps, (float)sum / (float)p.at_once);
+    };
+    if (__builtin_amdgcn_readfirstlane(cost(p.B, most) <= cost(n, min(4 * c, most)) + 7.f)) c = max(c, (most + 3) / 4);
+
+    int before = 0;
+    bool found = false;
+    each([&](int base, int steps) {
+        const int here = few_chunks(steps, c), upto = wave_sums(here);
+        const bool hit = by_seq ? base + lane == u && here > 0 : before + upto - here <= u && u < before + upto;
         const uint64_t who = __ballot(hit);
         if (who) {
-            const int l = __builtin_ctzll(who);
+            const int l = __builtin_ctzll(who), at = before + __builtin_amdgcn_readlane(upto - here, l);   // its first chunk's number
+            const int chunks = __builtin_amdgcn_readlane(here, l);
+            if (p.B > 64) look(base);
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             w.b = base + l;
             w.q0 = of(mine.q0);
@@ -137,16 +172,15 @@ __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u
             w.first = of(mine.first);
             w.c0 = tile * WG_COLS;
             w.cols = of(mine.cols);
-            const int at = before + of(upto - n);   // its first chunk's number
             w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
             w.slot = ((size_t)tile * p.Hkv + w.h) * p.places + at;
-            w.take(by_seq ? 0 : u - at, of(n), 128 * c, of(lo), of(hi));
-            return true;
+            w.take(by_seq ? 0 : u - at, chunks, 128 * c, of(lo), of(hi));
+            found = true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
-        if (!by_seq && before > u) return false;
-    }
-    return false;
+        return found || (!by_seq && before > u);
+    });
+    return found;
 }
 
 template <typename E, int D, int NT>

@@ -158,7 +158,7 @@ def test_workspace_covers_every_split():
             # the rule of the kernel: chunks of c 128 keys, at most `places` of them for any lengths
             if not whole and B <= 64:
                 at_once = max(1, 256 * {(64, 1): 4, (128, 1): 4, (192, 1): 3, (256, 1): 2, (64, 2): 3, (128, 2): 2}[D, out[1]] // (Hkv * tiles))
-                budget = max(2 * B, -(-2 * B // at_once) * at_once)
+                budget = max(2 * B, min(128 * B, -(-2 * B // at_once) * at_once))
                 for _ in range(4):
                     steps = [-(-int(x) // 32) for x in rng.randint(0, mkv + 1, B)]
                     chunks = lambda c: sum(1 if s <= max(24, 4 * c) else -(-s // (4 * c)) for s in steps)

@@ -116,7 +116,8 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         const int64_t at_once = std::max<int64_t>(1, slots_of_cu * kv4_few_per_cu(D, s.nt) / (Hkv * tiles));
         const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
         s.whole = items > (int64_t)KV4_MAX_COUNTERS || max_kv <= KV4_WHOLE_KEYS;
-        s.budget = (int)std::max<int64_t>(2 * (int64_t)B, rounds * at_once);
+        // up to 128 of a sequence, as many as one join takes in its time (131072 keys of one head: 1024 chunks 47.6 us)
+        s.budget = (int)std::max<int64_t>(2 * (int64_t)B, std::min<int64_t>(rounds * at_once, 128 * (int64_t)B));
         s.at_once = (int)at_once;
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
         s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);

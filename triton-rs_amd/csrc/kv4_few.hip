@@ -85,63 +85,20 @@ __device__ __forceinline__ int few_chunks(int steps, int c) {
     return steps < 0 ? 0 : steps <= max(KV4_WHOLE_KEYS / STEP, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
 }
 
-// The chunks of all sequences for one head and tile of columns stand in a row; workgroup u takes the u-th. Their
-// length is such that there are at most p.budget of them, whatever the lengths of the sequences: keys / budget or
-// keys / (budget - B / 2) where that is enough, else keys / (budget - B) (the budget is twice B or more). Sequences stay
-// whole where that is estimated to take no longer. With by_seq, sequence u's first chunk instead. A lane a sequence.
-template <int WG_COLS>
-__device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w) {
-    w.h = blockIdx.x;
-    int lo = 0, hi = 0;
-    if (p.whole) {   // sequence u, in one chunk
-        w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
-        w.take(0, 1, 0, lo, hi);
-        return w.cols > 0;
-    }
-    const int lane = threadIdx.x & 63;
-    Kv4Item mine;
-    auto look = [&](int base) {   // steps of this lane's sequence of 64 from base on, -1 without columns
-        mine.sequence<WG_COLS, STEP>(p, min(base + lane, p.B - 1), tile * WG_COLS, lo, hi);
-        return base + lane < p.B && mine.cols > 0 ? (hi - lo + STEP - 1) / STEP : -1;
-    };
-    // the first 256 sequences' steps stay in registers, their loads in flight together
-    constexpr int HELD = 4;
-    int held[HELD];
-    if (p.B > 64) {
-#pragma unroll
-        for (int g = HELD - 1; g > 0; --g) held[g] = look(64 * g);
-    }
-    held[0] = look(0);
-    auto each = [&](auto f) {   // f(base, steps) until it says so
-        if (f(0, held[0])) return;
-        if (p.B > 64) {
-#pragma unroll
-            for (int g = 1; g < HELD; ++g)
-                if (f(64 * g, held[g])) return;
-            for (int base = 64 * HELD; base < p.B; base += 64)
-                if (f(base, look(base))) return;
-        }
-    };
-    unsigned sum = 0;
-    int most = 0;
-    each([&](int, int steps) {
-        sum += wave_sum(max(steps, 0));
-        most = max(most, wave_max(max(steps, 0)));
-        return false;
-    });
-    int c = 1;   // in 128 keys: with no remainders, half a chunk a sequence, one a sequence
+// The length of chunks, in 128 keys, for sequences of `sum` steps together and `most` at most, total(c) their number:
+// at most p.budget of them, whatever the lengths. Keys / budget or keys / (budget - B / 2) where that is enough, else
+// keys / (budget - B) (the budget is twice B or more); or all sequences whole where that is estimated to take no longer.
+template <typename F>
+__device__ __forceinline__ int few_length(const Kv4AttnParams& p, unsigned sum, int most, F total) {
+    int c = 1;
     unsigned n = p.budget;
-    for (int rest = 0; rest <= 4; rest += 2) {
+    for (int rest = 0; rest <= 4; rest += 2) {   // no remainders, half a chunk a sequence, one a sequence
         const unsigned room = 4 * p.budget - rest * p.B;
         c = (int)max(1u, (sum + room - 1) / room);
         if (rest == 4) break;
-        unsigned total = 0;
-        each([&](int, int steps) {
-            total += wave_sum(few_chunks(steps, c));
-            return false;
-        });
-        if (total <= (unsigned)p.budget) {
-            n = total;
+        const unsigned t = total(c);
+        if (t <= (unsigned)p.budget) {
+            n = t;
             break;
         }
     }
@@ -153,34 +110,113 @@ __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u
         return 6.f * rounds + fmaxf(0.45f * rounds * (float)steps, (float)sum / (float)p.at_once);
     };
     if (__builtin_amdgcn_readfirstlane(cost(p.B, most) <= cost(n, min(4 * c, most)) + 7.f)) c = max(c, (most + 3) / 4);
+    return c;
+}
 
-    int before = 0;
-    bool found = false;
-    each([&](int base, int steps) {
+// What the waves of a workgroup tell each other of more than 64 sequences.
+struct FewFind {
+    unsigned total[4][4];   // per pass and wave
+    int most[4];
+    int hit[3];             // sequence (-1: none), its first chunk's number, its chunks
+};
+
+// The chunks of all sequences for one head and tile of columns stand in a row; workgroup u of 256 threads takes the
+// u-th. With by_seq, sequence u's first chunk instead. A lane a sequence, up to 64; a thread several, beyond (their
+// order in the row is that of the threads).
+template <int WG_COLS>
+__device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w, FewFind& find) {
+    w.h = blockIdx.x;
+    int lo = 0, hi = 0;
+    if (p.whole) {   // sequence u, in one chunk
+        w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
+        w.take(0, 1, 0, lo, hi);
+        return w.cols > 0;
+    }
+    Kv4Item mine;
+    auto look = [&](int b) {   // steps of sequence b, -1 without columns
+        mine.sequence<WG_COLS, STEP>(p, min(b, p.B - 1), tile * WG_COLS, lo, hi);
+        return b < p.B && mine.cols > 0 ? (hi - lo + STEP - 1) / STEP : -1;
+    };
+    int at, chunks, c;
+    if (p.B <= 64) {
+        const int lane = threadIdx.x & 63, steps = look(lane);
+        c = few_length(p, wave_sum(max(steps, 0)), wave_max(max(steps, 0)), [&](int c) { return wave_sum(few_chunks(steps, c)); });
         const int here = few_chunks(steps, c), upto = wave_sums(here);
-        const bool hit = by_seq ? base + lane == u && here > 0 : before + upto - here <= u && u < before + upto;
-        const uint64_t who = __ballot(hit);
-        if (who) {
-            const int l = __builtin_ctzll(who), at = before + __builtin_amdgcn_readlane(upto - here, l);   // its first chunk's number
-            const int chunks = __builtin_amdgcn_readlane(here, l);
-            if (p.B > 64) look(base);
-            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            w.b = base + l;
-            w.q0 = of(mine.q0);
-            w.n = of(mine.n);
-            w.len = of(mine.len);
-            w.first = of(mine.first);
-            w.c0 = tile * WG_COLS;
-            w.cols = of(mine.cols);
-            w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
-            w.slot = ((size_t)tile * p.Hkv + w.h) * p.places + at;
-            w.take(by_seq ? 0 : u - at, chunks, 128 * c, of(lo), of(hi));
-            found = true;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-        return found || (!by_seq && before > u);
-    });
-    return found;
+        const uint64_t who = __ballot(by_seq ? lane == u && here > 0 : upto - here <= u && u < upto);
+        if (!who) return false;
+        const int l = __builtin_ctzll(who);
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+        at = of(upto - here);
+        chunks = of(here);
+        w.b = l;
+        w.q0 = of(mine.q0);
+        w.n = of(mine.n);
+        w.len = of(mine.len);
+        w.first = of(mine.first);
+        w.c0 = tile * WG_COLS;
+        w.cols = of(mine.cols);
+        lo = of(lo);
+        hi = of(hi);
+    } else {
+        const int wave = threadIdx.x >> 6;
+        constexpr int HELD = 4;   // of a thread's sequences, in registers, their loads in flight together
+        int held[HELD];
+#pragma unroll
+        for (int g = 0; g < HELD; ++g) held[g] = look(256 * g + threadIdx.x);
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int g = 0; g < HELD; ++g) f(256 * g + (int)threadIdx.x, held[g]);
+            for (int b = 256 * HELD + threadIdx.x; b < p.B; b += 256) f(b, look(b));
+        };
+        auto all = [&](int pass, unsigned v) {   // sum over the workgroup
+            v = wave_sum((int)v);
+            if ((threadIdx.x & 63) == 0) find.total[pass][wave] = v;
+            __syncthreads();
+            return find.total[pass][0] + find.total[pass][1] + find.total[pass][2] + find.total[pass][3];
+        };
+        unsigned mine_sum = 0;
+        int mine_most = 0;
+        each([&](int, int steps) {
+            mine_sum += max(steps, 0);
+            mine_most = max(mine_most, steps);
+        });
+        auto mine_chunks = [&](int c) {
+            unsigned n = 0;
+            each([&](int, int steps) { n += few_chunks(steps, c); });
+            return n;
+        };
+        mine_most = wave_max(mine_most);
+        if ((threadIdx.x & 63) == 0) find.most[wave] = mine_most;
+        if (threadIdx.x == 0) find.hit[0] = -1;
+        const unsigned sum = all(0, mine_sum);
+        const int most = max(max(find.most[0], find.most[1]), max(find.most[2], find.most[3]));
+        int pass = 0;
+        c = __builtin_amdgcn_readfirstlane(few_length(p, sum, most, [&](int c) { return all(++pass, mine_chunks(c)); }));
+        const unsigned n = mine_chunks(c), upto = (unsigned)wave_sums((int)n);
+        all(3, n);
+        unsigned first = upto - n;   // number of this thread's first chunk
+        for (int x = 0; x < wave; ++x) first += find.total[3][x];
+        if (by_seq ? (u & 255) == (int)threadIdx.x : first <= (unsigned)u && (unsigned)u < first + n)
+            each([&](int b, int steps) {
+                const unsigned here = few_chunks(steps, c);
+                if (by_seq ? b == u && here > 0 : first <= (unsigned)u && (unsigned)u < first + here) {
+                    find.hit[0] = b;
+                    find.hit[1] = (int)first;
+                    find.hit[2] = (int)here;
+                }
+                first += here;
+            });
+        __syncthreads();
+        const int b = __builtin_amdgcn_readfirstlane(find.hit[0]);
+        if (b < 0) return false;
+        at = __builtin_amdgcn_readfirstlane(find.hit[1]);
+        chunks = __builtin_amdgcn_readfirstlane(find.hit[2]);
+        w.sequence<WG_COLS, STEP>(p, b, tile * WG_COLS, lo, hi);
+    }
+    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
+    w.slot = ((size_t)tile * p.Hkv + w.h) * p.places + at;
+    w.take(by_seq ? 0 : u - at, chunks, 128 * c, lo, hi);
+    return true;
 }
 
 template <typename E, int D, int NT>
@@ -191,8 +227,9 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
     __shared__ __align__(16) unsigned char ring[4][S::RING];
     __shared__ float ml[4][COLS][2];
     __shared__ int last;
+    __shared__ FewFind find;
     Kv4Item w;
-    if (!few_item<2 * COLS>(p, blockIdx.y, blockIdx.z, false, w)) return;
+    if (!few_item<2 * COLS>(p, blockIdx.y, blockIdx.z, false, w, find)) return;
     // one group of columns, its keys over four waves, or two over two
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kshift = w.cols <= COLS ? 2 : 1, kspl = 1 << kshift, g0 = wave & ~(kspl - 1);
@@ -386,10 +423,11 @@ template <typename E, int D, int NT>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnParams p) {
     __shared__ float4_t vals[256];
     __shared__ float ml[256][2];
+    __shared__ FewFind find;
     constexpr int COLS = 32 * NT;
     Kv4Item w;
     const int tile = p.tiles == 1 ? 0 : blockIdx.z / p.join_parts;
-    if (!few_item<COLS>(p, tile, blockIdx.y, true, w) || w.chunks == 1) return;
+    if (!few_item<COLS>(p, tile, blockIdx.y, true, w, find) || w.chunks == 1) return;
     const Kv4Sink<E, D> sink(p, w);
     const int e = (blockIdx.z - tile * p.join_parts) * 64 + (threadIdx.x & 63);
     sink.join_quads(e, threadIdx.x >> 6, 4, 64, e < w.cols * (D / 4), vals, ml);

@@ -105,6 +105,23 @@ extern "C" {
                                       total: i32) -> i32;
     fn fused_silu_mul_interleaved_f32(stream: *mut c_void, gate_up: u64, out: u64, inter: i32,
                                       total: i32) -> i32;
+    fn w4a16_kv4_cache_bytes(num_pages: i32, hkv: i32, d: i32, page_size: i32) -> usize;
+    fn w4a16_kv4_write(stream: *mut c_void, elem: i32, k: u64, v: u64, k_stride_t: i32,
+                       k_stride_h: i32, v_stride_t: i32, v_stride_h: i32, slots: u64, cache: u64,
+                       num_pages: i32, t: i32, hkv: i32, d: i32, page_size: i32) -> i32;
+    fn w4a16_kv4_read(stream: *mut c_void, elem: i32, cache: u64, slots: u64, k_out: u64,
+                      v_out: u64, k_stride_t: i32, k_stride_h: i32, v_stride_t: i32,
+                      v_stride_h: i32, num_pages: i32, t: i32, hkv: i32, d: i32,
+                      page_size: i32) -> i32;
+    fn w4a16_kv4_attention_workspace_size(t: i32, b: i32, hq: i32, hkv: i32, d: i32,
+                                          max_q_len: i32, max_kv_len: i32) -> usize;
+    fn w4a16_kv4_attention(stream: *mut c_void, elem: i32, q: u64, q_stride_t: i32,
+                           q_stride_h: i32, cache: u64, page_table: u64, kv_lens: u64, cu_q: u64,
+                           out: u64, out_stride_t: i32, out_stride_h: i32, lse: u64, t: i32,
+                           b: i32, hq: i32, hkv: i32, d: i32, num_pages: i32, page_size: i32,
+                           pages_per_seq: i32, max_q_len: i32, max_kv_len: i32, scale: f32,
+                           causal: i32, window: i32, workspace: u64,
+                           workspace_bytes: usize) -> i32;
 }
 
 /// The calling thread's last libw4a16 message, mapped onto the reference's error type:
@@ -419,6 +436,117 @@ pub fn silu_mul_interleaved_f32(stream: &HipStream, gate_up: u64, out: u64, inte
                                 total: i32) -> Result<(), RuntimeError> {
     // SAFETY: as above.
     check(unsafe { fused_silu_mul_interleaved_f32(stream.0, gate_up, out, inter, total) })
+}
+
+/// A 4-bit key/value cache and the element type of its rows.
+#[derive(Debug, Clone, Copy)]
+pub struct Kv4Cache {
+    /// Device buffer of `kv4_cache_bytes` bytes.
+    pub data: u64,
+    /// Pages.
+    pub num_pages: i32,
+    /// Key/value heads.
+    pub kv_heads: i32,
+    /// Dimensions of a head (64, 128, 192 or 256).
+    pub head_dim: i32,
+    /// Tokens of a page (a power of two, 16..1024).
+    pub page_size: i32,
+    /// Rows are bfloat16 (else fp16).
+    pub bf16: bool,
+}
+
+/// Rows `[tokens, heads, head_dim]`: device pointer, token and head strides in elements.
+#[derive(Debug, Clone, Copy)]
+pub struct Kv4Rows {
+    /// Device pointer.
+    pub data: u64,
+    /// Elements from token to token.
+    pub stride_t: i32,
+    /// Elements from head to head.
+    pub stride_h: i32,
+}
+
+/// `W4A16_BF16`.
+const BF16: i32 = 0x100;
+
+/// Bytes of a cache (its `data` is not looked at); 0: not supported.
+pub fn kv4_cache_bytes(c: &Kv4Cache) -> usize {
+    // SAFETY: pure function of its arguments.
+    unsafe { w4a16_kv4_cache_bytes(c.num_pages, c.kv_heads, c.head_dim, c.page_size) }
+}
+
+/// Quantises rows `k`, `v` into the slots (`i32[tokens]` on the device) of the cache.
+pub fn kv4_write(stream: &HipStream, c: &Kv4Cache, k: Kv4Rows, v: Kv4Rows, slots: u64,
+                 tokens: i32) -> Result<(), RuntimeError> {
+    // SAFETY: device pointers from hiprt_malloc; the library validates sizes and strides.
+    check(unsafe {
+        w4a16_kv4_write(stream.0, if c.bf16 { BF16 } else { 0 }, k.data, v.data, k.stride_t,
+                        k.stride_h, v.stride_t, v.stride_h, slots, c.data, c.num_pages, tokens,
+                        c.kv_heads, c.head_dim, c.page_size)
+    })
+}
+
+/// The rows that the slots hold, into `k_out` and `v_out`.
+pub fn kv4_read(stream: &HipStream, c: &Kv4Cache, slots: u64, k_out: Kv4Rows, v_out: Kv4Rows,
+                tokens: i32) -> Result<(), RuntimeError> {
+    // SAFETY: as above.
+    check(unsafe {
+        w4a16_kv4_read(stream.0, if c.bf16 { BF16 } else { 0 }, c.data, slots, k_out.data,
+                       v_out.data, k_out.stride_t, k_out.stride_h, v_out.stride_t, v_out.stride_h,
+                       c.num_pages, tokens, c.kv_heads, c.head_dim, c.page_size)
+    })
+}
+
+/// A batch of sequences for `kv4_attention`.
+#[derive(Debug, Clone, Copy)]
+pub struct Kv4Batch {
+    /// `i32[seqs, pages_per_seq]`.
+    pub page_table: u64,
+    /// `i32[seqs]`.
+    pub kv_lens: u64,
+    /// `i32[seqs + 1]`, or 0: one query a sequence.
+    pub cu_q: u64,
+    /// Query rows.
+    pub tokens: i32,
+    /// Sequences.
+    pub seqs: i32,
+    /// Query heads.
+    pub heads: i32,
+    /// Columns of the page table.
+    pub pages_per_seq: i32,
+    /// No sequence has more queries.
+    pub max_q_len: i32,
+    /// No sequence has more keys.
+    pub max_kv_len: i32,
+    /// Factor of q . k.
+    pub scale: f32,
+    /// A query sees no later token.
+    pub causal: bool,
+    /// And only this many up to its own (0: all).
+    pub window: i32,
+}
+
+/// Bytes of device workspace `kv4_attention` needs; its first 65536 are zero before the first call.
+pub fn kv4_attention_workspace_size(c: &Kv4Cache, b: &Kv4Batch) -> usize {
+    // SAFETY: pure function of its arguments.
+    unsafe {
+        w4a16_kv4_attention_workspace_size(b.tokens, b.seqs, b.heads, c.kv_heads, c.head_dim,
+                                           b.max_q_len, b.max_kv_len)
+    }
+}
+
+/// Attention of `q` over the cache into `out` (and `lse`, `f32[tokens, heads]`, unless 0).
+#[allow(clippy::too_many_arguments)]
+pub fn kv4_attention(stream: &HipStream, c: &Kv4Cache, b: &Kv4Batch, q: Kv4Rows, out: Kv4Rows,
+                     lse: u64, workspace: u64, workspace_bytes: usize) -> Result<(), RuntimeError> {
+    // SAFETY: as above; the workspace size is checked by the library.
+    check(unsafe {
+        w4a16_kv4_attention(stream.0, if c.bf16 { BF16 } else { 0 }, q.data, q.stride_t, q.stride_h,
+                            c.data, b.page_table, b.kv_lens, b.cu_q, out.data, out.stride_t,
+                            out.stride_h, lse, b.tokens, b.seqs, b.heads, c.kv_heads, c.head_dim,
+                            c.num_pages, c.page_size, b.pages_per_seq, b.max_q_len, b.max_kv_len,
+                            b.scale, b.causal as i32, b.window, workspace, workspace_bytes)
+    })
 }
 
 #[cfg(test)]

@@ -84,9 +84,11 @@ static int kv4_rows(bool write, void* stream, int elem, void* k, void* v, int32_
     return e == hipSuccess ? W4A16_OK : hip_fail(e, write ? "kv4 write launch" : "kv4 read launch");
 }
 
-// Which kernel, and how the keys are split. Few columns (up to 64) go to the kernel whose waves share them. The
-// keys are split as far as it takes to fill the places of workgroups that run at once, no further: each chunk
-// costs its partial results a round trip through memory.
+// Which kernel, and how the keys are split. Few columns (up to 64) go to the kernel whose waves share them: 8 sequences
+// of 8 queries, 8 heads of 4096 keys, D = 128, 64 columns, 37.5 us against 43.9 on the other, 96 columns 56.7 against
+// 45.5. Its waves take two tiles of 16 columns from 17 on (32 sequences, 24 columns: 46.9 us, one tile 65.0), where
+// registers allow (D <= 128). The keys are split as far as it takes to fill the places of workgroups that run at once,
+// no further: each chunk costs its partial results a round trip through memory.
 static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv) {
     Kv4AttnShape s{};
     const int64_t G = Hq / Hkv, C = (int64_t)(max_q < T ? max_q : T) * G, slots_of_cu = KV4_CUS;
@@ -98,10 +100,12 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
     s.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
     size_t slots = 0;
     if (s.many) {
-        // Up to two tiles a compute unit, the longest one sets the time: two groups of waves share its keys. Not where
-        // the tiles are of one length (a chunk behind a long context) and fill the device by themselves.
+        // Up to two tiles a compute unit, the longest one sets the time: two groups of waves share its keys (a prompt of
+        // 2048, 32 heads: 66 us, one group 75; 1344 tiles of 7 prompts: 58, one 45). Not where the tiles are of one
+        // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664).
         s.groups = D <= 128 && items <= 2 * KV4_CUS && !(items >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
         const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
+        // (chunks of 512 keys or more: 64 queries over 4096 keys, 32 heads of D = 128, 39.9 us; of 256 52.3, 1024 41.5)
         int64_t want = std::min((at_once + items - 1) / items, ((int64_t)max_kv + 511) / 512);
         if (items > (int64_t)KV4_MAX_COUNTERS) want = 1;
         want = std::max<int64_t>(1, want);

@@ -225,7 +225,7 @@ def attention_path(P, T, B, Hq, Hkv, D, max_q, max_kv):
     ([4, 9], [900, 1000], 10, 2, 192, 32, 0, ("few", 1, 18, 1)),
     ([1] * 130, [(37 * i) % 331 + 600 * (i == 7) for i in range(130)], 2, 1, 64, 16, 0, ("few", 1, 910, 0)),
     ([1] * 300, [(53 * i) % 200 + 1100 * (i % 97 == 5) for i in range(300)], 2, 1, 64, 16, 0, ("few", 1, 1024, 0)),
-    ([1] * 1100, [(29 * i) % 60 + 1000 * (i % 250 == 90) for i in range(1100)], 2, 1, 64, 16, 0, ("few", 1, 3072, 0)),
+    ([1] * 1100, [(29 * i) % 60 + 1000 * (i % 250 == 90) for i in range(1100)], 2, 2, 64, 16, 0, ("few", 1, 2560, 0)),
     # many: two groups of waves on a tile, one of them, keys in one chunk and in several
     ([300, 70], [300, 500], 2, 1, 128, 32, 0, ("many", 2, 1)),
     ([90], [2500], 4, 2, 64, 16, 0, ("many", 2, 5)),

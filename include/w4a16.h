@@ -362,7 +362,7 @@ W4A16_API int w4a16_fused_moe_prepared(void* stream, const void* x, const float*
  * `slot / page_size` is slot `slot`.
  *
  * A row x[0, D) is quantised over the range that it and 0 span: scale = (max - min) / 15 rounded
- * to fp32, then to the element type; zero = rint(-min / scale); n = clamp(rint(x / scale) + zero,
+ * to fp32, then to the element type; zero = min(rint(-min / scale), 15); n = clamp(rint(x / scale) + zero,
  * 0, 15), ties to even. A scale of 0 holds zeros; a row with an infinity or NaN is NaN throughout. */
 
 /* Bytes of a cache (0: not supported). A cache needs no initialisation. */
@@ -402,7 +402,7 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  * sequence are left as they were in out and lse. max_q_len and max_kv_len bound the sequences of the call (they choose the split of the work);
  * a kv_lens entry beyond max_kv_len or the table's width counts as that, a negative one as 0, and
  * queries of a sequence beyond max_q_len are left as they were. Sequences must not share rows of q.
- * The new tokens' rows are written before the call, on the same stream. At most 2^30 keys a
+ * out may be q itself, at its strides. The new tokens' rows are written before the call, on the same stream. At most 2^30 keys a
  * sequence, 2^36 in all (B max_kv_len), 65535 sequences and 2^27 query rows T Hq.
  *
  * workspace (256-byte aligned, w4a16_kv4_attention_workspace_size bytes) is caller-owned, its

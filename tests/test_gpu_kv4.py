@@ -309,6 +309,29 @@ def test_rows_that_are_not_finite(dtype, nq, lens):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("vscale", [2e4, 4e3])
+@pytest.mark.parametrize("nq,L,at", [(1, 90, 3), (1, 90, 88), (90, 600, 3), (90, 600, 555)])
+def test_value_rows_of_nan_at_no_weight(dtype, nq, L, at, vscale):
+    """A value row of NaN makes the queries NaN that see it, though its weight is e^-200 and less of the sum's
+    and the other values are large; where all queries see a step of keys, and where some do not. (At 2e4 some
+    of fp16's rows hold an infinity themselves.)"""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, dtype, vscale=vscale)
+    k = rows(torch.Generator().manual_seed(1), 1, 2, 64, dtype)
+    k[:] = -40.0
+    b.q = (b.q.float().abs() + 1).to(dtype)
+    v = torch.full_like(k, float("nan"))
+    P.kv4_write(k.cuda(), v.cuda(), b.cache, (b.table[0, at // 16:at // 16 + 1] * 16 + at % 16).cuda())
+    out, lse = b.gpu(P)
+    b.v[0][at] = np.nan
+    bad = np.isnan(b.v[0]).any(-1)                                      # [key, head]
+    want = np.stack([bad[:L - nq + 1 + i].any(0) for i in range(nq)]).repeat(2, 1)
+    assert (torch.isnan(out).cpu().numpy() == want[..., None]).all() and not torch.isnan(lse).any()
+    if vscale < 1e4:
+        assert (want == (np.arange(nq) + L - nq >= at)[:, None]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("nq,L,window", [(1, 90, 50), (5, 300, 0), (5, 300, 77), (150, 200, 0), (150, 400, 70)])
 def test_rows_that_a_query_does_not_see(dtype, nq, L, window):
     """What masked tokens hold moves no bit of a query's result: any bytes before the window and behind the
@@ -415,6 +438,17 @@ def test_strided_queries_and_outputs(nq):
     out = torch.zeros((Hq, 2 * nq, D), dtype=F16, device="cuda").transpose(0, 1)
     _, lse = b.gpu(P, q=qkv[:, :Hq], out=out)
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("nq,lens,D", [([1, 1], [1500, 40], 128), ([9, 2], [900, 1100], 256), ([200, 130], [300, 1500], 64)])
+def test_out_in_the_place_of_q(nq, lens, D):
+    """A program that keeps no second buffer: out is q, through one chunk and several, and either join."""
+    P = need_gpu()
+    b = Batch(P, nq, lens, 8, 2, D, 16, F16)
+    want, _ = b.gpu(P)
+    q = b.q.cuda()
+    got, _ = b.gpu(P, q=q, out=q)
+    assert got is q and torch.equal(got, want)
 
 
 def test_no_work():

@@ -87,6 +87,9 @@ __device__ __forceinline__ float kb_all(float v, F f) {
     return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float kb_sum(float v) { return kb_all(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ uint32_t kb_umax(uint32_t v) {
+    return __float_as_uint(kb_all(__uint_as_float(v), [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }));
+}
 __device__ __forceinline__ float kb_max(float v) { return kb_all(v, [](float a, float b) { return fmaxf(a, b); }); }
 
 // over the 16 lanes of a row: neighbours, pairs, halves mirrored, the row mirrored
@@ -103,8 +106,8 @@ __device__ __forceinline__ float row_min(float v) {
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
 
-// A scale of NaN (a row that held an infinity or NaN, n = z = 0) as the largest number: the weight of a column that
-// does not see the token is then 0, of one that does it is infinity, and its product with n - z NaN.
+// A scale of NaN (a row that held an infinity or NaN) as the largest number: the weight of a column that does not
+// see the token is then 0. For one that does see it, see value_room().
 __device__ __forceinline__ float seen_scale(float s) { return fminf(s, FLT_MAX); }
 
 // What a workgroup takes of sequence b, key/value head h: columns from c0 on, of keys [k0, k1) of this chunk.
@@ -159,7 +162,7 @@ struct Kv4Cols {
     float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
     float most[NT];        // the same, -infinity until a column has seen a key
     float room[NT];        // what logits less m may be: p_j s_j <= 2^KV4_WEIGHT_LOG2
-    float vtop[NT];        // a power of two above the largest value scale that a column has seen; 0 before it
+    float vtop[NT];        // a power of two above the largest value scale that a column has seen; 0 before it, NaN for good
     float vleast;          // the least of them of all columns
     float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
 
@@ -267,20 +270,27 @@ struct Kv4Cols {
         return Seen{lo[t] - at, min(hi[t], end) - at, bad};
     }
 
-    // Room for the value scales of a step, those that a column sees: what others see does not move its reference.
-    // vmax: the largest of them all, of this lane or more; of(t): of this lane's, the largest that columns t see.
-    template <typename F>
-    __device__ __forceinline__ void value_room(float vmax, F of) {
-        if (!__any(vmax > vleast)) return;   // rare after the first steps
+    // Room for the value scales vs of a step, those that a column sees: what others see does not move its reference.
+    // vmax: the largest of them all, of this lane or more, as bits (NaN beyond all numbers). A value row of NaN makes
+    // the columns NaN that see it, whatever its weight.
+    __device__ __forceinline__ void value_room(uint32_t vmax, const float (&vs)[2][4], int j, int end, int bad, int kb) {
+        if (!__any(vmax > __float_as_uint(vleast))) return;   // rare after the first steps
         vleast = INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float top = kb_max(of(t));
+            const Seen in = seen(t, j, end, bad, kb);
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = max(top, in(s, i) ? __float_as_uint(vs[s][i]) : 0u);
+            top = kb_umax(top);
             // 2 to 4 times the largest; value scales below 2^-60 share one
-            const int e = min(126, max(-60, (int)(__float_as_uint(top) >> 23) - 127 + 2));
-            const bool up = top > vtop[t];
+            const int e = min(126, max(-60, (int)(top >> 23) - 127 + 2));
+            const bool up = top > __float_as_uint(vtop[t]);
             float fresh = pow2(e), left = (float)(KV4_WEIGHT_LOG2 - e);
             asm("" : "+v"(fresh), "+v"(left));   // (selects, not a branch)
+            if (top >= __float_as_uint(FLT_MAX)) fresh = __builtin_nanf("");   // (no number is above it)
             vtop[t] = up ? fresh : vtop[t];
             room[t] = up ? left : room[t];
             most[t] = most[t] == -INFINITY ? most[t] : room[t];   // (the next logits raise m where that is too little)
@@ -349,6 +359,10 @@ struct Kv4Cols {
         for (int t = 0; t < NT; ++t) {
             l[t] = kb_sum(l[t]);
             if (most[t] == -INFINITY && l[t] == 0.f) m[t] = -FLT_MAX;
+            if (__any(vtop[t] != vtop[t])) {   // a value row of NaN was seen
+#pragma unroll
+                for (int x = 0; x < VT; ++x) o[t][x] += vtop[t] != vtop[t] ? vtop[t] : 0.f;
+            }
         }
     }
 };

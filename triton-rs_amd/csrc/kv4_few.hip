@@ -324,25 +324,17 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[t][s] = mfma16x16x32(f, a.qf[t][x], acc[t][s]);
             }
-        float ks[2][4], vs[2][4], vmax = 0.f;
+        float ks[2][4], vs[2][4];
+        uint32_t vmax = 0;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 ks[s][i] = param_scale<E>(kp[s][i]) * a.kscale;
                 vs[s][i] = param_scale<E>(vp[s][i]);
-                vmax = fmaxf(vmax, vs[s][i]);
+                vmax = max(vmax, __float_as_uint(vs[s][i]));
             }
-        a.value_room(vmax, [&](int t) {
-            if (whole) return vmax;
-            const auto in = a.seen(t, j, end, here, kb);
-            float top = 0.f;   // (fmaxf: NaN aside)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, in(s, i) ? vs[s][i] : 0.f);
-            return top;
-        });
+        a.value_room(vmax, vs, j, end, here, kb);
         if (!whole) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)

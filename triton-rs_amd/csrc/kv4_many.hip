@@ -20,8 +20,8 @@ struct ManyLds {
     static constexpr int KW = D / 32, VT = D / 16;
     half8_t k[4][KW][64];      // block, word of the quarter row, lane
     half8_t v[2][VT][64];      // pair of blocks, tile of the result, lane (first block's two pairs, second's)
-    float ks[64], vs[64];      // scales of the tokens, those of keys times kscale
-    float vtop[4];             // the largest of a block's value scales
+    float ks[64], vs[64];      // scales of the tokens, those of keys times kscale, those of values by seen_scale
+    uint32_t vtop[4];          // the largest of a block's value scales, as bits (NaN beyond all numbers)
     int live[4];               // tokens of a block that there are (0 or less: none)
 };
 
@@ -95,7 +95,10 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
     float4_t f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = param_scale<E>(t.vp[i]);
-    const float top = kb_max(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(f[i]));
+    top = kb_umax(top);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = seen_scale(f[i]);
     if (col == 0) *reinterpret_cast<float4_t*>(&s.vs[16 * wave + 4 * kb]) = f;
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
             for (int b = 0; b < 2; ++b) bad |= (s.live[2 * half + b] <= 0 ? 1 : 0) << b;
             bad = __builtin_amdgcn_readfirstlane(bad);
             const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad;
-            const float vmax = fmaxf(s.vtop[2 * half], s.vtop[2 * half + 1]);
+            const uint32_t vmax = max(s.vtop[2 * half], s.vtop[2 * half + 1]);
             // operands from LDS all at once, ahead of the products that take them: one wait instead of eight
             half8_t kf[2][C::KW], vf[C::VT];
 #pragma unroll
@@ -198,15 +201,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            a.value_room(vmax, [&](int n) {
-                const auto in = a.seen(n, jh, a.jhi, bad, kb);
-                float top = 0.f;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, (vs[b][i] < FLT_MAX && in(b, i)) ? vs[b][i] : 0.f);
-                return top;
-            });
+            a.value_room(vmax, vs, jh, a.jhi, bad, kb);
             float x[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, whole, jh, a.jhi, bad, kb);

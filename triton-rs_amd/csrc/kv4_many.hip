@@ -6,11 +6,11 @@
 // take them (16 bytes a lane, no bank conflicts), while the step before is computed from the other half
 // of the LDS: one barrier a step. The packed words come two steps ahead into registers.
 //
-// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, bf16, 666 us: 813 TFLOP/s, 69 % of a
-// large matrix product's 1185. The matrix cores are busy in 32 % of the cycles, the vector unit in 56 %;
+// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, bf16, 660 us: 820 TFLOP/s, 69 % of a
+// large matrix product's 1185. The matrix cores are busy in 32 % of the cycles, the vector unit in 52 %;
 // two waves a SIMD is what the results leave registers for, each a chain of products, softmax and products. Steps of 32 keys with a barrier each took 861 us, logits of one half beside the
-// weights of the other 754. A prompt of 2048 66 us: the last tile's 2048 keys one after another, halved
-// by a second group of waves. 7 prompts of up to 1500, 16 heads of D = 64, 47 us.
+// weights of the other 754. A prompt of 2048 64 us: the last tile's 2048 keys one after another, halved
+// by a second group of waves. 7 prompts of up to 1500, 16 heads of D = 64, 44 us.
 #include "kv4_attn_body.h"
 
 namespace w4a16 {

@@ -7,7 +7,7 @@
 // Bound by memory: 2 D bytes of a row against D / 2 + 4. A workgroup takes 16 tokens of one head, a
 // row 16 lanes of D / 16 dimensions each (a column of the value layout), so a wave's four rows write
 // 256 contiguous bytes of keys and of values where their slots are consecutive. Vector instructions are
-// kept to about 13 an element (writing; division, conversion and clamping one by one took twice as
+// kept to about 18 an element, addresses included (writing; division, conversion and clamping one by one took twice as
 // long as the memory): extremes as ordered 16-bit integers in pairs, and x / s rounded by two additions.
 // Measured, bf16, 8 heads of D = 128: 8192 tokens written in 12.1 us (3.5 TB/s), read back in 9.6 (4.4); 65536
 // read in 78 (4.4; a large copy reaches 4.8). A few rows take 3 us a kernel, 7 a call.

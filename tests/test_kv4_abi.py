@@ -152,7 +152,7 @@ def test_workspace_covers_every_split():
             assert out[2] == 1 or -(-C // 128) * B * Hkv <= 16384
         else:
             tiles = -(-C // (32 * out[1]))
-            whole = mkv <= 768 or tiles * B * Hkv > 16384
+            whole = mkv <= 512 or tiles * B * Hkv > 16384
             slots = 0 if whole else tiles * Hkv * out[2] * (-(-min(C, 32 * out[1]) // 16) * 16)
             assert out[2] >= B
             # the rule of the kernel: chunks of c 128 keys, at most `places` of them for any lengths
@@ -161,7 +161,7 @@ def test_workspace_covers_every_split():
                 budget = max(2 * B, min(128 * B, -(-2 * B // at_once) * at_once))
                 for _ in range(4):
                     steps = [-(-int(x) // 32) for x in rng.randint(0, mkv + 1, B)]
-                    chunks = lambda c: sum(1 if s <= max(24, 4 * c) else -(-s // (4 * c)) for s in steps)
+                    chunks = lambda c: sum(1 if s <= max(16, 4 * c) else -(-s // (4 * c)) for s in steps)
                     for rest in (0, 2, 4):
                         c = max(1, -(-sum(steps) // (4 * budget - rest * B)))
                         if rest == 4 or chunks(c) <= budget:

@@ -399,11 +399,12 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  * A query that sees no key: out 0, lse -infinity. What a query does not see moves no bit of its
  * result, whatever the cache holds there; a key or value row of NaN that it does see makes it NaN.
  * Keys in a page whose number is outside [0, num_pages) are not seen. Rows of q outside every
- * sequence are left as they were in out and lse. max_q_len and max_kv_len bound the sequences of the call (they choose the split of the work);
- * a kv_lens entry beyond max_kv_len or the table's width counts as that, a negative one as 0, and
- * queries of a sequence beyond max_q_len are left as they were. Sequences must not share rows of q.
- * out may be q itself, at its strides. The new tokens' rows are written before the call, on the same stream. At most 2^30 keys a
- * sequence, 2^36 in all (B max_kv_len), 65535 sequences and 2^27 query rows T Hq.
+ * sequence are left as they were in out and lse. max_q_len and max_kv_len bound the sequences of
+ * the call (they choose the kernels and the split of the work); a kv_lens entry beyond max_kv_len
+ * or the table's width counts as that, a negative one as 0, and queries of a sequence beyond
+ * max_q_len are left as they were. Sequences must not share rows of q. out may be q itself, at its
+ * strides. The new tokens' rows are written before the call, on the same stream. At most 2^30 keys
+ * a sequence, 2^36 in all (B max_kv_len), 65535 sequences and 2^27 query rows T Hq.
  *
  * workspace (256-byte aligned, w4a16_kv4_attention_workspace_size bytes) is caller-owned, its
  * first W4A16_KV4_COUNTER_BYTES zero at its first use; every call leaves them zero, so one workspace

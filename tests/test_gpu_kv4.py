@@ -243,6 +243,31 @@ def test_every_path(dtype, nq, lens, Hq, Hkv, D, page, window, path):
     assert torch.equal(out, again), "the same call twice"
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,lens,Hq,Hkv,D,window", [
+    ([1, 1, 400, 1, 1], [300, 1, 420, 450, 64], 8, 2, 64, 0),                   # whole sequences beside one prompt
+    ([1, 500, 16, 1, 0, 17, 2], [2300, 900, 700, 1, 40, 1100, 0], 8, 2, 128, 0),    # 16 queries of 4 heads: the most
+    ([300, 1, 3, 32, 33], [2600, 1900, 1200, 800, 33], 4, 2, 256, 500),
+    ([200] + [1] * 80, [900] + [(37 * i) % 800 + 1 for i in range(80)], 2, 2, 64, 0),
+    ([1] * 150 + [300, 129, 1], [(31 * i) % 600 + 1 for i in range(150)] + [2100, 140, 9], 4, 1, 128, 0),
+])
+def test_single_tokens_beside_prompts(dtype, nq, lens, Hq, Hkv, D, window):
+    """A batch most of whose sequences are far shorter than the longest runs on both kernels."""
+    import ctypes
+    P = need_gpu()
+    path = (ctypes.c_int32 * 4)()
+    P.lib().w4a16_internal_kv4_path(sum(nq), len(nq), Hq, Hkv, D, max(nq), max(lens), path)
+    assert path[0] == 2 and path[3] == 64 // (Hq // Hkv)
+    b = Batch(P, nq, lens, Hq, Hkv, D, 16, dtype)
+    ws = P.kv4_attention_workspace(b.q.cuda(), b.cache, len(nq), max(nq), max(lens))
+    first = None
+    for _ in range(3):
+        out, lse = b.gpu(P, window=window, workspace=ws)
+        b.check(out, lse, window=window)
+        first = out if first is None else first
+        assert torch.equal(out, first) and int(ws[:P.KV4_COUNTER_BYTES].sum()) == 0
+
+
 def test_long_sequence_and_workspace_of_many_calls():
     """70,000 keys; one workspace through calls of other shapes, back and forth."""
     P = need_gpu()

@@ -47,13 +47,14 @@ struct Kv4AttnParams {
     const int32_t* cu_q;              // [B + 1], or null: one query a sequence
     int q_st, q_sh, o_st, o_sh;
     int num_pages, pages_per_seq, T, B, Hq, Hkv, page_shift, max_q, max_kv;
+    int least_q, most_q;              // sequences of fewer or more queries are another kernel's
     float scale_log2;                 // scale * log2(e)
     int causal, window;
     uint32_t* counters;               // one a tile of columns, zero between calls
-    float* partials;                  // [tile][B][Hkv][splits] of slot_cols (D + 2) floats
+    float* partials;                  // by number of chunk, slot_cols (D + 2) floats each
     // from the shape
     int G, slot_cols;
-    int tiles, splits, chunk, pair_tiles;        // kv4_many.hip
+    int tiles, splits, chunk, pair_tiles, rows;  // kv4_many.hip
     int places, budget, at_once, whole, join_apart, join_parts;   // kv4_few.hip
 };
 constexpr size_t KV4_MAX_COUNTERS = 16384;
@@ -63,14 +64,15 @@ struct Kv4AttnShape {
     int tiles;         // tiles of columns of a sequence and key/value head
     int slot_cols;     // columns of a chunk's partial results
     // many: groups of four waves a workgroup; chunks of the keys, at most, and their length; long and short tiles of
-    // columns by turns
-    int groups, splits, chunk;
+    // columns by turns; tiles of all sequences of a head, at most (0: every sequence has a row of `tiles`)
+    int groups, splits, chunk, rows;
     bool pair_tiles;
     // few: chunks of all sequences of a head, at most, about how many are wanted, and how many run at once; whole: one a sequence;
     // join_apart: chunks are joined by a kernel of their own
     int places, budget, at_once;
     bool whole, join_apart;
     size_t partial_bytes;
+    int few_q;         // many: sequences of up to this many queries go to kv4_few.hip first (0: none do)
 };
 // Workgroups of kv4_few.hip that a compute unit holds, by registers (95, 142; 125, 194; 159; 193 of D = 64, 128, 192, 256
 // with one and, up to 128, two column tiles a wave) and LDS.

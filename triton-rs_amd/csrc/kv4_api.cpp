@@ -96,22 +96,31 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
     s.nt = s.many || (C > 16 && D <= 128) ? 2 : 1;
     const int wg_cols = s.many ? 128 : 32 * s.nt;
     const int64_t tiles = std::max<int64_t>(1, (C + wg_cols - 1) / wg_cols);
-    const int64_t items = std::max<int64_t>(1, tiles * B * Hkv);
+    int64_t items = std::max<int64_t>(1, tiles * B * Hkv);
     s.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
     size_t slots = 0;
     if (s.many) {
+        // Up to 1024 sequences share one row of tiles where that is less than half of as many as the longest has for each:
+        // no more tiles than T rows of q make. (Finding its own costs a workgroup a microsecond.)
+        const int64_t rows = std::max<int64_t>(1, (T * G + 127 * (int64_t)B) / 128);
+        int64_t full = items;   // about as many as there are
+        if (B > 1 && B <= 1024 && 2 * rows < tiles * B && rows <= 65535) {
+            s.rows = (int)rows;
+            items = rows * Hkv;
+            full = std::max<int64_t>(1, (T * G + 127) / 128 * Hkv);
+        }
         // Up to two tiles a compute unit, the longest one sets the time: two groups of waves share its keys (a prompt of
         // 2048, 32 heads: 66 us, one group 75; 1344 tiles of 7 prompts: 58, one 45). Not where the tiles are of one
         // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664).
-        s.groups = D <= 128 && items <= 2 * KV4_CUS && !(items >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
+        s.groups = D <= 128 && full <= 2 * KV4_CUS && !(full >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
         const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
         // (chunks of 512 keys or more: 64 queries over 4096 keys, 32 heads of D = 128, 39.9 us; of 256 52.3, 1024 41.5)
-        int64_t want = std::min((at_once + items - 1) / items, ((int64_t)max_kv + 511) / 512);
+        int64_t want = std::min((at_once + full - 1) / full, ((int64_t)max_kv + 511) / 512);
         if (items > (int64_t)KV4_MAX_COUNTERS) want = 1;
         want = std::max<int64_t>(1, want);
         s.chunk = (int)std::max<int64_t>(128, (((int64_t)max_kv + want - 1) / want + 127) / 128 * 128);
         s.splits = std::max(1, (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk));
-        s.pair_tiles = items * s.splits <= at_once;
+        s.pair_tiles = full * s.splits <= at_once;
         s.slot_cols = wg_cols;
         if (want > 1) slots = (size_t)items * want;   // (splits or more: enough for a smaller max_kv, too)
     } else {
@@ -131,7 +140,27 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         s.join_apart = !s.whole && (chunks > KV4_JOIN_CHUNKS || C * D * 4 * chunks >= KV4_JOIN_BYTES);
     }
     s.partial_bytes = slots * s.slot_cols * (D + 2) * sizeof(float);
+    // Few rows for what the sequences may have: single tokens among prompts. Walking a long cache for 128 columns of which
+    // few are there holds up the rest (31 single tokens and a chunk of 1024, 4096 keys each, 32 heads on 8, D = 128: 382 us
+    // on the kernel for many columns alone, 161 on both).
+    const int few_q = (int)(64 / G);
+    s.few_q = s.many && B > 1 && few_q > 0 && 4 * (int64_t)T < (int64_t)B * max_q ? few_q : 0;
     return s;
+}
+// The part of such a batch that runs on kv4_few.hip.
+static Kv4AttnShape kv4_few_part(const Kv4AttnShape& s, int T, int B, int Hq, int Hkv, int D, int max_kv) {
+    return kv4_attention_shape(T, B, Hq, Hkv, D, s.few_q, max_kv);
+}
+// Workspace beyond the counters.
+static size_t kv4_partial_bytes(const Kv4AttnShape& s, int T, int B, int Hq, int Hkv, int D, int max_kv) {
+    return s.partial_bytes + (s.few_q ? kv4_few_part(s, T, B, Hq, Hkv, D, max_kv).partial_bytes : 0);
+}
+static void kv4_params(Kv4AttnParams& p, const Kv4AttnShape& s, int D, int max_q, int T) {
+    p.max_q = max_q < T ? max_q : T;
+    p.slot_cols = s.slot_cols;
+    p.rows = s.rows; p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
+    p.places = s.places; p.budget = s.budget; p.at_once = s.at_once; p.whole = s.whole; p.join_apart = s.join_apart;
+    p.join_parts = (int)((std::min<int64_t>((int64_t)p.max_q * p.G, 32 * s.nt) * (D / 4) + 63) / 64);
 }
 
 }  // namespace w4a16
@@ -182,16 +211,16 @@ static int check_attention(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_
 W4A16_API size_t w4a16_kv4_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D,
                                                     int32_t max_q_len, int32_t max_kv_len) {
     if (check_attention(T, B, Hq, Hkv, D, max_q_len, max_kv_len)) return 0;
-    return W4A16_KV4_COUNTER_BYTES + kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len).partial_bytes;
+    return W4A16_KV4_COUNTER_BYTES + kv4_partial_bytes(kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len), T, B, Hq, Hkv, D, max_kv_len);
 }
 
 // Which kernel a call runs, so that tests can hold a case to the path it is for; not part of the public header.
 // out: {1, column tiles a wave, chunks a head at most, joined by a kernel of their own} few columns; {2, wave
-// groups, chunks, 0} many.
+// groups, chunks, queries of sequences that run on the other (0: none do)} many.
 W4A16_API void w4a16_internal_kv4_path(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q_len,
                                        int32_t max_kv_len, int32_t* out) {
     const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
-    const int32_t few[4] = {1, s.nt, s.places, s.join_apart}, many[4] = {2, s.groups, s.splits, 0};
+    const int32_t few[4] = {1, s.nt, s.places, s.join_apart}, many[4] = {2, s.groups, s.splits, s.few_q};
     for (int i = 0; i < 4; ++i) out[i] = s.many ? many[i] : few[i];
 }
 
@@ -218,7 +247,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     if (int rc = check_rows("q", q, q_stride_t, q_stride_h, T, Hq, D, false)) return rc;
     if (int rc = check_rows("out", out, out_stride_t, out_stride_h, T, Hq, D, true)) return rc;
     const Kv4AttnShape s = kv4_attention_shape(T, B, Hq, Hkv, D, max_q_len, max_kv_len);
-    const size_t need = W4A16_KV4_COUNTER_BYTES + s.partial_bytes;
+    const size_t need = W4A16_KV4_COUNTER_BYTES + kv4_partial_bytes(s, T, B, Hq, Hkv, D, max_kv_len);
     if (!workspace || workspace_bytes < need)
         return fail(W4A16_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace ? workspace_bytes : (size_t)0, need);
     if (!aligned(workspace, 256)) return fail(W4A16_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
@@ -228,18 +257,28 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.q_st = q_stride_t; p.q_sh = q_stride_h; p.o_st = out_stride_t; p.o_sh = out_stride_h;
     p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
     p.page_shift = __builtin_ctz((unsigned)page_size);
-    p.max_q = max_q_len < T ? max_q_len : T; p.max_kv = max_kv_len;
+    p.max_kv = max_kv_len;
     p.scale_log2 = scale_log2; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
     p.counters = static_cast<uint32_t*>(workspace);
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
-    p.G = Hq / Hkv; p.slot_cols = s.slot_cols;
-    p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
-    p.places = s.places; p.budget = s.budget; p.at_once = s.at_once; p.whole = s.whole; p.join_apart = s.join_apart;
-    p.join_parts = (int)((std::min<int64_t>((int64_t)p.max_q * p.G, 32 * s.nt) * (D / 4) + 63) / 64);
+    p.G = Hq / Hkv;
+    p.least_q = 1; p.most_q = INT32_MAX;
     (void)hipGetLastError();
     const bool bf16 = elem == W4A16_BF16;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = s.many ? launch_kv4_many(bf16, D, p, s, st) : launch_kv4_few(bf16, D, p, s, st);
+    hipError_t e = hipSuccess;
+    if (s.few_q) {
+        const Kv4AttnShape f = kv4_few_part(s, T, B, Hq, Hkv, D, max_kv_len);
+        Kv4AttnParams few = p;
+        kv4_params(few, f, D, s.few_q, T);
+        few.most_q = s.few_q;
+        if (s.splits > 1) few.counters += s.rows ? (size_t)s.rows * Hkv : (size_t)s.tiles * B * Hkv;
+        few.partials += s.partial_bytes / sizeof(float);
+        e = launch_kv4_few(bf16, D, few, f, st);
+        p.least_q = s.few_q + 1;
+    }
+    kv4_params(p, s, D, max_q_len, T);
+    if (e == hipSuccess) e = s.many ? launch_kv4_many(bf16, D, p, s, st) : launch_kv4_few(bf16, D, p, s, st);
     return e == hipSuccess ? W4A16_OK : hip_fail(e, "kv4 attention launch");
 }
 

@@ -92,6 +92,18 @@ __device__ __forceinline__ uint32_t kb_umax(uint32_t v) {
 }
 __device__ __forceinline__ float kb_max(float v) { return kb_all(v, [](float a, float b) { return fmaxf(a, b); }); }
 
+// over the lanes of a wave: inclusive f-sums (f(0, v) = v)
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));   // one lane up the row, two, four, eight
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));   // the last of a row to the next
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // the last of the lower half to the upper
+    return v;
+}
+__device__ __forceinline__ int wave_sums(int v) { return wave_scan(v, [](int a, int b) { return a + b; }); }
 // over the 16 lanes of a row: neighbours, pairs, halves mirrored, the row mirrored
 __device__ __forceinline__ float row_min(float v) {
     auto step = [&](auto ctrl) {
@@ -131,7 +143,7 @@ struct Kv4Item {
         q0 = p.cu_q ? min(max(cu0, 0), p.T) : b;
         const int q1 = p.cu_q ? min(max(cu1, 0), p.T) : b + 1;
         n = min(q1 - q0, p.max_q);
-        cols = n * p.G - c0;
+        cols = q1 - q0 < p.least_q || q1 - q0 > p.most_q ? 0 : n * p.G - c0;
         const long long cap = (long long)p.pages_per_seq << p.page_shift;
         len = (int)max(0ll, min((long long)min(kv, p.max_kv), cap));
         first = len - (q1 - q0);

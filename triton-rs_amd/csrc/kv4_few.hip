@@ -72,18 +72,6 @@ __device__ __forceinline__ void take(uint32_t (&dst)[D / 32], const unsigned cha
     }
 }
 
-// over the lanes of a wave: inclusive f-sums (f(0, v) = v)
-template <typename F>
-__device__ __forceinline__ int wave_scan(int v, F f) {
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));   // one lane up the row, two, four, eight
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));   // the last of a row to the next
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));   // the last of the lower half to the upper
-    return v;
-}
-__device__ __forceinline__ int wave_sums(int v) { return wave_scan(v, [](int a, int b) { return a + b; }); }
 __device__ __forceinline__ unsigned wave_sum(int v) { return (unsigned)__builtin_amdgcn_readlane(wave_sums(v), 63); }
 __device__ __forceinline__ int wave_max(int v) { return __builtin_amdgcn_readlane(wave_scan(v, [](int a, int b) { return max(a, b); }), 63); }
 

@@ -108,6 +108,38 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
     }
 }
 
+// Sequence and tile of 128 columns of this workgroup, and its chunk of the keys: those with the longest rows first, or
+// (where all workgroups run at once) long and short ones by turns. p.rows: the tiles of all sequences stand in one row,
+// each sequence's longest first, so that the workgroups of a prompt among single tokens lie side by side.
+__device__ __forceinline__ bool many_tile(const Kv4AttnParams& p, int& b, int& tile, int& chunk, size_t& at) {
+    if (!p.rows) {
+        const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
+        chunk = blockIdx.z - z * p.splits;
+        b = blockIdx.y;
+        tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
+        at = ((size_t)tile * p.B + b) * p.Hkv + blockIdx.x;
+        return true;
+    }
+    chunk = blockIdx.z;
+    at = (size_t)blockIdx.y * p.Hkv + blockIdx.x;
+    const int u = blockIdx.y;
+    for (int base = 0, before = 0; base < p.B; base += 64) {
+        const int s = base + (threadIdx.x & 63), in = min(s, p.B - 1);
+        const int n = min(max(p.cu_q[in + 1], 0), p.T) - min(max(p.cu_q[in], 0), p.T);
+        const int mine = s < p.B && n >= p.least_q ? (min(n, p.max_q) * p.G + 127) / 128 : 0;
+        const int upto = before + wave_sums(mine);
+        const uint64_t who = __ballot(u < upto);
+        if (who) {
+            const int l = __builtin_ctzll(who);
+            b = base + l;
+            tile = __builtin_amdgcn_readlane(upto, l) - 1 - u;
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
 template <typename E, int D, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void kv4_many_kernel(Kv4AttnParams p) {
     constexpr int NT = 2, COLS = 16 * NT, STEP = 64, ALL = STEP * GROUPS;
@@ -116,16 +148,14 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     __shared__ float ml[4 * COLS][2];
     __shared__ int last;
     Kv4Item w;
-    // columns of long rows first, or (where all workgroups run at once) long and short by turns
-    const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
-    const int tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
-    int lo, hi;
+    int b, tile, chunk;
     w.h = blockIdx.x;
-    w.sequence<4 * COLS, STEP>(p, blockIdx.y, tile * 4 * COLS, lo, hi);
+    if (!many_tile(p, b, tile, chunk, w.at)) return;
+    int lo, hi;
+    w.sequence<4 * COLS, STEP>(p, b, tile * 4 * COLS, lo, hi);
     const int chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
-    w.take(p.splits == 1 ? 0 : blockIdx.z - z * p.splits, chunks, p.chunk, lo, hi);
+    w.take(chunk, chunks, p.chunk, lo, hi);
     if (w.cols <= 0 || w.split >= chunks) return;
-    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
     w.slot = w.at * p.splits;
     // wave `wave` of group `group`: the group takes every GROUPS-th step of the keys
     const int lane = threadIdx.x & 63, number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3, group = number >> 2;
@@ -276,7 +306,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
 
 template <typename E, int D>
 static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
-    const dim3 grid(p.Hkv, p.B, s.tiles * s.splits);
+    const dim3 grid = s.rows ? dim3(p.Hkv, s.rows, s.splits) : dim3(p.Hkv, p.B, s.tiles * s.splits);
     if constexpr (D <= 128)
         if (s.groups == 2) {
             kv4_many_kernel<E, D, 2><<<grid, 512, 0, st>>>(p);

@@ -152,7 +152,7 @@ def test_workspace_covers_every_split():
             if 1 < B <= 1024 and 2 * max(1, (T * G + 127 * B) // 128) < rows:
                 rows = max(1, (T * G + 127 * B) // 128)      # one row of tiles: no more than T rows of q make
             slots = 0 if out[2] == 1 else rows * Hkv * out[2] * 128
-            assert out[2] == 1 or rows * Hkv <= 16384
+            assert out[2] == 1 or rows * Hkv <= 4096
             assert out[3] == (64 // G if B > 1 and 4 * T < B * mq else 0)
             if out[3]:           # and the partial results of what runs on the other kernel
                 few = P.lib().w4a16_kv4_attention_workspace_size(T, B, Hkv * G, Hkv, D, out[3], mkv) - 65536

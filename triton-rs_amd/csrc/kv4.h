@@ -50,7 +50,7 @@ struct Kv4AttnParams {
     int least_q, most_q;              // sequences of fewer or more queries are another kernel's
     float scale_log2;                 // scale * log2(e)
     int causal, window;
-    uint32_t* counters;               // one a tile of columns, zero between calls
+    uint32_t* counters;               // kv4_few.hip: one a sequence, head and tile, zero between calls
     float* partials;                  // by number of chunk, slot_cols (D + 2) floats each
     // from the shape
     int G, slot_cols;

@@ -20,6 +20,7 @@ constexpr int KV4_CUS = 256;
 static_assert(KV4_MAX_COUNTERS * sizeof(uint32_t) == W4A16_KV4_COUNTER_BYTES, "counters fill their area");
 constexpr int KV4_MAX_KEYS = 1 << 30;   // of a sequence: positions a few steps further still are int32
 constexpr int64_t KV4_MAX_ALL_KEYS = 1ll << 36;   // of all sequences: their steps of 32 are summed in 32 bits
+constexpr int64_t KV4_MAX_SPLIT_TILES = 4096;   // of 128 columns, 66 KB of partial results (D = 128) a chunk each
 constexpr int KV4_MAX_ROWS = 1 << 27;   // rows of one call: 16 threads each of a 32-bit count of threads
 
 // Up to this much a sequence's and head's last workgroup joins itself; more is a kernel's, which costs its launch
@@ -114,12 +115,13 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664).
         s.groups = D <= 128 && full <= 2 * KV4_CUS && !(full >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
         const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
-        // (chunks of 512 keys or more: 64 queries over 4096 keys, 32 heads of D = 128, 39.9 us; of 256 52.3, 1024 41.5)
+        // (chunks of 512 keys or more: with a join in the kernel 64 queries over 4096 keys, 32 heads of D = 128, took
+        // 39.9 us so, of 256 52.3, of 1024 41.5)
         int64_t most = std::max<int64_t>(1, std::min((at_once + full - 1) / full, ((int64_t)max_kv + 511) / 512));
-        if (items > (int64_t)KV4_MAX_COUNTERS) most = 1;
+        if (items > KV4_MAX_SPLIT_TILES) most = 1;
         auto chunk = [&](int64_t n) { return std::max<int64_t>(128, (((int64_t)max_kv + n - 1) / n + 127) / 128 * 128); };
         // A last round for a few workgroups costs as much as a full one, and one besides its keys some 384 of them: 154
-        // queries of 24 heads on one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 78.0.
+        // queries of 24 heads on one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 67.6.
         auto cost = [&](int64_t n) { return (full * n + at_once - 1) / at_once * (chunk(n) + 384); };
         const int64_t even = std::min(most, std::max<int64_t>(1, at_once / full));
         s.chunk = (int)chunk(cost(even) <= cost(most) ? even : most);
@@ -276,7 +278,6 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
         Kv4AttnParams few = p;
         kv4_params(few, f, D, s.few_q, T);
         few.most_q = s.few_q;
-        if (s.splits > 1) few.counters += s.rows ? (size_t)s.rows * Hkv : (size_t)s.tiles * B * Hkv;
         few.partials += s.partial_bytes / sizeof(float);
         e = launch_kv4_few(bf16, D, few, f, st);
         p.least_q = s.few_q + 1;

@@ -501,11 +501,10 @@ struct Kv4Sink {
             join_quads(e, share, shares, span, e < quads && share < shares, vals, ml);
         }
     }
-    // The same for kv4_many.hip, 128 columns of partial results as lanes have them: per column (m, 1 / l) over all
-    // chunks, then the values, four quads a thread and two chunks of each in flight.
-    template <int THREADS>
-    __device__ __forceinline__ void join_lanes(int live, float* ml, int* last) const {
-        if (!splitk_arrive(p.counters + w.at, w.chunks, last)) return;
+    // For kv4_many.hip, 128 columns of partial results as lanes have them: per column (m, 1 / l) over all
+    // chunks, then the values of part `part` of PARTS, two chunks in flight.
+    template <int PARTS>
+    __device__ __forceinline__ void join_lanes(int live, float* ml, int part) const {
         const int chunks = w.chunks;
         const float* heads = item + (size_t)p.slot_cols * D;
         if ((int)threadIdx.x < live) {
@@ -518,41 +517,32 @@ struct Kv4Sink {
             }
             ml[2 * threadIdx.x] = mm;
             ml[2 * threadIdx.x + 1] = ll == 0.f ? 0.f : 1.f / ll;
-            lse(w.c0 + threadIdx.x, mm, ll);
+            if (part == 0) lse(w.c0 + threadIdx.x, mm, ll);
         }
         __syncthreads();
-        constexpr int U = 4, QUADS = 32 * D;   // of 128 columns
+        constexpr int QUADS = 32 * D / PARTS;   // of 128 columns
+        static_assert(QUADS % 256 == 0, "whole rounds");
 #pragma unroll 1
-        for (int e0 = threadIdx.x; e0 < QUADS; e0 += THREADS * U) {
-            float4_t v[U];
-            float mm[U];
-            int c[U], d[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                lane_place(e0 + THREADS * u, c[u], d[u]);
-                mm[u] = ml[2 * min(c[u], live - 1)];
-                v[u] = float4_t{0.f, 0.f, 0.f, 0.f};
-            }
+        for (int e = part * QUADS + threadIdx.x; e < (part + 1) * QUADS; e += 256) {
+            int c, d;
+            lane_place(e, c, d);
+            const int at = min(c, live - 1);
+            const float mm = ml[2 * at];
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
             for (int s0 = 0; s0 < chunks; s0 += 2) {
-                float4_t x[U][2];
-                float f[U][2];
+                float4_t x[2];
+                float f[2];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int y = 0; y < 2; ++y) {
+                    const size_t s = min(s0 + y, chunks - 1);
+                    f[y] = __hip_atomic_load(heads + s * slot_floats + 2 * at, __ATOMIC_RELAXED, SCOPE_DEVICE);
+                    x[y] = ld_partial4<SCOPE_DEVICE>(item + s * slot_floats + 4 * e);
+                }
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const size_t s = min(s0 + y, chunks - 1);
-                        f[u][y] = __hip_atomic_load(heads + s * slot_floats + 2 * min(c[u], live - 1), __ATOMIC_RELAXED, SCOPE_DEVICE);
-                        x[u][y] = ld_partial4<SCOPE_DEVICE>(item + s * slot_floats + 4 * (e0 + THREADS * u));
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-                        if (s0 + y < chunks) v[u] += x[u][y] * __builtin_amdgcn_exp2f(f[u][y] - mm[u]);
+                for (int y = 0; y < 2; ++y)
+                    if (s0 + y < chunks) v += x[y] * __builtin_amdgcn_exp2f(f[y] - mm);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c[u] < live) out(w.c0 + c[u], d[u], v[u], ml[2 * c[u] + 1]);
+            if (c < live) out(w.c0 + c, d, v, ml[2 * c + 1]);
         }
     }
     // Partial results as lanes have them: number of a quad, and place of quad e

@@ -15,6 +15,8 @@
 
 namespace w4a16 {
 
+constexpr int MANY_STEP = 64;   // keys of a step
+
 template <int D>
 struct ManyLds {
     static constexpr int KW = D / 32, VT = D / 16;
@@ -110,17 +112,18 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
 
 // Sequence and tile of 128 columns of this workgroup, and its chunk of the keys: those with the longest rows first, or
 // (where all workgroups run at once) long and short ones by turns. p.rows: the tiles of all sequences stand in one row,
-// each sequence's longest first, so that the workgroups of a prompt among single tokens lie side by side.
-__device__ __forceinline__ bool many_tile(const Kv4AttnParams& p, int& b, int& tile, int& chunk, size_t& at) {
+// each sequence's longest first, so that the workgroups of a prompt among single tokens lie side by side. place:
+// tile and chunk, or (p.rows) chunk.
+__device__ __forceinline__ bool many_tile(const Kv4AttnParams& p, int place, int& b, int& tile, int& chunk, size_t& at) {
     if (!p.rows) {
-        const int z = p.splits == 1 ? blockIdx.z : blockIdx.z / p.splits;
-        chunk = blockIdx.z - z * p.splits;
+        const int z = p.splits == 1 ? place : place / p.splits;
+        chunk = place - z * p.splits;
         b = blockIdx.y;
         tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
         at = ((size_t)tile * p.B + b) * p.Hkv + blockIdx.x;
         return true;
     }
-    chunk = blockIdx.z;
+    chunk = place;
     at = (size_t)blockIdx.y * p.Hkv + blockIdx.x;
     const int u = blockIdx.y;
     for (int base = 0, before = 0; base < p.B; base += 64) {
@@ -140,23 +143,25 @@ __device__ __forceinline__ bool many_tile(const Kv4AttnParams& p, int& b, int& t
     return false;
 }
 
+__device__ __forceinline__ bool many_item(const Kv4AttnParams& p, int place, Kv4Item& w) {
+    int b, tile, chunk, lo, hi;
+    w.h = blockIdx.x;
+    if (!many_tile(p, place, b, tile, chunk, w.at)) return false;
+    w.sequence<128, MANY_STEP>(p, b, tile * 128, lo, hi);
+    const int chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
+    w.take(chunk, chunks, p.chunk, lo, hi);
+    w.slot = w.at * p.splits;
+    return w.cols > 0 && chunk < chunks;
+}
+
 template <typename E, int D, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void kv4_many_kernel(Kv4AttnParams p) {
-    constexpr int NT = 2, COLS = 16 * NT, STEP = 64, ALL = STEP * GROUPS;
+    constexpr int NT = 2, COLS = 16 * NT, STEP = MANY_STEP, ALL = STEP * GROUPS;
     typedef Kv4Cols<E, D, NT> C;
     __shared__ ManyLds<D> lds[2][GROUPS];
     __shared__ float ml[4 * COLS][2];
-    __shared__ int last;
     Kv4Item w;
-    int b, tile, chunk;
-    w.h = blockIdx.x;
-    if (!many_tile(p, b, tile, chunk, w.at)) return;
-    int lo, hi;
-    w.sequence<4 * COLS, STEP>(p, b, tile * 4 * COLS, lo, hi);
-    const int chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
-    w.take(chunk, chunks, p.chunk, lo, hi);
-    if (w.cols <= 0 || w.split >= chunks) return;
-    w.slot = w.at * p.splits;
+    if (!many_item(p, blockIdx.z, w)) return;
     // wave `wave` of group `group`: the group takes every GROUPS-th step of the keys
     const int lane = threadIdx.x & 63, number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3, group = number >> 2;
     const int col = lane & 15, kb = lane >> 4;
@@ -300,19 +305,36 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
             }
         if (kb == 0 && c < a.n) sink.put_ml(a.c + c, a.m[n], a.l[n]);
     }
-    if (w.chunks == 1) return;
-    sink.template join_lanes<256 * GROUPS>(min(4 * COLS, w.cols), &ml[0][0], &last);
+}
+
+// Joins the chunks of one tile: an eighth of its values a workgroup. (The last of the chunks' own workgroups took longer:
+// 64 queries over 4096 keys, 32 heads of D = 128, 8 chunks, 40.1 us, so 29.7; two chunks of 400 over 2000 40.2, 39.3.)
+constexpr int MANY_PARTS = 8;
+template <typename E, int D>
+__global__ __launch_bounds__(256) void kv4_many_join_kernel(Kv4AttnParams p) {
+    __shared__ float ml[128][2];
+    Kv4Item w;
+    const int part = blockIdx.z % MANY_PARTS;
+    if (!many_item(p, blockIdx.z / MANY_PARTS * p.splits, w) || w.chunks == 1) return;   // (its results are in place)
+    const Kv4Sink<E, D> sink(p, w);
+    sink.template join_lanes<MANY_PARTS>(min(128, w.cols), &ml[0][0], part);
 }
 
 template <typename E, int D>
 static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
     const dim3 grid = s.rows ? dim3(p.Hkv, s.rows, s.splits) : dim3(p.Hkv, p.B, s.tiles * s.splits);
+    auto join = [&] {
+        const dim3 parts(grid.x, grid.y, (s.rows ? 1 : s.tiles) * MANY_PARTS);
+        if (s.splits > 1) kv4_many_join_kernel<E, D><<<parts, 256, 0, st>>>(p);
+    };
     if constexpr (D <= 128)
         if (s.groups == 2) {
             kv4_many_kernel<E, D, 2><<<grid, 512, 0, st>>>(p);
+            join();
             return;
         }
     kv4_many_kernel<E, D, 1><<<grid, 256, 0, st>>>(p);
+    join();
 }
 
 hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {

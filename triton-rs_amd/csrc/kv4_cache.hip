@@ -224,9 +224,13 @@ __device__ __forceinline__ void dequantise8(uint32_t x, uint32_t par, uint32_t (
             f[2 * i] = __builtin_fmaf((float)(((x & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu), s, nzs);
             f[2 * i + 1] = __builtin_fmaf((float)((((x >> 4) & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu), s, nzs);
         }
-        if (s > 0x1p123f) {
+        if (s > 0x1p123f) {   // z s, or the result, may pass fp32: n - z first, then one product
+            const float z = (float)(par >> 16);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = fminf(fmaxf(f[i], -0x1.fep127f), 0x1.fep127f);
+            for (int i = 0; i < 8; ++i) {
+                const float v = ((float)((x >> (4 * i)) & 15u) - z) * s;
+                f[i] = fminf(fmaxf(v, -0x1.fep127f), 0x1.fep127f);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = pack2(E{}, f[2 * i], f[2 * i + 1]);

@@ -194,8 +194,8 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4RowParams p) {
     if (c < 2) *reinterpret_cast<uint32_t*>(block + 16 * D + 64 * c + 4 * tok) = c ? pv : pk;
 }
 
-// Eight nibbles as RNE_E((n - z) s) in four words. fp16: n - z is exact, so one fp16 product rounds once; bf16: the fma
-// gives (n - z) s exactly. Where 15 s passes the largest finite value (by less than a step) the result is that.
+// Eight nibbles as RNE_E((n - z) s) in four words. fp16: n - z is exact, so one fp16 product rounds once; bf16:
+// (n - z) s is exact in fp32. Where 15 s passes the largest finite value (by less than a step) the result is that.
 template <typename E>
 __device__ __forceinline__ void dequantise8(uint32_t x, uint32_t par, uint32_t (&o)[4]) {
     const float s = elem_f32<E>(par);
@@ -217,20 +217,14 @@ __device__ __forceinline__ void dequantise8(uint32_t x, uint32_t par, uint32_t (
         o[2] = perm(as_u32(a[1]), as_u32(a[0]), 0x07060302u);
         o[3] = perm(as_u32(a[3]), as_u32(a[2]), 0x07060302u);
     } else {
-        const float nzs = -(float)(par >> 16) * s;
+        // (z s may pass fp32 where (n - z) s does not; the bound of a row of NaN is NaN, and so is the middle of three)
+        const float z = (float)(par >> 16), most = s == s ? 0x1.fep127f : s;
         float f[8];
+        auto value = [&](uint32_t n) { return __builtin_amdgcn_fmed3f(((float)n - z) * s, -most, most); };
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // bytes: nibbles 2 i and 2 i + 1
-            f[2 * i] = __builtin_fmaf((float)(((x & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu), s, nzs);
-            f[2 * i + 1] = __builtin_fmaf((float)((((x >> 4) & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu), s, nzs);
-        }
-        if (s > 0x1p123f) {   // z s, or the result, may pass fp32: n - z first, then one product
-            const float z = (float)(par >> 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = ((float)((x >> (4 * i)) & 15u) - z) * s;
-                f[i] = fminf(fmaxf(v, -0x1.fep127f), 0x1.fep127f);
-            }
+            f[2 * i] = value(((x & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu);
+            f[2 * i + 1] = value((((x >> 4) & 0x0F0F0F0Fu) >> (8 * i)) & 0xFFu);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = pack2(E{}, f[2 * i], f[2 * i + 1]);

@@ -392,8 +392,10 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  * j < kv_lens[b] where (causal != 0) j <= i and (window > 0) j > i - window:
  *   out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j), lse = ln sum_j p_j (nullable, fp32
  *   [T, Hq]), both over the unrounded values (n - zero) scale that the cache holds. Sums are fp32;
- *   p_j times the value row's scale is rounded to fp16 before its product with n - zero (scales
- *   below 2^-60 count as 2^-60 in how p_j is scaled for that), bf16 queries are taken in fp16 under
+ *   p_j times the value row's scale is rounded to fp16 before its product with n - zero: by 2^-11 of
+ *   it, or 2^-32 of the query's largest such product where that is more (a scale below 2^-60 counts
+ *   as 2^-60 in that largest), so a value row of any size that has no weight takes no bits from the
+ *   others. bf16 queries are taken in fp16 under
  *   a power of two that the queries of up to 128 (query, head) pairs share (what lies 2^27 below
  *   their largest loses bits), and out is rounded once (to its type's largest finite value).
  * A query that sees no key: out 0, lse -infinity. What a query does not see moves no bit of its

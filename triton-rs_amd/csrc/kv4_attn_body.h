@@ -18,10 +18,12 @@
 // either block of 16, which is how the second product takes them as its operand (the sum over the
 // tokens may run in any order as long as the values follow), so no logit or weight passes between lanes
 // or through LDS. q is scaled by a power of two (wave-wide) into fp16's range, exactly for fp16 and bf16
-// alike but for what lies 2^27 below the largest. A weight p_j s_j is rounded to fp16; the reference m is
-// such that all of them are below 2^16, and raised (with the sums scaled down) only where a logit passes
-// the room that it and the value scales leave, 8 in base 2, so maxima pass between lanes only then. A
-// column's reference follows what the column sees, nothing else. Sums are fp32.
+// alike but for what lies 2^27 below the largest. A weight p_j s_j is rounded to fp16 (2^-11, of what the matrix
+// cores take the type with the most bits); the reference m is such that the largest of them is 2^7 when it is set and
+// 2^15 at most, so it follows logits and value scales together: a row of large values and no weight takes no bits
+// from the others. It is raised (with the sums scaled down) only where a step's largest logit and largest value
+// scale would pass 2^15, so maxima pass between lanes only then. A column's reference follows what the column sees,
+// nothing else. Sums are fp32.
 #pragma once
 #include <cfloat>
 
@@ -31,14 +33,37 @@
 
 namespace w4a16 {
 
-constexpr int KV4_WEIGHT_LOG2 = 15;   // p_j s_j <= 2^15
-constexpr float KV4_ROOM = 8.0f;      // a raise leaves the largest p_j at 2^-8 of what it may be
+constexpr float KV4_MOST = 15.f;   // p_j s_j <= 2^15
+constexpr float KV4_ROOM = 7.f;    // a raise leaves the largest at 2^-7 to 2^-8 of that
+// Value scales are taken times 2^-VALUE_DOWN, and smaller ones than LEAST_SCALE (all zero in fp16) as that in the
+// reference: p_j stays between 2^-98, at the largest bf16 scale, and 2^95, so that a sum of 2^30 fits fp32.
+template <typename E>
+constexpr int VALUE_DOWN = __is_same(E, half_t) ? 0 : 20;
+template <typename E>
+constexpr float LEAST_SCALE = __is_same(E, half_t) ? 0x1p-24f : 0x1p-80f;
 
 template <typename E>
 __device__ __forceinline__ float param_scale(uint32_t w) {
     if constexpr (__is_same(E, half_t)) return (float)__builtin_bit_cast(half_t, (uint16_t)w);
     else return bf16_bits_to_f32(w);   // the shift drops the upper half
 }
+
+template <typename E>
+__device__ __forceinline__ float value_scale(uint32_t w) {
+    if constexpr (VALUE_DOWN<E> == 0) return param_scale<E>(w);
+    else return param_scale<E>(w) * (1.f / (1 << VALUE_DOWN<E>));
+}
+// log2 of a number above value scales, from the bits of their largest (NaN beyond all numbers)
+template <typename E>
+__device__ __forceinline__ float log2_above(uint32_t top) {
+    return (float)((int)(max(top, __builtin_bit_cast(uint32_t, LEAST_SCALE<E>)) >> 23) - 126);
+}
+// what sum_j (p_j s_j) (n_j - z_j) is multiplied by, l = sum_j p_j
+template <typename E>
+__device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : (float)(1 << VALUE_DOWN<E>) / l; }
+// Square root of the factor from reference m to mm: references of steps, waves and chunks may lie further apart than
+// fp32's exponents reach (value scales do), where a sum of p_j is far from 1 as well. It is multiplied twice.
+__device__ __forceinline__ float half_fall(float m, float mm) { return __builtin_amdgcn_exp2f(0.5f * (m - mm)); }
 
 __device__ __forceinline__ half8_t as_h8(half2_t a, half2_t b, half2_t c, half2_t d) {
     const u32x4 t = {as_u32(a), as_u32(b), as_u32(c), as_u32(d)};
@@ -104,23 +129,8 @@ __device__ __forceinline__ int wave_scan(int v, F f) {
     return v;
 }
 __device__ __forceinline__ int wave_sums(int v) { return wave_scan(v, [](int a, int b) { return a + b; }); }
-// over the 16 lanes of a row: neighbours, pairs, halves mirrored, the row mirrored
-__device__ __forceinline__ float row_min(float v) {
-    auto step = [&](auto ctrl) {
-        v = fminf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true)));
-    };
-    step(std::integral_constant<int, 0xB1>{});
-    step(std::integral_constant<int, 0x4E>{});
-    step(std::integral_constant<int, 0x141>{});
-    step(std::integral_constant<int, 0x140>{});
-    return v;
-}
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
-
-// A scale of NaN (a row that held an infinity or NaN) as the largest number: the weight of a column that does not
-// see the token is then 0. For one that does see it, see value_room().
-__device__ __forceinline__ float seen_scale(float s) { return fminf(s, FLT_MAX); }
 
 // What a workgroup takes of sequence b, key/value head h: columns from c0 on, of keys [k0, k1) of this chunk.
 struct Kv4Item {
@@ -172,10 +182,7 @@ struct Kv4Cols {
     half8_t qf[NT][KW];
     float kscale;          // logits in base 2 are kscale s (q . (n - z))
     float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
-    float most[NT];        // the same, -infinity until a column has seen a key
-    float room[NT];        // what logits less m may be: p_j s_j <= 2^KV4_WEIGHT_LOG2
-    float vtop[NT];        // a power of two above the largest value scale that a column has seen; 0 before it, NaN for good
-    float vleast;          // the least of them of all columns
+    float most[NT];        // KV4_MOST, -infinity until a column has seen a key
     float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
 
     // the rows of q, as they are
@@ -262,9 +269,6 @@ struct Kv4Cols {
             }
             m[t] = l[t] = 0.f;
             most[t] = -INFINITY;
-            vleast = 0.f;
-            room[t] = (float)KV4_WEIGHT_LOG2;
-            vtop[t] = hi[t] > lo[t] ? 0.f : INFINITY;   // (one that sees nothing asks for no room)
 #pragma unroll
             for (int x = 0; x < VT; ++x) o[t][x] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
@@ -282,40 +286,32 @@ struct Kv4Cols {
         return Seen{lo[t] - at, min(hi[t], end) - at, bad};
     }
 
-    // Room for the value scales vs of a step, those that a column sees: what others see does not move its reference.
-    // vmax: the largest of them all, of this lane or more, as bits (NaN beyond all numbers). A value row of NaN makes
-    // the columns NaN that see it, whatever its weight.
-    __device__ __forceinline__ void value_room(uint32_t vmax, const float (&vs)[2][4], int j, int end, int bad, int kb) {
-        if (!__any(vmax > __float_as_uint(vleast))) return;   // rare after the first steps
-        vleast = INFINITY;
+    // A value row of NaN (its scale is) makes those columns NaN that see it, whatever its weight, and no others. Where all
+    // see it its weights do that; here, where some do not, they become 0 and the columns NaN by themselves.
+    __device__ __forceinline__ void value_nan(float (&vs)[2][4], int j, int end, int bad, int kb) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const Seen in = seen(t, j, end, bad, kb);
-            uint32_t top = 0;
+            uint32_t hit = 0;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = max(top, in(s, i) ? __float_as_uint(vs[s][i]) : 0u);
-            top = kb_umax(top);
-            // 2 to 4 times the largest; value scales below 2^-60 share one
-            const int e = min(126, max(-60, (int)(top >> 23) - 127 + 2));
-            const bool up = top > __float_as_uint(vtop[t]);
-            float fresh = pow2(e), left = (float)(KV4_WEIGHT_LOG2 - e);
-            asm("" : "+v"(fresh), "+v"(left));   // (selects, not a branch)
-            if (top >= __float_as_uint(FLT_MAX)) fresh = __builtin_nanf("");   // (no number is above it)
-            vtop[t] = up ? fresh : vtop[t];
-            room[t] = up ? left : room[t];
-            most[t] = most[t] == -INFINITY ? most[t] : room[t];   // (the next logits raise m where that is too little)
-            vleast = fminf(vleast, vtop[t]);
+                for (int i = 0; i < 4; ++i) hit |= (in(s, i) & (vs[s][i] != vs[s][i])) ? 1u : 0u;
+            const float add = kb_umax(hit) ? __builtin_nanf("") : 0.f;
+#pragma unroll
+            for (int x = 0; x < VT; ++x) o[t][x] += add;
         }
-        vleast = row_min(vleast);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vs[s][i] = fmaxf(vs[s][i], 0.f);
     }
 
     // Logits less m of 32 tokens from j on for columns t: acc = q . (n - z), ks = key scale times kscale, of the
-    // lane's tokens j + 16 s + 4 kb + i. whole: every column sees all 32; else tokens from `end` on and those
-    // of blocks in `bad` are not seen. Raises m where they pass it by too much.
-    __device__ __forceinline__ void logits(int t, float (&x)[2][4], const float4_t (&acc)[2], const float (&ks)[2][4], bool whole,
-                                           int j, int end, int bad, int kb) {
+    // lane's tokens j + 16 s + 4 kb + i; vs = value scales, 2^above more than any of them. whole: every column sees
+    // all 32; else tokens from `end` on and those of blocks in `bad` are not seen. Raises m where a weight may pass 2^15.
+    __device__ __forceinline__ void logits(int t, float (&x)[2][4], const float4_t (&acc)[2], const float (&ks)[2][4], const float (&vs)[2][4],
+                                           float above, bool whole, int j, int end, int bad, int kb) {
         float top = -INFINITY;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -333,17 +329,26 @@ struct Kv4Cols {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[s][i]);
-        if (__any(top > most[t])) {
+        if (__any(top > most[t] - above)) {   // rare after the first steps
+            top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = vs[s][i];
+                    asm volatile("" : "+v"(v));   // (else all steps take the scales' exponents ahead: 740 us for the 660 of kv4_many.hip)
+                    top = fmaxf(top, x[s][i] + log2_above<E>(__float_as_uint(fmaxf(v, 0.f))));   // (NaN as 0)
+                }
             top = kb_max(top);
             const bool up = top > most[t];
-            const float by = up ? top - (room[t] - KV4_ROOM) : 0.f;
+            const float by = up ? top - (KV4_MOST - KV4_ROOM) : 0.f;
             // (a column's first keys: nothing summed yet)
-            const float fall = most[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-by);
+            const float fall = most[t] == -INFINITY ? 0.f : half_fall(0.f, by);
             m[t] += by;
-            l[t] *= fall;
+            l[t] = l[t] * fall * fall;
 #pragma unroll
-            for (int y = 0; y < VT; ++y) o[t][y] *= fall;
-            most[t] = up ? room[t] : most[t];
+            for (int y = 0; y < VT; ++y) o[t][y] *= fall * fall;
+            most[t] = up ? KV4_MOST : most[t];
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -351,7 +356,7 @@ struct Kv4Cols {
         }
     }
 
-    // Their weights p_j s_j as operand, vs = value scales (seen_scale of them where `whole` is not); the sum of p_j.
+    // Their weights p_j s_j as operand; the sum of p_j.
     __device__ __forceinline__ half8_t weights(int t, const float (&x)[2][4], const float (&vs)[2][4]) {
         half8_t w;
 #pragma unroll
@@ -371,10 +376,6 @@ struct Kv4Cols {
         for (int t = 0; t < NT; ++t) {
             l[t] = kb_sum(l[t]);
             if (most[t] == -INFINITY && l[t] == 0.f) m[t] = -FLT_MAX;
-            if (__any(vtop[t] != vtop[t])) {   // a value row of NaN was seen
-#pragma unroll
-                for (int x = 0; x < VT; ++x) o[t][x] += vtop[t] != vtop[t] ? vtop[t] : 0.f;
-            }
         }
     }
 };
@@ -455,15 +456,15 @@ struct Kv4Sink {
                 float mn = m;
 #pragma unroll
                 for (int y = 0; y < 8; ++y) mn = fmaxf(mn, __uint_as_float((uint32_t)h[y]));
-                const float f = __builtin_amdgcn_exp2f(m - mn);
-                v *= f;
-                l *= f;
+                const float f = half_fall(m, mn);
+                v *= f * f;
+                l = l * f * f;
 #pragma unroll
                 for (int y = 0; y < 8; ++y)
                     if (s0 + shares * y < chunks) {
-                        const float g = __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)h[y]) - mn);
-                        v += x[y] * g;
-                        l += __uint_as_float((uint32_t)(h[y] >> 32)) * g;
+                        const float g = half_fall(__uint_as_float((uint32_t)h[y]), mn);
+                        v += x[y] * (g * g);
+                        l += __uint_as_float((uint32_t)(h[y] >> 32)) * g * g;
                     }
                 m = mn;
             }
@@ -475,19 +476,19 @@ struct Kv4Sink {
             if (on && share == 0) {
                 float mm = m;
                 for (int x = 1; x < shares; ++x) mm = fmaxf(mm, ml[threadIdx.x + x * span][0]);
-                const float f = __builtin_amdgcn_exp2f(m - mm);
-                v *= f;
-                l *= f;
+                const float f = half_fall(m, mm);
+                v *= f * f;
+                l = l * f * f;
                 for (int x = 1; x < shares; ++x) {
-                    const float g = __builtin_amdgcn_exp2f(ml[threadIdx.x + x * span][0] - mm);
-                    v += vals[threadIdx.x + x * span] * g;
-                    l += ml[threadIdx.x + x * span][1] * g;
+                    const float g = half_fall(ml[threadIdx.x + x * span][0], mm);
+                    v += vals[threadIdx.x + x * span] * (g * g);
+                    l += ml[threadIdx.x + x * span][1] * g * g;
                 }
                 m = mm;
             }
         }
         if (on && share == 0) {
-            out(w.c0 + c, d, v, l == 0.f ? 0.f : 1.f / l);
+            out(w.c0 + c, d, v, over_sum<E>(l));
             if (d == 0) lse(w.c0 + c, m, l);
         }
     }
@@ -512,11 +513,12 @@ struct Kv4Sink {
             for (int s = 0; s < chunks; ++s) {
                 const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(heads + s * slot_floats + 2 * threadIdx.x), __ATOMIC_RELAXED, SCOPE_DEVICE);
                 const float mx = __uint_as_float((uint32_t)x), mn = fmaxf(mm, mx);
-                ll = ll * __builtin_amdgcn_exp2f(mm - mn) + __uint_as_float((uint32_t)(x >> 32)) * __builtin_amdgcn_exp2f(mx - mn);
+                const float f = half_fall(mm, mn), g = half_fall(mx, mn);
+                ll = ll * f * f + __uint_as_float((uint32_t)(x >> 32)) * g * g;
                 mm = mn;
             }
             ml[2 * threadIdx.x] = mm;
-            ml[2 * threadIdx.x + 1] = ll == 0.f ? 0.f : 1.f / ll;
+            ml[2 * threadIdx.x + 1] = over_sum<E>(ll);
             if (part == 0) lse(w.c0 + threadIdx.x, mm, ll);
         }
         __syncthreads();

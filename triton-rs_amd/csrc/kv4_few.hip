@@ -320,21 +320,16 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 ks[s][i] = param_scale<E>(kp[s][i]) * a.kscale;
-                vs[s][i] = param_scale<E>(vp[s][i]);
+                vs[s][i] = value_scale<E>(vp[s][i]);
                 vmax = max(vmax, __float_as_uint(vs[s][i]));
             }
-        a.value_room(vmax, vs, j, end, here, kb);
-        if (!whole) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vs[s][i] = seen_scale(vs[s][i]);
-        }
+        const float above = log2_above<E>(vmax);
+        if (!whole && __any(above > 128.f)) a.value_nan(vs, j, end, here, kb);   // (a scale of NaN)
         half8_t pw[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float x[2][4];
-            a.logits(t, x, acc[t], ks, whole, j, end, here, kb);
+            a.logits(t, x, acc[t], ks, vs, above, whole, j, end, here, kb);
             pw[t] = a.weights(t, x, vs);
         }
         half2_t vz1[4], vz16[4];
@@ -395,10 +390,11 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
             for (int x = 1; x < kspl; ++x) mm = fmaxf(mm, ml[g0 + x][16 * t + c][0]);
             float4_t r = {0.f, 0.f, 0.f, 0.f};
             for (int x = 0; x < kspl; ++x) {
-                ll += ml[g0 + x][16 * t + c][1] * __builtin_amdgcn_exp2f(ml[g0 + x][16 * t + c][0] - mm);
+                const float f = half_fall(ml[g0 + x][16 * t + c][0], mm);
+                ll += ml[g0 + x][16 * t + c][1] * f * f;
                 r += *reinterpret_cast<const float4_t*>(reds + x * RING_FLOATS + c * S::ROW + d);
             }
-            sink.put(a.c + 16 * t + c, d, r, ll == 0.f ? 0.f : 1.f / ll);
+            sink.put(a.c + 16 * t + c, d, r, over_sum<E>(ll));
             if (d == 0) sink.put_ml(a.c + 16 * t + c, mm, ll);
         }
     }

@@ -22,8 +22,8 @@ struct ManyLds {
     static constexpr int KW = D / 32, VT = D / 16;
     half8_t k[4][KW][64];      // block, word of the quarter row, lane
     half8_t v[2][VT][64];      // pair of blocks, tile of the result, lane (first block's two pairs, second's)
-    float ks[64], vs[64];      // scales of the tokens, those of keys times kscale, those of values by seen_scale
-    uint32_t vtop[4];          // the largest of a block's value scales, as bits (NaN beyond all numbers)
+    float ks[64], vs[64];      // scales of the tokens, those of keys times kscale
+    float above[4];            // of a block's value scales: log2_above
     int live[4];               // tokens of a block that there are (0 or less: none)
 };
 
@@ -96,16 +96,14 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
     if (kb == 0) s.ks[16 * wave + col] = param_scale<E>(t.kc) * kscale;
     float4_t f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = param_scale<E>(t.vp[i]);
+    for (int i = 0; i < 4; ++i) f[i] = value_scale<E>(t.vp[i]);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(f[i]));
     top = kb_umax(top);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = seen_scale(f[i]);
     if (col == 0) *reinterpret_cast<float4_t*>(&s.vs[16 * wave + 4 * kb]) = f;
     if (lane == 0) {
-        s.vtop[wave] = top;
+        s.above[wave] = log2_above<E>(top);
         s.live[wave] = live;
     }
 }
@@ -217,29 +215,29 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
                     vs[b][i] = fv[i];
                 }
             }
-            int bad = 0;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) bad |= (s.live[2 * half + b] <= 0 ? 1 : 0) << b;
-            bad = __builtin_amdgcn_readfirstlane(bad);
-            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad;
-            const uint32_t vmax = max(s.vtop[2 * half], s.vtop[2 * half + 1]);
-            // operands from LDS all at once, ahead of the products that take them: one wait instead of eight
+            // operands from LDS all at once, ahead of what takes them: one wait instead of eight
             half8_t kf[2][C::KW], vf[C::VT];
+            const int live0 = s.live[2 * half], live1 = s.live[2 * half + 1];
+            const float above0 = s.above[2 * half], above1 = s.above[2 * half + 1];
 #pragma unroll
             for (int x = 0; x < C::KW; ++x)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) kf[b][x] = s.k[2 * half + b][x][lane];
             __builtin_amdgcn_sched_barrier(0);
+            const int bad = __builtin_amdgcn_readfirstlane((live0 <= 0 ? 1 : 0) | (live1 <= 0 ? 2 : 0));
+            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad;
+            const float above = fmaxf(above0, above1);
 #pragma unroll
             for (int x = 0; x < C::KW; ++x)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            a.value_room(vmax, vs, jh, a.jhi, bad, kb);
+            if (__builtin_expect(__any(above > 128.f), 0))   // (a scale of NaN)
+                if (!whole) a.value_nan(vs, jh, a.jhi, bad, kb);
             float x[NT][2][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, whole, jh, a.jhi, bad, kb);
+            for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, vs, above, whole, jh, a.jhi, bad, kb);
 #pragma unroll
             for (int x = 0; x < C::VT; ++x) vf[x] = s.v[half][x][lane];
             __builtin_amdgcn_sched_barrier(0);
@@ -273,9 +271,9 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float m1 = mls[128 * n + lane], mm = fmaxf(a.m[n], m1);
-                const float f0 = __builtin_amdgcn_exp2f(a.m[n] - mm), f1 = __builtin_amdgcn_exp2f(m1 - mm);
+                const float h0 = half_fall(a.m[n], mm), h1 = half_fall(m1, mm), f0 = h0 * h0, f1 = h1 * h1;
                 a.m[n] = mm;
-                a.l[n] = a.l[n] * f0 + mls[128 * n + 64 + lane] * f1;
+                a.l[n] = a.l[n] * h0 * h0 + mls[128 * n + 64 + lane] * h1 * h1;
 #pragma unroll
                 for (int x = 0; x < C::VT; ++x) a.o[n][x] = a.o[n][x] * f0 + o[(n * C::VT + x) * 64 + lane] * f1;
             }
@@ -286,7 +284,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     for (int n = 0; n < NT; ++n) {
         if (group) break;
         const int c = 16 * n + col;
-        const float inv = a.l[n] == 0.f ? 0.f : 1.f / a.l[n];
+        const float inv = over_sum<E>(a.l[n]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll

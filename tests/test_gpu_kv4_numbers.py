@@ -1,5 +1,5 @@
 """The 4-bit key/value cache at the ends of its numbers' range: rows near the type's largest value, value rows many powers
-of two apart. Compared with 64 bits (kv4_plain.py)."""
+of two apart, queries of any magnitude. Compared with 64 bits (kv4_plain.py)."""
 import numpy as np
 import pytest
 import torch
@@ -124,3 +124,35 @@ def test_value_rows_of_all_scales(dtype, low, high, nq, L):
         P.kv4_write(k16, v.to(dtype).cuda(), b.cache, slots)
         b.k[0], b.v[0] = plain.quantise(k16.cpu())[3], plain.quantise(v.to(dtype))[3]
         close(b, *b.gpu(P))
+
+
+@pytest.mark.parametrize("q,k,scale", [(2.0 ** 114, 2.0 ** -116, 0.125), (2.0 ** 120, 2.0 ** -122, 0.125), (1.5 * 2.0 ** 125, 2.0 ** -128, 0.125),
+                                       (2.0 ** 122, 1.0, 2.0 ** -124), (2.0 ** 60, 2.0 ** -120, 2.0 ** 60), (2.0 ** -110, 2.0 ** 108, 0.125),
+                                       (2.0 ** -125, 2.0 ** 100, 2.0 ** 24), (0.25, 2.0 ** 12, 2.0 ** -14), (1.0, 2.0 ** -40, 2.0 ** 38)])
+@pytest.mark.parametrize("nq,L", [(1, 90), (1, 1500), (90, 200)])
+def test_queries_of_any_magnitude(q, k, scale, nq, L):
+    """bfloat16 queries up to the type's end, whose logits are ordinary numbers."""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, BF16, kscale=k)
+    b.q = (b.q.double().clamp(-1.9, 1.9) * q).to(BF16)
+    assert torch.isfinite(b.q).all() and torch.isfinite(torch.tensor(b.k[0])).all()
+    out, lse = b.gpu(P, scale=scale)
+    assert torch.isfinite(out).all()
+    close(b, out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("nq,L", [(1, 90), (90, 200)])
+def test_keys_orthogonal_to_large_queries(nq, L):
+    """q . k = 0 exactly, beside a factor that passes fp32's range: a logit of 0."""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, BF16)
+    b.q[:] = 0
+    b.q[..., 0] = 2.0 ** 126
+    t = torch.arange(L)
+    slots = (b.table[0, t // 16] * 16 + t % 16).int().cuda()
+    k = rows(torch.Generator().manual_seed(2), L, 2, 64, BF16).float() * 2.0 ** 110
+    k[..., 0] = 0
+    _, v16 = P.kv4_read(b.cache, slots, BF16)
+    P.kv4_write(k.to(BF16).cuda(), v16, b.cache, slots)
+    b.k[0], b.v[0] = plain.quantise(k.to(BF16))[3], plain.quantise(v16.cpu())[3]
+    close(b, *b.gpu(P))

@@ -48,7 +48,8 @@ struct Kv4AttnParams {
     int q_st, q_sh, o_st, o_sh;
     int num_pages, pages_per_seq, T, B, Hq, Hkv, page_shift, max_q, max_kv;
     int least_q, most_q;              // sequences of fewer or more queries are another kernel's
-    float scale_log2;                 // scale * log2(e)
+    float scale_mant;                 // scale * log2(e) = scale_mant 2^scale_exp, |scale_mant| < 1
+    int scale_exp;
     int causal, window;
     uint32_t* counters;               // kv4_few.hip: one a sequence, head and tile, zero between calls
     float* partials;                  // by number of chunk, slot_cols (D + 2) floats each

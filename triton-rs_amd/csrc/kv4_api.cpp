@@ -264,7 +264,7 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
     p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
     p.page_shift = __builtin_ctz((unsigned)page_size);
     p.max_kv = max_kv_len;
-    p.scale_log2 = scale_log2; p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
+    p.scale_mant = std::frexp(scale_log2, &p.scale_exp); p.causal = causal != 0; p.window = window < (1 << 30) ? window : 1 << 30;
     p.counters = static_cast<uint32_t*>(workspace);
     p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A16_KV4_COUNTER_BYTES);
     p.G = Hq / Hkv;

@@ -53,11 +53,9 @@ __device__ __forceinline__ float value_scale(uint32_t w) {
     if constexpr (VALUE_DOWN<E> == 0) return param_scale<E>(w);
     else return param_scale<E>(w) * (1.f / (1 << VALUE_DOWN<E>));
 }
-// log2 of a number above value scales, from the bits of their largest (NaN beyond all numbers)
-template <typename E>
-__device__ __forceinline__ float log2_above(uint32_t top) {
-    return (float)((int)(max(top, __builtin_bit_cast(uint32_t, LEAST_SCALE<E>)) >> 23) - 126);
-}
+// log2 of a number above value scales, from the bits of their largest (NaN beyond all numbers), of `least` at least
+__device__ __forceinline__ float log2_above(uint32_t top, uint32_t least) { return (float)((int)(max(top, least) >> 23) - 126); }
+constexpr uint32_t INF_BITS32 = 0x7F800000u;
 // what sum_j (p_j s_j) (n_j - z_j) is multiplied by, l = sum_j p_j
 template <typename E>
 __device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : (float)(1 << VALUE_DOWN<E>) / l; }
@@ -180,7 +178,9 @@ struct Kv4Cols {
     int jlo, jhi;          // keys that some column sees, of the chunk
     int all_lo, all_hi;    // keys that every column sees
     half8_t qf[NT][KW];
-    float kscale;          // logits in base 2 are kscale s (q . (n - z))
+    float kscale;          // logits in base 2 are 2^shift kscale s (q . (n - z)), shift 0 but for numbers far from 1
+    int shift;
+    uint32_t least;        // for log2_above: LEAST_SCALE, or infinity, which takes every step to uncommon()
     float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
     float most[NT];        // KV4_MOST, -infinity until a column has seen a key
     float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
@@ -245,12 +245,17 @@ struct Kv4Cols {
     }
 
     // q in operand order under the power of two that `top`, the largest of the rows, gives: 2^13 to 2^14, or (fp16,
-    // whose own range is enough) less where q is small
+    // whose own range is enough: no bit is lost upwards) less where q is small, more where it is larger
     __device__ __forceinline__ void start(const Kv4AttnParams& p, float top) {
         constexpr bool F16 = __is_same(E, half_t);
-        const int e2 = top > 0.f ? min(F16 ? 15 : 100, max(F16 ? -14 : -100, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
+        const int e2 = top > 0.f ? min(F16 ? 15 : 126, max(F16 ? 0 : -114, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
         const float up = pow2(e2);
-        kscale = p.scale_log2 * pow2(-e2);
+        // a key scale (below 2^126) times kscale does not overflow, and what is below fp32's normal range is of no
+        // account in a logit; the rest of the factor comes last
+        const int e = __builtin_amdgcn_readfirstlane(p.scale_exp - e2), a = min(-1, max(-60, e));
+        kscale = p.scale_mant * pow2(a);
+        shift = e - a;
+        least = shift ? INF_BITS32 : __builtin_bit_cast(uint32_t, LEAST_SCALE<E>);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -286,6 +291,23 @@ struct Kv4Cols {
         return Seen{lo[t] - at, min(hi[t], end) - at, bad};
     }
 
+    // What few steps need before their logits: those with a value scale of NaN, or all where `shift` is not 0. (Two tests, and
+    // two branches of either column tile, cost 1024 queries over 32768 keys 690 us, 683 two tests in one place.)
+    __device__ __forceinline__ void uncommon(float4_t (&acc)[NT][2], float (&ks)[2][4], float (&vs)[2][4], float above, bool whole, int j,
+                                             int end, int bad, int kb) {
+        if (__builtin_expect(!__any(above > 128.f), 1)) return;
+        if (shift) {   // the whole factor, on the products
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t][s][i] = __builtin_ldexpf(acc[t][s][i] * ks[s][i], shift);
+                    ks[s][i] = 1.f;
+                }
+        }
+        if (!whole) value_nan(vs, j, end, bad, kb);
+    }
     // A value row of NaN (its scale is) makes those columns NaN that see it, whatever its weight, and no others. Where all
     // see it its weights do that; here, where some do not, they become 0 and the columns NaN by themselves.
     __device__ __forceinline__ void value_nan(float (&vs)[2][4], int j, int end, int bad, int kb) {
@@ -337,7 +359,7 @@ struct Kv4Cols {
                 for (int i = 0; i < 4; ++i) {
                     float v = vs[s][i];
                     asm volatile("" : "+v"(v));   // (else all steps take the scales' exponents ahead: 740 us for the 660 of kv4_many.hip)
-                    top = fmaxf(top, x[s][i] + log2_above<E>(__float_as_uint(fmaxf(v, 0.f))));   // (NaN as 0)
+                    top = fmaxf(top, x[s][i] + log2_above(__float_as_uint(fmaxf(v, LEAST_SCALE<E>)), 0u));   // (NaN as the least)
                 }
             top = kb_max(top);
             const bool up = top > most[t];

@@ -323,8 +323,8 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
                 vs[s][i] = value_scale<E>(vp[s][i]);
                 vmax = max(vmax, __float_as_uint(vs[s][i]));
             }
-        const float above = log2_above<E>(vmax);
-        if (!whole && __any(above > 128.f)) a.value_nan(vs, j, end, here, kb);   // (a scale of NaN)
+        const float above = log2_above(vmax, a.least);
+        a.uncommon(acc, ks, vs, above, whole, j, end, here, kb);
         half8_t pw[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {

@@ -23,7 +23,7 @@ struct ManyLds {
     half8_t k[4][KW][64];      // block, word of the quarter row, lane
     half8_t v[2][VT][64];      // pair of blocks, tile of the result, lane (first block's two pairs, second's)
     float ks[64], vs[64];      // scales of the tokens, those of keys times kscale
-    float above[4];            // of a block's value scales: log2_above
+    float above[4];            // log2_above of a block's value scales
     int live[4];               // tokens of a block that there are (0 or less: none)
 };
 
@@ -65,7 +65,7 @@ __device__ __forceinline__ void load_packed(Packed<D>& t, const unsigned char* b
 
 // Block `wave` of a step into LDS; its tokens [dead, live) (the others' parameters may be anything)
 template <typename E, int D>
-__device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int live, float kscale, int wave, int lane) {
+__device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int live, float kscale, uint32_t least, int wave, int lane) {
     const int col = lane & 15, kb = lane >> 4;
     t.kc = col >= dead && col < live ? t.kc : 0u;
 #pragma unroll
@@ -103,7 +103,7 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
     top = kb_umax(top);
     if (col == 0) *reinterpret_cast<float4_t*>(&s.vs[16 * wave + 4 * kb]) = f;
     if (lane == 0) {
-        s.above[wave] = log2_above<E>(top);
+        s.above[wave] = log2_above(top, least);
         s.live[wave] = live;
     }
 }
@@ -186,14 +186,14 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     __syncthreads();
 
     if (any) {   // (only a first step holds tokens before what its columns see)
-        unpack<E, D>(lds[0][group], t, w.see_lo(p, w.n <= 1 ? 0 : w.c0 / p.G) - (w.k0 + STEP * group + 16 * wave), live, a.kscale, wave, lane);
+        unpack<E, D>(lds[0][group], t, w.see_lo(p, w.n <= 1 ? 0 : w.c0 / p.G) - (w.k0 + STEP * group + 16 * wave), live, a.kscale, a.least, wave, lane);
         fetch(w.k0 + ALL);
     }
     __syncthreads();
     int buf = 0;
     for (int j = w.k0; j < w.k1; j += ALL, buf ^= 1) {
         if (j + ALL < w.k1) {
-            unpack<E, D>(lds[buf ^ 1][group], t, 0, live, a.kscale, wave, lane);
+            unpack<E, D>(lds[buf ^ 1][group], t, 0, live, a.kscale, a.least, wave, lane);
             fetch(j + 2 * ALL);
         }
         const ManyLds<D>& s = lds[buf][group];
@@ -233,8 +233,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            if (__builtin_expect(__any(above > 128.f), 0))   // (a scale of NaN)
-                if (!whole) a.value_nan(vs, jh, a.jhi, bad, kb);
+            a.uncommon(acc, ks, vs, above, whole, jh, a.jhi, bad, kb);
             float x[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], ks, vs, above, whole, jh, a.jhi, bad, kb);

@@ -1,5 +1,5 @@
-"""The 4-bit key/value cache at the ends of its numbers' range: rows near the type's largest value, value rows many powers
-of two apart, queries of any magnitude. Compared with 64 bits (kv4_plain.py)."""
+"""The 4-bit key/value cache at the ends of its numbers' range: rows near the type's largest value, value rows and queries
+many powers of two apart, queries of any magnitude. Compared with 64 bits (kv4_plain.py)."""
 import numpy as np
 import pytest
 import torch
@@ -156,3 +156,22 @@ def test_keys_orthogonal_to_large_queries(nq, L):
     P.kv4_write(k.to(BF16).cuda(), v16, b.cache, slots)
     b.k[0], b.v[0] = plain.quantise(k.to(BF16))[3], plain.quantise(v16.cpu())[3]
     close(b, *b.gpu(P))
+
+
+@pytest.mark.parametrize("far", [2.0 ** 30, 2.0 ** 60, 2.0 ** 115, 2.0 ** -30, 2.0 ** -100])
+@pytest.mark.parametrize("nq,L,Hq", [(1, 90, 8), (1, 1500, 24), (5, 300, 8), (90, 200, 4)])
+def test_queries_of_many_magnitudes(far, nq, L, Hq):
+    """One query row many powers of two larger or smaller than its neighbours costs them no bits."""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], Hq, 2, 64, 16, BF16)
+    odd = (nq // 2, 1)
+    b.q[odd] = (b.q[odd].double() * far).to(BF16)
+    close(b, *b.gpu(P), but=(odd,) if far > 1 else ())   # (its own logits are far beyond what exp tells apart)
+    # and the others' results do not depend on it
+    first = b.gpu(P)
+    b.q[odd] = b.q[odd] * 0 + 1
+    second = b.gpu(P)
+    keep = torch.ones(first[1].shape, dtype=torch.bool)
+    keep[odd] = False
+    tol = 2.0 ** -7 * first[0].double().abs().max()
+    assert float((first[0].double() - second[0].double()).abs()[keep.cuda()].max()) <= tol

@@ -17,8 +17,8 @@
 // keys 32 at a time. With S^T = K Q^T a lane has the logits of one column at tokens 4 (lane / 16) + i of
 // either block of 16, which is how the second product takes them as its operand (the sum over the
 // tokens may run in any order as long as the values follow), so no logit or weight passes between lanes
-// or through LDS. q is scaled by a power of two (wave-wide) into fp16's range, exactly for fp16 and bf16
-// alike but for what lies 2^27 below the largest. A weight p_j s_j is rounded to fp16 (2^-11, of what the matrix
+// or through LDS. q is scaled by powers of two into fp16's range: exactly for fp16, for bf16 but for what
+// lies 2^24 below a row's largest. A weight p_j s_j is rounded to fp16 (2^-11, of what the matrix
 // cores take the type with the most bits); the reference m is such that the largest of them is 2^7 when it is set and
 // 2^15 at most, so it follows logits and value scales together: a row of large values and no weight takes no bits
 // from the others. It is raised (with the sums scaled down) only where a step's largest logit and largest value
@@ -179,8 +179,8 @@ struct Kv4Cols {
     int all_lo, all_hi;    // keys that every column sees
     half8_t qf[NT][KW];
     float kscale;          // logits in base 2 are 2^shift kscale s (q . (n - z)), shift 0 but for numbers far from 1
-    int shift;
-    uint32_t least;        // for log2_above: LEAST_SCALE, or infinity, which takes every step to uncommon()
+    int shift[NT];         // (of column lane % 16) or from the others'
+    uint32_t least;        // for log2_above: LEAST_SCALE, or (some shift is not 0) infinity: every step goes to uncommon()
     float m[NT], l[NT];    // reference and sum of p_j = exp2(logit - m)
     float most[NT];        // KV4_MOST, -infinity until a column has seen a key
     float4_t o[NT][VT];    // of column lane % 16, dimensions (4 (lane / 16) + i) D / 16 + x in o[t][x][i]
@@ -211,53 +211,83 @@ struct Kv4Cols {
         all_hi = w.see_hi(p, i0);
     }
 
-    // the largest |q| of the wave's rows, infinities and NaN aside
-    __device__ __forceinline__ float largest() const {
+    // |q| of the wave's rows, infinities and NaN aside: the largest of each column, the largest and the smallest of these
+    // (zeros aside)
+    struct Sizes { float top, low, own[NT]; };
+    __device__ __forceinline__ Sizes sizes() const {
         typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
         constexpr uint32_t inf = __is_same(E, half_t) ? 0x7C00u : 0x7F80u;
-        ushort2_t top = {0, 0};   // (bits of non-negative numbers are ordered)
+        uint32_t most[NT], low = ~0u, top = 0;   // (bits of non-negative numbers are ordered)
+        bool odd = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+            ushort2_t m = {0, 0};
 #pragma unroll
             for (int x = 0; x < KW; ++x) {
                 const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, v[e] & 0x7FFF7FFFu));
+                for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, v[e] & 0x7FFF7FFFu));
             }
-        uint32_t most = max((uint32_t)top[0], (uint32_t)top[1]);
-        if (__any(most >= inf)) {
-            most = 0;
+            most[t] = max((uint32_t)m[0], (uint32_t)m[1]);
+            odd |= most[t] >= inf;
+        }
+        if (__any(odd)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                most[t] = 0;
 #pragma unroll
                 for (int x = 0; x < KW; ++x) {
                     const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t a = (v[e >> 1] >> (16 * (e & 1))) & 0x7FFFu;
-                        most = max(most, a < inf ? a : 0u);
+                        most[t] = max(most[t], a < inf ? a : 0u);
                     }
                 }
+            }
+        }
+        Sizes r;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            most[t] = kb_umax(most[t]);
+            r.own[t] = param_scale<E>(most[t]);
+            top = max(top, most[t]);
+            low = min(low, most[t] - 1);   // (0 as the largest)
         }
 #pragma unroll
-        for (int x = 1; x < 16; x <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, x));
-        return kb_max(param_scale<E>(most));
+        for (int x = 1; x < 16; x <<= 1) {
+            top = max(top, (uint32_t)__shfl_xor((int)top, x));
+            low = min(low, (uint32_t)__shfl_xor((int)low, x));
+        }
+        r.top = param_scale<E>(top);
+        r.low = param_scale<E>(low == ~0u ? top : low + 1);
+        return r;
     }
-
-    // q in operand order under the power of two that `top`, the largest of the rows, gives: 2^13 to 2^14, or (fp16,
-    // whose own range is enough: no bit is lost upwards) less where q is small, more where it is larger
-    __device__ __forceinline__ void start(const Kv4AttnParams& p, float top) {
+    // The power of two that takes queries of which `top` is the largest into fp16: to 2^13 to 2^14, or (fp16, whose own
+    // range is enough: no bit is lost upwards) less where they are small, more where they are larger.
+    __device__ __forceinline__ static int power(float top) {
         constexpr bool F16 = __is_same(E, half_t);
-        const int e2 = top > 0.f ? min(F16 ? 15 : 126, max(F16 ? 0 : -114, 13 - (int)(__float_as_uint(top) >> 23) + 127)) : 0;
-        const float up = pow2(e2);
+        return top > 0.f ? min(F16 ? 15 : 126, max(F16 ? 0 : -114, 13 - exponent(top))) : 0;
+    }
+    __device__ __forceinline__ static int exponent(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }
+
+    // q in operand order under the power of two of the largest of the rows; bf16 rows whose own largest is less than 2^-6
+    // of it have one of their own, so that what lies 2^24 below a row's largest loses bits at most. (r.top, r.low: of the
+    // wave's rows or more, the same in all waves that share kscale and least.)
+    __device__ __forceinline__ void start(const Kv4AttnParams& p, const Sizes& r) {
+        constexpr bool F16 = __is_same(E, half_t);
+        constexpr int APART = 6;
+        const int e2 = power(r.top), far = exponent(r.top) - APART;
         // a key scale (below 2^126) times kscale does not overflow, and what is below fp32's normal range is of no
         // account in a logit; the rest of the factor comes last
         const int e = __builtin_amdgcn_readfirstlane(p.scale_exp - e2), a = min(-1, max(-60, e));
         kscale = p.scale_mant * pow2(a);
-        shift = e - a;
-        least = shift ? INF_BITS32 : __builtin_bit_cast(uint32_t, LEAST_SCALE<E>);
+        least = __any(e != a || (!F16 && exponent(r.low) < far)) ? INF_BITS32 : __builtin_bit_cast(uint32_t, LEAST_SCALE<E>);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            const int et = !F16 && r.own[t] > 0.f && exponent(r.own[t]) < far ? power(r.own[t]) : e2;
+            const float up = pow2(et);
+            shift[t] = p.scale_exp - et - a;
 #pragma unroll
             for (int x = 0; x < KW; ++x) {
                 const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
@@ -291,18 +321,18 @@ struct Kv4Cols {
         return Seen{lo[t] - at, min(hi[t], end) - at, bad};
     }
 
-    // What few steps need before their logits: those with a value scale of NaN, or all where `shift` is not 0. (Two tests, and
+    // What few steps need before their logits: those with a value scale of NaN, or all where a `shift` is not 0. (Two tests, and
     // two branches of either column tile, cost 1024 queries over 32768 keys 690 us, 683 two tests in one place.)
     __device__ __forceinline__ void uncommon(float4_t (&acc)[NT][2], float (&ks)[2][4], float (&vs)[2][4], float above, bool whole, int j,
                                              int end, int bad, int kb) {
         if (__builtin_expect(!__any(above > 128.f), 1)) return;
-        if (shift) {   // the whole factor, on the products
+        if (least == INF_BITS32) {   // the whole factor, on the products
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) acc[t][s][i] = __builtin_ldexpf(acc[t][s][i] * ks[s][i], shift);
+                    for (int t = 0; t < NT; ++t) acc[t][s][i] = __builtin_ldexpf(acc[t][s][i] * ks[s][i], shift[t]);
                     ks[s][i] = 1.f;
                 }
         }

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
         const int at = beg + s * stride;
         if (at < end) fetch(s, at, pages.page(at >> 4), pages.page((at >> 4) + 1));
     }
-    a.start(p, a.largest());
+    a.start(p, a.sizes());
 
     int slot = 0;
     // the pages of the step that takes this one's slot

@@ -177,12 +177,16 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     };
     const bool any = w.k0 < w.k1;
     if (any) fetch(w.k0);
-    // one power of two for the workgroup's rows of q
-    float top = a.largest();
-    if (lane == 0 && group == 0) ml[wave][0] = top;   // (the groups have the same rows)
+    // one factor of the key scales for the workgroup's rows of q
+    typename C::Sizes q = a.sizes();
+    if (lane == 0 && group == 0) {   // (the groups have the same rows)
+        ml[wave][0] = q.top;
+        ml[wave][1] = q.top > 0.f ? q.low : INFINITY;
+    }
     __syncthreads();
-    top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
-    a.start(p, top);
+    q.top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
+    q.low = fminf(fminf(ml[0][1], ml[1][1]), fminf(ml[2][1], ml[3][1]));
+    a.start(p, q);
     __syncthreads();
 
     if (any) {   // (only a first step holds tokens before what its columns see)

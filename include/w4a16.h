@@ -399,7 +399,9 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  *   powers of two (what lies 2^24 below the largest of a query and head loses bits), and out is
  *   rounded once (to its type's largest finite value).
  * A query that sees no key: out 0, lse -infinity. What a query does not see moves no bit of its
- * result, whatever the cache holds there; a key or value row of NaN that it does see makes it NaN.
+ * result, whatever the cache holds there; a key or value row of NaN that it does see makes it NaN,
+ * and so does an infinity or NaN of its own where it sees a key. (A scale q . k that fp32 does not
+ * hold has no defined result.)
  * Keys in a page whose number is outside [0, num_pages) are not seen. Rows of q outside every
  * sequence are left as they were in out and lse. max_q_len and max_kv_len bound the sequences of
  * the call (they choose the kernels and the split of the work); a kv_lens entry beyond max_kv_len

@@ -1,5 +1,5 @@
-"""The 4-bit key/value cache at the ends of its numbers' range: rows near the type's largest value, value rows and queries
-many powers of two apart, queries of any magnitude. Compared with 64 bits (kv4_plain.py)."""
+"""The 4-bit key/value cache at the ends of its numbers' range: rows near the type's largest value, value
+rows and queries many powers of two apart, infinities. Compared with 64 bits (kv4_plain.py)."""
 import numpy as np
 import pytest
 import torch
@@ -175,3 +175,25 @@ def test_queries_of_many_magnitudes(far, nq, L, Hq):
     keep[odd] = False
     tol = 2.0 ** -7 * first[0].double().abs().max()
     assert float((first[0].double() - second[0].double()).abs()[keep.cuda()].max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,L", [(1, 1), (1, 90), (1, 1500), (90, 200)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_queries_are_nan(dtype, nq, L, sign):
+    """An infinite query has no softmax: its logits are infinities of either sign or NaN. Also where all of them
+    are -infinity, which is not a row that sees nothing."""
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, dtype)
+    t = torch.arange(L)
+    slots = (b.table[0, t // 16] * 16 + t % 16).int().cuda()
+    k = rows(torch.Generator().manual_seed(2), L, 2, 64, dtype)
+    k[..., 7] = -3.0
+    _, v16 = P.kv4_read(b.cache, slots, dtype)
+    P.kv4_write(k.cuda(), v16, b.cache, slots)
+    b.k[0], b.v[0] = plain.quantise(k)[3], plain.quantise(v16.cpu())[3]
+    b.q[nq // 2, 1, 7] = sign * float("inf")
+    out, lse = b.gpu(P)
+    assert torch.isnan(out[nq // 2, 1]).all() and torch.isnan(lse[nq // 2, 1])
+    assert int(torch.isnan(out).sum()) == 64
+    close(b, out, lse, but=((nq // 2, 1),))

@@ -212,9 +212,10 @@ struct Kv4Cols {
     }
 
     // |q| of the wave's rows, infinities and NaN aside: the largest of each column, the largest and the smallest of these
-    // (zeros aside)
+    // (zeros aside). Infinities become NaN: a query that has one is NaN where it sees a key, as infinite logits have no
+    // softmax, while all of them -infinity would look like a query that sees none.
     struct Sizes { float top, low, own[NT]; };
-    __device__ __forceinline__ Sizes sizes() const {
+    __device__ __forceinline__ Sizes sizes() {
         typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
         constexpr uint32_t inf = __is_same(E, half_t) ? 0x7C00u : 0x7F80u;
         uint32_t most[NT], low = ~0u, top = 0;   // (bits of non-negative numbers are ordered)
@@ -237,12 +238,14 @@ struct Kv4Cols {
                 most[t] = 0;
 #pragma unroll
                 for (int x = 0; x < KW; ++x) {
-                    const u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
+                    u32x4 v = __builtin_bit_cast(u32x4, qf[t][x]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t a = (v[e >> 1] >> (16 * (e & 1))) & 0x7FFFu;
                         most[t] = max(most[t], a < inf ? a : 0u);
+                        v[e >> 1] |= a < inf ? 0u : 0x7FFFu << (16 * (e & 1));
                     }
+                    qf[t][x] = __builtin_bit_cast(half8_t, v);
                 }
             }
         }

@@ -100,13 +100,19 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
     int64_t items = std::max<int64_t>(1, tiles * B * Hkv);
     s.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
     size_t slots = 0;
+    // Few rows for what the sequences may have: single tokens among prompts. Walking a long cache for 128 columns of which
+    // few are there holds up the rest (31 single tokens and a chunk of 1024, 4096 keys each, 32 heads on 8, D = 128: 382 us
+    // on the kernel for many columns alone, 161 on both).
+    const int few_q = (int)(64 / G);
+    s.few_q = s.many && B > 1 && few_q > 0 && 4 * (int64_t)T < (int64_t)B * max_q ? few_q : 0;
     if (s.many) {
         // Up to 1024 sequences share one row of tiles where that is less than half of as many as the longest has for each:
         // no more tiles than T rows of q make. (Finding its own costs a workgroup a microsecond.)
         const int64_t rows = std::max<int64_t>(1, (T * G + 127 * (int64_t)B) / 128);
         int64_t full = items;   // about as many as there are
         if (B > 1 && B <= 1024 && 2 * rows < tiles * B && rows <= 65535) {
-            s.rows = (int)rows;
+            // (launched: those of sequences that run here, which have a query at least, or more than few_q)
+            s.rows = (int)std::max<int64_t>(1, (T * G + 127 * std::min<int64_t>(B, T / (s.few_q + 1))) / 128);
             items = rows * Hkv;
             full = std::max<int64_t>(1, (T * G + 127) / 128 * Hkv);
         }
@@ -117,18 +123,15 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
         // (chunks of 512 keys or more: with a join in the kernel 64 queries over 4096 keys, 32 heads of D = 128, took
         // 39.9 us so, of 256 52.3, of 1024 41.5)
-        int64_t most = std::max<int64_t>(1, std::min((at_once + full - 1) / full, ((int64_t)max_kv + 511) / 512));
+        // as many as run at once: a last round for a few workgroups costs as much as a full one (154 queries of 24 heads on
+        // one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 67.6)
+        int64_t most = std::max<int64_t>(1, std::min(at_once / full, ((int64_t)max_kv + 511) / 512));
         if (items > KV4_MAX_SPLIT_TILES) most = 1;
-        auto chunk = [&](int64_t n) { return std::max<int64_t>(128, (((int64_t)max_kv + n - 1) / n + 127) / 128 * 128); };
-        // A last round for a few workgroups costs as much as a full one, and one besides its keys some 384 of them: 154
-        // queries of 24 heads on one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 67.6.
-        auto cost = [&](int64_t n) { return (full * n + at_once - 1) / at_once * (chunk(n) + 384); };
-        const int64_t even = std::min(most, std::max<int64_t>(1, at_once / full));
-        s.chunk = (int)chunk(cost(even) <= cost(most) ? even : most);
+        s.chunk = (int)std::max<int64_t>(128, (((int64_t)max_kv + most - 1) / most + 127) / 128 * 128);
         s.splits = std::max(1, (int)(((int64_t)max_kv + s.chunk - 1) / s.chunk));
         s.pair_tiles = full * s.splits <= at_once;
         s.slot_cols = wg_cols;
-        if (most > 1) slots = (size_t)items * most;   // (splits or more: enough for a smaller max_kv, too)
+        if (most > 1) slots = (size_t)items * most;   // (which grows with max_kv, and splits are no more: enough for a smaller one, too)
     } else {
         // chunks of a head and tile: what runs at once, or several rounds of it; B sequences have one each at least,
         // and a remainder
@@ -146,11 +149,6 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
         s.join_apart = !s.whole && (chunks > KV4_JOIN_CHUNKS || C * D * 4 * chunks >= KV4_JOIN_BYTES);
     }
     s.partial_bytes = slots * s.slot_cols * (D + 2) * sizeof(float);
-    // Few rows for what the sequences may have: single tokens among prompts. Walking a long cache for 128 columns of which
-    // few are there holds up the rest (31 single tokens and a chunk of 1024, 4096 keys each, 32 heads on 8, D = 128: 382 us
-    // on the kernel for many columns alone, 161 on both).
-    const int few_q = (int)(64 / G);
-    s.few_q = s.many && B > 1 && few_q > 0 && 4 * (int64_t)T < (int64_t)B * max_q ? few_q : 0;
     return s;
 }
 // The part of such a batch that runs on kv4_few.hip.

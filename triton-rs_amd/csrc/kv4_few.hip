@@ -127,6 +127,7 @@ __device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u
     if (p.whole) {   // sequence u, in one chunk
         w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
         w.take(0, 1, 0, lo, hi);
+        w.at = w.slot = 0;   // (no partial results)
         return w.cols > 0;
     }
     Kv4Item mine;

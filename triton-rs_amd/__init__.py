@@ -734,6 +734,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     _kv4_index(kv_lens, "kv_lens", dev, (B,))
     if cu_q is not None:
         _kv4_index(cu_q, "cu_q", dev, (B + 1,))
+    elif T != B:   # (also where one is 0, and there would be nothing to launch)
+        raise InvalidArgument(f"without cu_q every sequence has one query ({T} queries, {B} sequences)")
     if max_q_len is None:
         max_q_len = 1 if cu_q is None else max(1, T)
     if max_kv_len is None:

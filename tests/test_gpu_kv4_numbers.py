@@ -197,3 +197,15 @@ def test_infinite_queries_are_nan(dtype, nq, L, sign):
     assert torch.isnan(out[nq // 2, 1]).all() and torch.isnan(lse[nq // 2, 1])
     assert int(torch.isnan(out).sum()) == 64
     close(b, out, lse, but=((nq // 2, 1),))
+
+
+@pytest.mark.parametrize("dtype,k,v,scale", [(BF16, 2.0 ** 120, 1.0, 2.0 ** -122), (BF16, 1.0, 2.0 ** 125, 0.125), (F16, 300.0, 1.0, 2.0 ** -9),
+                                             (F16, 1.0, 1.2e4, 0.125), (F16, 2.0 ** -12, 2.0 ** -12, 2.0 ** 9), (BF16, 2.0 ** -124, 2.0 ** -50, 2.0 ** 121)])
+@pytest.mark.parametrize("nq,L", [(1, 90), (1, 1500), (90, 200)])
+def test_keys_and_values_at_the_ends(dtype, k, v, scale, nq, L):
+    P = need_gpu()
+    b = Batch(P, [nq], [L], 4, 2, 64, 16, dtype, kscale=k, vscale=v)
+    assert np.isfinite(b.k[0]).all() and np.isfinite(b.v[0]).all()
+    out, lse = b.gpu(P, scale=scale)
+    assert torch.isfinite(out).all()
+    close(b, out, lse, scale=scale)

@@ -395,9 +395,8 @@ W4A16_API int w4a16_kv4_read(void* stream, int elem, const void* cache, const in
  *   p_j times the value row's scale is rounded to fp16 before its product with n - zero: by 2^-11 of
  *   it, or 2^-32 of the query's largest such product where that is more (a scale below 2^-60 counts
  *   as 2^-60 in that largest), so a value row of any size that has no weight takes no bits from the
- *   others. bf16 queries are taken in fp16 under
- *   powers of two (what lies 2^24 below the largest of a query and head loses bits), and out is
- *   rounded once (to its type's largest finite value).
+ *   others. bf16 queries are taken in fp16 under powers of two (what lies 2^24 below the largest of
+ *   a query and head loses bits), and out is rounded once (to its type's largest finite value).
  * A query that sees no key: out 0, lse -infinity. What a query does not see moves no bit of its
  * result, whatever the cache holds there; a key or value row of NaN that it does see makes it NaN,
  * and so does an infinity or NaN of its own where it sees a key. (A scale q . k that fp32 does not

@@ -720,7 +720,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     logarithm of each row's sum of exponentials. A row that sees no key is 0, its lse -infinity; rows
     of q behind the last sequence are left as they were in out and lse (0 in an out made here).
     max_q_len, max_kv_len: bounds on the batch (T, or 1 without cu_q, and the table's width unless
-    given). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
+    given; close ones make a better plan and a far smaller workspace). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
     given."""
     pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
     qst, qsh = _kv4_rows(q, "q", _ELEM, dev)

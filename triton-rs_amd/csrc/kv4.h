@@ -75,12 +75,12 @@ struct Kv4AttnShape {
     size_t partial_bytes;
     int few_q;         // many: sequences of up to this many queries go to kv4_few.hip first (0: none do)
 };
-// Workgroups of kv4_few.hip that a compute unit holds, by registers (95, 142; 125, 194; 159; 193 of D = 64, 128, 192, 256
-// with one and, up to 128, two column tiles a wave) and LDS.
+// Workgroups of kv4_few.hip that are planned for a compute unit: what registers (90, 130; 123, 187; 157; 190 of D = 64, 128,
+// 192, 256 with one and, up to 128, two column tiles a wave) and LDS leave room for, one less at D = 64 with one tile.
 constexpr int kv4_few_per_cu(int D, int nt) { return nt == 2 ? (D == 64 ? 3 : 2) : D <= 128 ? 4 : D == 192 ? 3 : 2; }
 constexpr int KV4_WHOLE_KEYS = 512;   // keys that kv4_few.hip leaves in one chunk
 hipError_t launch_kv4_few(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
-// Waves of kv4_many.hip a SIMD, by registers (some 150, 221, 388 and 496 of D = 64, 128, 192 and 256).
+// Waves of kv4_many.hip a SIMD, by registers (144, 213, 376 and 485 of D = 64, 128, 192 and 256).
 constexpr int kv4_many_simd_waves(int D, int groups) { return D == 64 && groups == 1 ? 3 : D <= 128 ? 2 : 1; }
 hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st);
 

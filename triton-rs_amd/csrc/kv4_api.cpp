@@ -102,7 +102,7 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
     size_t slots = 0;
     // Few rows for what the sequences may have: single tokens among prompts. Walking a long cache for 128 columns of which
     // few are there holds up the rest (31 single tokens and a chunk of 1024, 4096 keys each, 32 heads on 8, D = 128: 382 us
-    // on the kernel for many columns alone, 161 on both).
+    // on the kernel for many columns alone, 181 on both; 139 in a call each, where the chunk's tiles are counted alone and split).
     const int few_q = (int)(64 / G);
     s.few_q = s.many && B > 1 && few_q > 0 && 4 * (int64_t)T < (int64_t)B * max_q ? few_q : 0;
     if (s.many) {
@@ -116,15 +116,14 @@ static Kv4AttnShape kv4_attention_shape(int T, int B, int Hq, int Hkv, int D, in
             items = rows * Hkv;
             full = std::max<int64_t>(1, (T * G + 127) / 128 * Hkv);
         }
-        // Up to two tiles a compute unit, the longest one sets the time: two groups of waves share its keys (a prompt of
-        // 2048, 32 heads: 66 us, one group 75; 1344 tiles of 7 prompts: 58, one 45). Not where the tiles are of one
-        // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664).
+        // Up to two tiles a compute unit: two groups of waves share a tile's keys (a prompt of
+        // 2048, 32 heads: 64 us, one group 75; 1344 tiles of 7 prompts: 58, one 45). Not where the tiles are of one
+        // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664, before the reference followed the value scales).
         s.groups = D <= 128 && full <= 2 * KV4_CUS && !(full >= KV4_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
         const int64_t at_once = slots_of_cu * kv4_many_simd_waves(D, s.groups) / s.groups;
-        // (chunks of 512 keys or more: with a join in the kernel 64 queries over 4096 keys, 32 heads of D = 128, took
-        // 39.9 us so, of 256 52.3, of 1024 41.5)
-        // as many as run at once: a last round for a few workgroups costs as much as a full one (154 queries of 24 heads on
-        // one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 67.6)
+        // Chunks of 512 keys or more (64 queries over 4096 keys, 32 heads on 8 of D = 128, 30.5 us so, of 256 34.3, of 1024
+        // 36.3; over 2048 26.0, 25.4, 34.4), as many as run at once: a last round for a few workgroups costs as much as a full
+        // one (154 queries of 24 heads on one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 69.4).
         int64_t most = std::max<int64_t>(1, std::min(at_once / full, ((int64_t)max_kv + 511) / 512));
         if (items > KV4_MAX_SPLIT_TILES) most = 1;
         s.chunk = (int)std::max<int64_t>(128, (((int64_t)max_kv + most - 1) / most + 127) / 128 * 128);

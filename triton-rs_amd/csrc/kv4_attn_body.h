@@ -391,7 +391,7 @@ struct Kv4Cols {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float v = vs[s][i];
-                    asm volatile("" : "+v"(v));   // (else all steps take the scales' exponents ahead: 740 us for the 660 of kv4_many.hip)
+                    asm volatile("" : "+v"(v));   // (else all steps take the scales' exponents ahead: 740 us for the 668 of kv4_many.hip)
                     top = fmaxf(top, x[s][i] + log2_above(__float_as_uint(fmaxf(v, LEAST_SCALE<E>)), 0u));   // (NaN as the least)
                 }
             top = kb_max(top);

@@ -9,7 +9,7 @@
 //
 // Measured: 4 sequences of 65536 keys, 32 heads on 8 of D = 128, 65 us a call, 4.4 TB/s (a large copy
 // reaches 4.8): 61 in this kernel, which issues vector instructions in half of its cycles, 5 in the join.
-// 48 sequences of up to 4096 keys 40 us, 3.1 TB/s, every step as fast but a start and an end of some
+// 48 sequences of up to 4096 keys 39 us, 3.2 TB/s, every step as fast but a start and an end of some
 // 6 us. One of 500 keys 9.5 us: launch, lengths, pages, first keys and the join of the waves one
 // after another. 8 drafts of 5 tokens over windows of 4096 keys, 16 heads on 2 of D = 256, 27 us,
 // 22 of them here with four steps a wave, likewise a chain.
@@ -99,9 +99,9 @@ __device__ __forceinline__ int few_length(const Kv4AttnParams& p, unsigned sum, 
             break;
         }
     }
-    // In steps of a full device (0.85 us at D = 128): a round of workgroups costs 6 besides its steps, a step of one
-    // workgroup alone 0.45, joining 7. Whole and in two, 8 heads of D = 128: 128 sequences of 1000 keys 35, 49 us, 256
-    // of 900 60, 103; 48 of 4096 56, 54.
+    // In steps of a full device (0.85 us at D = 128, the only one these were measured at): a round of workgroups costs 6 besides its steps, a step of one
+    // workgroup alone 0.45, joining 7. Whole and in two, 8 heads of D = 128: 128 sequences of 1000 keys 34, 49 us, 256
+    // of 900 58, 103; 48 of 4096 56, 54.
     auto cost = [&](unsigned chunks, int steps) {
         const float rounds = (float)((chunks + p.at_once - 1) / p.at_once);
         return 6.f * rounds + fmaxf(0.45f * rounds * (float)steps, (float)sum / (float)p.at_once);

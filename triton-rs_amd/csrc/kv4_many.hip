@@ -6,11 +6,14 @@
 // take them (16 bytes a lane, no bank conflicts), while the step before is computed from the other half
 // of the LDS: one barrier a step. The packed words come two steps ahead into registers.
 //
-// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, bf16, 660 us: 820 TFLOP/s, 69 % of a
-// large matrix product's 1185. The matrix cores are busy in 32 % of the cycles, the vector unit in 52 %;
+// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, bf16, 668 us: 810 TFLOP/s, 68 % of a
+// large matrix product's 1185. The matrix cores are busy in 32 % of the cycles, the vector unit in 55 %;
 // two waves a SIMD is what the results leave registers for, each a chain of products, softmax and products. Steps of 32 keys with a barrier each took 861 us, logits of one half beside the
-// weights of the other 754. A prompt of 2048 64 us: the last tile's 2048 keys one after another, halved
-// by a second group of waves. 7 prompts of up to 1500, 16 heads of D = 64, 44 us.
+// weights of the other 754. A prompt of 2048 64 us: 512 workgroups, one to a compute unit for
+// their LDS, a long tile and then a short one, 2080 keys together everywhere; at the rate above these are some 42 us, and the
+// rest stands around them in either (pages, q, first blocks, the groups' join). 7 prompts of up to 1500, 16 heads of D = 64,
+// 45 us. One wave a SIMD from D = 192 on: 512 queries over 8192 keys, 12 heads on 4 of 192, 102 us, 300 over 20000, 16 on 2 of
+// 256, 230, a third of that product's rate.
 #include "kv4_attn_body.h"
 
 namespace w4a16 {
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
 }
 
 // Joins the chunks of one tile: an eighth of its values a workgroup. (The last of the chunks' own workgroups took longer:
-// 64 queries over 4096 keys, 32 heads of D = 128, 8 chunks, 40.1 us, so 29.7; two chunks of 400 over 2000 40.2, 39.3.)
+// 64 queries over 4096 keys, 32 heads of D = 128, 8 chunks, 40.1 us, so 30; two chunks of 400 over 2000 40.2, 39.3.)
 constexpr int MANY_PARTS = 8;
 template <typename E, int D>
 __global__ __launch_bounds__(256) void kv4_many_join_kernel(Kv4AttnParams p) {

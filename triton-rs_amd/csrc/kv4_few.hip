@@ -14,11 +14,10 @@
 // after another. 8 drafts of 5 tokens over windows of 4096 keys, 16 heads on 2 of D = 256, 27 us,
 // 22 of them here with four steps a wave, likewise a chain.
 #include "kv4_attn_body.h"
+#include "kv_few.h"
 #include "lds_dma.h"
 
 namespace w4a16 {
-
-constexpr int STEP = 32;   // keys of a step
 
 template <int D>
 struct FewShape {
@@ -72,153 +71,8 @@ __device__ __forceinline__ void take(uint32_t (&dst)[D / 32], const unsigned cha
     }
 }
 
-__device__ __forceinline__ unsigned wave_sum(int v) { return (unsigned)__builtin_amdgcn_readlane(wave_sums(v), 63); }
-__device__ __forceinline__ int wave_max(int v) { return __builtin_amdgcn_readlane(wave_scan(v, [](int a, int b) { return max(a, b); }), 63); }
-
-// Chunks of `steps` steps of keys in chunks of c 128 (4 c steps); -1: no columns here. Up to 512 keys stay whole, as a
-// chunk more costs its partial results' way to the last one and back: one sequence, 8 heads of D = 128, 500 keys 9.0 us
-// whole, 9.8 in chunks, 700 keys 11.0, 9.4; 4 drafts of 5 tokens, 8 heads a group, 500 keys 19.8, 20.5, 700 23.5, 17.2.
-__device__ __forceinline__ int few_chunks(int steps, int c) {
-    return steps < 0 ? 0 : steps <= max(KV4_WHOLE_KEYS / STEP, 4 * c) ? 1 : (steps + 4 * c - 1) / (4 * c);
-}
-
-// The length of chunks, in 128 keys, for sequences of `sum` steps together and `most` at most, total(c) their number:
-// at most p.budget of them, whatever the lengths. Keys / budget or keys / (budget - B / 2) where that is enough, else
-// keys / (budget - B) (the budget is twice B or more); or all sequences whole where that is estimated to take no longer.
-template <typename F>
-__device__ __forceinline__ int few_length(const Kv4AttnParams& p, unsigned sum, int most, F total) {
-    int c = 1;
-    unsigned n = p.budget;
-    for (int rest = 0; rest <= 4; rest += 2) {   // no remainders, half a chunk a sequence, one a sequence
-        const unsigned room = 4 * p.budget - rest * p.B;
-        c = (int)max(1u, (sum + room - 1) / room);
-        if (rest == 4) break;
-        const unsigned t = total(c);
-        if (t <= (unsigned)p.budget) {
-            n = t;
-            break;
-        }
-    }
-    // In steps of a full device (0.85 us at D = 128, the only one these were measured at): a round of workgroups costs 6 besides its steps, a step of one
-    // workgroup alone 0.45, joining 7. Whole and in two, 8 heads of D = 128: 128 sequences of 1000 keys 34, 49 us, 256
-    // of 900 58, 103; 48 of 4096 56, 54.
-    auto cost = [&](unsigned chunks, int steps) {
-        const float rounds = (float)((chunks + p.at_once - 1) / p.at_once);
-        return 6.f * rounds + fmaxf(0.45f * rounds * (float)steps, (float)sum / (float)p.at_once);
-    };
-    if (__builtin_amdgcn_readfirstlane(cost(p.B, most) <= cost(n, min(4 * c, most)) + 7.f)) c = max(c, (most + 3) / 4);
-    return c;
-}
-
-// What the waves of a workgroup tell each other of more than 64 sequences.
-struct FewFind {
-    unsigned total[4][4];   // per pass and wave
-    int most[4];
-    int hit[3];             // sequence (-1: none), its first chunk's number, its chunks
-};
-
-// The chunks of all sequences for one head and tile of columns stand in a row; workgroup u of 256 threads takes the
-// u-th. With by_seq, sequence u's first chunk instead. A lane a sequence, up to 64; a thread several, beyond (their
-// order in the row is that of the threads).
-template <int WG_COLS>
-__device__ __forceinline__ bool few_item(const Kv4AttnParams& p, int tile, int u, bool by_seq, Kv4Item& w, FewFind& find) {
-    w.h = blockIdx.x;
-    int lo = 0, hi = 0;
-    if (p.whole) {   // sequence u, in one chunk
-        w.sequence<WG_COLS, STEP>(p, u, tile * WG_COLS, lo, hi);
-        w.take(0, 1, 0, lo, hi);
-        w.at = w.slot = 0;   // (no partial results)
-        return w.cols > 0;
-    }
-    Kv4Item mine;
-    auto look = [&](int b) {   // steps of sequence b, -1 without columns
-        mine.sequence<WG_COLS, STEP>(p, min(b, p.B - 1), tile * WG_COLS, lo, hi);
-        return b < p.B && mine.cols > 0 ? (hi - lo + STEP - 1) / STEP : -1;
-    };
-    int at, chunks, c;
-    if (p.B <= 64) {
-        const int lane = threadIdx.x & 63, steps = look(lane);
-        c = few_length(p, wave_sum(max(steps, 0)), wave_max(max(steps, 0)), [&](int c) { return wave_sum(few_chunks(steps, c)); });
-        const int here = few_chunks(steps, c), upto = wave_sums(here);
-        const uint64_t who = __ballot(by_seq ? lane == u && here > 0 : upto - here <= u && u < upto);
-        if (!who) return false;
-        const int l = __builtin_ctzll(who);
-        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-        at = of(upto - here);
-        chunks = of(here);
-        w.b = l;
-        w.q0 = of(mine.q0);
-        w.n = of(mine.n);
-        w.len = of(mine.len);
-        w.first = of(mine.first);
-        w.c0 = tile * WG_COLS;
-        w.cols = of(mine.cols);
-        lo = of(lo);
-        hi = of(hi);
-    } else {
-        const int wave = threadIdx.x >> 6;
-        constexpr int HELD = 4;   // of a thread's sequences, in registers, their loads in flight together
-        int held[HELD];
-#pragma unroll
-        for (int g = 0; g < HELD; ++g) held[g] = look(256 * g + threadIdx.x);
-        auto each = [&](auto f) {
-#pragma unroll
-            for (int g = 0; g < HELD; ++g) f(256 * g + (int)threadIdx.x, held[g]);
-            for (int b = 256 * HELD + threadIdx.x; b < p.B; b += 256) f(b, look(b));
-        };
-        auto all = [&](int pass, unsigned v) {   // sum over the workgroup
-            v = wave_sum((int)v);
-            if ((threadIdx.x & 63) == 0) find.total[pass][wave] = v;
-            __syncthreads();
-            return find.total[pass][0] + find.total[pass][1] + find.total[pass][2] + find.total[pass][3];
-        };
-        unsigned mine_sum = 0;
-        int mine_most = 0;
-        each([&](int, int steps) {
-            mine_sum += max(steps, 0);
-            mine_most = max(mine_most, steps);
-        });
-        auto mine_chunks = [&](int c) {
-            unsigned n = 0;
-            each([&](int, int steps) { n += few_chunks(steps, c); });
-            return n;
-        };
-        mine_most = wave_max(mine_most);
-        if ((threadIdx.x & 63) == 0) find.most[wave] = mine_most;
-        if (threadIdx.x == 0) find.hit[0] = -1;
-        const unsigned sum = all(0, mine_sum);
-        const int most = max(max(find.most[0], find.most[1]), max(find.most[2], find.most[3]));
-        int pass = 0;
-        c = __builtin_amdgcn_readfirstlane(few_length(p, sum, most, [&](int c) { return all(++pass, mine_chunks(c)); }));
-        const unsigned n = mine_chunks(c), upto = (unsigned)wave_sums((int)n);
-        all(3, n);
-        unsigned first = upto - n;   // number of this thread's first chunk
-        for (int x = 0; x < wave; ++x) first += find.total[3][x];
-        if (by_seq ? (u & 255) == (int)threadIdx.x : first <= (unsigned)u && (unsigned)u < first + n)
-            each([&](int b, int steps) {
-                const unsigned here = few_chunks(steps, c);
-                if (by_seq ? b == u && here > 0 : first <= (unsigned)u && (unsigned)u < first + here) {
-                    find.hit[0] = b;
-                    find.hit[1] = (int)first;
-                    find.hit[2] = (int)here;
-                }
-                first += here;
-            });
-        __syncthreads();
-        const int b = __builtin_amdgcn_readfirstlane(find.hit[0]);
-        if (b < 0) return false;
-        at = __builtin_amdgcn_readfirstlane(find.hit[1]);
-        chunks = __builtin_amdgcn_readfirstlane(find.hit[2]);
-        w.sequence<WG_COLS, STEP>(p, b, tile * WG_COLS, lo, hi);
-    }
-    w.at = ((size_t)tile * p.B + w.b) * p.Hkv + w.h;
-    w.slot = ((size_t)tile * p.Hkv + w.h) * p.places + at;
-    w.take(by_seq ? 0 : u - at, chunks, 128 * c, lo, hi);
-    return true;
-}
-
 template <typename E, int D, int NT>
-__global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(KvAttnParams p) {
     typedef FewShape<D> S;
     typedef Kv4Cols<E, D, NT> C;
     constexpr int COLS = 16 * NT;
@@ -226,7 +80,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
     __shared__ float ml[4][COLS][2];
     __shared__ int last;
     __shared__ FewFind find;
-    Kv4Item w;
+    KvItem w;
     if (!few_item<2 * COLS>(p, blockIdx.y, blockIdx.z, false, w, find)) return;
     // one group of columns, its keys over four waves, or two over two
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -237,7 +91,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
     a.load(p, w, w.c0 + (wave >> kshift) * COLS, lane);
     const int stride = STEP << kshift, beg = (a.jlo & ~(STEP - 1)) + STEP * (wave & (kspl - 1)), end = a.jhi;
     unsigned char* const mine = ring[wave];
-    const Kv4Pages pages(p, w, S::BLOCK);
+    const KvPages pages(p, w, S::BLOCK);
     int bad = 0;   // bits 2 slot + s: block s of a slot lies in no page
     auto fetch = [&](int slot, int at, int pa, int pb) {
         bring<D>(mine + slot * 2 * S::BLOCK, pages.block(pa, at >> 4), lane);
@@ -359,7 +213,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
     a.finish();
 
     // the waves of a group join their shares of the keys
-    const Kv4Sink<E, D> sink(p, w);
+    const KvSink<E, D, VALUE_DOWN<E>> sink(p, w);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
         if (kb == 0) {
@@ -395,7 +249,7 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
                 ll += ml[g0 + x][16 * t + c][1] * f * f;
                 r += *reinterpret_cast<const float4_t*>(reds + x * RING_FLOATS + c * S::ROW + d);
             }
-            sink.put(a.c + 16 * t + c, d, r, over_sum<E>(ll));
+            sink.put(a.c + 16 * t + c, d, r, over_sum<VALUE_DOWN<E>>(ll));
             if (d == 0) sink.put_ml(a.c + 16 * t + c, mm, ll);
         }
     }
@@ -403,35 +257,25 @@ __global__ __launch_bounds__(256, kv4_few_per_cu(D, NT)) void kv4_few_kernel(Kv4
     sink.join(min(2 * COLS, w.cols), reinterpret_cast<float4_t*>(&ring[0][0]), reinterpret_cast<float(*)[2]>(&ring[0][4096]), &last);
 }
 
-// Joins the chunks of one sequence and head where that is more than one workgroup does in passing: 64 quads of
-// values a workgroup, a quarter of the chunks a wave.
 template <typename E, int D, int NT>
-__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnParams p) {
-    __shared__ float4_t vals[256];
-    __shared__ float ml[256][2];
-    __shared__ FewFind find;
-    constexpr int COLS = 32 * NT;
-    Kv4Item w;
-    const int tile = p.tiles == 1 ? 0 : blockIdx.z / p.join_parts;
-    if (!few_item<COLS>(p, tile, blockIdx.y, true, w, find) || w.chunks == 1) return;
-    const Kv4Sink<E, D> sink(p, w);
-    const int e = (blockIdx.z - tile * p.join_parts) * 64 + (threadIdx.x & 63);
-    sink.join_quads(e, threadIdx.x >> 6, 4, 64, e < w.cols * (D / 4), vals, ml);
+__global__ __launch_bounds__(256) void kv4_join_kernel(KvAttnParams p) {
+    __shared__ FewJoin lds;
+    few_join<E, D, NT, VALUE_DOWN<E>>(p, lds);
 }
 
 template <typename E, int D, int NT>
-static void run(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+static void run(const KvAttnShape& s, const KvAttnParams& p, hipStream_t st) {
     kv4_few_kernel<E, D, NT><<<dim3(p.Hkv, s.tiles, s.places), 256, 0, st>>>(p);
     if (p.join_apart) kv4_join_kernel<E, D, NT><<<dim3(p.Hkv, p.B, s.tiles * p.join_parts), 256, 0, st>>>(p);
 }
 template <typename E, int D>
-static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+static void go(const KvAttnShape& s, const KvAttnParams& p, hipStream_t st) {
     if constexpr (D <= 128)
         if (s.nt == 2) return run<E, D, 2>(s, p, st);
     run<E, D, 1>(s, p, st);
 }
 
-hipError_t launch_kv4_few(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {
+hipError_t launch_kv4_few(bool bf16, int D, const KvAttnParams& p, const KvAttnShape& s, hipStream_t st) {
     switch (D) {
         case 64: bf16 ? go<bf16_t, 64>(s, p, st) : go<half_t, 64>(s, p, st); break;
         case 128: bf16 ? go<bf16_t, 128>(s, p, st) : go<half_t, 128>(s, p, st); break;

@@ -15,10 +15,9 @@
 // 45 us. One wave a SIMD from D = 192 on: 512 queries over 8192 keys, 12 heads on 4 of 192, 102 us, 300 over 20000, 16 on 2 of
 // 256, 230, a third of that product's rate.
 #include "kv4_attn_body.h"
+#include "kv_many.h"
 
 namespace w4a16 {
-
-constexpr int MANY_STEP = 64;   // keys of a step
 
 template <int D>
 struct ManyLds {
@@ -111,57 +110,13 @@ __device__ __forceinline__ void unpack(ManyLds<D>& s, Packed<D> t, int dead, int
     }
 }
 
-// Sequence and tile of 128 columns of this workgroup, and its chunk of the keys: those with the longest rows first, or
-// (where all workgroups run at once) long and short ones by turns. p.rows: the tiles of all sequences stand in one row,
-// each sequence's longest first, so that the workgroups of a prompt among single tokens lie side by side. place:
-// tile and chunk, or (p.rows) chunk.
-__device__ __forceinline__ bool many_tile(const Kv4AttnParams& p, int place, int& b, int& tile, int& chunk, size_t& at) {
-    if (!p.rows) {
-        const int z = p.splits == 1 ? place : place / p.splits;
-        chunk = place - z * p.splits;
-        b = blockIdx.y;
-        tile = !p.pair_tiles ? p.tiles - 1 - z : z < (p.tiles + 1) / 2 ? p.tiles - 1 - z : z - (p.tiles + 1) / 2;
-        at = ((size_t)tile * p.B + b) * p.Hkv + blockIdx.x;
-        return true;
-    }
-    chunk = place;
-    at = (size_t)blockIdx.y * p.Hkv + blockIdx.x;
-    const int u = blockIdx.y;
-    for (int base = 0, before = 0; base < p.B; base += 64) {
-        const int s = base + (threadIdx.x & 63), in = min(s, p.B - 1);
-        const int n = min(max(p.cu_q[in + 1], 0), p.T) - min(max(p.cu_q[in], 0), p.T);
-        const int mine = s < p.B && n >= p.least_q ? (min(n, p.max_q) * p.G + 127) / 128 : 0;
-        const int upto = before + wave_sums(mine);
-        const uint64_t who = __ballot(u < upto);
-        if (who) {
-            const int l = __builtin_ctzll(who);
-            b = base + l;
-            tile = __builtin_amdgcn_readlane(upto, l) - 1 - u;
-            return true;
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
-    }
-    return false;
-}
-
-__device__ __forceinline__ bool many_item(const Kv4AttnParams& p, int place, Kv4Item& w) {
-    int b, tile, chunk, lo, hi;
-    w.h = blockIdx.x;
-    if (!many_tile(p, place, b, tile, chunk, w.at)) return false;
-    w.sequence<128, MANY_STEP>(p, b, tile * 128, lo, hi);
-    const int chunks = p.splits == 1 ? 1 : max(1, (int)(((unsigned)(hi - lo) + p.chunk - 1) / (unsigned)p.chunk));
-    w.take(chunk, chunks, p.chunk, lo, hi);
-    w.slot = w.at * p.splits;
-    return w.cols > 0 && chunk < chunks;
-}
-
 template <typename E, int D, int GROUPS>
-__global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void kv4_many_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void kv4_many_kernel(KvAttnParams p) {
     constexpr int NT = 2, COLS = 16 * NT, STEP = MANY_STEP, ALL = STEP * GROUPS;
     typedef Kv4Cols<E, D, NT> C;
     __shared__ ManyLds<D> lds[2][GROUPS];
     __shared__ float ml[4 * COLS][2];
-    Kv4Item w;
+    KvItem w;
     if (!many_item(p, blockIdx.z, w)) return;
     // wave `wave` of group `group`: the group takes every GROUPS-th step of the keys
     const int lane = threadIdx.x & 63, number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3, group = number >> 2;
@@ -169,7 +124,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     C a;
     a.load(p, w, w.c0 + wave * COLS, lane);
 
-    const Kv4Pages pages(p, w, kv4_block_bytes(D));
+    const KvPages pages(p, w, kv4_block_bytes(D));
     Packed<D> t;
     int live = 0;   // tokens of this wave's block of the step in t
     // (beyond the keys: their last block again, none of it alive)
@@ -285,12 +240,12 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
             }
         }
     }
-    const Kv4Sink<E, D> sink(p, w);
+    const KvSink<E, D, VALUE_DOWN<E>> sink(p, w);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         if (group) break;
         const int c = 16 * n + col;
-        const float inv = over_sum<E>(a.l[n]);
+        const float inv = over_sum<VALUE_DOWN<E>>(a.l[n]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -311,21 +266,14 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
     }
 }
 
-// Joins the chunks of one tile: an eighth of its values a workgroup. (The last of the chunks' own workgroups took longer:
-// 64 queries over 4096 keys, 32 heads of D = 128, 8 chunks, 40.1 us, so 30; two chunks of 400 over 2000 40.2, 39.3.)
-constexpr int MANY_PARTS = 8;
 template <typename E, int D>
-__global__ __launch_bounds__(256) void kv4_many_join_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256) void kv4_many_join_kernel(KvAttnParams p) {
     __shared__ float ml[128][2];
-    Kv4Item w;
-    const int part = blockIdx.z % MANY_PARTS;
-    if (!many_item(p, blockIdx.z / MANY_PARTS * p.splits, w) || w.chunks == 1) return;   // (its results are in place)
-    const Kv4Sink<E, D> sink(p, w);
-    sink.template join_lanes<MANY_PARTS>(min(128, w.cols), &ml[0][0], part);
+    many_join<E, D, VALUE_DOWN<E>>(p, &ml[0][0]);
 }
 
 template <typename E, int D>
-static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
+static void go(const KvAttnShape& s, const KvAttnParams& p, hipStream_t st) {
     const dim3 grid = s.rows ? dim3(p.Hkv, s.rows, s.splits) : dim3(p.Hkv, p.B, s.tiles * s.splits);
     auto join = [&] {
         const dim3 parts(grid.x, grid.y, (s.rows ? 1 : s.tiles) * MANY_PARTS);
@@ -341,7 +289,7 @@ static void go(const Kv4AttnShape& s, const Kv4AttnParams& p, hipStream_t st) {
     join();
 }
 
-hipError_t launch_kv4_many(bool bf16, int D, const Kv4AttnParams& p, const Kv4AttnShape& s, hipStream_t st) {
+hipError_t launch_kv4_many(bool bf16, int D, const KvAttnParams& p, const KvAttnShape& s, hipStream_t st) {
     switch (D) {
         case 64: bf16 ? go<bf16_t, 64>(s, p, st) : go<half_t, 64>(s, p, st); break;
         case 128: bf16 ? go<bf16_t, 128>(s, p, st) : go<half_t, 128>(s, p, st); break;

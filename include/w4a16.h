@@ -347,6 +347,61 @@ W4A16_API int w4a16_fused_moe_prepared(void* stream, const void* x, const float*
                                        int32_t block_m, void* workspace, size_t workspace_bytes,
                                        void* out);
 
+/* ------------------------------------------------------------------ norm and rotary positions
+ * Not in the reference for these types (its rms_norm and residual_add are fp32 and fp16 kernels of
+ * their own, crates/triton-kernels): what a program whose linear layers run here needs ahead of them and
+ * behind them. `elem` is 0 (fp16) or W4A16_BF16, the type of all rows. Rows are [T, H, K] (or [T, H, D])
+ * with strides in elements along T and H, contiguous along the last; they need no alignment but an
+ * element's and no particular size. An output may be the tensor that it is made from, at its strides; it
+ * must not otherwise overlap an input. Nothing is allocated. At most 2^30 rows in a call. */
+
+/* h = x + residual (nullable: h = x), y = h / sqrt(mean(h^2) + eps) * weight[K], in fp32 for each row of
+ * K <= 65536 elements. residual_out takes h (both or neither; it may be residual itself), out takes y,
+ * each rounded once (beyond its type's range to infinity); y is made from the unrounded h. Squares that fp32 does not
+ * hold are scaled: any finite h has its y. A row with a NaN is NaN throughout, one with infinities NaN
+ * there and 0 elsewhere. */
+W4A16_API int w4a16_rms_norm(void* stream, int elem, const void* x, int32_t x_stride_t, int32_t x_stride_h,
+                             const void* residual, int32_t r_stride_t, int32_t r_stride_h,
+                             void* residual_out, int32_t ro_stride_t, int32_t ro_stride_h,
+                             const void* weight, void* out, int32_t out_stride_t, int32_t out_stride_h,
+                             int32_t T, int32_t H, int32_t K, float eps);
+
+/* The same with y in 8 bits: out is e4m3 (1 sign, 4 exponent, 3 mantissa bits; largest value 448, no
+ * infinities; strides in bytes), scales fp32 [T, H, K / group] contiguous, one for `group` elements (32,
+ * 64, 128, 256 or 512, of which K is a multiple) or for a row (0): scale = max(max |y| / 448, 2^-100), out =
+ * y / scale rounded to nearest even, so that out * scale stands for y. A group with a NaN has a scale of
+ * NaN. */
+W4A16_API int w4a16_rms_norm_8bit(void* stream, int elem, const void* x, int32_t x_stride_t,
+                                  int32_t x_stride_h, const void* residual, int32_t r_stride_t,
+                                  int32_t r_stride_h, void* residual_out, int32_t ro_stride_t,
+                                  int32_t ro_stride_h, const void* weight, void* out, int32_t out_stride_t,
+                                  int32_t out_stride_h, float* scales, int32_t T, int32_t H, int32_t K,
+                                  int32_t group, float eps);
+
+/* Radians per position of each pair of dimensions, inv_freq[rot / 2] (host memory; no GPU access):
+ * f_i = base^(-2 i / rot), i = 0 .. rot / 2 - 1, and for contexts longer than a model was trained on
+ *   LINEAR  f_i / factor
+ *   BASE    f_i of base * factor^(rot / (rot - 2))
+ *   RAMP    f_i (share + (1 - share) / factor), share = clamp((t - slow) / (fast - slow), 0, 1), t the turns
+ *           that f_i makes over original_length positions: what turns `fast` times or more stays, what turns `slow`
+ *           times or less is slowed by the factor. */
+typedef enum { W4A16_ROPE_PLAIN = 0, W4A16_ROPE_LINEAR = 1, W4A16_ROPE_BASE = 2, W4A16_ROPE_RAMP = 3 } w4a16_rope_scaling;
+W4A16_API int w4a16_rope_frequencies(int32_t rot, double base, int scaling, double factor,
+                                     double original_length, double slow, double fast, double* inv_freq);
+
+/* Rotary positions: in rows q [T, Hq, D] and k [T, Hkv, D] (nullable, with Hkv = 0) of tokens at
+ * positions[T] (any int32), pair i < rot / 2 of dimensions, (i, i + rot / 2) or (interleaved != 0) (2 i, 2 i + 1),
+ * (a, b) becomes magnitude * (a cos w - b sin w, a sin w + b cos w), w = positions[t] * inv_freq[i]
+ * (device memory, fp64, any frequencies). Dimensions from rot on are copied. Angles are fp64, products fp32;
+ * results are rounded once (to their type's largest finite value beyond that). 1024 heads of 1024
+ * dimensions at most; rot is even. */
+W4A16_API int w4a16_rope(void* stream, int elem, const void* q, int32_t q_stride_t, int32_t q_stride_h,
+                         void* q_out, int32_t qo_stride_t, int32_t qo_stride_h, const void* k,
+                         int32_t k_stride_t, int32_t k_stride_h, void* k_out, int32_t ko_stride_t,
+                         int32_t ko_stride_h, const int32_t* positions, const double* inv_freq,
+                         float magnitude, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t rot,
+                         int32_t interleaved);
+
 /* ------------------------------------------------------------------ key/value cache in 4 bits
  * Not in the reference (it has neither cache nor attention): what a program whose linear layers
  * run here needs between its q, k, v projection and its output projection. `elem` is 0 (fp16) or

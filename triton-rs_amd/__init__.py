@@ -78,6 +78,7 @@ EXPORTED = (
     "w4a16_moe_gemm", "fused_silu_mul_interleaved_f16", "fused_silu_mul_interleaved_f32",
     "w4a16_moe_sum",
     "w4a16_fused_moe_workspace_size", "w4a16_fused_moe", "w4a16_fused_moe_prepared",
+    "w4a16_rms_norm", "w4a16_rms_norm_8bit", "w4a16_rope_frequencies", "w4a16_rope",
     "w4a16_kv4_cache_bytes", "w4a16_kv4_write", "w4a16_kv4_read",
     "w4a16_kv4_attention_workspace_size", "w4a16_kv4_attention",
     "hiprt_create", "hiprt_destroy", "hiprt_module_load", "hiprt_module_unload", "hiprt_launch",
@@ -136,6 +137,12 @@ def lib() -> ctypes.CDLL:
                                       _P, _I, _I, _I, _P, _Z, _P]
         L.w4a16_fused_moe_prepared.argtypes = [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I,
                                                _P, _Z, _P]
+        rows = [_P, _I, _I]   # rows at a token and a head stride
+        _F, _D = ctypes.c_float, ctypes.c_double
+        L.w4a16_rms_norm.argtypes = [_P, _I] + rows * 3 + [_P] + rows + [_I] * 3 + [_F]
+        L.w4a16_rms_norm_8bit.argtypes = [_P, _I] + rows * 3 + [_P] + rows + [_P] + [_I] * 4 + [_F]
+        L.w4a16_rope_frequencies.argtypes = [_I, _D, _I, _D, _D, _D, _D, ctypes.POINTER(_D)]
+        L.w4a16_rope.argtypes = [_P, _I] + rows * 4 + [_P, _P, _F] + [_I] * 6
         L.w4a16_kv4_cache_bytes.restype = ctypes.c_size_t
         L.w4a16_kv4_cache_bytes.argtypes = [_I] * 4
         L.w4a16_kv4_write.argtypes = [_P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I]
@@ -573,10 +580,185 @@ def fused_moe_prepared(x, router_logits, w13: PreparedWeights, w2: PreparedWeigh
     return out
 
 
+# ------------------------------------------------------------------ tensors of calls made once a layer and step
+
+_Tensor = torch.Tensor
+_INT32_MAX = 2 ** 31 - 1   # (ctypes drops what lies above, silently)
+
+
+# (each check of a tensor is the one test that a good call pays; _require says what is wrong with a bad one)
+
+def _tensor(t, name: str, dtypes, index: int):
+    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
+        _require(t, name, dtypes, torch.device("cuda", index))
+
+
+def _rows(t, name: str, dtypes, index: int, shape=None):
+    """(token stride, head stride) of rows [T, H, D] with contiguous D."""
+    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
+        _require(t, name, dtypes, torch.device("cuda", index))
+    if t.shape != shape if shape is not None else t.dim() != 3:
+        raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
+    st, sh, sd = t.stride()
+    if sd != 1:
+        raise InvalidArgument(f"{name} must be contiguous along its last dimension")
+    if st > _INT32_MAX or sh > _INT32_MAX or t.shape[0] > _INT32_MAX:
+        raise InvalidArgument(f"{name}: rows and strides are 32-bit ({t.shape[0]} rows at {st}, {sh})")
+    return st, sh
+
+
+def _index(t, name: str, index: int, shape=None):
+    if not isinstance(t, _Tensor) or t.dtype is not torch.int32 or t.get_device() != index:
+        _require(t, name, _INT32, torch.device("cuda", index))
+    if not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise InvalidArgument(f"{name} must be a contiguous int32 tensor" + ("" if shape is None else f" {list(shape)}"))
+
+
+def _call_on(index: int, fn, *args) -> None:
+    """fn(stream, *args) on the device's current stream, with the device as the current one (kernels
+    are launched on the current device). Pointers go as plain integers and the stream without an
+    object around it: a decode step makes many of these calls, each a few microseconds of host time."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(stream, *args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(stream, *args)
+    if rc != OK:
+        check(rc)
+
+
+# ------------------------------------------------------------------ norm and rotary positions
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _norm_rows(t, name: str, dtypes, index: int, shape):
+    """(T, H, K, token stride, head stride) of rows [T, K] or [T, H, K]."""
+    _tensor(t, name, dtypes, index)
+    if t.shape != shape if shape is not None else t.dim() not in (2, 3):
+        raise InvalidArgument(f"{name} must be {list(shape) if shape is not None else '[T, K] or [T, H, K]'}, not {list(t.shape)}")
+    T, H, K = (t.shape[0], 1, t.shape[1]) if t.dim() == 2 else t.shape
+    st = t.stride()
+    if K > 1 and st[-1] != 1:
+        raise InvalidArgument(f"{name} must be contiguous along its last dimension")
+    st, sh = st[0], (st[1] if t.dim() == 3 else 0)
+    if max(T, H, K, st, sh) > _INT32_MAX:
+        raise InvalidArgument(f"{name}: sizes and strides are 32-bit ({list(t.shape)} at {st}, {sh})")
+    return T, H, K, st, sh
+
+
+def _rms_norm(x, weight, eps, residual, residual_out, out, scales, group, fn, out_dtype):
+    index = x.get_device() if isinstance(x, _Tensor) else -1
+    if index < 0:
+        _require(x, "x", _ELEM)
+    T, H, K, st, sh = _norm_rows(x, "x", _ELEM, index, None)
+    _tensor(weight, "weight", (x.dtype,), index)
+    if weight.shape != (K,) or not weight.is_contiguous():
+        raise InvalidArgument(f"weight must be a contiguous [{K}] tensor")
+    r = ro = (None, 0, 0)
+    if residual is not None:
+        if residual_out is None:
+            residual_out = residual
+        r = (residual.data_ptr(), *_norm_rows(residual, "residual", (x.dtype,), index, x.shape)[3:])
+        ro = (residual_out.data_ptr(), *_norm_rows(residual_out, "residual_out", (x.dtype,), index, x.shape)[3:])
+    elif residual_out is not None:
+        raise InvalidArgument("residual_out without residual")
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    ost, osh = _norm_rows(out, "out", (out_dtype or x.dtype,), index, x.shape)[3:]
+    if out_dtype is None:
+        _call_on(index, fn, _elem_flag(x), x.data_ptr(), st, sh, *r, *ro, weight.data_ptr(), out.data_ptr(), ost, osh, T, H, K, eps)
+        return out
+    if group < 0 or (group and K % group):
+        raise InvalidArgument(f"group {group}: 0 (a row), or a divisor of {K}")
+    shape = (*x.shape[:-1], K // (group or K) if K else 0)
+    if scales is None:
+        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    _tensor(scales, "scales", (torch.float32,), index)
+    if scales.shape != shape or not scales.is_contiguous():
+        raise InvalidArgument(f"scales must be a contiguous {list(shape)} tensor")
+    _call_on(index, fn, _elem_flag(x), x.data_ptr(), st, sh, *r, *ro, weight.data_ptr(), out.data_ptr(), ost, osh,
+             scales.data_ptr(), T, H, K, group, eps)
+    return out, scales
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+             residual_out: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = h / sqrt(mean(h^2) + eps) * weight along the last dimension of x [T, K] or [T, H, K] (fp16 or
+    bfloat16; any strides but along K), h = x + residual where one is given. The sum h goes to
+    residual_out (residual itself unless given), rounded; y is made from the unrounded sum. out may be x."""
+    return _rms_norm(x, weight, eps, residual, residual_out, out, None, -1, lib().w4a16_rms_norm, None)
+
+
+def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group: int = 0,
+                  residual: torch.Tensor | None = None, residual_out: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """(out, scales): rms_norm's y as e4m3 (torch.float8_e4m3fn) with an fp32 scale for every `group`
+    elements (32, 64, 128, 256 or 512) or for a row (0): y = out * scale, scales [T, K / group] ([T, 1] for
+    rows: what torch._scaled_mm takes)."""
+    return _rms_norm(x, weight, eps, residual, residual_out, out, scales, group, lib().w4a16_rms_norm_8bit, E4M3)
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3}
+
+
+class Rope:
+    """Rotary positions of heads: the frequencies of rot / 2 pairs of dimensions (fp64, on the device),
+    whether a pair is (2 i, 2 i + 1) (interleaved) or (i, i + rot / 2), and a factor on the result.
+
+    base, scaling, factor, original_length, slow, fast: as w4a16_rope_frequencies takes them. Or
+    inv_freq: radians per position of each pair, of any origin."""
+
+    def __init__(self, rot: int | None = None, base: float = 10000.0, interleaved: bool = False, scaling: str = "none",
+                 factor: float = 1.0, original_length: float = 0.0, slow: float = 1.0, fast: float = 32.0,
+                 magnitude: float = 1.0, inv_freq=None, device="cuda"):
+        if inv_freq is None:
+            if rot is None:
+                raise InvalidArgument("give rot, or inv_freq")
+            if scaling not in ROPE_SCALINGS:
+                raise InvalidArgument(f"unknown scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
+            if not 0 < rot <= _INT32_MAX:
+                raise InvalidArgument(f"rot={rot} must be even and positive")
+            host = (ctypes.c_double * max(1, min(rot, 1 << 16) // 2))()
+            check(lib().w4a16_rope_frequencies(rot, base, ROPE_SCALINGS[scaling], factor, original_length, slow, fast, host))
+            inv_freq = torch.tensor(list(host), dtype=torch.float64)
+        inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64)
+        if inv_freq.dim() != 1 or inv_freq.numel() < 1 or (rot is not None and inv_freq.numel() * 2 != rot):
+            raise InvalidArgument(f"inv_freq must have a frequency for each pair, [rot / 2], not {list(inv_freq.shape)}")
+        self.inv_freq = inv_freq.to(device).contiguous()
+        self.rot, self.interleaved, self.magnitude = 2 * inv_freq.numel(), bool(interleaved), float(magnitude)
+
+
+def rope(q: torch.Tensor, positions: torch.Tensor, rope: Rope, k: torch.Tensor | None = None,
+         q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """q [T, heads, D] and k [T, kv heads, D] (fp16 or bfloat16) rotated at positions (int32 [T]) into q_out
+    and k_out (in place unless given), which are returned: (q_out, k_out), or q_out without k."""
+    index = q.get_device() if isinstance(q, _Tensor) else -1
+    if index < 0:
+        _require(q, "q", _ELEM)
+    qst, qsh = _rows(q, "q", _ELEM, index)
+    T, Hq, D = q.shape
+    q_out = q if q_out is None else q_out
+    qost, qosh = _rows(q_out, "q_out", (q.dtype,), index, q.shape)
+    _index(positions, "positions", index, (T,))
+    _tensor(rope.inv_freq, "rope.inv_freq", (torch.float64,), index)
+    Hkv, krows = 0, (None, 0, 0, None, 0, 0)
+    if k is not None:
+        Hkv = k.shape[1] if k.dim() == 3 else 0
+        kst, ksh = _rows(k, "k", (q.dtype,), index, (T, Hkv, D))
+        k_out = k if k_out is None else k_out
+        krows = (k.data_ptr(), kst, ksh, k_out.data_ptr(), *_rows(k_out, "k_out", (q.dtype,), index, k.shape))
+    elif k_out is not None:
+        raise InvalidArgument("k_out without k")
+    _call_on(index, lib().w4a16_rope, _elem_flag(q), q.data_ptr(), qst, qsh, q_out.data_ptr(), qost, qosh, *krows,
+             positions.data_ptr(), rope.inv_freq.data_ptr(), rope.magnitude, T, Hq, Hkv, D, rope.rot, int(rope.interleaved))
+    return q_out if k is None else (q_out, k_out)
+
+
 # ------------------------------------------------------------------ key/value cache in 4 bits
 
 KV4_COUNTER_BYTES = 65536
-_Tensor = torch.Tensor
 
 
 def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -606,62 +788,17 @@ def _kv4_cache_shape(cache: torch.Tensor):
     return pages, Hkv, blocks * 16, D, index
 
 
-_INT32_MAX = 2 ** 31 - 1   # (ctypes drops what lies above, silently)
-
-
-# (each check of a tensor is the one test that a good call pays; _require says what is wrong with a bad one)
-
-def _kv4_tensor(t, name: str, dtypes, index: int):
-    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
-        _require(t, name, dtypes, torch.device("cuda", index))
-
-
-def _kv4_rows(t, name: str, dtypes, index: int, shape=None):
-    """(token stride, head stride) of rows [T, H, D] with contiguous D."""
-    if not isinstance(t, _Tensor) or t.dtype not in dtypes or t.get_device() != index:
-        _require(t, name, dtypes, torch.device("cuda", index))
-    if t.shape != shape if shape is not None else t.dim() != 3:
-        raise InvalidArgument(f"{name} must be {list(shape) if shape else '[T, heads, D]'}, not {list(t.shape)}")
-    st, sh, sd = t.stride()
-    if sd != 1:
-        raise InvalidArgument(f"{name} must be contiguous along its last dimension")
-    if st > _INT32_MAX or sh > _INT32_MAX or t.shape[0] > _INT32_MAX:
-        raise InvalidArgument(f"{name}: rows and strides are 32-bit ({t.shape[0]} rows at {st}, {sh})")
-    return st, sh
-
-
-def _kv4_index(t, name: str, index: int, shape=None):
-    if not isinstance(t, _Tensor) or t.dtype is not torch.int32 or t.get_device() != index:
-        _require(t, name, _INT32, torch.device("cuda", index))
-    if not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise InvalidArgument(f"{name} must be a contiguous int32 tensor" + ("" if shape is None else f" {list(shape)}"))
-
-
-def _call_on(index: int, fn, *args) -> None:
-    """fn(stream, *args) on the device's current stream, with the device as the current one (kernels
-    are launched on the current device). Pointers go as plain integers and the stream without an
-    object around it: a decode step makes many of these calls, each a few microseconds of host time."""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(stream, *args)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(stream, *args)
-    if rc != OK:
-        check(rc)
-
-
 def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     """Quantises rows k, v [T, kv heads, D] (fp16 or bfloat16; any token and head strides that are
     multiples of 8) to 4 bits into the slots (int32 [T], page * page_size + offset) of the cache,
     which it returns. A row whose slot is negative or beyond the cache is passed over; slots of one
     call must differ from each other."""
     pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
-    _kv4_tensor(k, "k", _ELEM, dev)
+    _tensor(k, "k", _ELEM, dev)
     shape = (k.shape[0] if k.dim() else 0, Hkv, D)
-    kst, ksh = _kv4_rows(k, "k", _ELEM, dev, shape)
-    vst, vsh = _kv4_rows(v, "v", (k.dtype,), dev, shape)
-    _kv4_index(slots, "slots", dev, shape[:1])
+    kst, ksh = _rows(k, "k", _ELEM, dev, shape)
+    vst, vsh = _rows(v, "v", (k.dtype,), dev, shape)
+    _index(slots, "slots", dev, shape[:1])
     _call_on(dev, lib().w4a16_kv4_write, _elem_flag(k), k.data_ptr(), v.data_ptr(), kst, ksh, vst, vsh,
              slots.data_ptr(), cache.data_ptr(), pages, shape[0], Hkv, D, page)
     return cache
@@ -672,7 +809,7 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
     type that they were written in (`dtype`, or that of k_out and v_out). Rows whose slot is negative
     or beyond the cache are left as they were in k_out and v_out (0 where these are not given)."""
     pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
-    _kv4_index(slots, "slots", dev)
+    _index(slots, "slots", dev)
     if slots.dim() != 1:
         raise InvalidArgument("slots must be 1-D")
     shape = (slots.shape[0], Hkv, D)
@@ -680,8 +817,8 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
         raise InvalidArgument("give both k_out and v_out, or neither")
     if k_out is None:
         k_out, v_out = torch.zeros((2, *shape), dtype=dtype, device=cache.device)
-    kst, ksh = _kv4_rows(k_out, "k_out", _ELEM, dev, shape)
-    vst, vsh = _kv4_rows(v_out, "v_out", (k_out.dtype,), dev, shape)
+    kst, ksh = _rows(k_out, "k_out", _ELEM, dev, shape)
+    vst, vsh = _rows(v_out, "v_out", (k_out.dtype,), dev, shape)
     _call_on(dev, lib().w4a16_kv4_read, _elem_flag(k_out), cache.data_ptr(), slots.data_ptr(),
              k_out.data_ptr(), v_out.data_ptr(), kst, ksh, vst, vsh, pages, shape[0], Hkv, D, page)
     return k_out, v_out
@@ -723,17 +860,17 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     given; close ones make a better plan and a far smaller workspace). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
     given."""
     pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
-    qst, qsh = _kv4_rows(q, "q", _ELEM, dev)
+    qst, qsh = _rows(q, "q", _ELEM, dev)
     T, Hq, Dq = shape = q.shape
     if Dq != D:
         raise InvalidArgument(f"q has heads of {Dq} dimensions, the cache {D}")
-    _kv4_index(page_table, "page_table", dev)
+    _index(page_table, "page_table", dev)
     if page_table.dim() != 2:
         raise InvalidArgument("page_table must be [sequences, pages per sequence]")
     B, per = page_table.shape
-    _kv4_index(kv_lens, "kv_lens", dev, (B,))
+    _index(kv_lens, "kv_lens", dev, (B,))
     if cu_q is not None:
-        _kv4_index(cu_q, "cu_q", dev, (B + 1,))
+        _index(cu_q, "cu_q", dev, (B + 1,))
     elif T != B:   # (also where one is 0, and there would be nothing to launch)
         raise InvalidArgument(f"without cu_q every sequence has one query ({T} queries, {B} sequences)")
     if max_q_len is None:
@@ -744,9 +881,9 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         raise InvalidArgument(f"max_q_len, max_kv_len and window are 32-bit ({max_q_len}, {max_kv_len}, {window})")
     if out is None:
         out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
-    ost, osh = _kv4_rows(out, "out", (q.dtype,), dev, shape)
+    ost, osh = _rows(out, "out", (q.dtype,), dev, shape)
     if lse is not None:
-        _kv4_tensor(lse, "lse", (torch.float32,), dev)
+        _tensor(lse, "lse", (torch.float32,), dev)
         if lse.shape != (T, Hq) or not lse.is_contiguous():
             raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
     if T == 0 or B == 0:
@@ -754,7 +891,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     if workspace is None:
         workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
     else:
-        _kv4_tensor(workspace, "workspace", (torch.uint8,), dev)
+        _tensor(workspace, "workspace", (torch.uint8,), dev)
         if not workspace.is_contiguous():
             raise InvalidArgument("workspace must be contiguous")
     _call_on(dev, lib().w4a16_kv4_attention, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),

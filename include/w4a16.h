@@ -484,6 +484,75 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
                                   int32_t max_kv_len, float scale, int32_t causal, int32_t window,
                                   void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------ key/value cache in 8 bits
+ * Not in the reference. Twice the bytes of the cache in 4 bits at a sixteenth of its rounding, and rows come
+ * by sequence: their blocks share a scale. `elem` is 0 (fp16) or W4A16_BF16, the type of k, v, q and out; a
+ * cache holds no type.
+ *
+ * A cache holds num_pages pages of page_size tokens (a power of two, 16..1024) of Hkv heads of D
+ * dimensions (64, 128, 192 or 256): [num_pages][Hkv][page_size / 16] blocks of 32 D + 16 bytes,
+ * 16-byte aligned. A block holds 16 tokens of one head, each byte an e4m3 number: keys (token t, dimension d at
+ * 256 (d / 16) + 16 t + d % 16); from 16 D values (token 4 u + i, dimension r D / 16 + 4 g + e at 1024 g + 256 u +
+ * 16 r + 4 e + i); from 32 D two fp32 scales, of the keys and of the values, powers of two; then a 32-bit word whose bit t
+ * (16 + t) says that token t's keys (values) are not finite, and four bytes of zeros. A number n stands for n * scale.
+ *
+ * A block's scale is the smallest 2^e, e >= -60, of which 448 are no less than the largest magnitude that it holds;
+ * x is held as x / scale rounded to nearest even. A row with an infinity or NaN is NaN throughout (and
+ * does not count for the scale). Tokens are appended: a block that holds tokens of the sequence already keeps its
+ * scale, or raises it to what the new rows need; the older numbers are then rounded at the new one, which leaves
+ * them as they were except below 2^-6 scales. */
+
+/* Bytes of a cache (0: not supported). A cache needs no initialisation. */
+W4A16_API size_t w4a16_kv8_cache_bytes(int32_t num_pages, int32_t Hkv, int32_t D, int32_t page_size);
+
+/* Appends rows k, v [T, Hkv, D] (strides in elements, multiples of 8; 16-byte aligned) to their sequences:
+ * rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q null: row b, T = B) are sequence b's tokens up to kv_lens[b] - 1, the
+ * last of them there, token j in page page_table[b * pages_per_seq + j / page_size]. Its tokens before the first of these
+ * are in the cache already. Rows outside every sequence or beyond max_q_len of one (T is always enough), tokens before 0 or
+ * beyond the table, pages outside [0, num_pages) and sequences of more than 2^30 tokens are passed over.
+ * A block that this call writes must belong to one of its sequences only.
+ * inv_freq (nullable, [rot / 2]): k is rotated first, as w4a16_rope does but without a rounding in between (what fp32
+ * does not hold counts as infinite), at positions[T] or (null) each token's place in its sequence; so is q [T, Hq, D]
+ * (nullable, with Hq = 0), into q_out (q itself, at its strides, or apart from it), with w4a16_rope's results; rows of q outside
+ * every sequence are left as they were (given positions: are rotated too). At most 2^22 tokens and 65535 sequences in a call. */
+W4A16_API int w4a16_kv8_write(void* stream, int elem, const void* k, int32_t k_stride_t, int32_t k_stride_h,
+                              const void* v, int32_t v_stride_t, int32_t v_stride_h, const void* q,
+                              int32_t q_stride_t, int32_t q_stride_h, void* q_out, int32_t qo_stride_t,
+                              int32_t qo_stride_h, const int32_t* positions, const double* inv_freq,
+                              float magnitude, int32_t rot, int32_t interleaved, void* cache,
+                              const int32_t* page_table, const int32_t* kv_lens, const int32_t* cu_q,
+                              int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t num_pages,
+                              int32_t page_size, int32_t pages_per_seq, int32_t max_q_len);
+
+/* The rows that the slots (page * page_size + token, as for w4a16_kv4_read) hold, rounded to the element
+ * type (to its largest finite value beyond that), into k_out, v_out [T, Hkv, D] (strides in elements, multiples of
+ * 8; 16-byte aligned; rows not over each other). Rows whose slot is negative or beyond the cache are left
+ * as they were. A slot may be named more than once. */
+W4A16_API int w4a16_kv8_read(void* stream, int elem, const void* cache, const int32_t* slots, void* k_out,
+                             int32_t k_stride_t, int32_t k_stride_h, void* v_out, int32_t v_stride_t,
+                             int32_t v_stride_h, int32_t num_pages, int32_t T, int32_t Hkv, int32_t D,
+                             int32_t page_size);
+
+/* Attention of queries q [T, Hq, D] over the cache: arguments, masks, limits, workspace and what is left as it
+ * was as for w4a16_kv4_attention. out and lse are over the unrounded values n * scale that the cache holds. Products and sums
+ * are fp32; p_j times the scale of the value row's block is rounded to fp16 before its product with n: by 2^-12 of it, or
+ * 2^-33 of the query's largest such product where that is more; out is rounded once (to its type's largest finite
+ * value beyond that). What a query does not see moves no bit of its result, whatever the cache holds there; a
+ * key or value row of NaN that it does see makes it NaN, and so does an infinity or NaN of its own where it
+ * sees a key. (A scale q . k that fp32 does not hold has no defined result.) */
+#define W4A16_KV8_COUNTER_BYTES 65536
+W4A16_API size_t w4a16_kv8_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv,
+                                                    int32_t D, int32_t max_q_len,
+                                                    int32_t max_kv_len);
+W4A16_API int w4a16_kv8_attention(void* stream, int elem, const void* q, int32_t q_stride_t,
+                                  int32_t q_stride_h, const void* cache, const int32_t* page_table,
+                                  const int32_t* kv_lens, const int32_t* cu_q, void* out,
+                                  int32_t out_stride_t, int32_t out_stride_h, float* lse, int32_t T,
+                                  int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t num_pages,
+                                  int32_t page_size, int32_t pages_per_seq, int32_t max_q_len,
+                                  int32_t max_kv_len, float scale, int32_t causal, int32_t window,
+                                  void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ runtime
  * A HIP backend for the reference's DeviceRuntime trait (crates/triton-runtime/src/
  * lib.rs:64-85): load a code object, launch a kernel by name with KernelArg-style

@@ -81,6 +81,8 @@ EXPORTED = (
     "w4a16_rms_norm", "w4a16_rms_norm_8bit", "w4a16_rope_frequencies", "w4a16_rope",
     "w4a16_kv4_cache_bytes", "w4a16_kv4_write", "w4a16_kv4_read",
     "w4a16_kv4_attention_workspace_size", "w4a16_kv4_attention",
+    "w4a16_kv8_cache_bytes", "w4a16_kv8_write", "w4a16_kv8_read",
+    "w4a16_kv8_attention_workspace_size", "w4a16_kv8_attention",
     "hiprt_create", "hiprt_destroy", "hiprt_module_load", "hiprt_module_unload", "hiprt_launch",
     "hiprt_stream_create", "hiprt_stream_destroy", "hiprt_stream_synchronize", "hiprt_malloc",
     "hiprt_free", "hiprt_memcpy_htod_async", "hiprt_memcpy_dtoh_async", "hiprt_memset_async",
@@ -151,6 +153,13 @@ def lib() -> ctypes.CDLL:
         L.w4a16_kv4_attention_workspace_size.argtypes = [_I] * 7
         L.w4a16_kv4_attention.argtypes = [_P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P] + \
             [_I] * 10 + [ctypes.c_float, _I, _I, _P, _Z]
+        L.w4a16_kv8_cache_bytes.restype = ctypes.c_size_t
+        L.w4a16_kv8_cache_bytes.argtypes = [_I] * 4
+        L.w4a16_kv8_write.argtypes = [_P, _I] + rows * 4 + [_P, _P, _F, _I, _I] + [_P] * 4 + [_I] * 9
+        L.w4a16_kv8_read.argtypes = [_P, _I, _P, _P] + rows * 2 + [_I] * 5
+        L.w4a16_kv8_attention_workspace_size.restype = ctypes.c_size_t
+        L.w4a16_kv8_attention_workspace_size.argtypes = [_I] * 7
+        L.w4a16_kv8_attention.argtypes = L.w4a16_kv4_attention.argtypes
         L.hiprt_create.argtypes = [_I, ctypes.POINTER(_P)]
         L.hiprt_destroy.argtypes = [_P]
         L.hiprt_module_load.argtypes = [_P, _P, _Z, ctypes.POINTER(_P)]
@@ -756,9 +765,71 @@ def rope(q: torch.Tensor, positions: torch.Tensor, rope: Rope, k: torch.Tensor |
     return q_out if k is None else (q_out, k_out)
 
 
+# ------------------------------------------------------------------ attention over a paged cache
+
+KV_COUNTER_BYTES = KV4_COUNTER_BYTES = KV8_COUNTER_BYTES = 65536
+
+
+def _attention_workspace(shape_of, fn, q, cache, num_seqs, max_q_len, max_kv_len) -> torch.Tensor:
+    _, Hkv, _, D, _ = shape_of(cache)
+    T, Hq = q.shape[:2]
+    if max(T, num_seqs, max_q_len, max_kv_len) > _INT32_MAX:
+        raise InvalidArgument(f"sizes are 32-bit ({T}, {num_seqs}, {max_q_len}, {max_kv_len})")
+    need = fn(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
+    if need == 0:
+        check(ERR_INVALID_ARG)
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
+    ws[:KV_COUNTER_BYTES].zero_()
+    return ws
+
+
+def _attention(shape_of, workspace_of, fn, q, cache, page_table, kv_lens, cu_q, max_q_len, max_kv_len, scale, causal, window,
+               out, lse, workspace) -> torch.Tensor:
+    pages, Hkv, page, D, dev = shape_of(cache)
+    qst, qsh = _rows(q, "q", _ELEM, dev)
+    T, Hq, Dq = shape = q.shape
+    if Dq != D:
+        raise InvalidArgument(f"q has heads of {Dq} dimensions, the cache {D}")
+    _index(page_table, "page_table", dev)
+    if page_table.dim() != 2:
+        raise InvalidArgument("page_table must be [sequences, pages per sequence]")
+    B, per = page_table.shape
+    _index(kv_lens, "kv_lens", dev, (B,))
+    if cu_q is not None:
+        _index(cu_q, "cu_q", dev, (B + 1,))
+    elif T != B:   # (also where one is 0, and there would be nothing to launch)
+        raise InvalidArgument(f"without cu_q every sequence has one query ({T} queries, {B} sequences)")
+    if max_q_len is None:
+        max_q_len = 1 if cu_q is None else max(1, T)
+    if max_kv_len is None:
+        max_kv_len = per * page
+    if max_q_len > _INT32_MAX or max_kv_len > _INT32_MAX or window > _INT32_MAX:
+        raise InvalidArgument(f"max_q_len, max_kv_len and window are 32-bit ({max_q_len}, {max_kv_len}, {window})")
+    if out is None:
+        out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
+    ost, osh = _rows(out, "out", (q.dtype,), dev, shape)
+    if lse is not None:
+        _tensor(lse, "lse", (torch.float32,), dev)
+        if lse.shape != (T, Hq) or not lse.is_contiguous():
+            raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
+    if T == 0 or B == 0:
+        return out
+    if workspace is None:
+        workspace = workspace_of(q, cache, B, max_q_len, max_kv_len)
+    else:
+        _tensor(workspace, "workspace", (torch.uint8,), dev)
+        if not workspace.is_contiguous():
+            raise InvalidArgument("workspace must be contiguous")
+    _call_on(dev, fn, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),
+             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
+             out.data_ptr(), ost, osh, None if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, pages, page,
+             per, max_q_len, max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window,
+             workspace.data_ptr(), workspace.numel())
+    return out
+
+
 # ------------------------------------------------------------------ key/value cache in 4 bits
 
-KV4_COUNTER_BYTES = 65536
 
 
 def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -830,16 +901,7 @@ def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int,
     max_q_len and this max_kv_len or a smaller one. A call of another shape may need more, a smaller
     one too: a workspace for several is as large as the largest of theirs. Calls that may overlap in
     time need one each."""
-    _, Hkv, _, D, _ = _kv4_cache_shape(cache)
-    T, Hq = q.shape[:2]
-    if max(T, num_seqs, max_q_len, max_kv_len) > _INT32_MAX:
-        raise InvalidArgument(f"sizes are 32-bit ({T}, {num_seqs}, {max_q_len}, {max_kv_len})")
-    need = lib().w4a16_kv4_attention_workspace_size(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
-    if need == 0:
-        check(ERR_INVALID_ARG)
-    ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
-    ws[:KV4_COUNTER_BYTES].zero_()
-    return ws
+    return _attention_workspace(_kv4_cache_shape, lib().w4a16_kv4_attention_workspace_size, q, cache, num_seqs, max_q_len, max_kv_len)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -859,11 +921,59 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     max_q_len, max_kv_len: bounds on the batch (T, or 1 without cu_q, and the table's width unless
     given; close ones make a better plan and a far smaller workspace). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
     given."""
-    pages, Hkv, page, D, dev = _kv4_cache_shape(cache)
-    qst, qsh = _rows(q, "q", _ELEM, dev)
-    T, Hq, Dq = shape = q.shape
-    if Dq != D:
-        raise InvalidArgument(f"q has heads of {Dq} dimensions, the cache {D}")
+    return _attention(_kv4_cache_shape, kv4_attention_workspace, lib().w4a16_kv4_attention, q, cache, page_table, kv_lens, cu_q,
+                      max_q_len, max_kv_len, scale, causal, window, out, lse, workspace)
+
+
+# ------------------------------------------------------------------ key/value cache in 8 bits
+
+def kv8_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
+              device="cuda") -> torch.Tensor:
+    """An empty 8-bit key/value cache: uint8 [num_pages, num_kv_heads, page_size / 16,
+    32 head_dim + 16], e4m3 with a scale for each block of 16 tokens and head (the layout is in
+    include/w4a16.h). head_dim 64, 128, 192 or 256, page_size a power of two from 16 to 1024."""
+    if max(num_pages, num_kv_heads, head_dim, page_size) > _INT32_MAX or \
+            lib().w4a16_kv8_cache_bytes(num_pages, num_kv_heads, head_dim, page_size) == 0:
+        raise Unsupported(f"no 8-bit cache of {num_pages} pages of {page_size} tokens, "
+                          f"{num_kv_heads} heads of {head_dim}")
+    return torch.zeros((num_pages, num_kv_heads, page_size // 16, 32 * head_dim + 16),
+                       dtype=torch.uint8, device=device)
+
+
+def _kv8_cache_shape(cache: torch.Tensor):
+    """(pages, kv heads, page size, head dim, device index) of a cache tensor."""
+    index = cache.get_device() if isinstance(cache, _Tensor) else -1
+    if index < 0 or cache.dtype is not torch.uint8:
+        _require(cache, "cache", (torch.uint8,))
+    shape = cache.shape
+    if len(shape) != 4 or not cache.is_contiguous():
+        raise InvalidArgument("cache must be a contiguous [pages, kv heads, page_size / 16, 32 D + 16] tensor")
+    pages, Hkv, blocks, width = shape
+    D = (width - 16) // 32
+    if D < 1 or width != 32 * D + 16:
+        raise InvalidArgument(f"cache has blocks of {width} bytes, not 32 D + 16")
+    return pages, Hkv, blocks * 16, D, index
+
+
+def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+              cu_q: torch.Tensor | None = None, max_q_len: int | None = None, rope: Rope | None = None,
+              positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Appends rows k, v [T, kv heads, D] (fp16 or bfloat16; token and head strides that are multiples of 8) to
+    the sequences of an 8-bit cache, which it returns.
+
+    Rows cu_q[b] .. cu_q[b + 1] (int32 [B + 1]; None: one row each, T = B) are sequence b's newest tokens, the
+    last of them at token kv_lens[b] - 1 (int32 [B]; lengths with the new tokens) of pages page_table[b] (int32
+    [B, pages per sequence]). Rows outside every sequence (padding behind cu_q[B]), tokens beyond the table and
+    pages that do not exist are passed over. Blocks of 16 tokens share a scale, which later rows may raise.
+    max_q_len: a bound on the new tokens of a sequence (T unless given; a close one makes a smaller launch).
+    rope: k is rotated first, in fp32, at positions (int32 [T]) or each token's place in its sequence, and q [T,
+    heads, D], where given, into q_out (in place unless given) in the same launch."""
+    pages, Hkv, page, D, dev = _kv8_cache_shape(cache)
+    _tensor(k, "k", _ELEM, dev)
+    T = k.shape[0] if k.dim() else 0
+    kst, ksh = _rows(k, "k", _ELEM, dev, (T, Hkv, D))
+    vst, vsh = _rows(v, "v", (k.dtype,), dev, (T, Hkv, D))
     _index(page_table, "page_table", dev)
     if page_table.dim() != 2:
         raise InvalidArgument("page_table must be [sequences, pages per sequence]")
@@ -871,35 +981,68 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     _index(kv_lens, "kv_lens", dev, (B,))
     if cu_q is not None:
         _index(cu_q, "cu_q", dev, (B + 1,))
-    elif T != B:   # (also where one is 0, and there would be nothing to launch)
-        raise InvalidArgument(f"without cu_q every sequence has one query ({T} queries, {B} sequences)")
     if max_q_len is None:
         max_q_len = 1 if cu_q is None else max(1, T)
-    if max_kv_len is None:
-        max_kv_len = per * page
-    if max_q_len > _INT32_MAX or max_kv_len > _INT32_MAX or window > _INT32_MAX:
-        raise InvalidArgument(f"max_q_len, max_kv_len and window are 32-bit ({max_q_len}, {max_kv_len}, {window})")
-    if out is None:
-        out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
-    ost, osh = _rows(out, "out", (q.dtype,), dev, shape)
-    if lse is not None:
-        _tensor(lse, "lse", (torch.float32,), dev)
-        if lse.shape != (T, Hq) or not lse.is_contiguous():
-            raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
+    if max(B, per, max_q_len) > _INT32_MAX:
+        raise InvalidArgument(f"sizes are 32-bit ({B}, {per}, {max_q_len})")
+    Hq, qrows, turn = 0, (None, 0, 0, None, 0, 0), (None, None, 0.0, 0, 0)
+    if rope is not None:
+        _tensor(rope.inv_freq, "rope.inv_freq", (torch.float64,), dev)
+        if positions is not None:
+            _index(positions, "positions", dev, (T,))
+        turn = (None if positions is None else positions.data_ptr(), rope.inv_freq.data_ptr(), rope.magnitude, rope.rot, int(rope.interleaved))
+        if q is not None:
+            Hq = q.shape[1] if q.dim() == 3 else 0
+            qst, qsh = _rows(q, "q", (k.dtype,), dev, (T, Hq, D))
+            q_out = q if q_out is None else q_out
+            qrows = (q.data_ptr(), qst, qsh, q_out.data_ptr(), *_rows(q_out, "q_out", (q.dtype,), dev, q.shape))
+    elif positions is not None or q is not None:
+        raise InvalidArgument("positions and q are for a rotation: give rope")
+    if q is None and q_out is not None:
+        raise InvalidArgument("q_out without q")
     if T == 0 or B == 0:
-        return out
-    if workspace is None:
-        workspace = kv4_attention_workspace(q, cache, B, max_q_len, max_kv_len)
-    else:
-        _tensor(workspace, "workspace", (torch.uint8,), dev)
-        if not workspace.is_contiguous():
-            raise InvalidArgument("workspace must be contiguous")
-    _call_on(dev, lib().w4a16_kv4_attention, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),
-             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
-             out.data_ptr(), ost, osh, None if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, pages, page,
-             per, max_q_len, max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window,
-             workspace.data_ptr(), workspace.numel())
-    return out
+        return cache
+    _call_on(dev, lib().w4a16_kv8_write, _elem_flag(k), k.data_ptr(), kst, ksh, v.data_ptr(), vst, vsh, *qrows, *turn,
+             cache.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, B, Hq,
+             Hkv, D, pages, page, per, max_q_len)
+    return cache
+
+
+def kv8_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_out=None, v_out=None):
+    """(k, v) [T, kv heads, D]: the rows that the slots (int32 [T], page * page_size + offset) of the cache hold,
+    rounded to `dtype`, or that of k_out and v_out. Rows whose slot is negative or beyond the cache are left as
+    they were in k_out and v_out (0 where these are not given)."""
+    pages, Hkv, page, D, dev = _kv8_cache_shape(cache)
+    _index(slots, "slots", dev)
+    if slots.dim() != 1:
+        raise InvalidArgument("slots must be 1-D")
+    shape = (slots.shape[0], Hkv, D)
+    if (k_out is None) != (v_out is None):
+        raise InvalidArgument("give both k_out and v_out, or neither")
+    if k_out is None:
+        k_out, v_out = torch.zeros((2, *shape), dtype=dtype, device=cache.device)
+    kst, ksh = _rows(k_out, "k_out", _ELEM, dev, shape)
+    vst, vsh = _rows(v_out, "v_out", (k_out.dtype,), dev, shape)
+    _call_on(dev, lib().w4a16_kv8_read, _elem_flag(k_out), cache.data_ptr(), slots.data_ptr(), k_out.data_ptr(), kst, ksh,
+             v_out.data_ptr(), vst, vsh, pages, shape[0], Hkv, D, page)
+    return k_out, v_out
+
+
+def kv8_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int, max_q_len: int,
+                            max_kv_len: int) -> torch.Tensor:
+    """A workspace for kv8_attention calls, as kv4_attention_workspace makes it."""
+    return _attention_workspace(_kv8_cache_shape, lib().w4a16_kv8_attention_workspace_size, q, cache, num_seqs, max_q_len, max_kv_len)
+
+
+def kv8_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                  cu_q: torch.Tensor | None = None, max_q_len: int | None = None,
+                  max_kv_len: int | None = None, scale: float | None = None, causal: bool = True,
+                  window: int = 0, out=None, lse=None, workspace=None) -> torch.Tensor:
+    """softmax(scale q k^T) v over the keys and values of an 8-bit cache; returns out [T, heads, D]. Arguments,
+    masks, results and workspace are kv4_attention's; the new tokens' keys and values are in the cache already
+    (kv8_write), and q may be of either type, whatever the cache was written from."""
+    return _attention(_kv8_cache_shape, kv8_attention_workspace, lib().w4a16_kv8_attention, q, cache, page_table, kv_lens, cu_q,
+                      max_q_len, max_kv_len, scale, causal, window, out, lse, workspace)
 
 
 # ------------------------------------------------------------------ kernel level (reference names)

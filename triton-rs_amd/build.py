@@ -35,7 +35,8 @@ SOURCES = ["api.cpp", "hiprt.cpp", "kernels_gemv.hip", "kernels_prefill.hip", "k
            "direct.hip", "direct_gptq.hip", "direct_gptq_bf16.hip", "direct_awq.hip", "direct_awq_bf16.hip",
            "direct_prep.hip", "direct_moe_gptq.hip", "direct_moe_awq.hip", "direct_moe_prep.hip",
            "layer_api.cpp", "norm.hip", "rope.hip",
-           "kv_api.cpp", "kv4_api.cpp", "kv4_cache.hip", "kv4_few.hip", "kv4_many.hip"]
+           "kv_api.cpp", "kv4_api.cpp", "kv4_cache.hip", "kv4_few.hip", "kv4_many.hip",
+           "kv8_api.cpp", "kv8_cache.hip", "kv8_few.hip", "kv8_many.hip"]
 
 
 def _obj(src: str) -> str:

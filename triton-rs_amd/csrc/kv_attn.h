@@ -26,6 +26,7 @@ struct KvAttnParams {
     int least_q, most_q;              // sequences of fewer or more queries are another kernel's
     float scale_mant;                 // scale * log2(e) = scale_mant 2^scale_exp, |scale_mant| < 1
     int scale_exp;
+    float scale_log2;                 // scale * log2(e)
     int causal, window;
     uint32_t* counters;               // few columns: one a sequence, head and tile, zero between calls
     float* partials;                  // by number of chunk, slot_cols (D + 2) floats each

@@ -20,39 +20,18 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
         turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
     }
     __syncthreads();
-    // eight elements of a row (PAIRS), or eight and their eight partners; then those beyond rot
-    const int turned = PAIRS ? (p.rot + 7) / 8 : (half + 7) / 8, units = turned + (p.D - p.rot + 7) / 8;
+    const int turned = turned_units(p.rot, PAIRS), units = row_units(p.rot, p.D, PAIRS);
     static_assert(ROPE_MAX_D / 8 + 1 <= 256, "a row's units are threads of one workgroup");
     const int rows = 256 / units, heads = p.rows[0].H + p.rows[1].H;
-    const int mine = threadIdx.x / units;
+    const int mine = threadIdx.x / units, u = threadIdx.x - mine * units;
     if (mine >= rows) return;
-    const int u = threadIdx.x - mine * units;
     for (int r = mine; r < live * heads; r += rows) {
         const int t = r / heads, hh = r - t * heads;
         const RopeRows& w = p.rows[hh >= p.rows[0].H];
         const int h = hh >= p.rows[0].H ? hh - p.rows[0].H : hh;
-        const uint16_t* x = static_cast<const uint16_t*>(w.x) + (size_t)(t0 + t) * w.st + (size_t)h * w.sh;
-        uint16_t* o = static_cast<uint16_t*>(w.out) + (size_t)(t0 + t) * w.o_st + (size_t)h * w.o_sh;
-        const float2* a = turn + t * half;
-        if (u >= turned) {
-            const int e = p.rot + 8 * (u - turned);
-            if (x != o) store8(o + e, load8(x + e, p.D - e), p.D - e);
-        } else if constexpr (PAIRS) {
-            float f[8];
-            to_f32<E>(load8(x + 8 * u, p.rot - 8 * u), f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rotate<E>(f[2 * i], f[2 * i + 1], a[min(4 * u + i, half - 1)]);
-            store8(o + 8 * u, from_f32<E>(f), p.rot - 8 * u);
-        } else {
-            float f[8], g[8];
-            to_f32<E>(load8(x + 8 * u, half - 8 * u), f);
-            to_f32<E>(load8(x + half + 8 * u, half - 8 * u), g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rotate<E>(f[i], g[i], a[min(8 * u + i, half - 1)]);
-            store8(o + 8 * u, from_f32<E>(f), half - 8 * u);
-            store8(o + half + 8 * u, from_f32<E>(g), half - 8 * u);
-        }
-        }
+        turn_unit<E, PAIRS>(static_cast<const uint16_t*>(w.x) + (size_t)(t0 + t) * w.st + (size_t)h * w.sh,
+                            static_cast<uint16_t*>(w.out) + (size_t)(t0 + t) * w.o_st + (size_t)h * w.o_sh, turn + t * half, u, turned, p.rot, p.D);
+    }
 }
 
 template <typename E>

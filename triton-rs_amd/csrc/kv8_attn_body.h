@@ -8,7 +8,8 @@
 // type, so the first product has no rounding but that of its fp32 sum. A scale acts on a whole 16 x 16 tile of logits:
 // s_k in the factor that softmax's base 2 needs anyway, s_v as its exponent, added to the logit. What is
 // exponentiated is log2(p_j s_v): the weight that the second product takes, rounded to fp16 (2^-12 of it; of what the
-// matrix cores take the type with the most bits). The sum of p_j is that of a tile's weights times 1 / s_v. The
+// matrix cores take the type with the most bits). The sum of p_j is that of a tile's weights times 1 / s_v; where all of a lane's
+// weights of a tile are below 2^-100, which fp32 may not hold although p_j counts (s_v far below the others), p_j is exponentiated by itself. The
 // reference m follows the largest weight p_j s_v, which is 2^8 when it is set and 2^15 at most: it is raised (with the sums
 // scaled down) only where a weight would pass that, so maxima pass between lanes only then, and a block of
 // large values and no weight takes no bits from the others. Scales are 2^-60 to 2^120, so a sum of 2^30 p_j
@@ -26,6 +27,7 @@ namespace w4a16 {
 
 constexpr float KV8_MOST = 15.f;   // p_j s_v <= 2^15
 constexpr float KV8_ROOM = 7.f;    // a raise leaves the largest at 2^-7 of that
+constexpr float KV8_LOW = -100.f;  // log2 of weights whose p_j is exponentiated by itself
 
 // Two e4m3 bytes (the low or the high ones) of a word in the type of an operand, exactly.
 template <typename E, bool HIGH>
@@ -47,7 +49,8 @@ __device__ __forceinline__ uint32_t token_bytes(int lo, int hi, int kb) {
     return from & to;
 }
 
-// What logits and weights take of a block's last 16 bytes.
+// What logits and weights take of a block's last 16 bytes. (there: a token of it is seen; else its scales may be anything, and
+// a NaN would pass into the sums by way of weights of zero.)
 struct Kv8Scale {
     float key;       // scale of its keys, times scale log2(e)
     float value;     // log2 of the scale of its values
@@ -135,9 +138,9 @@ struct Kv8Cols {
 
     // log2(p_j s_v) of 32 tokens from j on for columns t: acc = q . n of the lane's tokens j + 16 s + 4 kb + i. whole: every
     // column sees all 32 and no row is NaN; else tokens from `end` on and those of blocks in `bad` are not seen. Raises m where
-    // a weight would pass 2^15.
-    __device__ __forceinline__ void logits(int t, float (&x)[2][4], const float4_t (&acc)[2], const Kv8Scale (&s)[2], bool whole, int j,
-                                           int end, int bad, int kb) {
+    // a weight would pass 2^15. back: what a block's weights count in the sum of p_j, 1 / s_v (or 0 where they are counted here).
+    __device__ __forceinline__ void logits(int t, float (&x)[2][4], float (&back)[2], const float4_t (&acc)[2], const Kv8Scale (&s)[2], bool whole,
+                                           int j, int end, int bad, int kb) {
         float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -165,11 +168,14 @@ struct Kv8Cols {
                 for (int y = 0; y < VT; ++y) o[t][y] += add;
             }
         }
+        const float low = fminf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[b][i]);
-        if (__any(top > most[t])) {   // rare after the first steps
+#pragma unroll
+        for (int b = 0; b < 2; ++b) back[b] = s[b].back;
+        if (__any((top > most[t]) | (low < KV8_LOW))) {   // rare after the first steps
             top = kb_max(top);
             const bool up = top > most[t];
             const float by = up ? top - (KV8_MOST - KV8_ROOM) : 0.f;
@@ -184,11 +190,20 @@ struct Kv8Cols {
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[b][i] -= by;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const bool alone = fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])) < KV8_LOW;
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p += __builtin_amdgcn_exp2f(x[b][i] - s[b].value);
+                l[t] += alone ? p : 0.f;
+                back[b] = alone ? 0.f : back[b];
+            }
         }
     }
 
     // The weights as operand; the sum of p_j.
-    __device__ __forceinline__ half8_t weights(int t, const float (&x)[2][4], const Kv8Scale (&s)[2]) {
+    __device__ __forceinline__ half8_t weights(int t, const float (&x)[2][4], const float (&back)[2]) {
         half8_t w;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -198,7 +213,7 @@ struct Kv8Cols {
                 f[i] = __builtin_amdgcn_exp2f(x[b][i]);
                 w[4 * b + i] = (half_t)f[i];
             }
-            l[t] = __builtin_fmaf((f[0] + f[1]) + (f[2] + f[3]), s[b].back, l[t]);
+            l[t] = __builtin_fmaf((f[0] + f[1]) + (f[2] + f[3]), back[b], l[t]);
         }
         return w;
     }

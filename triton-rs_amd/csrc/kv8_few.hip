@@ -63,7 +63,8 @@ __global__ __launch_bounds__(256, kv8_few_per_cu(D, NT)) void kv8_few_kernel(KvA
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[t][b] = mfma16x16x32(f, a.qf[t][x], acc[t][b]);
             }
-        const Kv8Scale sc[2] = {Kv8Scale::of(s.tail[0], p.scale_log2, !(bad & 1)), Kv8Scale::of(s.tail[1], p.scale_log2, !(bad & 2) && j + 16 < end)};
+        const Kv8Scale sc[2] = {Kv8Scale::of(s.tail[0], p.scale_log2, !(bad & 1) && j + 16 > a.jlo),
+                                Kv8Scale::of(s.tail[1], p.scale_log2, !(bad & 2) && j + 16 < end && j + 32 > a.jlo)};
         const bool whole = j >= a.all_lo && j + STEP <= a.all_hi && j + STEP <= end && !bad && !(sc[0].nan | sc[1].nan);
         // bytes of tokens that no column sees may be anything
         uint32_t mask[2] = {~0u, ~0u};
@@ -73,9 +74,9 @@ __global__ __launch_bounds__(256, kv8_few_per_cu(D, NT)) void kv8_few_kernel(KvA
         half8_t pw[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float x[2][4];
-            a.logits(t, x, acc[t], sc, whole, j, end, bad, kb);
-            pw[t] = a.weights(t, x, sc);
+            float x[2][4], back[2];
+            a.logits(t, x, back, acc[t], sc, whole, j, end, bad, kb);
+            pw[t] = a.weights(t, x, back);
         }
 #pragma unroll
         for (int g = 0; g < D / 64; ++g)

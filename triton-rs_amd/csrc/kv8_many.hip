@@ -40,7 +40,7 @@ __device__ __forceinline__ void unpack(ManyLds<E, D>& s, const Packed<D>& t, int
         }
     }
     if (lane == 0) {
-        s.scale[wave] = Kv8Scale::of(t.tail, factor, live > 0);
+        s.scale[wave] = Kv8Scale::of(t.tail, factor, live > 0 && dead < 16);
         s.live[wave] = live;
     }
 }
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
             // operands from LDS all at once, ahead of what takes them: one wait instead of eight
             typename C::vec_t kf[2][C::KW];
             half8_t vf[C::VT];
-            const Kv8Scale sc[2] = {s.scale[2 * half], s.scale[2 * half + 1]};
+            Kv8Scale sc[2] = {s.scale[2 * half], s.scale[2 * half + 1]};
             const int live0 = s.live[2 * half], live1 = s.live[2 * half + 1];
 #pragma unroll
             for (int x = 0; x < C::KW; ++x)
@@ -105,22 +105,24 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
                 for (int b = 0; b < 2; ++b) kf[b][x] = s.k[2 * half + b][x][lane];
             __builtin_amdgcn_sched_barrier(0);
             const int bad = __builtin_amdgcn_readfirstlane((live0 <= 0 ? 1 : 0) | (live1 <= 0 ? 2 : 0));
-            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad && !__builtin_amdgcn_readfirstlane(sc[0].nan | sc[1].nan);
+            sc[0].nan = __builtin_amdgcn_readfirstlane(sc[0].nan);
+            sc[1].nan = __builtin_amdgcn_readfirstlane(sc[1].nan);
+            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad && !(sc[0].nan | sc[1].nan);
 #pragma unroll
             for (int x = 0; x < C::KW; ++x)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            float x[NT][2][4];
+            float x[NT][2][4], back[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) a.logits(n, x[n], acc[n], sc, whole, jh, a.jhi, bad, kb);
+            for (int n = 0; n < NT; ++n) a.logits(n, x[n], back[n], acc[n], sc, whole, jh, a.jhi, bad, kb);
 #pragma unroll
             for (int x = 0; x < C::VT; ++x) vf[x] = s.v[half][x][lane];
             __builtin_amdgcn_sched_barrier(0);
-            half8_t pw[NT];
+                half8_t pw[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) pw[n] = a.weights(n, x[n], sc);
+            for (int n = 0; n < NT; ++n) pw[n] = a.weights(n, x[n], back[n]);
 #pragma unroll
             for (int x = 0; x < C::VT; ++x)
 #pragma unroll

@@ -12,6 +12,8 @@ every computation runs in the HIP library, and loading fails loudly when it is m
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 import torch  # loaded first so the process has one HIP runtime (same SONAME)
@@ -20,6 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libw4a16.so")
 HSACO_PATH = os.path.join(HERE, "w4a16_typed.hsaco")
 META_PATH = os.path.join(HERE, "w4a16_typed.json")
+CALLS_PATH = os.path.join(HERE, "_calls.so")
 
 FMT_GPTQ, FMT_GPTQ_SYM, FMT_AWQ = 0, 1, 2
 BF16 = 0x100   # W4A16_BF16: bfloat16 activations, scales and output (OR-ed into the format)
@@ -181,6 +184,25 @@ def lib() -> ctypes.CDLL:
         L.hiprt_event_elapsed_ms.argtypes = [_P, _P, ctypes.POINTER(ctypes.c_float)]
         _lib = L
     return _lib
+
+
+_calls = None
+
+
+def _load_calls():
+    """The native module of the calls that are made once a layer and step (csrc/calls.cpp)."""
+    global _calls
+    lib()
+    if not os.path.exists(CALLS_PATH):
+        raise ImportError(f"{CALLS_PATH} is missing: run `python triton-rs_amd/build.py` "
+                          "(or __graft_entry__.build()) first")
+    loader = importlib.machinery.ExtensionFileLoader("_calls", CALLS_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_calls", CALLS_PATH, loader=loader))
+    loader.exec_module(module)
+    # (a build of torch without a GPU runtime has no streams, and no tensor that a call would take)
+    module.setup(InvalidArgument, check, getattr(torch._C, "_cuda_getCurrentRawStream", None))
+    _calls = module
+    return module
 
 
 def check(rc: int) -> None:
@@ -642,62 +664,12 @@ def _call_on(index: int, fn, *args) -> None:
 E4M3 = torch.float8_e4m3fn
 
 
-def _norm_rows(t, name: str, dtypes, index: int, shape):
-    """(T, H, K, token stride, head stride) of rows [T, K] or [T, H, K]."""
-    _tensor(t, name, dtypes, index)
-    if t.shape != shape if shape is not None else t.dim() not in (2, 3):
-        raise InvalidArgument(f"{name} must be {list(shape) if shape is not None else '[T, K] or [T, H, K]'}, not {list(t.shape)}")
-    T, H, K = (t.shape[0], 1, t.shape[1]) if t.dim() == 2 else t.shape
-    st = t.stride()
-    if K > 1 and st[-1] != 1:
-        raise InvalidArgument(f"{name} must be contiguous along its last dimension")
-    st, sh = st[0], (st[1] if t.dim() == 3 else 0)
-    if max(T, H, K, st, sh) > _INT32_MAX:
-        raise InvalidArgument(f"{name}: sizes and strides are 32-bit ({list(t.shape)} at {st}, {sh})")
-    return T, H, K, st, sh
-
-
-def _rms_norm(x, weight, eps, residual, residual_out, out, scales, group, fn, out_dtype):
-    index = x.get_device() if isinstance(x, _Tensor) else -1
-    if index < 0:
-        _require(x, "x", _ELEM)
-    T, H, K, st, sh = _norm_rows(x, "x", _ELEM, index, None)
-    _tensor(weight, "weight", (x.dtype,), index)
-    if weight.shape != (K,) or not weight.is_contiguous():
-        raise InvalidArgument(f"weight must be a contiguous [{K}] tensor")
-    r = ro = (None, 0, 0)
-    if residual is not None:
-        if residual_out is None:
-            residual_out = residual
-        r = (residual.data_ptr(), *_norm_rows(residual, "residual", (x.dtype,), index, x.shape)[3:])
-        ro = (residual_out.data_ptr(), *_norm_rows(residual_out, "residual_out", (x.dtype,), index, x.shape)[3:])
-    elif residual_out is not None:
-        raise InvalidArgument("residual_out without residual")
-    if out is None:
-        out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-    ost, osh = _norm_rows(out, "out", (out_dtype or x.dtype,), index, x.shape)[3:]
-    if out_dtype is None:
-        _call_on(index, fn, _elem_flag(x), x.data_ptr(), st, sh, *r, *ro, weight.data_ptr(), out.data_ptr(), ost, osh, T, H, K, eps)
-        return out
-    if group < 0 or (group and K % group):
-        raise InvalidArgument(f"group {group}: 0 (a row), or a divisor of {K}")
-    shape = (*x.shape[:-1], K // (group or K) if K else 0)
-    if scales is None:
-        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
-    _tensor(scales, "scales", (torch.float32,), index)
-    if scales.shape != shape or not scales.is_contiguous():
-        raise InvalidArgument(f"scales must be a contiguous {list(shape)} tensor")
-    _call_on(index, fn, _elem_flag(x), x.data_ptr(), st, sh, *r, *ro, weight.data_ptr(), out.data_ptr(), ost, osh,
-             scales.data_ptr(), T, H, K, group, eps)
-    return out, scales
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
              residual_out: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = h / sqrt(mean(h^2) + eps) * weight along the last dimension of x [T, K] or [T, H, K] (fp16 or
     bfloat16; any strides but along K), h = x + residual where one is given. The sum h goes to
     residual_out (residual itself unless given), rounded; y is made from the unrounded sum. out may be x."""
-    return _rms_norm(x, weight, eps, residual, residual_out, out, None, -1, lib().w4a16_rms_norm, None)
+    return (_calls or _load_calls()).rms_norm(x, weight, eps, residual, residual_out, out, None, None)
 
 
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group: int = 0,
@@ -706,7 +678,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, grou
     """(out, scales): rms_norm's y as e4m3 (torch.float8_e4m3fn) with an fp32 scale for every `group`
     elements (32, 64, 128, 256 or 512) or for a row (0): y = out * scale, scales [T, K / group] ([T, 1] for
     rows: what torch._scaled_mm takes)."""
-    return _rms_norm(x, weight, eps, residual, residual_out, out, scales, group, lib().w4a16_rms_norm_8bit, E4M3)
+    return (_calls or _load_calls()).rms_norm(x, weight, eps, residual, residual_out, out, scales, group)
 
 
 ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3}
@@ -743,89 +715,14 @@ def rope(q: torch.Tensor, positions: torch.Tensor, rope: Rope, k: torch.Tensor |
          q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
     """q [T, heads, D] and k [T, kv heads, D] (fp16 or bfloat16) rotated at positions (int32 [T]) into q_out
     and k_out (in place unless given), which are returned: (q_out, k_out), or q_out without k."""
-    index = q.get_device() if isinstance(q, _Tensor) else -1
-    if index < 0:
-        _require(q, "q", _ELEM)
-    qst, qsh = _rows(q, "q", _ELEM, index)
-    T, Hq, D = q.shape
+    (_calls or _load_calls()).rope(q, positions, rope.inv_freq, rope.magnitude, rope.interleaved, k, q_out, k_out)
     q_out = q if q_out is None else q_out
-    qost, qosh = _rows(q_out, "q_out", (q.dtype,), index, q.shape)
-    _index(positions, "positions", index, (T,))
-    _tensor(rope.inv_freq, "rope.inv_freq", (torch.float64,), index)
-    Hkv, krows = 0, (None, 0, 0, None, 0, 0)
-    if k is not None:
-        Hkv = k.shape[1] if k.dim() == 3 else 0
-        kst, ksh = _rows(k, "k", (q.dtype,), index, (T, Hkv, D))
-        k_out = k if k_out is None else k_out
-        krows = (k.data_ptr(), kst, ksh, k_out.data_ptr(), *_rows(k_out, "k_out", (q.dtype,), index, k.shape))
-    elif k_out is not None:
-        raise InvalidArgument("k_out without k")
-    _call_on(index, lib().w4a16_rope, _elem_flag(q), q.data_ptr(), qst, qsh, q_out.data_ptr(), qost, qosh, *krows,
-             positions.data_ptr(), rope.inv_freq.data_ptr(), rope.magnitude, T, Hq, Hkv, D, rope.rot, int(rope.interleaved))
-    return q_out if k is None else (q_out, k_out)
+    return q_out if k is None else (q_out, k if k_out is None else k_out)
 
 
 # ------------------------------------------------------------------ attention over a paged cache
 
 KV_COUNTER_BYTES = KV4_COUNTER_BYTES = KV8_COUNTER_BYTES = 65536
-
-
-def _attention_workspace(shape_of, fn, q, cache, num_seqs, max_q_len, max_kv_len) -> torch.Tensor:
-    _, Hkv, _, D, _ = shape_of(cache)
-    T, Hq = q.shape[:2]
-    if max(T, num_seqs, max_q_len, max_kv_len) > _INT32_MAX:
-        raise InvalidArgument(f"sizes are 32-bit ({T}, {num_seqs}, {max_q_len}, {max_kv_len})")
-    need = fn(T, num_seqs, Hq, Hkv, D, max_q_len, max_kv_len)
-    if need == 0:
-        check(ERR_INVALID_ARG)
-    ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
-    ws[:KV_COUNTER_BYTES].zero_()
-    return ws
-
-
-def _attention(shape_of, workspace_of, fn, q, cache, page_table, kv_lens, cu_q, max_q_len, max_kv_len, scale, causal, window,
-               out, lse, workspace) -> torch.Tensor:
-    pages, Hkv, page, D, dev = shape_of(cache)
-    qst, qsh = _rows(q, "q", _ELEM, dev)
-    T, Hq, Dq = shape = q.shape
-    if Dq != D:
-        raise InvalidArgument(f"q has heads of {Dq} dimensions, the cache {D}")
-    _index(page_table, "page_table", dev)
-    if page_table.dim() != 2:
-        raise InvalidArgument("page_table must be [sequences, pages per sequence]")
-    B, per = page_table.shape
-    _index(kv_lens, "kv_lens", dev, (B,))
-    if cu_q is not None:
-        _index(cu_q, "cu_q", dev, (B + 1,))
-    elif T != B:   # (also where one is 0, and there would be nothing to launch)
-        raise InvalidArgument(f"without cu_q every sequence has one query ({T} queries, {B} sequences)")
-    if max_q_len is None:
-        max_q_len = 1 if cu_q is None else max(1, T)
-    if max_kv_len is None:
-        max_kv_len = per * page
-    if max_q_len > _INT32_MAX or max_kv_len > _INT32_MAX or window > _INT32_MAX:
-        raise InvalidArgument(f"max_q_len, max_kv_len and window are 32-bit ({max_q_len}, {max_kv_len}, {window})")
-    if out is None:
-        out = (torch.empty if cu_q is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
-    ost, osh = _rows(out, "out", (q.dtype,), dev, shape)
-    if lse is not None:
-        _tensor(lse, "lse", (torch.float32,), dev)
-        if lse.shape != (T, Hq) or not lse.is_contiguous():
-            raise InvalidArgument(f"lse must be a contiguous [{T}, {Hq}] tensor")
-    if T == 0 or B == 0:
-        return out
-    if workspace is None:
-        workspace = workspace_of(q, cache, B, max_q_len, max_kv_len)
-    else:
-        _tensor(workspace, "workspace", (torch.uint8,), dev)
-        if not workspace.is_contiguous():
-            raise InvalidArgument("workspace must be contiguous")
-    _call_on(dev, fn, _elem_flag(q), q.data_ptr(), qst, qsh, cache.data_ptr(),
-             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
-             out.data_ptr(), ost, osh, None if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, pages, page,
-             per, max_q_len, max_kv_len, D ** -0.5 if scale is None else scale, int(causal), window,
-             workspace.data_ptr(), workspace.numel())
-    return out
 
 
 # ------------------------------------------------------------------ key/value cache in 4 bits
@@ -901,7 +798,7 @@ def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int,
     max_q_len and this max_kv_len or a smaller one. A call of another shape may need more, a smaller
     one too: a workspace for several is as large as the largest of theirs. Calls that may overlap in
     time need one each."""
-    return _attention_workspace(_kv4_cache_shape, lib().w4a16_kv4_attention_workspace_size, q, cache, num_seqs, max_q_len, max_kv_len)
+    return (_calls or _load_calls()).attention_workspace(4, q, cache, num_seqs, max_q_len, max_kv_len)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -921,8 +818,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     max_q_len, max_kv_len: bounds on the batch (T, or 1 without cu_q, and the table's width unless
     given; close ones make a better plan and a far smaller workspace). workspace: from kv4_attention_workspace, kept between calls; made for the call unless
     given."""
-    return _attention(_kv4_cache_shape, kv4_attention_workspace, lib().w4a16_kv4_attention, q, cache, page_table, kv_lens, cu_q,
-                      max_q_len, max_kv_len, scale, causal, window, out, lse, workspace)
+    return (_calls or _load_calls()).attention(4, q, cache, page_table, kv_lens, cu_q, max_q_len, max_kv_len, scale, causal, window, out,
+                                               lse, workspace)
 
 
 # ------------------------------------------------------------------ key/value cache in 8 bits
@@ -940,21 +837,6 @@ def kv8_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int =
                        dtype=torch.uint8, device=device)
 
 
-def _kv8_cache_shape(cache: torch.Tensor):
-    """(pages, kv heads, page size, head dim, device index) of a cache tensor."""
-    index = cache.get_device() if isinstance(cache, _Tensor) else -1
-    if index < 0 or cache.dtype is not torch.uint8:
-        _require(cache, "cache", (torch.uint8,))
-    shape = cache.shape
-    if len(shape) != 4 or not cache.is_contiguous():
-        raise InvalidArgument("cache must be a contiguous [pages, kv heads, page_size / 16, 32 D + 16] tensor")
-    pages, Hkv, blocks, width = shape
-    D = (width - 16) // 32
-    if D < 1 or width != 32 * D + 16:
-        raise InvalidArgument(f"cache has blocks of {width} bytes, not 32 D + 16")
-    return pages, Hkv, blocks * 16, D, index
-
-
 def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
               cu_q: torch.Tensor | None = None, max_q_len: int | None = None, rope: Rope | None = None,
               positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
@@ -969,69 +851,28 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table:
     max_q_len: a bound on the new tokens of a sequence (T unless given; a close one makes a smaller launch).
     rope: k is rotated first, in fp32, at positions (int32 [T]) or each token's place in its sequence, and q [T,
     heads, D], where given, into q_out (in place unless given) in the same launch."""
-    pages, Hkv, page, D, dev = _kv8_cache_shape(cache)
-    _tensor(k, "k", _ELEM, dev)
-    T = k.shape[0] if k.dim() else 0
-    kst, ksh = _rows(k, "k", _ELEM, dev, (T, Hkv, D))
-    vst, vsh = _rows(v, "v", (k.dtype,), dev, (T, Hkv, D))
-    _index(page_table, "page_table", dev)
-    if page_table.dim() != 2:
-        raise InvalidArgument("page_table must be [sequences, pages per sequence]")
-    B, per = page_table.shape
-    _index(kv_lens, "kv_lens", dev, (B,))
-    if cu_q is not None:
-        _index(cu_q, "cu_q", dev, (B + 1,))
-    if max_q_len is None:
-        max_q_len = 1 if cu_q is None else max(1, T)
-    if max(B, per, max_q_len) > _INT32_MAX:
-        raise InvalidArgument(f"sizes are 32-bit ({B}, {per}, {max_q_len})")
-    Hq, qrows, turn = 0, (None, 0, 0, None, 0, 0), (None, None, 0.0, 0, 0)
-    if rope is not None:
-        _tensor(rope.inv_freq, "rope.inv_freq", (torch.float64,), dev)
-        if positions is not None:
-            _index(positions, "positions", dev, (T,))
-        turn = (None if positions is None else positions.data_ptr(), rope.inv_freq.data_ptr(), rope.magnitude, rope.rot, int(rope.interleaved))
-        if q is not None:
-            Hq = q.shape[1] if q.dim() == 3 else 0
-            qst, qsh = _rows(q, "q", (k.dtype,), dev, (T, Hq, D))
-            q_out = q if q_out is None else q_out
-            qrows = (q.data_ptr(), qst, qsh, q_out.data_ptr(), *_rows(q_out, "q_out", (q.dtype,), dev, q.shape))
-    elif positions is not None or q is not None:
-        raise InvalidArgument("positions and q are for a rotation: give rope")
-    if q is None and q_out is not None:
-        raise InvalidArgument("q_out without q")
-    if T == 0 or B == 0:
-        return cache
-    _call_on(dev, lib().w4a16_kv8_write, _elem_flag(k), k.data_ptr(), kst, ksh, v.data_ptr(), vst, vsh, *qrows, *turn,
-             cache.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, B, Hq,
-             Hkv, D, pages, page, per, max_q_len)
-    return cache
+    turn = (None, None, None) if rope is None else (rope.inv_freq, rope.magnitude, rope.interleaved)
+    return (_calls or _load_calls()).kv8_write(k, v, cache, page_table, kv_lens, cu_q, max_q_len, *turn, positions, q, q_out)
 
 
 def kv8_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_out=None, v_out=None):
     """(k, v) [T, kv heads, D]: the rows that the slots (int32 [T], page * page_size + offset) of the cache hold,
     rounded to `dtype`, or that of k_out and v_out. Rows whose slot is negative or beyond the cache are left as
     they were in k_out and v_out (0 where these are not given)."""
-    pages, Hkv, page, D, dev = _kv8_cache_shape(cache)
-    _index(slots, "slots", dev)
-    if slots.dim() != 1:
-        raise InvalidArgument("slots must be 1-D")
-    shape = (slots.shape[0], Hkv, D)
     if (k_out is None) != (v_out is None):
         raise InvalidArgument("give both k_out and v_out, or neither")
     if k_out is None:
-        k_out, v_out = torch.zeros((2, *shape), dtype=dtype, device=cache.device)
-    kst, ksh = _rows(k_out, "k_out", _ELEM, dev, shape)
-    vst, vsh = _rows(v_out, "v_out", (k_out.dtype,), dev, shape)
-    _call_on(dev, lib().w4a16_kv8_read, _elem_flag(k_out), cache.data_ptr(), slots.data_ptr(), k_out.data_ptr(), kst, ksh,
-             v_out.data_ptr(), vst, vsh, pages, shape[0], Hkv, D, page)
+        if not isinstance(cache, _Tensor) or not isinstance(slots, _Tensor) or cache.dim() != 4:
+            raise InvalidArgument("cache and slots must be tensors, cache as kv8_cache makes it")
+        k_out, v_out = torch.zeros((2, slots.numel(), cache.shape[1], (cache.shape[3] - 16) // 32), dtype=dtype, device=cache.device)
+    (_calls or _load_calls()).kv8_read(cache, slots, k_out, v_out)
     return k_out, v_out
 
 
 def kv8_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int, max_q_len: int,
                             max_kv_len: int) -> torch.Tensor:
     """A workspace for kv8_attention calls, as kv4_attention_workspace makes it."""
-    return _attention_workspace(_kv8_cache_shape, lib().w4a16_kv8_attention_workspace_size, q, cache, num_seqs, max_q_len, max_kv_len)
+    return (_calls or _load_calls()).attention_workspace(8, q, cache, num_seqs, max_q_len, max_kv_len)
 
 
 def kv8_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -1041,8 +882,8 @@ def kv8_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     """softmax(scale q k^T) v over the keys and values of an 8-bit cache; returns out [T, heads, D]. Arguments,
     masks, results and workspace are kv4_attention's; the new tokens' keys and values are in the cache already
     (kv8_write), and q may be of either type, whatever the cache was written from."""
-    return _attention(_kv8_cache_shape, kv8_attention_workspace, lib().w4a16_kv8_attention, q, cache, page_table, kv_lens, cu_q,
-                      max_q_len, max_kv_len, scale, causal, window, out, lse, workspace)
+    return (_calls or _load_calls()).attention(8, q, cache, page_table, kv_lens, cu_q, max_q_len, max_kv_len, scale, causal, window, out,
+                                               lse, workspace)
 
 
 # ------------------------------------------------------------------ kernel level (reference names)

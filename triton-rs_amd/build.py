@@ -4,6 +4,7 @@ Outputs (next to this file):
   libw4a16.so         C ABI of include/w4a16.h (kernels embedded as a gfx950 fat binary)
   w4a16_typed.hsaco   code object with the reference-named kernels, for hiprt_module_load
   w4a16_typed.json    launch metadata for that code object
+  _calls.so           CPython module of the calls made once a layer and step (csrc/calls.cpp)
 
 Every HIP compile line carries `-Xclang -target-feature -Xclang -packed-fp32-ops`, which
 turns off packed-fp32 instruction selection on this target.
@@ -24,9 +25,11 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libw4a16.so")
 HSACO = os.path.join(HERE, "w4a16_typed.hsaco")
 META = os.path.join(HERE, "w4a16_typed.json")
+CALLS = os.path.join(HERE, "_calls.so")
 
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}"]
@@ -68,13 +71,35 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _compile_calls() -> str:
+    """calls.cpp with torch's headers: the host compiler, as torch's own extensions are built."""
+    import sysconfig
+
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    obj = _obj("calls.cpp")
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
+          "-c", os.path.join(CSRC, "calls.cpp"), "-o", obj])
+    return obj
+
+
+def _link_calls(obj: str) -> None:
+    """Its library is the one beside it; torch's are loaded before it."""
+    import torch
+    _run([CXX, "-shared", obj, "-o", CALLS + ".tmp", f"-L{HERE}", "-lw4a16", f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}",
+          "-ltorch_python", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"])
+    os.replace(CALLS + ".tmp", CALLS)
+
+
 def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
     # an object whose source is gone would still be linked by whoever takes all objects here
     for f in os.listdir(BUILD):
-        if f.endswith(".o") and os.path.join(BUILD, f) not in map(_obj, SOURCES):
+        if f.endswith(".o") and os.path.join(BUILD, f) not in map(_obj, [*SOURCES, "calls.cpp"]):
             os.remove(os.path.join(BUILD, f))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        fut_calls = ex.submit(_compile_calls)
         objs = list(ex.map(_compile, SOURCES))
         fut_hsaco = ex.submit(_run, [HIPCC, "-x", "hip", f"--offload-arch={ARCH}", *COMMON,
                                      "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "typed_module.hip"),
@@ -83,6 +108,7 @@ def build(verbose: bool = True) -> str:
     os.replace(HSACO + ".tmp", HSACO)
     _run([HIPCC, "-shared", "-fPIC", *objs, "-o", LIB + ".tmp"])
     os.replace(LIB + ".tmp", LIB)
+    _link_calls(fut_calls.result())
     meta = {
         "kernels": [
             {"name": name, "num_warps": 8, "threads_per_block": 256, "warp_size": 64,
@@ -96,13 +122,13 @@ def build(verbose: bool = True) -> str:
     with open(META, "w") as f:
         json.dump(meta, f, indent=2)
     if verbose:
-        print(f"built {LIB} and {HSACO}")
+        print(f"built {LIB}, {HSACO} and {CALLS}")
     return LIB
 
 
 def clean() -> None:
     shutil.rmtree(BUILD, ignore_errors=True)
-    for p in (LIB, HSACO, META):
+    for p in (LIB, HSACO, META, CALLS):
         if os.path.exists(p):
             os.remove(p)
 

@@ -15,7 +15,7 @@ static_assert(KV_COUNTER_BYTES == W4A16_KV8_COUNTER_BYTES, "counters fill their 
 
 constexpr int32_t KV8_MAX_TOKENS = 1 << 22;   // of a call that writes: their workgroups' threads are counted in 32 bits
 
-static const KvFormat KV8 = {"kv8 attention launch", kv8_few_per_cu, kv8_many_simd_waves, 512, 3.f, 3.5f, 12, 96 << 10,
+static const KvFormat KV8 = {"kv8 attention launch", kv8_few_per_cu, kv8_many_simd_waves, 512, 1.f, 3.f, 3.5f, 12, 96 << 10,
                              launch_kv8_few, launch_kv8_many};
 
 }  // namespace w4a16

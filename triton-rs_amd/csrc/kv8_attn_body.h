@@ -49,6 +49,7 @@ __device__ __forceinline__ uint32_t token_bytes(int lo, int hi, int kb) {
     return from & to;
 }
 
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 // What logits and weights take of a block's last 16 bytes. (there: a token of it is seen; else its scales may be anything, and
 // a NaN would pass into the sums by way of weights of zero.)
 struct Kv8Scale {
@@ -56,7 +57,7 @@ struct Kv8Scale {
     float value;     // log2 of the scale of its values
     float back;      // 1 / that scale
     uint32_t nan;    // rows that are not finite
-    __device__ __forceinline__ static Kv8Scale of(u32x4 tail, float factor, bool there) {
+    __device__ __forceinline__ static Kv8Scale of(u32x3 tail, float factor, bool there) {
         const uint32_t e = there ? (tail[1] >> 23) & 255u : 127u;
         return {there ? __uint_as_float(tail[0]) * factor : 0.f, (float)((int)e - 127), __uint_as_float((254u - e) << 23), there ? tail[2] : 0u};
     }
@@ -228,9 +229,10 @@ struct Kv8Cols {
     }
 };
 
-// A block's last 16 bytes, by a scalar load (constant address space: no kernel that reads them writes them).
-__device__ __forceinline__ u32x4 block_tail(const unsigned char* block, int D) {
-    return *(const __attribute__((address_space(4))) u32x4*)(block + 32 * D);
+// What of a block's last 16 bytes says something, in every lane: a vector load, which is waited for with the block's others. (A
+// scalar load is waited for with all scalar loads, the next step's among them: 64 us for the 55 of kv8_few.hip's 48 sequences.)
+__device__ __forceinline__ u32x3 block_tail(const unsigned char* block, int D) {
+    return *reinterpret_cast<const u32x3*>(at_bytes(block, 32 * D + vconst(0)));
 }
 
 }  // namespace w4a16

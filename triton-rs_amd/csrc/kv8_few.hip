@@ -10,13 +10,6 @@
 
 namespace w4a16 {
 
-// A step of 32 keys as this lane takes it.
-template <int D>
-struct FewStep {
-    u32x4 k[2][D / 64], v[2][D / 64], tail[2];
-    int bad;   // bit s: block s lies in no page
-};
-
 template <typename E, int D, int NT>
 __global__ __launch_bounds__(256, kv8_few_per_cu(D, NT)) void kv8_few_kernel(KvAttnParams p) {
     typedef Kv8Cols<E, D, NT> C;
@@ -37,76 +30,87 @@ __global__ __launch_bounds__(256, kv8_few_per_cu(D, NT)) void kv8_few_kernel(KvA
     a.load(p, w, w.c0 + (wave >> kshift) * COLS, lane);
     const int stride = STEP << kshift, beg = __builtin_amdgcn_readfirstlane((a.jlo & ~(STEP - 1)) + STEP * (wave & (kspl - 1))), end = __builtin_amdgcn_readfirstlane(a.jhi);
     const KvPages pages(p, w, kv8_block_bytes(D));
-    // (steps beyond the last load its last block again; none is computed)
-    auto fetch = [&](FewStep<D>& s, int at, int pa, int pb) {
-        const unsigned char* const block[2] = {pages.block(pa, at >> 4), pages.block(pb, (at >> 4) + 1)};
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-#pragma unroll
-            for (int g = 0; g < D / 64; ++g) s.k[b][g] = *reinterpret_cast<const u32x4*>(at_bytes(block[b], 1024 * g + 16 * lane));
-#pragma unroll
-            for (int g = 0; g < D / 64; ++g) s.v[b][g] = *reinterpret_cast<const u32x4*>(at_bytes(block[b], 16 * D + 1024 * g + 16 * lane));
-            s.tail[b] = block_tail(block[b], D);
-        }
-        s.bad = (pages.ok(pa) ? 0 : 1) | (pages.ok(pb) ? 0 : 2);
+    // One step of keys and one of values in registers: the next step's keys are loaded over this one's as soon as the first product
+    // has taken them, its values behind the second. (Steps beyond the last load its last block again; none is computed.)
+    u32x4 k[2][D / 64], v[2][D / 64];
+    u32x3 tail[2];
+    int bad = 0;   // bit b: block b of the step lies in no page
+    const unsigned char* block[2];
+    auto locate = [&](int at, int pa, int pb) {
+        block[0] = pages.block(pa, at >> 4);
+        block[1] = pages.block(pb, (at >> 4) + 1);
     };
-    auto compute = [&](const FewStep<D>& s, int j) {
-        const int bad = __builtin_amdgcn_readfirstlane(s.bad);
-        float4_t acc[NT][2];
+    auto load_keys = [&] {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int x = 0; x < C::KW; ++x)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const auto f = operand8<E>(s.k[b][x >> 1][2 * (x & 1)], s.k[b][x >> 1][2 * (x & 1) + 1]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t][b] = mfma16x16x32(f, a.qf[t][x], acc[t][b]);
-            }
-        const Kv8Scale sc[2] = {Kv8Scale::of(s.tail[0], p.scale_log2, !(bad & 1) && j + 16 > a.jlo),
-                                Kv8Scale::of(s.tail[1], p.scale_log2, !(bad & 2) && j + 16 < end && j + 32 > a.jlo)};
-        const bool whole = j >= a.all_lo && j + STEP <= a.all_hi && j + STEP <= end && !bad && !(sc[0].nan | sc[1].nan);
-        // bytes of tokens that no column sees may be anything
-        uint32_t mask[2] = {~0u, ~0u};
-        if (!whole)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) mask[b] = token_bytes(a.jlo - j - 16 * b, (bad >> b) & 1 ? 0 : end - j - 16 * b, kb);
-        half8_t pw[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float x[2][4], back[2];
-            a.logits(t, x, back, acc[t], sc, whole, j, end, bad, kb);
-            pw[t] = a.weights(t, x, back);
-        }
-#pragma unroll
-        for (int g = 0; g < D / 64; ++g)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const half8_t f = operand8<half_t>(s.v[0][g][e] & mask[0], s.v[1][g][e] & mask[1]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) a.o[t][4 * g + e] = mfma16x16x32(f, pw[t], a.o[t][4 * g + e]);
-            }
+            for (int g = 0; g < D / 64; ++g) k[b][g] = *reinterpret_cast<const u32x4*>(at_bytes(block[b], 1024 * g + 16 * lane));
     };
+    auto load_values = [&] {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int g = 0; g < D / 64; ++g) v[b][g] = *reinterpret_cast<const u32x4*>(at_bytes(block[b], 16 * D + 1024 * g + 16 * lane));
+    };
+    auto load_tails = [&] {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tail[b] = block_tail(block[b], D);
+    };
+    a.start();
     if (beg < end) {
-        FewStep<D> s0, s1;
         auto page = [&](int at, int b) { return pages.page((at >> 4) + b); };
-        int pa = page(beg + stride, 0), pb = page(beg + stride, 1);
-        fetch(s0, beg, page(beg, 0), page(beg, 1));
-        a.start();
-        for (int j = beg;; j += 2 * stride) {
-            fetch(s1, j + stride, pa, pb);
+        int pa = page(beg, 0), pb = page(beg, 1);
+        locate(beg, pa, pb);
+        load_keys();
+        load_tails();
+        load_values();
+        bad = (pages.ok(pa) ? 0 : 1) | (pages.ok(pb) ? 0 : 2);
+        pa = page(beg + stride, 0);
+        pb = page(beg + stride, 1);
+        for (int j = beg; j < end; j += stride) {
+            float4_t acc[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < C::KW; ++x)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const auto f = operand8<E>(k[b][x >> 1][2 * (x & 1)], k[b][x >> 1][2 * (x & 1) + 1]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t][b] = mfma16x16x32(f, a.qf[t][x], acc[t][b]);
+                }
+            locate(j + stride, pa, pb);
+            load_keys();
+            __builtin_amdgcn_sched_barrier(0);
+            const Kv8Scale sc[2] = {Kv8Scale::of(tail[0], p.scale_log2, !(bad & 1) && j + 16 > a.jlo),
+                                    Kv8Scale::of(tail[1], p.scale_log2, !(bad & 2) && j + 16 < end && j + 32 > a.jlo)};
+            const bool whole = j >= a.all_lo && j + STEP <= a.all_hi && j + STEP <= end && !bad && !__builtin_amdgcn_readfirstlane(sc[0].nan | sc[1].nan);
+            // bytes of tokens that no column sees may be anything
+            uint32_t mask[2] = {~0u, ~0u};
+            if (!whole)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) mask[b] = token_bytes(a.jlo - j - 16 * b, (bad >> b) & 1 ? 0 : end - j - 16 * b, kb);
+            half8_t pw[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x[2][4], back[2];
+                a.logits(t, x, back, acc[t], sc, whole, j, end, bad, kb);
+                pw[t] = a.weights(t, x, back);
+            }
+            load_tails();
+#pragma unroll
+            for (int g = 0; g < D / 64; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const half8_t f = operand8<half_t>(v[0][g][e] & mask[0], v[1][g][e] & mask[1]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) a.o[t][4 * g + e] = mfma16x16x32(f, pw[t], a.o[t][4 * g + e]);
+                }
+            load_values();
+            bad = __builtin_amdgcn_readfirstlane((pages.ok(pa) ? 0 : 1) | (pages.ok(pb) ? 0 : 2));
             pa = page(j + 2 * stride, 0);
             pb = page(j + 2 * stride, 1);
-            compute(s0, j);
-            if (j + stride >= end) break;
-            fetch(s0, j + 2 * stride, pa, pb);
-            pa = page(j + 3 * stride, 0);
-            pb = page(j + 3 * stride, 1);
-            compute(s1, j + stride);
-            if (j + 2 * stride >= end) break;
         }
-    } else {
-        a.start();
     }
     a.finish();
 

@@ -22,7 +22,8 @@ struct ManyLds {
 // A block (of this wave) as this lane takes it.
 template <int D>
 struct Packed {
-    u32x4 k[D / 64], v[D / 64], tail;
+    u32x4 k[D / 64], v[D / 64];
+    u32x3 tail;
 };
 
 // Block `wave` of a step into LDS; its tokens [dead, live) (the others' bytes may be anything)
@@ -61,9 +62,11 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
     const KvPages pages(p, w, kv8_block_bytes(D));
     Packed<D> t;
     int live = 0;   // tokens of this wave's block of the step in t
-    // (beyond the keys: their last block again, none of it alive)
+    // (beyond the keys: their last block again, none of it alive; the page of the step after it ahead of its use)
+    int page = 0;
+    auto block_of = [&](int j) { return ((j + STEP * group) >> 4) + wave; };
     auto fetch = [&](int j) {
-        const int blk = ((j + STEP * group) >> 4) + wave, page = pages.page(blk);
+        const int blk = block_of(j);
         live = pages.ok(page) ? w.k1 - 16 * blk : 0;
         const unsigned char* b = pages.block(page, blk);
 #pragma unroll
@@ -71,9 +74,13 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
 #pragma unroll
         for (int g = 0; g < D / 64; ++g) t.v[g] = *reinterpret_cast<const u32x4*>(at_bytes(b, 16 * D + 1024 * g + 16 * lane));
         t.tail = block_tail(b, D);
+        page = pages.page(block_of(j + ALL));
     };
     const bool any = w.k0 < w.k1;
-    if (any) fetch(w.k0);
+    if (any) {
+        page = pages.page(block_of(w.k0));
+        fetch(w.k0);
+    }
     a.start();
     if (any) {   // (only a first step holds tokens before what its columns see)
         unpack<E, D>(lds[0][group], t, w.see_lo(p, w.n <= 1 ? 0 : w.c0 / p.G) - (w.k0 + STEP * group + 16 * wave), live, p.scale_log2, wave, lane);

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv4_many_simd_waves(D, GROUPS)) void 
 template <typename E, int D>
 __global__ __launch_bounds__(256) void kv4_many_join_kernel(KvAttnParams p) {
     __shared__ float ml[128][2];
-    many_join<E, D, VALUE_DOWN<E>>(p, &ml[0][0]);
+    many_join<E, D, VALUE_DOWN<E>>(p, &ml[0][0], [](int e, int& c, int& d) { KvSink<E, D, VALUE_DOWN<E>>::lane_place(e, c, d); });
 }
 
 template <typename E, int D>

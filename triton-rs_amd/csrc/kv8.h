@@ -46,7 +46,7 @@ struct Kv8ReadParams {
 hipError_t launch_kv8_read(bool bf16, int D, const Kv8ReadParams& p, hipStream_t st);
 
 // Workgroups of kv8_few.hip that are planned for a compute unit, by registers.
-constexpr int kv8_few_per_cu(int D, int nt) { return nt == 2 ? 2 : D == 64 ? 4 : D == 128 ? 3 : 2; }
+constexpr int kv8_few_per_cu(int D, int nt) { return nt == 2 ? (D == 64 ? 3 : 2) : D <= 128 ? 4 : 2; }
 hipError_t launch_kv8_few(bool bf16, int D, const KvAttnParams& p, const KvAttnShape& s, hipStream_t st);
 // Waves of kv8_many.hip a SIMD, by registers.
 constexpr int kv8_many_simd_waves(int D, int groups) { return D <= 128 ? 2 : 1; }

@@ -10,11 +10,17 @@
 
 namespace w4a16 {
 
+// The 32 x 32 x 16 product: lane l has row (or column) l % 32 of an operand at k = 8 (l / 32) + (0..7), and column l % 32 of the
+// result at rows 8 (i / 4) + 4 (l / 32) + i % 4. The vector unit runs beside it (64 multiplications and additions of one
+// wave and the products of another: 164 ns, 131 and 125 alone; beside as much work in 16 x 16 x 32 products 200).
+__device__ __forceinline__ float16_t mfma32x32x16(half8_t a, half8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float16_t mfma32x32x16(bf16x8_t a, bf16x8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
 template <typename E, int D>
 struct ManyLds {
-    static constexpr int KW = D / 32, VT = D / 16;
-    typename vec8<E>::type k[4][KW][64];   // block, operand of a row, lane
-    half8_t v[2][VT][64];                  // pair of blocks, tile of the result, lane (first block's tokens, second's)
+    static constexpr int KW = D / 16, VT = D / 32;
+    typename vec8<E>::type k[2][KW][64];   // pair of blocks, 16 dimensions, lane (token l % 32 of the pair)
+    half8_t v[4][VT][64];                  // block, 32 dimensions, lane (its quads l / 32 and 2 + l / 32 of tokens)
     Kv8Scale scale[4];
     int live[4];                           // tokens of a block that there are (0 or less: none)
 };
@@ -29,15 +35,19 @@ struct Packed {
 // Block `wave` of a step into LDS; its tokens [dead, live) (the others' bytes may be anything)
 template <typename E, int D>
 __device__ __forceinline__ void unpack(ManyLds<E, D>& s, const Packed<D>& t, int dead, int live, float factor, int wave, int lane) {
-    const uint32_t mask = dead <= 0 && live >= 16 ? ~0u : token_bytes(dead, live, lane >> 4);
+    const int r = lane & 15, quad = lane >> 4;
+    const uint32_t mask = dead <= 0 && live >= 16 ? ~0u : token_bytes(dead, live, quad);
+    auto* const k = &s.k[wave >> 1][quad][16 * (wave & 1) + r];
+    auto* const v = reinterpret_cast<u32x2*>(&s.v[wave][0][r + 32 * (quad & 1)]) + (quad >> 1);
 #pragma unroll
     for (int g = 0; g < D / 64; ++g) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s.k[wave][2 * g + h][lane] = operand8<E>(t.k[g][2 * h], t.k[g][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) k[4 * g * 64 + 32 * h] = operand8<E>(t.k[g][2 * h], t.k[g][2 * h + 1]);
+        // dimension r D / 16 + x, x = 4 g + e, is row r + 16 (x % 2) of tile x / 2
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t w = t.v[g][e] & mask;
-            *(reinterpret_cast<u32x2*>(&s.v[wave >> 1][4 * g + e][lane]) + (wave & 1)) = u32x2{from_e4m3<half_t, false>(w), from_e4m3<half_t, true>(w)};
+            v[2 * ((2 * g + e / 2) * 64 + 16 * (e & 1))] = u32x2{from_e4m3<half_t, false>(w), from_e4m3<half_t, true>(w)};
         }
     }
     if (lane == 0) {
@@ -46,16 +56,164 @@ __device__ __forceinline__ void unpack(ManyLds<E, D>& s, const Packed<D>& t, int
     }
 }
 
+__device__ __forceinline__ float half_max(float v) {   // over a column's two lanes, 32 apart
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A wave's 32 columns, column lane % 32 in a lane; as Kv8Cols, whose comments hold here.
+template <typename E, int D>
+struct ManyCols {
+    typedef typename vec8<E>::type vec_t;
+    static constexpr int KW = D / 16, VT = D / 32;
+    int c, n, lo, hi, jlo, jhi, all_lo, all_hi;
+    vec_t qf[KW];          // dimensions 16 x + 8 (lane / 32) + (0..7)
+    float m, l, most;
+    float16_t o[VT];       // dimension r D / 16 + 2 y + z, r + 16 z = 8 (i / 4) + 4 (lane / 32) + i % 4, in o[y][i]
+
+    __device__ __forceinline__ void load(const KvAttnParams& p, const KvItem& w, int first_col, int lane) {
+        c = first_col;
+        n = min(32, w.n * p.G - c);
+        const int col = lane & 31, r = c + col, i = w.n == 1 ? 0 : r / p.G;
+        const bool in = col < n;
+        hi = in ? w.see_hi(p, i) : 0;
+        lo = in ? w.see_lo(p, i) : 0;
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (size_t)(w.q0 + i) * p.q_st + (size_t)(w.h * p.G + r - i * p.G) * p.q_sh + 8 * (lane >> 5);
+        constexpr uint32_t inf = __is_same(E, half_t) ? 0x7C00u : 0x7F80u;
+#pragma unroll
+        for (int x = 0; x < KW; ++x) {
+            u32x4 v = {0, 0, 0, 0};
+            if (in) v = *reinterpret_cast<const u32x4*>(src + 16 * x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {   // infinities become NaN
+                const uint32_t u = v[e], a = u & 0x7FFFu, b = (u >> 16) & 0x7FFFu;
+                v[e] = u | (a < inf ? 0u : 0x7FFFu) | (b < inf ? 0u : 0x7FFF0000u);
+            }
+            qf[x] = __builtin_bit_cast(vec_t, v);
+        }
+        const int i0 = w.n == 1 ? 0 : c / p.G, i1 = w.n == 1 ? 0 : (c + max(n, 1) - 1) / p.G;
+        jlo = max(w.k0, w.see_lo(p, i0));
+        jhi = n > 0 ? min(w.k1, w.see_hi(p, i1)) : 0;
+        all_lo = w.see_lo(p, i1);
+        all_hi = w.see_hi(p, i0);
+        m = l = 0.f;
+        most = -INFINITY;
+#pragma unroll
+        for (int y = 0; y < VT; ++y)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[y][e] = 0.f;
+    }
+
+    // Tokens j + 8 (i / 4) + 4 (lane / 32) + i % 4 of 32 from j on.
+    __device__ __forceinline__ void logits(float (&x)[16], float (&back)[2], const float16_t& acc, const Kv8Scale (&s)[2], bool whole, int j, int end,
+                                           int bad, int lane) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float off = s[b].value - m;
+#pragma unroll
+            for (int i = 8 * b; i < 8 * b + 8; ++i) x[i] = __builtin_fmaf(acc[i], s[b].key, off);
+        }
+        if (!whole) {
+            int at = j + 4 * (lane >> 5);
+            asm volatile("" : "+v"(at), "+s"(bad));   // (else kept over the loop: every token's distances, in registers)
+            const int from = lo - at, to = min(hi, end) - at;
+            uint32_t hit = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = 8 * (i / 4) + i % 4, b = i / 8, bit = (t + 4 * (lane >> 5)) & 15;
+                const bool in = (t >= from) & (t < to) & !((bad >> b) & 1);
+                if ((s[b].nan >> bit) & 1) x[i] = __builtin_nanf("");
+                if (!in) x[i] = -INFINITY;
+                hit |= in ? (s[b].nan >> (16 + bit)) & 1 : 0u;
+            }
+            if ((s[0].nan | s[1].nan) >> 16) {   // a value row of NaN makes those columns NaN that see it
+                const float add = half_max(hit ? 1.f : 0.f) > 0.f ? __builtin_nanf("") : 0.f;
+#pragma unroll
+                for (int y = 0; y < VT; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[y][i] += add;
+            }
+        }
+        float high[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = fmaxf(x[8 * b + i], x[8 * b + 4 + i]);
+            high[b] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            back[b] = s[b].back;
+        }
+        float top = fmaxf(high[0], high[1]);
+        if (__any((top > most) | (fminf(high[0], high[1]) < KV8_LOW))) {   // rare after the first steps
+            top = half_max(top);
+            const bool up = top > most;
+            const float by = up ? top - (KV8_MOST - KV8_ROOM) : 0.f;
+            const float fall = most == -INFINITY ? 0.f : half_fall(0.f, by);
+            m += by;
+            l = l * fall * fall;
+#pragma unroll
+            for (int y = 0; y < VT; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[y][i] *= fall * fall;
+            most = up ? KV8_MOST : most;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const bool alone = high[b] - by < KV8_LOW;
+                float p = 0.f;
+#pragma unroll
+                for (int i = 8 * b; i < 8 * b + 8; ++i) {
+                    x[i] -= by;
+                    p += __builtin_amdgcn_exp2f(x[i] - s[b].value);
+                }
+                l += alone ? p : 0.f;
+                back[b] = alone ? 0.f : back[b];
+            }
+        }
+    }
+    // Weights of block b as operand; the sum of p_j.
+    __device__ __forceinline__ half8_t weights(int b, const float (&x)[16], const float (&back)[2]) {
+        half8_t w;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            f[i] = __builtin_amdgcn_exp2f(x[8 * b + i]);
+            w[i] = (half_t)f[i];
+        }
+        l = __builtin_fmaf(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])), back[b], l);
+        return w;
+    }
+    __device__ __forceinline__ void finish() {
+        l = half_sum(l);
+        if (most == -INFINITY && l == 0.f) m = -FLT_MAX;
+    }
+    // Rows of the result: quad xq (four dimensions in a row) of rr-th row r
+    __device__ __forceinline__ static int row(int rr, int lane) { return 8 * (rr / 4) + 4 * (lane >> 5) + rr % 4; }
+    __device__ __forceinline__ float4_t quad(int rr, int xq) const {
+        return float4_t{o[2 * xq][rr], o[2 * xq][rr + 8], o[2 * xq + 1][rr], o[2 * xq + 1][rr + 8]};
+    }
+    // Partial results as lanes have them: number of a quad, and place of quad e
+    static constexpr int XQ = D / 64;
+    __device__ __forceinline__ static int lane_quad(int wave, int rr, int xq, int lane) { return ((wave * 8 + rr) * XQ + xq) * 64 + lane; }
+    __device__ __forceinline__ static void lane_place(int e, int& c, int& d) {
+        const int lane = e & 63, q = e >> 6, xq = q % XQ, u = q / XQ;
+        c = 32 * (u >> 3) + (lane & 31);
+        d = row(u & 7, lane) * (D / 16) + 4 * xq;
+    }
+};
+
 template <typename E, int D, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void kv8_many_kernel(KvAttnParams p) {
-    constexpr int NT = 2, COLS = 16 * NT, STEP = MANY_STEP, ALL = STEP * GROUPS;
-    typedef Kv8Cols<E, D, NT> C;
+    constexpr int COLS = 32, STEP = MANY_STEP, ALL = STEP * GROUPS;
+    typedef ManyCols<E, D> C;
     __shared__ ManyLds<E, D> lds[2][GROUPS];
     KvItem w;
     if (!many_item(p, blockIdx.z, w)) return;
     // wave `wave` of group `group`: the group takes every GROUPS-th step of the keys
     const int lane = threadIdx.x & 63, number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = number & 3, group = number >> 2;
-    const int col = lane & 15, kb = lane >> 4;
     C a;
     a.load(p, w, w.c0 + wave * COLS, lane);
 
@@ -80,9 +238,7 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
     if (any) {
         page = pages.page(block_of(w.k0));
         fetch(w.k0);
-    }
-    a.start();
-    if (any) {   // (only a first step holds tokens before what its columns see)
+        // (only a first step holds tokens before what its columns see)
         unpack<E, D>(lds[0][group], t, w.see_lo(p, w.n <= 1 ? 0 : w.c0 / p.G) - (w.k0 + STEP * group + 16 * wave), live, p.scale_log2, wave, lane);
         fetch(w.k0 + ALL);
     }
@@ -98,103 +254,94 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
         for (int half = 0; half < 2; ++half) {
             const int jh = j + STEP * group + 32 * half;
             if (jh >= a.jhi || jh + 32 <= a.jlo) continue;   // none of this wave's columns sees these
-            float4_t acc[NT][2];
+            float16_t acc;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 16; ++i) acc[i] = 0.f;
             // operands from LDS all at once, ahead of what takes them: one wait instead of eight
-            typename C::vec_t kf[2][C::KW];
-            half8_t vf[C::VT];
+            typename C::vec_t kf[C::KW];
+            half8_t vf[2][C::VT];
             Kv8Scale sc[2] = {s.scale[2 * half], s.scale[2 * half + 1]};
             const int live0 = s.live[2 * half], live1 = s.live[2 * half + 1];
 #pragma unroll
-            for (int x = 0; x < C::KW; ++x)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) kf[b][x] = s.k[2 * half + b][x][lane];
+            for (int x = 0; x < C::KW; ++x) kf[x] = s.k[half][x][lane];
             __builtin_amdgcn_sched_barrier(0);
             const int bad = __builtin_amdgcn_readfirstlane((live0 <= 0 ? 1 : 0) | (live1 <= 0 ? 2 : 0));
             sc[0].nan = __builtin_amdgcn_readfirstlane(sc[0].nan);
             sc[1].nan = __builtin_amdgcn_readfirstlane(sc[1].nan);
             const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad && !(sc[0].nan | sc[1].nan);
 #pragma unroll
-            for (int x = 0; x < C::KW; ++x)
+            for (int x = 0; x < C::KW; ++x) acc = mfma32x32x16(kf[x], a.qf[x], acc);
+            float x[16], back[2];
+            a.logits(x, back, acc, sc, whole, jh, a.jhi, bad, lane);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[n][b] = mfma16x16x32(kf[b][x], a.qf[n][x], acc[n][b]);
-            float x[NT][2][4], back[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) a.logits(n, x[n], back[n], acc[n], sc, whole, jh, a.jhi, bad, kb);
-#pragma unroll
-            for (int x = 0; x < C::VT; ++x) vf[x] = s.v[half][x][lane];
+                for (int y = 0; y < C::VT; ++y) vf[b][y] = s.v[2 * half + b][y][lane];
             __builtin_amdgcn_sched_barrier(0);
-                half8_t pw[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) pw[n] = a.weights(n, x[n], back[n]);
+            for (int b = 0; b < 2; ++b) {
+                const half8_t pw = a.weights(b, x, back);
 #pragma unroll
-            for (int x = 0; x < C::VT; ++x)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) a.o[n][x] = mfma16x16x32(vf[x], pw[n], a.o[n][x]);
+                for (int y = 0; y < C::VT; ++y) a.o[y] = mfma32x32x16(vf[b][y], pw, a.o[y]);
+            }
         }
         __syncthreads();
     }
     a.finish();
 
     if constexpr (GROUPS == 2) {   // the second group's share of the keys to the first
-        float4_t* const o = reinterpret_cast<float4_t*>(&lds[0][0]) + wave * (NT * C::VT) * 64;
-        float* const mls = reinterpret_cast<float*>(reinterpret_cast<float4_t*>(&lds[0][0]) + 4 * (NT * C::VT) * 64) + wave * NT * 128;
-        static_assert(4 * NT * C::VT * 64 * 16 + 4 * NT * 128 * 4 <= sizeof(lds), "results of four waves fit");
+        float4_t* const o = reinterpret_cast<float4_t*>(&lds[0][0]) + wave * (4 * C::VT) * 64;
+        float* const mls = reinterpret_cast<float*>(reinterpret_cast<float4_t*>(&lds[0][0]) + 4 * (4 * C::VT) * 64) + wave * 128;
+        static_assert(4 * 4 * C::VT * 64 * 16 + 4 * 128 * 4 <= sizeof(lds), "results of four waves fit");
         if (group) {
+            mls[lane] = a.m;
+            mls[64 + lane] = a.l;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mls[128 * n + lane] = a.m[n];
-                mls[128 * n + 64 + lane] = a.l[n];
+            for (int y = 0; y < C::VT; ++y)
 #pragma unroll
-                for (int x = 0; x < C::VT; ++x) o[(n * C::VT + x) * 64 + lane] = a.o[n][x];
-            }
+                for (int e = 0; e < 4; ++e) o[(4 * y + e) * 64 + lane] = float4_t{a.o[y][4 * e], a.o[y][4 * e + 1], a.o[y][4 * e + 2], a.o[y][4 * e + 3]};
         }
         __syncthreads();
-        if (group == 0) {
+        if (group) return;
+        const float m1 = mls[lane], mm = fmaxf(a.m, m1);
+        const float h0 = half_fall(a.m, mm), h1 = half_fall(m1, mm), f0 = h0 * h0, f1 = h1 * h1;
+        a.m = mm;
+        a.l = a.l * h0 * h0 + mls[64 + lane] * h1 * h1;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float m1 = mls[128 * n + lane], mm = fmaxf(a.m[n], m1);
-                const float h0 = half_fall(a.m[n], mm), h1 = half_fall(m1, mm), f0 = h0 * h0, f1 = h1 * h1;
-                a.m[n] = mm;
-                a.l[n] = a.l[n] * h0 * h0 + mls[128 * n + 64 + lane] * h1 * h1;
+        for (int y = 0; y < C::VT; ++y)
 #pragma unroll
-                for (int x = 0; x < C::VT; ++x) a.o[n][x] = a.o[n][x] * f0 + o[(n * C::VT + x) * 64 + lane] * f1;
+            for (int e = 0; e < 4; ++e) {
+                const float4_t u = o[(4 * y + e) * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a.o[y][4 * e + i] = a.o[y][4 * e + i] * f0 + u[i] * f1;
             }
-        }
     }
     const KvSink<E, D, 0> sink(p, w);
+    const int col = lane & 31;
+    const float inv = over_sum<0>(a.l);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        if (group) break;
-        const int c = 16 * n + col;
-        const float inv = over_sum<0>(a.l[n]);
+    for (int rr = 0; rr < 8; ++rr)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int x = 0; x < C::VT; x += 4) {
-                const float4_t v = {a.o[n][x][i], a.o[n][x + 1][i], a.o[n][x + 2][i], a.o[n][x + 3][i]};
-                // (chunks of partial results as they lie: 1 KiB a store and wave)
-                if (w.chunks > 1) {
-                    st_partial4<SCOPE_DEVICE>(sink.part + 4 * sink.lane_quad(wave, n, i, x, lane), v);
-                } else if (c < a.n) {
-                    if constexpr (C::VT % 8 == 0) {   // 16 bytes a store
-                        if (x % 8 == 4) sink.out8(a.c + c, (4 * kb + i) * C::VT + x - 4, float4_t{a.o[n][x - 4][i], a.o[n][x - 3][i], a.o[n][x - 2][i], a.o[n][x - 1][i]}, v, inv);
-                    } else {
-                        sink.out(a.c + c, (4 * kb + i) * C::VT + x, v, inv);
-                    }
+        for (int xq = 0; xq < C::XQ; ++xq) {
+            const float4_t v = a.quad(rr, xq);
+            // (chunks of partial results as they lie: 1 KiB a store and wave)
+            if (w.chunks > 1) {
+                st_partial4<SCOPE_DEVICE>(sink.part + 4 * C::lane_quad(wave, rr, xq, lane), v);
+            } else if (col < a.n) {
+                if constexpr (C::XQ % 2 == 0) {   // 16 bytes a store
+                    if (xq % 2) sink.out8(a.c + col, C::row(rr, lane) * (D / 16) + 4 * (xq - 1), a.quad(rr, xq - 1), v, inv);
+                } else {
+                    sink.out(a.c + col, C::row(rr, lane) * (D / 16) + 4 * xq, v, inv);
                 }
             }
-        if (kb == 0 && c < a.n) sink.put_ml(a.c + c, a.m[n], a.l[n]);
-    }
+        }
+    if (lane < 32 && col < a.n) sink.put_ml(a.c + col, a.m, a.l);
 }
 
 template <typename E, int D>
 __global__ __launch_bounds__(256) void kv8_many_join_kernel(KvAttnParams p) {
     __shared__ float ml[128][2];
-    many_join<E, D, 0>(p, &ml[0][0]);
+    many_join<E, D, 0>(p, &ml[0][0], [](int e, int& c, int& d) { ManyCols<E, D>::lane_place(e, c, d); });
 }
 
 template <typename E, int D>

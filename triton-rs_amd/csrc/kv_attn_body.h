@@ -212,10 +212,10 @@ struct KvSink {
             join_quads(e, share, shares, span, e < quads && share < shares, vals, ml);
         }
     }
-    // For kv4_many.hip, 128 columns of partial results as lanes have them: per column (m, 1 / l) over all
-    // chunks, then the values of part `part` of PARTS, two chunks in flight.
-    template <int PARTS>
-    __device__ __forceinline__ void join_lanes(int live, float* ml, int part) const {
+    // For many columns, 128 of them with partial results as lanes have them: per column (m, 1 / l) over all
+    // chunks, then the values of part `part` of PARTS, two chunks in flight. place(e, c, d): column and dimension of quad e.
+    template <int PARTS, typename P>
+    __device__ __forceinline__ void join_lanes(int live, float* ml, int part, P place) const {
         const int chunks = w.chunks;
         const float* heads = item + (size_t)p.slot_cols * D;
         if ((int)threadIdx.x < live) {
@@ -237,7 +237,7 @@ struct KvSink {
 #pragma unroll 1
         for (int e = part * QUADS + threadIdx.x; e < (part + 1) * QUADS; e += 256) {
             int c, d;
-            lane_place(e, c, d);
+            place(e, c, d);
             const int at = min(c, live - 1);
             const float mm = ml[2 * at];
             float4_t v = {0.f, 0.f, 0.f, 0.f};

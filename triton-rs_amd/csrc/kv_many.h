@@ -54,13 +54,13 @@ __device__ __forceinline__ bool many_item(const KvAttnParams& p, int place, KvIt
 // Joins the chunks of one tile: an eighth of its values a workgroup. (The last of the chunks' own workgroups took longer:
 // 64 queries over 4096 keys, 32 heads of D = 128, 8 chunks, 40.1 us, so 30; two chunks of 400 over 2000 40.2, 39.3.)
 constexpr int MANY_PARTS = 8;
-template <typename E, int D, int DOWN>
-__device__ __forceinline__ void many_join(const KvAttnParams& p, float* ml) {   // ml: two floats a column
+template <typename E, int D, int DOWN, typename P>
+__device__ __forceinline__ void many_join(const KvAttnParams& p, float* ml, P place) {   // ml: two floats a column
     KvItem w;
     const int part = blockIdx.z % MANY_PARTS;
     if (!many_item(p, blockIdx.z / MANY_PARTS * p.splits, w) || w.chunks == 1) return;   // (its results are in place)
     const KvSink<E, D, DOWN> sink(p, w);
-    sink.template join_lanes<MANY_PARTS>(min(128, w.cols), ml, part);
+    sink.template join_lanes<MANY_PARTS>(min(128, w.cols), ml, part, place);
 }
 
 }  // namespace w4a16

@@ -311,6 +311,41 @@ def test_rotation_of_queries_without_new_lengths():
     assert torch.equal(a, b) and torch.equal(out, P.rope(q, lens - 1, r, q_out=torch.empty_like(q)))
 
 
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("n", [None, [1000, 0, 3, 217], [17] * 70, [1, 0] * 600 + [200] * 3])
+def test_rotation_of_many_queries(n, explicit):
+    """Enough of them for a launch of their own: a row's bits do not depend on how many there are, nor do the keys' and values'; rows of
+    no sequence stay as they are. Without cu_q, too."""
+    P = need_gpu()
+    Hq, Hkv, D = 32, 1, 128
+    gen = torch.Generator().manual_seed(11)
+    B, before = (1100, 0) if n is None else (len(n), 5)
+    T = B if n is None else sum(n) + 12
+    assert T * Hq * D >= 4 << 20
+    n = n or [1] * B
+    lens = [x + int(torch.randint(0, 40, (1,), generator=gen)) for x in n]
+    per = -(-max(lens) // 16)
+    table = torch.randperm(B * per, generator=gen).view(B, per).int()
+    k = torch.randn((T, Hkv, D), generator=gen).bfloat16().cuda()
+    q = torch.randn((T, Hq, D), generator=gen).bfloat16().cuda()
+    cu = np.cumsum([before] + n)
+    places = torch.full((T,), -1, dtype=torch.int32)
+    for b in range(B):
+        places[cu[b]:cu[b + 1]] = torch.arange(lens[b] - n[b], lens[b])
+    r = P.Rope(D, interleaved=explicit)
+    kw = dict(rope=r, positions=places.cuda() if explicit else None)
+    if T != B:
+        kw.update(cu_q=i32(cu), max_q_len=max(n))
+    one, two = P.kv8_cache(B * per, Hkv, D, 16), P.kv8_cache(B * per, Hkv, D, 16)
+    P.kv8_write(k, k, one, table.cuda(), i32(lens), **kw)
+    out = torch.full_like(q, 5.0)
+    P.kv8_write(k, k, two, table.cuda(), i32(lens), q=q, q_out=out, **kw)
+    assert torch.equal(one, two)
+    mine = (places >= 0).cuda()
+    want = torch.cat([P.rope(q[i:i + 50], places[i:i + 50].cuda(), r, q_out=torch.empty_like(q[i:i + 50])) for i in range(0, T, 50)])
+    assert torch.equal(out[mine], want[mine]) and (explicit or (out[~mine] == 5).all())
+
+
 # ------------------------------------------------------------------ attention
 
 class Batch8(Batch):

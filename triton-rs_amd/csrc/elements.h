@@ -22,7 +22,7 @@ __device__ __forceinline__ Elems8 load8(const uint16_t* p, int n) {
     Elems8 r = {{0, 0, 0, 0}};
     if (n >= 8) {
         r = *reinterpret_cast<const Elems8*>(p);
-    } else {
+    } else if (n > 0) {
 #pragma unroll
         for (int e = 0; e < 7; ++e)
             if (e < n) r.w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
@@ -32,7 +32,7 @@ __device__ __forceinline__ Elems8 load8(const uint16_t* p, int n) {
 __device__ __forceinline__ void store8(uint16_t* p, const Elems8& v, int n) {
     if (n >= 8) {
         *reinterpret_cast<Elems8*>(p) = v;
-    } else {
+    } else if (n > 0) {
 #pragma unroll
         for (int e = 0; e < 7; ++e)
             if (e < n) p[e] = (uint16_t)(v.w[e >> 1] >> (16 * (e & 1)));

@@ -7,7 +7,10 @@
 //
 // Bound by memory: 4 D bytes of a token's rows in, 2 D out. A workgroup takes a block (16 tokens) of some heads, so no two
 // write one scale. Rows pass through LDS; then a thread has 16 bytes of the block, of keys 16 dimensions of
-// a token, of values four tokens of four dimensions. Queries are rotated by workgroups of their own in the same launch.
+// a token, of values four tokens of four dimensions. Few queries are rotated by workgroups of their own in the same launch.
+//
+// Measured, 8 heads of D = 128: 8192 tokens 16.9 us (50 MB, 3.0 TB/s), keys rotated on the way 24.7 (36 with fp64 sincospi for the
+// angles, all 16 rows of which began in one bank, and partners read one by one); 48 tokens of 48 sequences 4.6 and 5.6.
 #include "kv8.h"
 #include "kv_attn_body.h"
 #include "rotate.h"
@@ -60,35 +63,25 @@ __device__ __forceinline__ bool find_block(const Kv8WriteParams& p, int per_seq,
     return false;
 }
 
-enum Turn { NONE, HALVES, PAIRS };
+// how a key is rotated: pairs of dimensions i and i + rot / 2 (EIGHTS: rot / 2 is a multiple of eight, partners are read eight
+// by eight), or 2 i and 2 i + 1
+enum Turn { NONE, HALVES, EIGHTS, PAIRED };
 
 // Queries of one token, all heads, as rope.hip.
-template <typename E, Turn TURN, int THREADS>
+template <typename E, bool PAIRS, int THREADS>
 __device__ __forceinline__ void turn_queries(const Kv8WriteParams& p, int D, int t, float2* turn) {
     int position;
-    if (p.positions) {
-        position = p.positions[t];
-    } else {   // its place in the sequence that it is of
-        int b = t;
-        if (p.cu_q) {
-            b = -1;
-            for (int base = 0; base < p.B && b < 0; base += 64) {
-                const int s = base + (threadIdx.x & 63), in = min(s, p.B - 1);
-                const uint64_t who = __ballot(s < p.B && p.cu_q[in] <= t && t < p.cu_q[in + 1]);
-                if (who) b = base + __builtin_ctzll(who);
-            }
-            if (b < 0) return;   // of none: left as it is
-        }
-        position = p.cu_q ? p.kv_lens[b] - min(max(p.cu_q[b + 1], 0), p.T) + t : p.kv_lens[b] - 1;
-    }
+    if (p.positions) position = p.positions[t];
+    else if (!place_of(p.cu_q, p.kv_lens, p.B, p.T, t, position)) return;   // of no sequence: left as it is
     const int half = p.rot / 2;
     for (int i = threadIdx.x; i < half; i += THREADS) turn[i] = angle(position, p.inv_freq[i], p.magnitude);
     __syncthreads();
-    const int turned = turned_units(p.rot, TURN == PAIRS), units = row_units(p.rot, D, TURN == PAIRS);
+    const int units = row_units(p.rot, D, PAIRS);
     for (int e = threadIdx.x; e < units * p.q.H; e += THREADS) {
         const int h = e / units, u = e - h * units;
-        turn_unit<E, TURN == PAIRS>(static_cast<const uint16_t*>(p.q.x) + (size_t)t * p.q.st + (size_t)h * p.q.sh,
-                                    static_cast<uint16_t*>(p.q.out) + (size_t)t * p.q.o_st + (size_t)h * p.q.o_sh, turn, u, turned, p.rot, D);
+        const uint16_t* x = static_cast<const uint16_t*>(p.q.x) + (size_t)t * p.q.st + (size_t)h * p.q.sh;
+        uint16_t* o = static_cast<uint16_t*>(p.q.out) + (size_t)t * p.q.o_st + (size_t)h * p.q.o_sh;
+        store_turned<E, PAIRS>(load_unit<PAIRS>(x, x == o, u, p.rot, D), x == o, o, turn, u, p.rot, D);
     }
 }
 
@@ -97,9 +90,9 @@ __global__ __launch_bounds__(2 * D) void kv8_write_kernel(Kv8WriteParams p, int 
     constexpr int ROW = D + 8, THREADS = 2 * D;
     __shared__ __align__(16) uint16_t rows[2][16][ROW];
     __shared__ uint32_t top[2][16];                     // largest magnitude of a row, as bits
-    __shared__ float2 turn[TURN == NONE ? 1 : 16][TURN == NONE ? 1 : D / 2];
+    __shared__ __align__(16) float2 turn[TURN == NONE ? 1 : 16][TURN == NONE ? 1 : D / 2 + 2];   // 16 rows, each four banks on
     if ((int)blockIdx.x >= items * groups) {
-        if constexpr (TURN != NONE) turn_queries<E, TURN, THREADS>(p, D, blockIdx.x - items * groups, &turn[0][0]);
+        if constexpr (TURN != NONE) turn_queries<E, TURN == PAIRED, THREADS>(p, D, blockIdx.x - items * groups, &turn[0][0]);
         return;
     }
     const int item = blockIdx.x / groups, h0 = (blockIdx.x - item * groups) * heads;
@@ -145,8 +138,25 @@ __global__ __launch_bounds__(2 * D) void kv8_write_kernel(Kv8WriteParams p, int 
             if (t >= from && t < to) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) f[e] = elem_to_f32<E>(src[c + e]);
-                if constexpr (TURN == HALVES) {
-                    const int half = p.rot / 2;
+                const int half = p.rot / 2;
+                if constexpr (TURN == EIGHTS) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const int d = c + 8 * g;
+                        if (d < p.rot) {
+                            const bool low = d < half;
+                            const int i = low ? d : d - half;
+                            float other[8];
+                            to_f32<E>(*reinterpret_cast<const Elems8*>(src + (low ? d + half : i)), other);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                float u = low ? f[8 * g + e] : other[e], w = low ? other[e] : f[8 * g + e];
+                                turn_pair(u, w, turn[t][i + e]);
+                                f[8 * g + e] = low ? u : w;
+                            }
+                        }
+                    }
+                } else if constexpr (TURN == HALVES) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int d = c + e;
@@ -158,7 +168,7 @@ __global__ __launch_bounds__(2 * D) void kv8_write_kernel(Kv8WriteParams p, int 
                             f[e] = low ? u : v;
                         }
                     }
-                } else if constexpr (TURN == PAIRS) {
+                } else if constexpr (TURN == PAIRED) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 2)
                         if (c + e < p.rot) turn_pair(f[e], f[e + 1], turn[t][(c + e) >> 1]);
@@ -297,13 +307,25 @@ static void write(const Kv8WriteParams& p, hipStream_t st) {
     const unsigned grid = (unsigned)items * groups + (p.q.H ? p.T : 0);
     const int per_seq = direct ? (int)per : 0;
     if (!p.inv_freq) kv8_write_kernel<E, D, NONE><<<grid, 2 * D, 0, st>>>(p, per_seq, items, groups, heads);
-    else if (p.interleaved) kv8_write_kernel<E, D, PAIRS><<<grid, 2 * D, 0, st>>>(p, per_seq, items, groups, heads);
+    else if (p.interleaved) kv8_write_kernel<E, D, PAIRED><<<grid, 2 * D, 0, st>>>(p, per_seq, items, groups, heads);
+    else if (p.rot % 16 == 0) kv8_write_kernel<E, D, EIGHTS><<<grid, 2 * D, 0, st>>>(p, per_seq, items, groups, heads);
     else kv8_write_kernel<E, D, HALVES><<<grid, 2 * D, 0, st>>>(p, per_seq, items, groups, heads);
 }
 template <typename E, int D>
 static void read(const Kv8ReadParams& p, hipStream_t st) { kv8_read_kernel<E, D><<<dim3((p.T + 15) / 16, p.Hkv), 256, 0, st>>>(p); }
 
-hipError_t launch_kv8_write(bool bf16, int D, const Kv8WriteParams& p, hipStream_t st) {
+hipError_t launch_kv8_write(bool bf16, int D, const Kv8WriteParams& all, hipStream_t st) {
+    Kv8WriteParams p = all;
+    // Many queries are rotated by a launch of their own: beside the registers of the keys' rows too few of them are in flight. 8192
+    // tokens, 32 heads of D = 128: 42 us in the same launch, 31 apart; 512 tokens 0.5 and 4.3.
+    if (p.q.H && (int64_t)p.T * p.q.H * D >= 4 << 20) {
+        RopeParams r{};
+        r.rows[0] = p.q;
+        r.positions = p.positions; r.kv_lens = p.kv_lens; r.cu_q = p.cu_q; r.B = p.B;
+        r.inv_freq = p.inv_freq; r.magnitude = p.magnitude; r.T = p.T; r.D = D; r.rot = p.rot; r.interleaved = p.interleaved;
+        if (hipError_t e = launch_rope(bf16, r, st)) return e;
+        p.q = {};
+    }
     switch (D) {
         case 64: bf16 ? write<bf16_t, 64>(p, st) : write<half_t, 64>(p, st); break;
         case 128: bf16 ? write<bf16_t, 128>(p, st) : write<half_t, 128>(p, st); break;

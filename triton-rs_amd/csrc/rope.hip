@@ -1,46 +1,78 @@
 // Rotary positions: pair (a, b) of a row, dimensions (i, i + rot / 2) or (2 i, 2 i + 1), at position n becomes
 // m (a cos w - b sin w, a sin w + b cos w), w = n f_i, in fp32, rounded once.
 //
-// An angle is taken modulo a whole turn in fp64 (a position of 10^6 in fp32 would be off by 0.06 rad) and its
-// sine and cosine, fp64 rounded to fp32, are computed once a token for all heads, in LDS. The two products of a
+// An angle is taken modulo a whole turn in fp64 (a position of 10^6 in fp32 would be off by 0.06 rad); its
+// sine and cosine (rotate.h) are computed once a token for all heads, in LDS. The two products of a
 // result are rounded before their difference or sum, so that every kernel that rotates gives the same bits.
-// Bound by memory: a row in, a row out.
+// Bound by memory: a row in, a row out. 8192 tokens, 40 heads of D = 128, 168 MB: 37 us (4.5 TB/s), rot = 64, 90 or 96 of it
+// 40, 41 and 37; 16 tokens 3.7.
 #include "elements.h"
 #include "layer.h"
 #include "rotate.h"
 
 namespace w4a16 {
 
-template <typename E, bool PAIRS>
+constexpr int ROPE_TOKENS = 2;   // of a workgroup, at most
+struct RowPlace { const uint16_t* x; uint16_t* o; };
+
+template <typename E, bool PAIRS, bool GIVEN>   // GIVEN: positions are
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
     extern __shared__ float2 turn[];   // [tokens][rot / 2]
+    [[maybe_unused]] __shared__ int none[ROPE_TOKENS];   // tokens of no sequence
     const int half = p.rot / 2, t0 = blockIdx.x * tokens, live = min(tokens, p.T - t0);
-    for (int i = threadIdx.x; i < live * half; i += 256) {
-        const int t = i / half;
-        turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
-    }
-    __syncthreads();
-    const int turned = turned_units(p.rot, PAIRS), units = row_units(p.rot, p.D, PAIRS);
+    const int units = row_units(p.rot, p.D, PAIRS);
     static_assert(ROPE_MAX_D / 8 + 1 <= 256, "a row's units are threads of one workgroup");
-    const int rows = 256 / units, heads = p.rows[0].H + p.rows[1].H;
+    const int rows = 256 / units, heads = p.rows[0].H + p.rows[1].H, all = live * heads;
     const int mine = threadIdx.x / units, u = threadIdx.x - mine * units;
-    if (mine >= rows) return;
-    for (int r = mine; r < live * heads; r += rows) {
-        const int t = r / heads, hh = r - t * heads;
-        const RopeRows& w = p.rows[hh >= p.rows[0].H];
-        const int h = hh >= p.rows[0].H ? hh - p.rows[0].H : hh;
-        turn_unit<E, PAIRS>(static_cast<const uint16_t*>(w.x) + (size_t)(t0 + t) * w.st + (size_t)h * w.sh,
-                            static_cast<uint16_t*>(w.out) + (size_t)(t0 + t) * w.o_st + (size_t)h * w.o_sh, turn + t * half, u, turned, p.rot, p.D);
+    auto row = [&](int r, int& t) {   // row r of the workgroup
+        t = r / heads;
+        const int hh = r - t * heads;
+        const bool second = hh >= p.rows[0].H;
+        const RopeRows& w = p.rows[second];
+        const int h = second ? hh - p.rows[0].H : hh;
+        return RowPlace{static_cast<const uint16_t*>(w.x) + (size_t)(t0 + t) * w.st + (size_t)h * w.sh,
+                        static_cast<uint16_t*>(w.out) + (size_t)(t0 + t) * w.o_st + (size_t)h * w.o_sh};
+    };
+    for (int r0 = 0; r0 < all; r0 += rows) {
+        const int r = r0 + mine;
+        const bool some = mine < rows && r < all;
+        Unit v{};
+        int t = 0;
+        RowPlace at{};
+        if (some) {
+            at = row(r, t);
+            v = load_unit<PAIRS>(at.x, at.x == at.o, u, p.rot, p.D);
+        }
+        if (r0 == 0) {   // while the first rows are on their way
+            if constexpr (GIVEN) {
+                for (int i = threadIdx.x; i < live * half; i += 256) {
+                    const int t = i / half;
+                    turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
+                }
+            } else {   // a wave a token
+                for (int t = threadIdx.x >> 6; t < live; t += 4) {
+                    int position = 0;
+                    const bool found = place_of(p.cu_q, p.kv_lens, p.B, p.T, t0 + t, position);
+                    if ((threadIdx.x & 63) == 0) none[t] = !found;
+                    for (int i = threadIdx.x & 63; i < half; i += 64) turn[t * half + i] = angle(position, p.inv_freq[i], p.magnitude);
+                }
+            }
+            __syncthreads();
+        }
+        if (some && (GIVEN || !none[t])) store_turned<E, PAIRS>(v, at.x == at.o, at.o, turn + t * half, u, p.rot, p.D);
     }
 }
 
 template <typename E>
 static void go(const RopeParams& p, hipStream_t st) {
-    const int tokens = p.T >= 4096 ? 4 : 1;
+    // Two tokens a workgroup where all of them are more than are resident at once; with one its angles and barrier count (8192
+    // tokens, 40 heads of D = 64 20 us and 18), with four a CU's workgroups all wait at once (40 heads of 128, pairs: 38 and 43 us).
+    const int tokens = p.T >= 2048 ? ROPE_TOKENS : 1;
     const dim3 grid((unsigned)((p.T + tokens - 1) / tokens));
     const size_t lds = sizeof(float2) * tokens * (p.rot / 2);
-    if (p.interleaved) rope_kernel<E, true><<<grid, 256, lds, st>>>(p, tokens);
-    else rope_kernel<E, false><<<grid, 256, lds, st>>>(p, tokens);
+    auto* const kernel = p.positions ? p.interleaved ? rope_kernel<E, true, true> : rope_kernel<E, false, true>
+                                     : p.interleaved ? rope_kernel<E, true, false> : rope_kernel<E, false, false>;
+    kernel<<<grid, 256, lds, st>>>(p, tokens);
 }
 
 hipError_t launch_rope(bool bf16, const RopeParams& p, hipStream_t st) {

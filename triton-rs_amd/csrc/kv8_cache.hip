@@ -25,6 +25,14 @@ __device__ __forceinline__ uint32_t rescale(uint32_t w, float ratio) {
     return to_e4m3(byte_f32(w, 0) * ratio, byte_f32(w, 1) * ratio, byte_f32(w, 2) * ratio, byte_f32(w, 3) * ratio);
 }
 
+// The largest of 16 lanes' numbers (lanes 16 i ..), all of which are active.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false));   // rotated by 8, 4, 2, 1 lanes
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xF, 0xF, false));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xF, 0xF, false));
+}
+
 // The new tokens of sequence b: rows q0.. of the call at positions [lo, hi) of the sequence; row of position lo.
 struct Append { int lo, hi, row; };
 __device__ __forceinline__ Append append(const Kv8WriteParams& p, int b) {
@@ -189,18 +197,15 @@ __global__ __launch_bounds__(2 * D) void kv8_write_kernel(Kv8WriteParams p, int 
                         f[4 * i + e] = elem_to_f32<E>(w[e >> 1] >> (16 * (e & 1)));
                         most = max(most, __float_as_uint(f[4 * i + e]) & 0x7FFFFFFFu);
                     }
-                    atomicMax(&top[1][t], most);
+                    most = row_max(most);
+                    if (r == 0) atomicMax(&top[1][t], most);
                 }
             }
         }
         __syncthreads();
-        uint32_t most = 0, odd = 0;   // largest finite row, rows that are not
-#pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const uint32_t v = top[values][t];
-            if (v >= 0x7F800000u) odd |= 1u << t;
-            else most = max(most, v);
-        }
+        // largest finite row, and rows that are not (16 lanes have a row each, the wave's others the same)
+        const uint32_t theirs = top[values][x & 15], odd = (uint32_t)__ballot(theirs >= 0x7F800000u) & 0xFFFFu;
+        const uint32_t most = row_max(theirs >= 0x7F800000u ? 0u : theirs);
         // most <= 448 2^e: 448 is 1.75 2^8
         int e2 = max((int)(most >> 23) - 127 - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0), KV8_LEAST_EXP);
         const float need = pow2(e2), old = __uint_as_float(values ? tail[1] : tail[0]);

@@ -16,7 +16,7 @@ static_assert(KV_COUNTER_BYTES == W4A16_KV4_COUNTER_BYTES, "counters fill their 
 // 8 of 128 KB 28.3, 26.5; 5 of 84 KB 32.6, 33.1. 8 heads: 16 chunks 22.6, 19.1; 10 chunks 21.4, 23.3; 4 35.2, 38.4.
 constexpr int KV4_JOIN_CHUNKS = 12;
 constexpr int64_t KV4_JOIN_BYTES = 96 << 10;
-static const KvFormat KV4 = {"kv4 attention launch", kv4_few_per_cu, kv4_many_simd_waves, KV4_WHOLE_KEYS, 1.f, 6.f, 7.f,
+static const KvFormat KV4 = {"kv4 attention launch", kv4_few_per_cu, kv4_many_simd_waves, KV4_WHOLE_KEYS, [](int) { return 0.45f; }, 6.f, 7.f,
                              KV4_JOIN_CHUNKS, KV4_JOIN_BYTES, launch_kv4_few, launch_kv4_many};
 
 static int kv4_rows(bool write, void* stream, int elem, void* k, void* v, int32_t k_st, int32_t k_sh, int32_t v_st,

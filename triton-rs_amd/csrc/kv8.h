@@ -45,8 +45,12 @@ struct Kv8ReadParams {
 };
 hipError_t launch_kv8_read(bool bf16, int D, const Kv8ReadParams& p, hipStream_t st);
 
-// Workgroups of kv8_few.hip that are planned for a compute unit, by registers.
-constexpr int kv8_few_per_cu(int D, int nt) { return nt == 2 ? (D == 64 ? 3 : 2) : D <= 128 ? 4 : 2; }
+// Workgroups of kv8_few.hip that a compute unit has registers for, and those that the keys are split for: the four waves of one
+// have enough of the cache on its way (D = 64: of two), and each further chunk costs its partial results' way. In us, for one, two,
+// four a compute unit: 1 sequence, 8 heads of D = 128, 16000 keys 15.3, 16.7, 19.9; 16 of 16000 94.9, 99.3, 103.8; 8 of 3 queries, 2000
+// keys 16.4, 17.5, 19.5; 4 of 16 heads of D = 64, 16000 keys 35.9, 30.8, 33.6.
+constexpr int kv8_few_occupancy(int D, int nt) { return nt == 2 ? (D == 64 ? 3 : 2) : D <= 128 ? 4 : 2; }
+constexpr int kv8_few_per_cu(int D) { return D == 64 ? 2 : 1; }
 hipError_t launch_kv8_few(bool bf16, int D, const KvAttnParams& p, const KvAttnShape& s, hipStream_t st);
 // Waves of kv8_many.hip a SIMD, by registers.
 constexpr int kv8_many_simd_waves(int D, int groups) { return D <= 128 ? 2 : 1; }

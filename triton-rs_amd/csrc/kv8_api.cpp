@@ -15,7 +15,19 @@ static_assert(KV_COUNTER_BYTES == W4A16_KV8_COUNTER_BYTES, "counters fill their 
 
 constexpr int32_t KV8_MAX_TOKENS = 1 << 22;   // of a call that writes: their workgroups' threads are counted in 32 bits
 
-static const KvFormat KV8 = {"kv8 attention launch", kv8_few_per_cu, kv8_many_simd_waves, 512, 1.f, 3.f, 3.5f, 12, 96 << 10,
+// Keys in one chunk: 500 keys of one sequence, 8 heads of D = 128, 7.9 us whole, 9.3 in chunks, 1000 keys 10.5, 9.5; 4 drafts of 5
+// tokens, 8 heads a group, 500 keys 13.1, 15.4.
+constexpr int KV8_WHOLE_KEYS = 512;
+// Up to this much a sequence's and head's last workgroup joins itself (us; itself, a kernel of its own): 1 sequence, 8 heads of
+// D = 128, 31 chunks 13.2, 11.1; 5 queries of 8 heads a group, D = 256, 16 chunks of 40 KB 38.5, 25.1; 8 sequences of 3 queries, 4
+// chunks of 6 KB 16.4, 17.2; 32 of 6, 24 KB in one 28.0, 34.0; 4 sequences, 8 chunks 36.3, 38.1.
+constexpr int KV8_JOIN_CHUNKS = 12;
+constexpr int64_t KV8_JOIN_BYTES = 96 << 10;
+// One sequence alone, 8 heads of D = 128, takes 0.17 us for a step of 32 keys, 256 workgroups together 0.41: 16 sequences of 16000
+// keys 123 us where a step alone is taken for 0.45 of the device's (whole), 95 from 0.55 to 0.7 (in two); 16 of 1000 keys 12.7
+// up to 0.6 (whole), 14.1 at 0.7.
+static const KvFormat KV8 = {"kv8 attention launch", [](int D, int) { return kv8_few_per_cu(D); }, kv8_many_simd_waves, KV8_WHOLE_KEYS,
+                             [](int per_cu) { return 0.6f / (float)per_cu; }, 3.f, 8.f, KV8_JOIN_CHUNKS, KV8_JOIN_BYTES,
                              launch_kv8_few, launch_kv8_many};
 
 }  // namespace w4a16

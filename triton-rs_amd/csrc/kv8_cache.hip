@@ -9,8 +9,9 @@
 // write one scale. Rows pass through LDS; then a thread has 16 bytes of the block, of keys 16 dimensions of
 // a token, of values four tokens of four dimensions. Few queries are rotated by workgroups of their own in the same launch.
 //
-// Measured, 8 heads of D = 128: 8192 tokens 16.9 us (50 MB, 3.0 TB/s), keys rotated on the way 24.7 (36 with fp64 sincospi for the
-// angles, all 16 rows of which began in one bank, and partners read one by one); 48 tokens of 48 sequences 4.6 and 5.6.
+// Measured, 8 heads of D = 128: 8192 tokens 15.0 us (50 MB, 3.3 TB/s), keys rotated on the way 21.0; 48 tokens of 48 sequences 4.4
+// and 5.3; 8192 tokens read 11.6 (4.3 TB/s). What is left is registers: 77 and 91 of a thread leave six and five waves a SIMD (in 64
+// it spills: 28 us), the next head's rows on their way beside this one's cost a wave and 1 us.
 #include "kv8.h"
 #include "kv_attn_body.h"
 #include "rotate.h"

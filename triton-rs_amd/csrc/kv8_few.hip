@@ -11,7 +11,7 @@
 namespace w4a16 {
 
 template <typename E, int D, int NT>
-__global__ __launch_bounds__(256, kv8_few_per_cu(D, NT)) void kv8_few_kernel(KvAttnParams p) {
+__global__ __launch_bounds__(256, kv8_few_occupancy(D, NT)) void kv8_few_kernel(KvAttnParams p) {
     typedef Kv8Cols<E, D, NT> C;
     constexpr int COLS = 16 * NT, ROW = D + 4;   // LDS row of a column's result
     __shared__ __align__(16) float red[4][16 * ROW];

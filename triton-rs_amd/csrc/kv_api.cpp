@@ -101,7 +101,7 @@ static KvAttnShape kv_attention_shape(const KvFormat& f, int T, int B, int Hq, i
         const int64_t rounds = (2 * (int64_t)B + at_once - 1) / at_once;
         s.whole = items > (int64_t)KV_MAX_COUNTERS || max_kv <= f.whole_keys;
         // up to 128 of a sequence, as many as one join takes in its time (131072 keys of one head: 1024 chunks 47.6 us)
-        s.budget = (int)std::max<int64_t>(2 * (int64_t)B, std::min<int64_t>((int64_t)(rounds * at_once * f.fill), 128 * (int64_t)B));
+        s.budget = (int)std::max<int64_t>(2 * (int64_t)B, std::min<int64_t>(rounds * at_once, 128 * (int64_t)B));
         s.at_once = (int)at_once;
         s.places = (int)(s.whole ? B : std::min<int64_t>(s.budget, (int64_t)B * (((int64_t)max_kv + 31) / 128 + 1)));
         s.slot_cols = (int)std::min<int64_t>(wg_cols, (C + 15) / 16 * 16);
@@ -124,7 +124,7 @@ static size_t kv_partial_bytes(const KvFormat& f, const KvAttnShape& s, int T, i
 static void kv_params(const KvFormat& f, KvAttnParams& p, const KvAttnShape& s, int D, int max_q, int T) {
     p.max_q = max_q < T ? max_q : T;
     p.slot_cols = s.slot_cols;
-    p.whole_keys = f.whole_keys; p.round_cost = f.round_cost; p.join_cost = f.join_cost;
+    p.whole_keys = f.whole_keys; p.step_alone = f.step_alone(f.few_per_cu(D, s.nt)); p.round_cost = f.round_cost; p.join_cost = f.join_cost;
     p.rows = s.rows; p.tiles = s.tiles; p.splits = s.splits; p.chunk = s.chunk; p.pair_tiles = s.pair_tiles;
     p.places = s.places; p.budget = s.budget; p.at_once = s.at_once; p.whole = s.whole; p.join_apart = s.join_apart;
     p.join_parts = (int)((std::min<int64_t>((int64_t)p.max_q * p.G, 32 * s.nt) * (D / 4) + 63) / 64);

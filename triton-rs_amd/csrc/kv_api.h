@@ -16,8 +16,8 @@ struct KvFormat {
     int (*few_per_cu)(int D, int nt);           // workgroups of the kernel for few columns that a compute unit holds
     int (*many_simd_waves)(int D, int groups);  // waves of the kernel for many columns that a SIMD holds
     int whole_keys;                             // keys that the kernel for few columns leaves in one chunk
-    float fill;                                 // chunks of the keys that the kernel for few columns wants, in rounds of a full device
-    float round_cost, join_cost;                // kv_few.h
+    float (*step_alone)(int per_cu);            // in steps of a full device (kv_few.h), as
+    float round_cost, join_cost;                // these
     int join_chunks;                            // up to this much a sequence's and head's last workgroup joins itself
     int64_t join_bytes;
     hipError_t (*launch_few)(bool bf16, int D, const KvAttnParams& p, const KvAttnShape& s, hipStream_t st);

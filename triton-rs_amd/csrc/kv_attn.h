@@ -35,7 +35,7 @@ struct KvAttnParams {
     int tiles, splits, chunk, pair_tiles, rows;  // many columns
     int places, budget, at_once, whole, join_apart, join_parts;   // few columns
     int whole_keys;                   // few columns: a sequence of up to so many keys is one chunk
-    float round_cost, join_cost;      // few columns: in steps of a full device (kv_few.h)
+    float step_alone, round_cost, join_cost;   // few columns: in steps of a full device (kv_few.h)
 };
 constexpr size_t KV_MAX_COUNTERS = 16384;
 struct KvAttnShape {

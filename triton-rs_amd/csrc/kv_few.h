@@ -34,12 +34,12 @@ __device__ __forceinline__ int few_length(const KvAttnParams& p, unsigned sum, i
             break;
         }
     }
-    // In steps of a full device (4 bits: 0.85 us at D = 128, the only one these were measured at): a round of workgroups costs
-    // p.round_cost (6) besides its steps, a step of one workgroup alone 0.45, joining p.join_cost (7). Whole and in two, 8 heads of D = 128: 128 sequences of 1000 keys 34, 49 us, 256
-    // of 900 58, 103; 48 of 4096 56, 54.
+    // In steps of a full device: a round of workgroups costs p.round_cost besides its steps, a step of one workgroup alone
+    // p.step_alone, joining p.join_cost. (In 4 bits 6, 0.45 and 7 of 0.85 us, measured at D = 128. Whole and in two, 8 heads: 128
+    // sequences of 1000 keys 34, 49 us, 256 of 900 58, 103; 48 of 4096 56, 54. In 8 bits 3, 0.6 and 8 of 0.41 us.)
     auto cost = [&](unsigned chunks, int steps) {
         const float rounds = (float)((chunks + p.at_once - 1) / p.at_once);
-        return p.round_cost * rounds + fmaxf(0.45f * rounds * (float)steps, (float)sum / (float)p.at_once);
+        return p.round_cost * rounds + fmaxf(p.step_alone * rounds * (float)steps, (float)sum / (float)p.at_once);
     };
     if (__builtin_amdgcn_readfirstlane(cost(p.B, most) <= cost(n, min(4 * c, most)) + p.join_cost)) c = max(c, (most + 3) / 4);
     return c;

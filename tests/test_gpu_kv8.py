@@ -314,8 +314,8 @@ def test_rotation_of_queries_without_new_lengths():
 @pytest.mark.parametrize("explicit", [False, True])
 @pytest.mark.parametrize("n", [None, [1000, 0, 3, 217], [17] * 70, [1, 0] * 600 + [200] * 3])
 def test_rotation_of_many_queries(n, explicit):
-    """Enough of them for a launch of their own: a row's bits do not depend on how many there are, nor do the keys' and values'; rows of
-    no sequence stay as they are. Without cu_q, too."""
+    """A row's bits do not depend on how many there are, nor do the keys' and values'; rows of no sequence stay as they are.
+    Without cu_q, too."""
     P = need_gpu()
     Hq, Hkv, D = 32, 1, 128
     gen = torch.Generator().manual_seed(11)

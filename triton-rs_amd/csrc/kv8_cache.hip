@@ -7,9 +7,11 @@
 //
 // Bound by memory: 4 D bytes of a token's rows in, 2 D out. A workgroup takes a block (16 tokens) of some heads, so no two
 // write one scale. Rows pass through LDS; then a thread has 16 bytes of the block, of keys 16 dimensions of
-// a token, of values four tokens of four dimensions. Few queries are rotated by workgroups of their own in the same launch.
+// a token, of values four tokens of four dimensions. Queries are rotated by workgroups of their own in the same launch (as
+// one of rope.hip's they took 4 to 10 us more, start and end).
 //
-// Measured, 8 heads of D = 128: 8192 tokens 15.0 us (50 MB, 3.3 TB/s), keys rotated on the way 21.0; 48 tokens of 48 sequences 4.4
+// Measured, 8 heads of D = 128: 8192 tokens 15.0 us (50 MB, 3.3 TB/s), keys rotated on the way 21.0, and 32
+// heads of queries 49 (184 MB, 3.8 TB/s); 48 tokens of 48 sequences 4.4
 // and 5.3; 8192 tokens read 11.6 (4.3 TB/s). What is left is registers: 77 and 91 of a thread leave six and five waves a SIMD (in 64
 // it spills: 28 us), the next head's rows on their way beside this one's cost a wave and 1 us.
 #include "kv8.h"
@@ -76,21 +78,45 @@ __device__ __forceinline__ bool find_block(const Kv8WriteParams& p, int per_seq,
 // by eight), or 2 i and 2 i + 1
 enum Turn { NONE, HALVES, EIGHTS, PAIRED };
 
+// The position of the row of token t in its sequence, rows cu_q[b] .. cu_q[b + 1] - 1 (without cu_q: row b) of which end at
+// token kv_lens[b] - 1. false: it is of none. By a whole wave: each step tells 64 parts of the sequences apart.
+__device__ __forceinline__ bool place_of(const Kv8WriteParams& p, int t, int& position) {
+    if (!p.cu_q) {
+        position = p.kv_lens[t] - 1;
+        return true;
+    }
+    int at = 0, n = p.B + 1;   // the last of cu_q[at .. at + n - 1] that is t or less
+    while (true) {
+        const int step = (n + 63) / 64, i = (threadIdx.x & 63) * step;
+        const int k = __popcll(__ballot(i < n && p.cu_q[at + min(i, n - 1)] <= t));
+        if (k == 0) return false;
+        at += (k - 1) * step;
+        n = min(step, n - (k - 1) * step);
+        if (step == 1) break;
+    }
+    if (at >= p.B) return false;
+    position = p.kv_lens[at] - min(max(p.cu_q[at + 1], 0), p.T) + t;
+    return true;
+}
+
 // Queries of one token, all heads, as rope.hip.
 template <typename E, bool PAIRS, int THREADS>
 __device__ __forceinline__ void turn_queries(const Kv8WriteParams& p, int D, int t, float2* turn) {
-    int position;
-    if (p.positions) position = p.positions[t];
-    else if (!place_of(p.cu_q, p.kv_lens, p.B, p.T, t, position)) return;   // of no sequence: left as it is
-    const int half = p.rot / 2;
-    for (int i = threadIdx.x; i < half; i += THREADS) turn[i] = angle(position, p.inv_freq[i], p.magnitude);
-    __syncthreads();
-    const int units = row_units(p.rot, D, PAIRS);
-    for (int e = threadIdx.x; e < units * p.q.H; e += THREADS) {
-        const int h = e / units, u = e - h * units;
+    const int half = p.rot / 2, units = row_units(p.rot, D, PAIRS), all = units * p.q.H;
+    for (int e0 = 0; e0 < all; e0 += THREADS) {
+        const int e = e0 + threadIdx.x, h = e / units, u = e - h * units;
         const uint16_t* x = static_cast<const uint16_t*>(p.q.x) + (size_t)t * p.q.st + (size_t)h * p.q.sh;
         uint16_t* o = static_cast<uint16_t*>(p.q.out) + (size_t)t * p.q.o_st + (size_t)h * p.q.o_sh;
-        store_turned<E, PAIRS>(load_unit<PAIRS>(x, x == o, u, p.rot, D), x == o, o, turn, u, p.rot, D);
+        Unit v{};
+        if (e < all) v = load_unit<PAIRS>(x, x == o, u, p.rot, D);
+        if (e0 == 0) {   // while the first of them are on their way
+            int position;
+            if (p.positions) position = p.positions[t];
+            else if (!place_of(p, t, position)) return;   // of no sequence: left as it is
+            for (int i = threadIdx.x; i < half; i += THREADS) turn[i] = angle(position, p.inv_freq[i], p.magnitude);
+            __syncthreads();
+        }
+        if (e < all) store_turned<E, PAIRS>(v, x == o, o, turn, u, p.rot, D);
     }
 }
 
@@ -320,18 +346,7 @@ static void write(const Kv8WriteParams& p, hipStream_t st) {
 template <typename E, int D>
 static void read(const Kv8ReadParams& p, hipStream_t st) { kv8_read_kernel<E, D><<<dim3((p.T + 15) / 16, p.Hkv), 256, 0, st>>>(p); }
 
-hipError_t launch_kv8_write(bool bf16, int D, const Kv8WriteParams& all, hipStream_t st) {
-    Kv8WriteParams p = all;
-    // Many queries are rotated by a launch of their own: beside the registers of the keys' rows too few of them are in flight. 8192
-    // tokens, 32 heads of D = 128: 42 us in the same launch, 31 apart; 512 tokens 0.5 and 4.3.
-    if (p.q.H && (int64_t)p.T * p.q.H * D >= 4 << 20) {
-        RopeParams r{};
-        r.rows[0] = p.q;
-        r.positions = p.positions; r.kv_lens = p.kv_lens; r.cu_q = p.cu_q; r.B = p.B;
-        r.inv_freq = p.inv_freq; r.magnitude = p.magnitude; r.T = p.T; r.D = D; r.rot = p.rot; r.interleaved = p.interleaved;
-        if (hipError_t e = launch_rope(bf16, r, st)) return e;
-        p.q = {};
-    }
+hipError_t launch_kv8_write(bool bf16, int D, const Kv8WriteParams& p, hipStream_t st) {
     switch (D) {
         case 64: bf16 ? write<bf16_t, 64>(p, st) : write<half_t, 64>(p, st); break;
         case 128: bf16 ? write<bf16_t, 128>(p, st) : write<half_t, 128>(p, st); break;

@@ -30,9 +30,7 @@ struct RopeRows {
 };
 struct RopeParams {
     RopeRows rows[2];         // queries, keys (H = 0: none)
-    const int32_t* positions; // [T], or null: a token's place in its sequence (rotate.h), and rows of none stay as they are
-    const int32_t *kv_lens, *cu_q;
-    int B;
+    const int32_t* positions; // [T]
     const double* inv_freq;   // [rot / 2]
     float magnitude;
     int T, D, rot;

@@ -15,10 +15,9 @@ namespace w4a16 {
 constexpr int ROPE_TOKENS = 2;   // of a workgroup, at most
 struct RowPlace { const uint16_t* x; uint16_t* o; };
 
-template <typename E, bool PAIRS, bool GIVEN>   // GIVEN: positions are
+template <typename E, bool PAIRS>
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
     extern __shared__ float2 turn[];   // [tokens][rot / 2]
-    [[maybe_unused]] __shared__ int none[ROPE_TOKENS];   // tokens of no sequence
     const int half = p.rot / 2, t0 = blockIdx.x * tokens, live = min(tokens, p.T - t0);
     const int units = row_units(p.rot, p.D, PAIRS);
     static_assert(ROPE_MAX_D / 8 + 1 <= 256, "a row's units are threads of one workgroup");
@@ -44,22 +43,13 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
             v = load_unit<PAIRS>(at.x, at.x == at.o, u, p.rot, p.D);
         }
         if (r0 == 0) {   // while the first rows are on their way
-            if constexpr (GIVEN) {
-                for (int i = threadIdx.x; i < live * half; i += 256) {
-                    const int t = i / half;
-                    turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
-                }
-            } else {   // a wave a token
-                for (int t = threadIdx.x >> 6; t < live; t += 4) {
-                    int position = 0;
-                    const bool found = place_of(p.cu_q, p.kv_lens, p.B, p.T, t0 + t, position);
-                    if ((threadIdx.x & 63) == 0) none[t] = !found;
-                    for (int i = threadIdx.x & 63; i < half; i += 64) turn[t * half + i] = angle(position, p.inv_freq[i], p.magnitude);
-                }
+            for (int i = threadIdx.x; i < live * half; i += 256) {
+                const int t = i / half;
+                turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
             }
             __syncthreads();
         }
-        if (some && (GIVEN || !none[t])) store_turned<E, PAIRS>(v, at.x == at.o, at.o, turn + t * half, u, p.rot, p.D);
+        if (some) store_turned<E, PAIRS>(v, at.x == at.o, at.o, turn + t * half, u, p.rot, p.D);
     }
 }
 
@@ -70,9 +60,8 @@ static void go(const RopeParams& p, hipStream_t st) {
     const int tokens = p.T >= 2048 ? ROPE_TOKENS : 1;
     const dim3 grid((unsigned)((p.T + tokens - 1) / tokens));
     const size_t lds = sizeof(float2) * tokens * (p.rot / 2);
-    auto* const kernel = p.positions ? p.interleaved ? rope_kernel<E, true, true> : rope_kernel<E, false, true>
-                                     : p.interleaved ? rope_kernel<E, true, false> : rope_kernel<E, false, false>;
-    kernel<<<grid, 256, lds, st>>>(p, tokens);
+    if (p.interleaved) rope_kernel<E, true><<<grid, 256, lds, st>>>(p, tokens);
+    else rope_kernel<E, false><<<grid, 256, lds, st>>>(p, tokens);
 }
 
 hipError_t launch_rope(bool bf16, const RopeParams& p, hipStream_t st) {

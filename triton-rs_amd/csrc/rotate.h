@@ -28,29 +28,6 @@ __device__ __forceinline__ float2 angle(int position, double f, float magnitude)
     return float2{n == 1 || n == 2 ? -x : x, n >= 2 ? -z : z};
 }
 
-// The position of the row of token t in its sequence, rows cu_q[b] .. cu_q[b + 1] - 1 (null: row b) of which end at token
-// kv_lens[b] - 1. false: it is of none. By a whole wave: each step tells 64 parts of the sequences apart.
-__device__ __forceinline__ bool place_of(const int32_t* cu_q, const int32_t* kv_lens, int B, int T, int t, int& position) {
-    int b = t;
-    if (cu_q) {
-        int at = 0, n = B + 1;   // the last of cu_q[at .. at + n - 1] that is t or less
-        while (true) {
-            const int step = (n + 63) / 64, i = (threadIdx.x & 63) * step;
-            const int k = __popcll(__ballot(i < n && cu_q[at + min(i, n - 1)] <= t));
-            if (k == 0) return false;
-            at += (k - 1) * step;
-            n = min(step, n - (k - 1) * step);
-            if (step == 1) break;
-        }
-        if (at >= B) return false;
-        b = at;
-        position = kv_lens[b] - min(max(cu_q[b + 1], 0), T) + t;
-    } else {
-        position = kv_lens[b] - 1;
-    }
-    return true;
-}
-
 // (a, b) turned, in fp32: each product is rounded, then their difference or sum (no contraction)
 __device__ __forceinline__ void turn_pair(float& a, float& b, float2 w) {
 #pragma clang fp contract(off)

@@ -188,9 +188,11 @@ static void go(const NormParams& p, hipStream_t st) {
     if (v <= 16) return run<E, Q8, 16, 1>(p, 256, st);
     if (v <= 32) return run<E, Q8, 16, 2>(p, 256, st);
     if (v <= 64) return run<E, Q8, 64, 1>(p, 256, st);
-    // A workgroup a row: two units a thread, so that a CU's rows are in different phases; one where few rows are there, whose
-    // time is one row's. bf16 with a residual: 8192 rows of 5120 64 us with one, 60 with two, 61 with four; 1 row of 4096 3.1, 3.6, 4.3.
-    const int vpt = v <= 1024 && (long long)p.T * p.H < 1024 ? 1 : v <= 2048 ? 2 : v <= 4096 ? 4 : 8;
+    // A workgroup a row: two units a thread, so that a CU's rows are in different phases; one where rows are few (2 waves a SIMD)
+    // and the time is one row's. bf16 with a residual: 8192 rows of 5120 64 us with one, 60 with two, 61 with four; 1 row of 4096
+    // 3.1, 3.6, 4.3; 64 of 8192 4.0, 4.1, 4.9. To 8 bits without: 777 rows of 5003 8.4, 6.8; 300 of 8192 5.3, 4.9.
+    const bool few = v <= 1024 && (long long)p.T * p.H * (waves(1) / 64) <= 2048;
+    const int vpt = few ? 1 : v <= 2048 ? 2 : v <= 4096 ? 4 : 8;
     if (vpt == 1) return run<E, Q8, WIDE, 1>(p, waves(1), st);
     if (vpt == 2) return run<E, Q8, WIDE, 2>(p, waves(2), st);
     if (vpt == 4) return run<E, Q8, WIDE, 4>(p, waves(4), st);

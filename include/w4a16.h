@@ -539,7 +539,7 @@ W4A16_API int w4a16_kv8_read(void* stream, int elem, const void* cache, const in
  * 2^-33 of the query's largest such product where that is more; out is rounded once (to its type's largest finite
  * value beyond that). What a query does not see moves no bit of its result, whatever the cache holds there; a
  * key or value row of NaN that it does see makes it NaN, and so does an infinity or NaN of its own where it
- * sees a key. (A scale q . k that fp32 does not hold has no defined result.) */
+ * sees a key. (A q . n, with n the key's numbers of at most 448, or a scale q . k that fp32 does not hold has no defined result.) */
 #define W4A16_KV8_COUNTER_BYTES 65536
 W4A16_API size_t w4a16_kv8_attention_workspace_size(int32_t T, int32_t B, int32_t Hq, int32_t Hkv,
                                                     int32_t D, int32_t max_q_len,

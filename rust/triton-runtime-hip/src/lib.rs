@@ -122,6 +122,47 @@ extern "C" {
                            pages_per_seq: i32, max_q_len: i32, max_kv_len: i32, scale: f32,
                            causal: i32, window: i32, workspace: u64,
                            workspace_bytes: usize) -> i32;
+    // norm and rotary positions
+    fn w4a16_rms_norm(stream: *mut c_void, elem: i32, x: u64, x_stride_t: i32, x_stride_h: i32,
+                      residual: u64, r_stride_t: i32, r_stride_h: i32, residual_out: u64,
+                      ro_stride_t: i32, ro_stride_h: i32, weight: u64, out: u64,
+                      out_stride_t: i32, out_stride_h: i32, t: i32, h: i32, k: i32,
+                      eps: f32) -> i32;
+    fn w4a16_rms_norm_8bit(stream: *mut c_void, elem: i32, x: u64, x_stride_t: i32,
+                           x_stride_h: i32, residual: u64, r_stride_t: i32, r_stride_h: i32,
+                           residual_out: u64, ro_stride_t: i32, ro_stride_h: i32, weight: u64,
+                           out: u64, out_stride_t: i32, out_stride_h: i32, scales: u64, t: i32,
+                           h: i32, k: i32, group: i32, eps: f32) -> i32;
+    fn w4a16_rope_frequencies(rot: i32, base: f64, scaling: i32, factor: f64,
+                              original_length: f64, slow: f64, fast: f64,
+                              inv_freq: *mut f64) -> i32;
+    fn w4a16_rope(stream: *mut c_void, elem: i32, q: u64, q_stride_t: i32, q_stride_h: i32,
+                  q_out: u64, qo_stride_t: i32, qo_stride_h: i32, k: u64, k_stride_t: i32,
+                  k_stride_h: i32, k_out: u64, ko_stride_t: i32, ko_stride_h: i32,
+                  positions: u64, inv_freq: u64, magnitude: f32, t: i32, hq: i32, hkv: i32,
+                  d: i32, rot: i32, interleaved: i32) -> i32;
+    // key/value cache in 8 bits
+    fn w4a16_kv8_cache_bytes(num_pages: i32, hkv: i32, d: i32, page_size: i32) -> usize;
+    fn w4a16_kv8_write(stream: *mut c_void, elem: i32, k: u64, k_stride_t: i32, k_stride_h: i32,
+                       v: u64, v_stride_t: i32, v_stride_h: i32, q: u64, q_stride_t: i32,
+                       q_stride_h: i32, q_out: u64, qo_stride_t: i32, qo_stride_h: i32,
+                       positions: u64, inv_freq: u64, magnitude: f32, rot: i32,
+                       interleaved: i32, cache: u64, page_table: u64, kv_lens: u64, cu_q: u64,
+                       t: i32, b: i32, hq: i32, hkv: i32, d: i32, num_pages: i32,
+                       page_size: i32, pages_per_seq: i32, max_q_len: i32) -> i32;
+    fn w4a16_kv8_read(stream: *mut c_void, elem: i32, cache: u64, slots: u64, k_out: u64,
+                      k_stride_t: i32, k_stride_h: i32, v_out: u64, v_stride_t: i32,
+                      v_stride_h: i32, num_pages: i32, t: i32, hkv: i32, d: i32,
+                      page_size: i32) -> i32;
+    fn w4a16_kv8_attention_workspace_size(t: i32, b: i32, hq: i32, hkv: i32, d: i32,
+                                          max_q_len: i32, max_kv_len: i32) -> usize;
+    fn w4a16_kv8_attention(stream: *mut c_void, elem: i32, q: u64, q_stride_t: i32,
+                           q_stride_h: i32, cache: u64, page_table: u64, kv_lens: u64, cu_q: u64,
+                           out: u64, out_stride_t: i32, out_stride_h: i32, lse: u64, t: i32,
+                           b: i32, hq: i32, hkv: i32, d: i32, num_pages: i32, page_size: i32,
+                           pages_per_seq: i32, max_q_len: i32, max_kv_len: i32, scale: f32,
+                           causal: i32, window: i32, workspace: u64,
+                           workspace_bytes: usize) -> i32;
 }
 
 /// The calling thread's last libw4a16 message, mapped onto the reference's error type:
@@ -438,7 +479,7 @@ pub fn silu_mul_interleaved_f32(stream: &HipStream, gate_up: u64, out: u64, inte
     check(unsafe { fused_silu_mul_interleaved_f32(stream.0, gate_up, out, inter, total) })
 }
 
-/// A 4-bit key/value cache and the element type of its rows.
+/// A key/value cache in 4 bits (or, for the `kv8_` functions, in 8) and the element type of its rows.
 #[derive(Debug, Clone, Copy)]
 pub struct Kv4Cache {
     /// Device buffer of `kv4_cache_bytes` bytes.
@@ -497,7 +538,7 @@ pub fn kv4_read(stream: &HipStream, c: &Kv4Cache, slots: u64, k_out: Kv4Rows, v_
     })
 }
 
-/// A batch of sequences for `kv4_attention`.
+/// A batch of sequences for `kv4_attention`, `kv8_write` and `kv8_attention`.
 #[derive(Debug, Clone, Copy)]
 pub struct Kv4Batch {
     /// `i32[seqs, pages_per_seq]`.
@@ -542,6 +583,121 @@ pub fn kv4_attention(stream: &HipStream, c: &Kv4Cache, b: &Kv4Batch, q: Kv4Rows,
     // SAFETY: as above; the workspace size is checked by the library.
     check(unsafe {
         w4a16_kv4_attention(stream.0, if c.bf16 { BF16 } else { 0 }, q.data, q.stride_t, q.stride_h,
+                            c.data, b.page_table, b.kv_lens, b.cu_q, out.data, out.stride_t,
+                            out.stride_h, lse, b.tokens, b.seqs, b.heads, c.kv_heads, c.head_dim,
+                            c.num_pages, c.page_size, b.pages_per_seq, b.max_q_len, b.max_kv_len,
+                            b.scale, b.causal as i32, b.window, workspace, workspace_bytes)
+    })
+}
+
+/// Root-mean-square norm of rows `[tokens, heads, dims]`: `h = x + residual`, `out = h / sqrt(mean(h^2) + eps) * weight`;
+/// `residual` (read and written), unless its `data` is 0, takes h.
+#[allow(clippy::too_many_arguments)]
+pub fn rms_norm(stream: &HipStream, bf16: bool, x: Kv4Rows, residual: Kv4Rows, weight: u64, out: Kv4Rows, tokens: i32,
+                heads: i32, dims: i32, eps: f32) -> Result<(), RuntimeError> {
+    // SAFETY: device pointers from hiprt_malloc; the library validates sizes and strides.
+    check(unsafe {
+        w4a16_rms_norm(stream.0, if bf16 { BF16 } else { 0 }, x.data, x.stride_t, x.stride_h, residual.data,
+                       residual.stride_t, residual.stride_h, residual.data, residual.stride_t, residual.stride_h, weight,
+                       out.data, out.stride_t, out.stride_h, tokens, heads, dims, eps)
+    })
+}
+
+/// The same to e4m3 bytes (strides of `out` in bytes) with one scale for `group` elements (0: a row), `f32[tokens, heads,
+/// dims / group]`.
+#[allow(clippy::too_many_arguments)]
+pub fn rms_norm_8bit(stream: &HipStream, bf16: bool, x: Kv4Rows, residual: Kv4Rows, weight: u64, out: Kv4Rows, scales: u64,
+                     tokens: i32, heads: i32, dims: i32, group: i32, eps: f32) -> Result<(), RuntimeError> {
+    // SAFETY: as above.
+    check(unsafe {
+        w4a16_rms_norm_8bit(stream.0, if bf16 { BF16 } else { 0 }, x.data, x.stride_t, x.stride_h, residual.data,
+                            residual.stride_t, residual.stride_h, residual.data, residual.stride_t, residual.stride_h,
+                            weight, out.data, out.stride_t, out.stride_h, scales, tokens, heads, dims, group, eps)
+    })
+}
+
+/// A rotation: `f64[rot / 2]` radians a position on the device (`rope_frequencies` makes them on the host).
+#[derive(Debug, Clone, Copy)]
+pub struct Rope {
+    /// Device pointer.
+    pub inv_freq: u64,
+    /// Dimensions that are rotated.
+    pub rot: i32,
+    /// Factor of the result.
+    pub magnitude: f32,
+    /// Pairs are neighbours (else halves).
+    pub interleaved: bool,
+}
+
+/// Frequencies without scaling for longer contexts.
+pub fn rope_frequencies(rot: i32, base: f64) -> Result<Vec<f64>, RuntimeError> {
+    let mut f = vec![0f64; rot.max(0) as usize / 2];
+    // SAFETY: the library refuses an odd rot, or one below 2, before it writes rot / 2 numbers.
+    check(unsafe { w4a16_rope_frequencies(rot, base, 0, 1.0, 0.0, 0.0, 0.0, f.as_mut_ptr()) })?;
+    Ok(f)
+}
+
+/// Rotates `q` and (unless its `data` is 0) `k` in place at `positions`, `i32[tokens]` on the device.
+#[allow(clippy::too_many_arguments)]
+pub fn rope(stream: &HipStream, bf16: bool, q: Kv4Rows, k: Kv4Rows, positions: u64, r: &Rope, tokens: i32, heads: i32,
+            kv_heads: i32, head_dim: i32) -> Result<(), RuntimeError> {
+    // SAFETY: as above.
+    check(unsafe {
+        w4a16_rope(stream.0, if bf16 { BF16 } else { 0 }, q.data, q.stride_t, q.stride_h, q.data, q.stride_t, q.stride_h,
+                   k.data, k.stride_t, k.stride_h, k.data, k.stride_t, k.stride_h, positions, r.inv_freq, r.magnitude,
+                   tokens, heads, if k.data == 0 { 0 } else { kv_heads }, head_dim, r.rot, r.interleaved as i32)
+    })
+}
+
+/// Bytes of a cache in 8 bits (its `data` is not looked at); 0: not supported.
+pub fn kv8_cache_bytes(c: &Kv4Cache) -> usize {
+    // SAFETY: pure function of its arguments.
+    unsafe { w4a16_kv8_cache_bytes(c.num_pages, c.kv_heads, c.head_dim, c.page_size) }
+}
+
+/// Appends rows `k`, `v` to the sequences of `b`; with `rope` keys are rotated on the way, and `q` (unless its `data` is 0) in
+/// place.
+#[allow(clippy::too_many_arguments)]
+pub fn kv8_write(stream: &HipStream, c: &Kv4Cache, b: &Kv4Batch, k: Kv4Rows, v: Kv4Rows, q: Kv4Rows,
+                 rope: Option<&Rope>) -> Result<(), RuntimeError> {
+    let (freq, rot, magnitude, pairs) = rope.map_or((0, 0, 1.0, 0), |r| (r.inv_freq, r.rot, r.magnitude, r.interleaved as i32));
+    // SAFETY: as above.
+    check(unsafe {
+        w4a16_kv8_write(stream.0, if c.bf16 { BF16 } else { 0 }, k.data, k.stride_t, k.stride_h, v.data, v.stride_t,
+                        v.stride_h, q.data, q.stride_t, q.stride_h, q.data, q.stride_t, q.stride_h, 0, freq, magnitude, rot,
+                        pairs, c.data, b.page_table, b.kv_lens, b.cu_q, b.tokens, b.seqs,
+                        if q.data == 0 { 0 } else { b.heads }, c.kv_heads, c.head_dim, c.num_pages, c.page_size,
+                        b.pages_per_seq, b.max_q_len)
+    })
+}
+
+/// The rows that the slots hold, into `k_out` and `v_out`.
+pub fn kv8_read(stream: &HipStream, c: &Kv4Cache, slots: u64, k_out: Kv4Rows, v_out: Kv4Rows,
+                tokens: i32) -> Result<(), RuntimeError> {
+    // SAFETY: as above.
+    check(unsafe {
+        w4a16_kv8_read(stream.0, if c.bf16 { BF16 } else { 0 }, c.data, slots, k_out.data, k_out.stride_t, k_out.stride_h,
+                       v_out.data, v_out.stride_t, v_out.stride_h, c.num_pages, tokens, c.kv_heads, c.head_dim,
+                       c.page_size)
+    })
+}
+
+/// Bytes of device workspace `kv8_attention` needs; its first 65536 are zero before the first call.
+pub fn kv8_attention_workspace_size(c: &Kv4Cache, b: &Kv4Batch) -> usize {
+    // SAFETY: pure function of its arguments.
+    unsafe {
+        w4a16_kv8_attention_workspace_size(b.tokens, b.seqs, b.heads, c.kv_heads, c.head_dim,
+                                           b.max_q_len, b.max_kv_len)
+    }
+}
+
+/// Attention of `q` over a cache in 8 bits into `out` (and `lse`, `f32[tokens, heads]`, unless 0).
+#[allow(clippy::too_many_arguments)]
+pub fn kv8_attention(stream: &HipStream, c: &Kv4Cache, b: &Kv4Batch, q: Kv4Rows, out: Kv4Rows,
+                     lse: u64, workspace: u64, workspace_bytes: usize) -> Result<(), RuntimeError> {
+    // SAFETY: as above; the workspace size is checked by the library.
+    check(unsafe {
+        w4a16_kv8_attention(stream.0, if c.bf16 { BF16 } else { 0 }, q.data, q.stride_t, q.stride_h,
                             c.data, b.page_table, b.kv_lens, b.cu_q, out.data, out.stride_t,
                             out.stride_h, lse, b.tokens, b.seqs, b.heads, c.kv_heads, c.head_dim,
                             c.num_pages, c.page_size, b.pages_per_seq, b.max_q_len, b.max_kv_len,

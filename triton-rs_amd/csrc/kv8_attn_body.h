@@ -230,7 +230,7 @@ struct Kv8Cols {
 };
 
 // What of a block's last 16 bytes says something, in every lane: a vector load, which is waited for with the block's others. (A
-// scalar load is waited for with all scalar loads, the next step's among them: 64 us for the 55 of kv8_few.hip's 48 sequences.)
+// scalar load is waited for with all scalar loads, the next step's among them: 48 sequences of kv8_few.hip 63.9 us, 63.5 so.)
 __device__ __forceinline__ u32x3 block_tail(const unsigned char* block, int D) {
     return *reinterpret_cast<const u32x3*>(at_bytes(block, 32 * D + vconst(0)));
 }

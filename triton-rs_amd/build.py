@@ -26,6 +26,7 @@ LIB = os.path.join(HERE, "libw4a16.so")
 HSACO = os.path.join(HERE, "w4a16_typed.hsaco")
 META = os.path.join(HERE, "w4a16_typed.json")
 CALLS = os.path.join(HERE, "_calls.so")
+CALLS_OBJ = os.path.join(BUILD, "module", "calls.o")   # (BUILD itself holds the library's objects, all of which a program may link)
 
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -77,11 +78,11 @@ def _compile_calls() -> str:
 
     import torch
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
-    obj = _obj("calls.cpp")
+    os.makedirs(os.path.dirname(CALLS_OBJ), exist_ok=True)
     _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
-          "-c", os.path.join(CSRC, "calls.cpp"), "-o", obj])
-    return obj
+          "-c", os.path.join(CSRC, "calls.cpp"), "-o", CALLS_OBJ])
+    return CALLS_OBJ
 
 
 def _link_calls(obj: str) -> None:
@@ -96,7 +97,7 @@ def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
     # an object whose source is gone would still be linked by whoever takes all objects here
     for f in os.listdir(BUILD):
-        if f.endswith(".o") and os.path.join(BUILD, f) not in map(_obj, [*SOURCES, "calls.cpp"]):
+        if f.endswith(".o") and os.path.join(BUILD, f) not in map(_obj, SOURCES):
             os.remove(os.path.join(BUILD, f))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         fut_calls = ex.submit(_compile_calls)

@@ -1,10 +1,14 @@
 // Attention over the 8-bit cache for many columns (prompts, chunks of them): bound by the matrix and
-// vector instructions. The mathematics is in kv8_attn_body.h.
+// vector instructions, of which one wave's overlap little with another's. The mathematics is in kv8_attn_body.h.
 //
 // A workgroup of four waves takes 128 columns, 32 a wave, and walks the keys 64 at a time: each wave turns
 // a block of 16 tokens into operands once for all four, in LDS and in the order in which lanes take them (16
 // bytes a lane, no bank conflicts), while the step before is computed from the other half of the LDS: one
-// barrier a step. The bytes come two steps ahead into registers.
+// barrier a step. The bytes come a step ahead into registers.
+//
+// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, 610 to 630 us (0.88 PFLOP/s, matrix cores busy 38 %, vector unit
+// some 45); a prompt of 2048 60 us, of 512 20. 64 columns a wave, one wave a SIMD, halve what is read from LDS and took 966
+// us, with the products and the vector instructions beside them in an order of their own 1580 (registers beyond 256 are moved).
 #include "kv8_attn_body.h"
 #include "kv_many.h"
 
@@ -32,28 +36,35 @@ struct Packed {
     u32x3 tail;
 };
 
-// Block `wave` of a step into LDS; its tokens [dead, live) (the others' bytes may be anything)
+// Piece i of UNPACK_PIECES of block b of a step into LDS; its tokens [dead, live) (the others' bytes may be anything)
+template <int D>
+constexpr int UNPACK_PIECES = 6 * (D / 64);
 template <typename E, int D>
-__device__ __forceinline__ void unpack(ManyLds<E, D>& s, const Packed<D>& t, int dead, int live, float factor, int wave, int lane) {
-    const int r = lane & 15, quad = lane >> 4;
-    const uint32_t mask = dead <= 0 && live >= 16 ? ~0u : token_bytes(dead, live, quad);
-    auto* const k = &s.k[wave >> 1][quad][16 * (wave & 1) + r];
-    auto* const v = reinterpret_cast<u32x2*>(&s.v[wave][0][r + 32 * (quad & 1)]) + (quad >> 1);
-#pragma unroll
-    for (int g = 0; g < D / 64; ++g) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) k[4 * g * 64 + 32 * h] = operand8<E>(t.k[g][2 * h], t.k[g][2 * h + 1]);
-        // dimension r D / 16 + x, x = 4 g + e, is row r + 16 (x % 2) of tile x / 2
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t w = t.v[g][e] & mask;
-            v[2 * ((2 * g + e / 2) * 64 + 16 * (e & 1))] = u32x2{from_e4m3<half_t, false>(w), from_e4m3<half_t, true>(w)};
-        }
+__device__ __forceinline__ void unpack_piece(ManyLds<E, D>& s, const Packed<D>& t, int i, uint32_t mask, int b, int lane) {
+    const int r = lane & 15, quad = lane >> 4, g = i / 6, h = i % 6;
+    if (h < 2) {
+        s.k[b >> 1][4 * g + quad][16 * (b & 1) + r + 32 * h] = operand8<E>(t.k[g][2 * h], t.k[g][2 * h + 1]);
+    } else {   // dimension r D / 16 + x, x = 4 g + e, is row r + 16 (x % 2) of tile x / 2
+        const int e = h - 2;
+        const uint32_t w = t.v[g][e] & mask;
+        reinterpret_cast<u32x2*>(&s.v[b][2 * g + e / 2][r + 32 * (quad & 1) + 16 * (e & 1)])[quad >> 1] =
+            u32x2{from_e4m3<half_t, false>(w), from_e4m3<half_t, true>(w)};
     }
+}
+__device__ __forceinline__ uint32_t live_bytes(int dead, int live, int lane) { return dead <= 0 && live >= 16 ? ~0u : token_bytes(dead, live, lane >> 4); }
+template <typename E, int D>
+__device__ __forceinline__ void unpack_scale(ManyLds<E, D>& s, const Packed<D>& t, int dead, int live, float factor, int b, int lane) {
     if (lane == 0) {
-        s.scale[wave] = Kv8Scale::of(t.tail, factor, live > 0 && dead < 16);
-        s.live[wave] = live;
+        s.scale[b] = Kv8Scale::of(t.tail, factor, live > 0 && dead < 16);
+        s.live[b] = live;
     }
+}
+template <typename E, int D>
+__device__ __forceinline__ void unpack(ManyLds<E, D>& s, const Packed<D>& t, int dead, int live, float factor, int b, int lane) {
+    const uint32_t mask = live_bytes(dead, live, lane);
+#pragma unroll
+    for (int i = 0; i < UNPACK_PIECES<D>; ++i) unpack_piece<E, D>(s, t, i, mask, b, lane);
+    unpack_scale<E, D>(s, t, dead, live, factor, b, lane);
 }
 
 __device__ __forceinline__ float half_max(float v) {   // over a column's two lanes, 32 apart
@@ -65,15 +76,23 @@ __device__ __forceinline__ float half_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The largest of three, one of which is not NaN. (The compiler's own first quiets what it has from another block, an instruction
+// an operand.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // A wave's 32 columns, column lane % 32 in a lane; as Kv8Cols, whose comments hold here.
 template <typename E, int D>
 struct ManyCols {
     typedef typename vec8<E>::type vec_t;
     static constexpr int KW = D / 16, VT = D / 32;
-    int c, n, lo, hi, jlo, jhi, all_lo, all_hi;
+    float16_t o[VT];       // dimension r D / 16 + 2 y + z, r + 16 z = 8 (i / 4) + 4 (lane / 32) + i % 4, in o[y][i]
     vec_t qf[KW];          // dimensions 16 x + 8 (lane / 32) + (0..7)
     float m, l, most;
-    float16_t o[VT];       // dimension r D / 16 + 2 y + z, r + 16 z = 8 (i / 4) + 4 (lane / 32) + i % 4, in o[y][i]
+    int c, n, lo, hi, jlo, jhi, all_lo, all_hi;
 
     __device__ __forceinline__ void load(const KvAttnParams& p, const KvItem& w, int first_col, int lane) {
         c = first_col;
@@ -108,15 +127,14 @@ struct ManyCols {
             for (int e = 0; e < 16; ++e) o[y][e] = 0.f;
     }
 
-    // Tokens j + 8 (i / 4) + 4 (lane / 32) + i % 4 of 32 from j on.
-    __device__ __forceinline__ void logits(float (&x)[16], float (&back)[2], const float16_t& acc, const Kv8Scale (&s)[2], bool whole, int j, int end,
-                                           int bad, int lane) {
+    // Tokens j + 8 (i / 4) + 4 (lane / 32) + i % 4 of 32 from j on: [from, to) of the lane's 16 logits
+    __device__ __forceinline__ void logits(float (&x)[16], const float16_t& acc, const Kv8Scale (&s)[2], int from, int to) const {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const float off = s[b].value - m;
-#pragma unroll
-            for (int i = 8 * b; i < 8 * b + 8; ++i) x[i] = __builtin_fmaf(acc[i], s[b].key, off);
-        }
+        for (int i = 0; i < 16; ++i)
+            if (i >= from && i < to) x[i] = __builtin_fmaf(acc[i], s[i / 8].key, s[i / 8].value - m);
+    }
+    // What is not seen, or not finite. whole: nothing of that.
+    __device__ __forceinline__ void mask(float (&x)[16], const Kv8Scale (&s)[2], bool whole, int j, int end, int bad, int lane) {
         if (!whole) {
             int at = j + 4 * (lane >> 5);
             asm volatile("" : "+v"(at), "+s"(bad));   // (else kept over the loop: every token's distances, in registers)
@@ -138,13 +156,13 @@ struct ManyCols {
                     for (int i = 0; i < 16; ++i) o[y][i] += add;
             }
         }
+    }
+    // The reference follows; how the lane's sums take a block's weights in back.
+    __device__ __forceinline__ void follow(float (&x)[16], float (&back)[2], const Kv8Scale (&s)[2]) {
         float high[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            float t[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = fmaxf(x[8 * b + i], x[8 * b + 4 + i]);
-            high[b] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            high[b] = max3(max3(x[8 * b], x[8 * b + 1], x[8 * b + 2]), max3(x[8 * b + 3], x[8 * b + 4], x[8 * b + 5]), max3(x[8 * b + 6], x[8 * b + 7], x[8 * b + 7]));
             back[b] = s[b].back;
         }
         float top = fmaxf(high[0], high[1]);
@@ -174,17 +192,21 @@ struct ManyCols {
             }
         }
     }
-    // Weights of block b as operand; the sum of p_j.
-    __device__ __forceinline__ half8_t weights(int b, const float (&x)[16], const float (&back)[2]) {
-        half8_t w;
-        float f[8];
+    // Weights [from, to) of the lane's 16; a block's as operand; the sum of p_j.
+    __device__ __forceinline__ static void weights(float (&x)[16], int from, int to) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            f[i] = __builtin_amdgcn_exp2f(x[8 * b + i]);
-            w[i] = (half_t)f[i];
-        }
+        for (int i = 0; i < 16; ++i)
+            if (i >= from && i < to) x[i] = __builtin_amdgcn_exp2f(x[i]);
+    }
+    __device__ __forceinline__ static half8_t operand(const float (&w)[16], int b) {
+        half8_t h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = (half_t)w[8 * b + i];
+        return h;
+    }
+    __device__ __forceinline__ void sum(const float (&w)[16], const float (&back)[2], int b) {
+        const float* f = w + 8 * b;
         l = __builtin_fmaf(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])), back[b], l);
-        return w;
     }
     __device__ __forceinline__ void finish() {
         l = half_sum(l);
@@ -205,6 +227,8 @@ struct ManyCols {
     }
 };
 
+// What stands before it is issued before what stands behind.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 template <typename E, int D, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void kv8_many_kernel(KvAttnParams p) {
     constexpr int COLS = 32, STEP = MANY_STEP, ALL = STEP * GROUPS;
@@ -244,16 +268,37 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
     }
     __syncthreads();
     int buf = 0;
+    // Two waves a SIMD (D <= 128): the next step is unpacked beside this one's products of keys, a half step's share each, and the
+    // instructions of the second product stand in this order (1024 queries over 32768 keys of 8 heads 618 us, 637 in the compiler's).
+    // One wave: all of it first, so that the bytes of the step behind it are a step ahead (2048 of D = 256 119 us, 124).
+    constexpr bool BESIDE = D <= 128;
+    constexpr int PIECES = UNPACK_PIECES<D> / 2;   // of a half step
     for (int j = w.k0; j < w.k1; j += ALL, buf ^= 1) {
-        if (j + ALL < w.k1) {
-            unpack<E, D>(lds[buf ^ 1][group], t, 0, live, p.scale_log2, wave, lane);
-            fetch(j + 2 * ALL);
-        }
         const ManyLds<E, D>& s = lds[buf][group];
+        ManyLds<E, D>& into = lds[buf ^ 1][group];   // the next step's (behind the last: that of no step)
+        const uint32_t bytes = live_bytes(0, live, lane);
+        if constexpr (!BESIDE)
+            if (j + ALL < w.k1) {
+                unpack<E, D>(into, t, 0, live, p.scale_log2, wave, lane);
+                fetch(j + 2 * ALL);
+            }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int jh = j + STEP * group + 32 * half;
-            if (jh >= a.jhi || jh + 32 <= a.jlo) continue;   // none of this wave's columns sees these
+            auto piece = [&](int i) { unpack_piece<E, D>(into, t, half * PIECES + i, bytes, wave, lane); };
+            auto rest = [&] {
+                if (half == 0) return;   // (the first half's share stands there)
+                unpack_scale<E, D>(into, t, 0, live, p.scale_log2, wave, lane);
+                fetch(j + 2 * ALL);
+            };
+            if (jh >= a.jhi || jh + 32 <= a.jlo) {   // none of this wave's columns sees these
+                if constexpr (BESIDE) {
+#pragma unroll
+                    for (int i = 0; i < PIECES; ++i) piece(i);
+                    rest();
+                }
+                continue;
+            }
             float16_t acc;
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[i] = 0.f;
@@ -264,25 +309,59 @@ __global__ __launch_bounds__(256 * GROUPS, kv8_many_simd_waves(D, GROUPS)) void 
             const int live0 = s.live[2 * half], live1 = s.live[2 * half + 1];
 #pragma unroll
             for (int x = 0; x < C::KW; ++x) kf[x] = s.k[half][x][lane];
-            __builtin_amdgcn_sched_barrier(0);
+            in_order();
             const int bad = __builtin_amdgcn_readfirstlane((live0 <= 0 ? 1 : 0) | (live1 <= 0 ? 2 : 0));
             sc[0].nan = __builtin_amdgcn_readfirstlane(sc[0].nan);
             sc[1].nan = __builtin_amdgcn_readfirstlane(sc[1].nan);
-            const bool whole = jh >= a.all_lo && jh + 32 <= a.all_hi && jh + 32 <= a.jhi && !bad && !(sc[0].nan | sc[1].nan);
+            // (& and no &&, which would be a branch ahead of the products: D = 192, 1024 over 16384 378 us, 340 so)
+            const bool whole = (jh >= a.all_lo) & (jh + 32 <= a.all_hi) & (jh + 32 <= a.jhi) & !bad & !(sc[0].nan | sc[1].nan);
 #pragma unroll
-            for (int x = 0; x < C::KW; ++x) acc = mfma32x32x16(kf[x], a.qf[x], acc);
+            for (int x = 0; x < C::KW; ++x) {
+                acc = mfma32x32x16(kf[x], a.qf[x], acc);
+                if constexpr (BESIDE) {
+                    in_order();
+#pragma unroll
+                    for (int i = x * PIECES / C::KW; i < (x + 1) * PIECES / C::KW; ++i) piece(i);
+                    in_order();
+                }
+            }
+            if constexpr (BESIDE) rest();
             float x[16], back[2];
-            a.logits(x, back, acc, sc, whole, jh, a.jhi, bad, lane);
+            a.logits(x, acc, sc, 0, 16);
+            a.mask(x, sc, whole, jh, a.jhi, bad, lane);
+            a.follow(x, back, sc);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int y = 0; y < C::VT; ++y) vf[b][y] = s.v[2 * half + b][y][lane];
-            __builtin_amdgcn_sched_barrier(0);
+            in_order();
+            if constexpr (BESIDE) {
+                C::weights(x, 0, 8);
+                half8_t pw = C::operand(x, 0);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const half8_t pw = a.weights(b, x, back);
+                for (int y = 0; y < C::VT; ++y) {
+                    a.o[y] = mfma32x32x16(vf[0][y], pw, a.o[y]);
+                    in_order();
+                    C::weights(x, 8 + y * 8 / C::VT, 8 + (y + 1) * 8 / C::VT);
+                    in_order();
+                }
+                pw = C::operand(x, 1);
 #pragma unroll
-                for (int y = 0; y < C::VT; ++y) a.o[y] = mfma32x32x16(vf[b][y], pw, a.o[y]);
+                for (int y = 0; y < C::VT; ++y) {
+                    a.o[y] = mfma32x32x16(vf[1][y], pw, a.o[y]);
+                    in_order();
+                    if (y < 2) a.sum(x, back, y);
+                    in_order();
+                }
+            } else {
+                C::weights(x, 0, 16);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const half8_t pw = C::operand(x, b);
+                    a.sum(x, back, b);
+#pragma unroll
+                    for (int y = 0; y < C::VT; ++y) a.o[y] = mfma32x32x16(vf[b][y], pw, a.o[y]);
+                }
             }
         }
         __syncthreads();

@@ -353,7 +353,7 @@ W4A16_API int w4a16_fused_moe_prepared(void* stream, const void* x, const float*
  * behind them. `elem` is 0 (fp16) or W4A16_BF16, the type of all rows. Rows are [T, H, K] (or [T, H, D])
  * with strides in elements along T and H, contiguous along the last; they need no alignment but an
  * element's and no particular size. An output may be the tensor that it is made from, at its strides; it
- * must not otherwise overlap an input. Nothing is allocated. At most 2^30 rows in a call. */
+ * must not otherwise overlap an input. Nothing is allocated. At most 2^30 rows of a tensor in a call. */
 
 /* h = x + residual (nullable: h = x), y = h / sqrt(mean(h^2) + eps) * weight[K], in fp32 for each row of
  * K <= 65536 elements. residual_out takes h (both or neither; it may be residual itself), out takes y,

@@ -310,6 +310,19 @@ def test_rope_strides_and_ends(dtype):
     assert [3, 7] in nan and [3, 39] in nan and all(n[1] in (7, 39) for n in nan)
 
 
+def test_rope_of_more_tokens_than_a_launch_has_threads_along_x():
+    P = need_gpu()
+    T = (1 << 25) + 70001   # two tokens a workgroup of 256: 2^32 threads and some
+    r = P.Rope(2)
+    positions = torch.arange(T, dtype=torch.int32, device="cuda") % 1000
+    q = torch.zeros((T, 1, 2), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    P.rope(q, positions, r)
+    w = positions.double()
+    want = torch.stack([w.cos(), w.sin()], 1)
+    assert ((q[:, 0].double() - want).abs().max() <= 2.0 ** -11 + 2.0 ** -22).item()   # (values of 1 at most: half a step of fp16, and fp32's)
+
+
 def test_rope_arguments():
     P = need_gpu()
     q, pos, r = torch.zeros((2, 4, 64), dtype=F16, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), P.Rope(64)

@@ -87,6 +87,7 @@ def _rope(P, **over):
     (dict(Hq=0), "bad sizes", False),
     (dict(D=0), "bad sizes", False),
     (dict(D=1040), "at most 1024 of 1024", True),
+    (dict(T=2 ** 30 // 4 + 1), "2^30", True),
     (dict(Hq=1025), "at most 1024", True),
     (dict(rot=0), "rot=0", False),
     (dict(rot=33), "rot=33", False),

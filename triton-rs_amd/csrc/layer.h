@@ -9,7 +9,7 @@
 namespace w4a16 {
 
 constexpr int NORM_MAX_K = 65536;   // elements of a row: 1024 threads of 64
-constexpr int64_t NORM_MAX_ROWS = 1ll << 30;
+constexpr int64_t LAYER_MAX_ROWS = 1ll << 30;   // of a call
 
 struct NormParams {   // rows [T, H, K], strides in elements, K contiguous
     const void *x, *residual, *weight;   // residual: null for none

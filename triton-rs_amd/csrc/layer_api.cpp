@@ -17,7 +17,7 @@ static int rms_norm(void* stream, int elem, const void* x, int32_t x_st, int32_t
     if (int rc = check_elem(elem)) return rc;
     if (T < 0 || H < 1 || K < 1) return fail(W4A16_ERR_INVALID_ARG, "bad sizes (T=%d H=%d K=%d)", T, H, K);
     if (K > NORM_MAX_K) return fail(W4A16_ERR_UNSUPPORTED, "K=%d: at most %d", K, NORM_MAX_K);
-    if ((int64_t)T * H > NORM_MAX_ROWS) return fail(W4A16_ERR_UNSUPPORTED, "%d x %d rows: at most 2^30 in a call", T, H);
+    if ((int64_t)T * H > LAYER_MAX_ROWS) return fail(W4A16_ERR_UNSUPPORTED, "%d x %d rows: at most 2^30 in a call", T, H);
     if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(W4A16_ERR_INVALID_ARG, "eps must be finite and not negative");
     if (group > 0 && (group < 32 || group > 512 || (group & (group - 1)) || K % group))
         return fail(W4A16_ERR_INVALID_ARG, "group %d: 0 (a row), 32, 64, 128, 256 or 512, and K=%d a multiple", group, K);
@@ -100,6 +100,8 @@ W4A16_API int w4a16_rope(void* stream, int elem, const void* q, int32_t q_stride
     if (T < 0 || Hq < 1 || Hkv < 0 || D < 1) return fail(W4A16_ERR_INVALID_ARG, "bad sizes (T=%d Hq=%d Hkv=%d D=%d)", T, Hq, Hkv, D);
     if (D > ROPE_MAX_D || Hq > KV_MAX_HEADS || Hkv > KV_MAX_HEADS)
         return fail(W4A16_ERR_UNSUPPORTED, "%d and %d heads of %d: at most %d of %d", Hq, Hkv, D, KV_MAX_HEADS, ROPE_MAX_D);
+    if ((int64_t)T * (Hq > Hkv ? Hq : Hkv) > LAYER_MAX_ROWS)
+        return fail(W4A16_ERR_UNSUPPORTED, "%d tokens of %d and %d rows: at most 2^30 in a call", T, Hq, Hkv);
     if (rot < 2 || rot % 2 || rot > D) return fail(W4A16_ERR_INVALID_ARG, "rot=%d: even, 2 to the head's %d dimensions", rot, D);
     if (!std::isfinite(magnitude)) return fail(W4A16_ERR_INVALID_ARG, "magnitude must be finite");
     if (!k != (Hkv == 0) || !k != !k_out) return fail(W4A16_ERR_INVALID_ARG, "k, k_out and Hkv: all or none");

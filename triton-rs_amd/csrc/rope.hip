@@ -18,7 +18,8 @@ struct RowPlace { const uint16_t* x; uint16_t* o; };
 template <typename E, bool PAIRS>
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
     extern __shared__ float2 turn[];   // [tokens][rot / 2]
-    const int half = p.rot / 2, t0 = blockIdx.x * tokens, live = min(tokens, p.T - t0);
+    const int half = p.rot / 2, t0 = (int)(blockIdx.y * gridDim.x + blockIdx.x) * tokens, live = min(tokens, p.T - t0);
+    if (live <= 0) return;
     const int units = row_units(p.rot, p.D, PAIRS);
     static_assert(ROPE_MAX_D / 8 + 1 <= 256, "a row's units are threads of one workgroup");
     const int rows = 256 / units, heads = p.rows[0].H + p.rows[1].H, all = live * heads;
@@ -58,7 +59,8 @@ static void go(const RopeParams& p, hipStream_t st) {
     // Two tokens a workgroup where all of them are more than are resident at once; with one its angles and barrier count (8192
     // tokens, 40 heads of D = 64 20 us and 18), with four a CU's workgroups all wait at once (40 heads of 128, pairs: 38 and 43 us).
     const int tokens = p.T >= 2048 ? ROPE_TOKENS : 1;
-    const dim3 grid((unsigned)((p.T + tokens - 1) / tokens));
+    const unsigned blocks = ((unsigned)p.T + tokens - 1) / tokens, x = blocks < 65536 ? blocks : 65536;   // (a launch's threads along x are 32-bit)
+    const dim3 grid(x, (blocks + x - 1) / x);
     const size_t lds = sizeof(float2) * tokens * (p.rot / 2);
     if (p.interleaved) rope_kernel<E, true><<<grid, 256, lds, st>>>(p, tokens);
     else rope_kernel<E, false><<<grid, 256, lds, st>>>(p, tokens);

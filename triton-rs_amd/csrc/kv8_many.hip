@@ -6,8 +6,8 @@
 // bytes a lane, no bank conflicts), while the step before is computed from the other half of the LDS: one
 // barrier a step. The bytes come a step ahead into registers.
 //
-// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, 610 to 630 us (0.88 PFLOP/s, matrix cores busy 38 %, vector unit
-// some 45); a prompt of 2048 60 us, of 512 20. 64 columns a wave, one wave a SIMD, halve what is read from LDS and took 966
+// Measured: 1024 queries over 32768 keys, 32 heads on 8 of D = 128, 600 to 625 us (0.88 PFLOP/s, matrix cores busy 42 %, vector unit
+// 51); a prompt of 2048 60 us, of 512 20. 64 columns a wave, one wave a SIMD, halve what is read from LDS and took 966
 // us, with the products and the vector instructions beside them in an order of their own 1580 (registers beyond 256 are moved).
 #include "kv8_attn_body.h"
 #include "kv_many.h"

@@ -11,7 +11,7 @@
 // one of rope.hip's they took 4 to 10 us more, start and end).
 //
 // Measured, 8 heads of D = 128: 8192 tokens 15.0 us (50 MB, 3.3 TB/s), keys rotated on the way 21.0, and 32
-// heads of queries 49 (184 MB, 3.8 TB/s); 48 tokens of 48 sequences 4.4
+// heads of queries 46 (184 MB, 4.0 TB/s); 48 tokens of 48 sequences 4.4
 // and 5.3; 8192 tokens read 11.6 (4.3 TB/s). What is left is registers: 77 and 91 of a thread leave six and five waves a SIMD (in 64
 // it spills: 28 us), the next head's rows on their way beside this one's cost a wave and 1 us.
 #include "kv8.h"
@@ -85,17 +85,19 @@ __device__ __forceinline__ bool place_of(const Kv8WriteParams& p, int t, int& po
         position = p.kv_lens[t] - 1;
         return true;
     }
+    const int lane = threadIdx.x & 63;
     int at = 0, n = p.B + 1;   // the last of cu_q[at .. at + n - 1] that is t or less
-    while (true) {
-        const int step = (n + 63) / 64, i = (threadIdx.x & 63) * step;
+    while (n > 64) {
+        const int step = (n + 63) / 64, i = lane * step;
         const int k = __popcll(__ballot(i < n && p.cu_q[at + min(i, n - 1)] <= t));
         if (k == 0) return false;
         at += (k - 1) * step;
         n = min(step, n - (k - 1) * step);
-        if (step == 1) break;
     }
-    if (at >= p.B) return false;
-    position = p.kv_lens[at] - min(max(p.cu_q[at + 1], 0), p.T) + t;
+    const int e = min(at + lane, p.B), first = p.cu_q[e], next = p.cu_q[min(e + 1, p.B)], len = p.kv_lens[min(e, p.B - 1)];
+    const int k = __popcll(__ballot(lane < n && first <= t));
+    if (k == 0 || at + k > p.B) return false;
+    position = __builtin_amdgcn_readlane(len, k - 1) - min(max(__builtin_amdgcn_readlane(next, k - 1), 0), p.T) + t;
     return true;
 }
 
@@ -332,9 +334,10 @@ static void write(const Kv8WriteParams& p, hipStream_t st) {
     const long long per = ((long long)(p.max_q < p.T ? p.max_q : p.T) + 30) / 16, all = (long long)p.T / 16 + 2 * (long long)p.B;
     const bool direct = per * p.B <= 2 * all;
     const int items = (int)(direct ? per * p.B : all);
-    // heads of a workgroup: one where few blocks are there, so that they fill the device
+    // Heads of a workgroup: one where few blocks are there, so that they fill the device; more share the angles. Beside queries a half
+    // of it will do: 5424 tokens, 8 heads, 32 of queries 35.4 us in one head a workgroup, 33.1 in two; without queries 18.9 and 19.5.
     int heads = 1;
-    while (heads < p.Hkv && (long long)items * ((p.Hkv + 2 * heads - 1) / (2 * heads)) >= 2048) heads *= 2;
+    while (heads < p.Hkv && (long long)items * ((p.Hkv + 2 * heads - 1) / (2 * heads)) >= (p.q.H ? 1024 : 2048)) heads *= 2;
     const int groups = (p.Hkv + heads - 1) / heads;
     const unsigned grid = (unsigned)items * groups + (p.q.H ? p.T : 0);
     const int per_seq = direct ? (int)per : 0;

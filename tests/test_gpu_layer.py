@@ -66,6 +66,23 @@ def test_norm(dtype, T, K, residual):
     check_8bit(q, s, y, 0)
 
 
+@TYPES
+@pytest.mark.parametrize("T,K,group", [(2100, 513, 0), (1100, 1031, 0), (600, 4096, 128), (300, 5003, 0), (333, 4608, 512), (130, 8191, 0)])
+def test_norm_of_many_rows(dtype, T, K, group):
+    """Rows that run with more elements a thread than a few rows of their width; in place."""
+    P = need_gpu()
+    gen = torch.Generator().manual_seed(T + K)
+    x = torch.randn((T, K), generator=gen).to(dtype).cuda()
+    r = (torch.randn((T, K), generator=gen) * 5).to(dtype).cuda()
+    w = (1 + 0.3 * torch.randn(K, generator=gen)).to(dtype).cuda()
+    h, y = plain.norm(x, w, 1e-5, r)
+    q, s = P.rms_norm_8bit(x, w, 1e-5, group=group, residual=r, residual_out=torch.empty_like(r))
+    check_8bit(q, s, y, group)
+    assert P.rms_norm(x, w, 1e-5, residual=r, out=x) is x
+    rounded_once(x, y, dtype, NORM_REL)
+    rounded_once(r, h, dtype, 2.0 ** -24)
+
+
 def check_8bit(q, s, y, group):
     """Scales are max |y| / 448 (2^-100 at least) within the norm's roundings and two more; numbers are half a step
     of e4m3 from y / scale, which is off by as much and three more."""

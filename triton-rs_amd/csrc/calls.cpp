@@ -1,7 +1,7 @@
 // Python's side of the calls that a program makes once a layer and step (norm, rotary positions, the caches'
 // attention, the 8-bit cache): checks of the tensors, then the C-ABI entry point, without a Python object on the
 // way. A decode step makes hundreds of these calls, of a few microseconds of GPU time each; in Python the checks and
-// ctypes' conversions took 7 us of a call's 9.5 (one row of rms_norm), of which this leaves half of one.
+// ctypes' conversions made a call of rms_norm 9.9 us, which takes 4.2 here.
 //
 // A module for CPython (built by build.py beside the library, imported by __init__.py): functions of positional
 // arguments, called by the functions of the same names there, which have the documentation.

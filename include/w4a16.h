@@ -369,8 +369,8 @@ W4A16_API int w4a16_rms_norm(void* stream, int elem, const void* x, int32_t x_st
 /* The same with y in 8 bits: out is e4m3 (1 sign, 4 exponent, 3 mantissa bits; largest value 448, no
  * infinities; strides in bytes), scales fp32 [T, H, K / group] contiguous, one for `group` elements (32,
  * 64, 128, 256 or 512, of which K is a multiple) or for a row (0): scale = max(max |y| / 448, 2^-100), out =
- * y / scale rounded to nearest even, so that out * scale stands for y. A group with a NaN has a scale of
- * NaN. */
+ * the fp32 quotient y / scale rounded to nearest even, so that out * scale stands for y. A group with a NaN has
+ * a scale of NaN; one with a y that fp32 does not hold an infinite scale, NaN there and 0 elsewhere. */
 W4A16_API int w4a16_rms_norm_8bit(void* stream, int elem, const void* x, int32_t x_stride_t,
                                   int32_t x_stride_h, const void* residual, int32_t r_stride_t,
                                   int32_t r_stride_h, void* residual_out, int32_t ro_stride_t,

@@ -1,0 +1,63 @@
+"""Norm and rotary positions where a rounding or fp32's range decides: numbers next to the middle of two of e4m3, an eps that
+outweighs rows, rows of several waves that are zero or not finite, magnitudes that take products past fp32."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_plain as plain
+from test_gpu_layer import BF16, E4M3, F16, NORM_REL, TYPES, need_gpu, rounded_once
+
+pytestmark = pytest.mark.gpu
+
+
+def near_the_middle(dtype):
+    """[groups, 32] positive weights, the first of each the largest m, the others next to the middle between two numbers of e4m3
+    times m / 448: 21 is one, and 21 / 448 is 3 / 64, so 3 m / 64 of any m that holds it is one but for the scale's rounding."""
+    bits = 11 if dtype == F16 else 8
+    first = np.arange(1, 2 ** bits // 3, 2, dtype=np.float64)
+    powers = 2.0 ** np.concatenate((np.arange(0, -11, -1), np.arange(0, -11, -1), np.arange(0, -9, -1)))   # (21 2^4 is the largest middle)
+    return torch.from_numpy(np.concatenate((first[:, None], 0.75 * first[:, None] * powers), 1)).to(dtype)
+
+
+@TYPES
+def test_8bit_next_to_the_middle(dtype):
+    """Rows of 1 and -1 and no eps: y is the weight itself, exactly. Each number is the fp32 quotient of it and the scale (itself an
+    fp32 quotient) rounded to nearest even, bit for bit: once a group, once a row."""
+    P = need_gpu()
+    w = near_the_middle(dtype)
+    assert torch.equal(w[:, 1].double() * 4, w[:, 0].double() * 3)
+    K = w.numel()
+    x = torch.where(torch.rand((3, K), generator=torch.Generator().manual_seed(0)) < 0.5, -1.0, 1.0).to(dtype)
+    assert torch.equal(P.rms_norm(x.cuda(), w.flatten().cuda(), 0.0).cpu(), x * w.flatten())
+    scale = w[:, 0].float() / 448.0
+    want = (w.float() / scale[:, None]).to(E4M3).float().flatten()
+    q, s = P.rms_norm_8bit(x.cuda(), w.flatten().cuda(), 0.0, group=32)
+    assert torch.equal(s.cpu(), scale.expand(3, -1)) and torch.equal(q.float().cpu(), x.float() * want)
+    for i in range(0, len(w), 7):
+        row = torch.cat((w[i], w[i, 1:20]))   # (of no width that a group has)
+        q, s = P.rms_norm_8bit(x[:, :51].contiguous().cuda(), row.cuda(), 0.0)
+        assert (s.cpu() == scale[i]).all() and torch.equal(q.float().cpu(), x[:, :51].float() * torch.cat((want[32 * i:32 * i + 32], want[32 * i + 1:32 * i + 20])))
+
+
+@TYPES
+@pytest.mark.parametrize("K", [64, 3000])
+def test_8bit_beyond_fp32(dtype, K):
+    """y beyond fp32 in a group: its scale is infinite, what is finite of it 0, what is not NaN; its neighbours are as ever."""
+    P = need_gpu()
+    if dtype == F16:
+        pytest.skip("no such y")
+    x = torch.ones((2, K), dtype=dtype)
+    x[0, 40] = 2.0 ** 20                        # y of about sqrt(K) 2^126 there, and beside it about 2^-20
+    w = torch.ones(K, dtype=dtype)
+    w[40] = 2.0 ** 127
+    w = w.cuda()
+    for group in (32, 0) if K == 64 else (0,):
+        q, s = P.rms_norm_8bit(x.cuda(), w, 1e-6, group=group)
+        q, s = q.float().cpu(), s.cpu()
+        at = 40 // (group or K)
+        part = slice(at * (group or K), (at + 1) * (group or K))
+        assert s[0, at] == float("inf") and torch.isfinite(s[1]).all()
+        assert q[0, 40].isnan() and not q[0, part].nan_to_num(0).any() and int(q[0].isnan().sum()) == 1
+        if group:
+            y = plain.norm(x, w, 1e-6)[1][0, :32]
+            assert torch.isfinite(s[0, 0]) and ((q[0, :32].double() * s[0, 0] - y).abs() <= y.abs() * (2.0 ** -4 + NORM_REL + 2.0 ** -22)).all()

@@ -1,6 +1,6 @@
 // Root-mean-square norm of rows with the residual's addition: h = x + r, y = h / sqrt(mean h^2 + eps) w,
 // in fp32; h rounded to the element type goes back as the residual, y to the element type, or to e4m3 with a
-// scale for every `group` elements: s = max(max |y| / 448, 2^-100), y / s rounded.
+// scale for every `group` elements: s = max(max |y| / 448, 2^-100), the fp32 quotient y / s rounded.
 //
 // Bound by memory: 2 bytes of x and 2 of r in, 2 of h and 2 (or 1) of y out. A row stays in the registers of
 // its threads, 8 VPT elements each, so that each byte passes once; the sum of squares (and the largest |y| of a
@@ -159,10 +159,16 @@ __global__ __launch_bounds__(TPR == WIDE ? 1024 : 256) void norm_kernel(NormPara
             }
             float s = m / 448.f;
             s = s < 0x1p-100f ? 0x1p-100f : s;   // (NaN stays)
-            const float by = 1.f / s;
+            // y / s in fp32 (y times the rounded 1 / s, and its rest: for s next to 2^-100 but for a unit), then to e4m3. Under an infinite
+            // scale what is finite is 0.
+            const float by = 1.f / s, rest = s == INFINITY ? 0.f : s;
             uint32_t q[2];
+            auto over = [&](float v) {
+                const float u = v * by;
+                return __builtin_fmaf(__builtin_fmaf(-u, rest, v), by, u);
+            };
 #pragma unroll
-            for (int g = 0; g < 2; ++g) q[g] = to_e4m3(y[i][4 * g] * by, y[i][4 * g + 1] * by, y[i][4 * g + 2] * by, y[i][4 * g + 3] * by);
+            for (int g = 0; g < 2; ++g) q[g] = to_e4m3(over(y[i][4 * g]), over(y[i][4 * g + 1]), over(y[i][4 * g + 2]), over(y[i][4 * g + 3]));
             if (n >= 8) {
                 *reinterpret_cast<Bytes8*>(out + e0) = Bytes8{{q[0], q[1]}};
             } else if (n > 0) {

@@ -39,16 +39,13 @@ def test_8bit_next_to_the_middle(dtype):
         assert (s.cpu() == scale[i]).all() and torch.equal(q.float().cpu(), x[:, :51].float() * torch.cat((want[32 * i:32 * i + 32], want[32 * i + 1:32 * i + 20])))
 
 
-@TYPES
 @pytest.mark.parametrize("K", [64, 3000])
-def test_8bit_beyond_fp32(dtype, K):
+def test_8bit_beyond_fp32(K):
     """y beyond fp32 in a group: its scale is infinite, what is finite of it 0, what is not NaN; its neighbours are as ever."""
     P = need_gpu()
-    if dtype == F16:
-        pytest.skip("no such y")
-    x = torch.ones((2, K), dtype=dtype)
+    x = torch.ones((2, K), dtype=BF16)
     x[0, 40] = 2.0 ** 20                        # y of about sqrt(K) 2^126 there, and beside it about 2^-20
-    w = torch.ones(K, dtype=dtype)
+    w = torch.ones(K, dtype=BF16)
     w[40] = 2.0 ** 127
     w = w.cuda()
     for group in (32, 0) if K == 64 else (0,):
@@ -61,3 +58,26 @@ def test_8bit_beyond_fp32(dtype, K):
         if group:
             y = plain.norm(x, w, 1e-6)[1][0, :32]
             assert torch.isfinite(s[0, 0]) and ((q[0, :32].double() * s[0, 0] - y).abs() <= y.abs() * (2.0 ** -4 + NORM_REL + 2.0 ** -22)).all()
+
+
+@TYPES
+@pytest.mark.parametrize("K", [700, 2100, 5003, 20000, 40000, 65536])
+def test_8bit_rows_without_a_scale_of_their_own(dtype, K):
+    """Rows of several waves that are zero, infinite or NaN, a scale a row, beside ordinary ones: many of each."""
+    P = need_gpu()
+    gen = torch.Generator().manual_seed(K)
+    T = 300 if K < 30000 else 60
+    x = torch.randn((T, K), generator=gen).to(dtype)
+    w = (1 + 0.3 * torch.randn(K, generator=gen)).to(dtype)
+    want, ws = (y[::6] for y in P.rms_norm_8bit(x.cuda(), w.cuda()))   # (as many rows: how a row is split may depend on that)
+    x[1::6] = 0
+    x[2::6, K - 1] = float("inf")
+    x[3::6, K // 3] = float("nan")
+    x[4::6] = -float("inf")
+    for _ in range(3):
+        q, s = P.rms_norm_8bit(x.cuda(), w.cuda())
+        q, s = q.float().cpu(), s.cpu()
+        assert torch.equal(q[::6], want.float().cpu()) and torch.equal(s[::6], ws.cpu()) and torch.isfinite(ws).all()
+        assert (s[1::6] == 2.0 ** -100).all() and not q[1::6].any()
+        for first in (2, 3, 4):
+            assert s[first::6].isnan().all() and q[first::6].isnan().all()

@@ -16,16 +16,17 @@ namespace w4a16 {
 
 constexpr int WIDE = 0;   // TPR: a workgroup a row
 
-// v of all threads of a row joined; 0 is neutral. Waves meet in lds, two places used in turn: who writes one has passed
-// the barrier behind which the other was written, so all have read this one.
+// v of all threads of a row joined; 0 is neutral. Waves meet in a place of lds: 0 for the sums of squares, 1 and 2 for what is the
+// largest of a row and of its result. 0 alone is used twice, with 1 between: who writes it again has passed the barrier behind
+// which 1 was written, so all have read it. (1 and 2 apart, as there is no second sum of a row that is zero or not finite.)
 template <int TPR, typename F>
-__device__ __forceinline__ float row_all(float v, float (&lds)[2][16], int turn, F f) {
+__device__ __forceinline__ float row_all(float v, float (&lds)[3][16], int place, F f) {
     constexpr int IN_WAVE = TPR == 16 ? 16 : 64;
 #pragma unroll
     for (int x = 1; x < IN_WAVE; x <<= 1) v = f(v, __shfl_xor(v, x));
     if constexpr (TPR == WIDE) {
         const int waves = blockDim.x >> 6;
-        float* const at = lds[turn & 1];
+        float* const at = lds[place];
         if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
         if (threadIdx.x < 16 && (int)threadIdx.x >= waves) at[threadIdx.x] = 0.f;
         __syncthreads();
@@ -62,7 +63,7 @@ template <typename E, bool Q8, int TPR, int VPT>
 __global__ __launch_bounds__(TPR == WIDE ? 1024 : 256) void norm_kernel(NormParams p) {
     const int per_row = TPR == WIDE ? (int)blockDim.x : TPR, RPB = TPR == WIDE ? 1 : 256 / per_row;
     constexpr bool SHORT = TPR == 16 && VPT == 1;
-    __shared__ float lds[2][16];
+    __shared__ float lds[3][16];
     const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RPB + (TPR == WIDE ? 0 : threadIdx.x / per_row);
     if (row >= (long long)p.T * p.H) return;   // (a row's threads agree)
     const int t = p.H == 1 ? (int)row : (int)((unsigned)row / (unsigned)p.H), h = p.H == 1 ? 0 : (int)row - t * p.H;
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(TPR == WIDE ? 1024 : 256) void norm_kernel(NormPara
     }
     if constexpr (Q8) {
         unsigned char* out = static_cast<unsigned char*>(p.out) + (size_t)t * p.o_st + (size_t)h * p.o_sh;
-        if (!p.group) most = row_all<TPR>(most, lds, 1, larger);
+        if (!p.group) most = row_all<TPR>(most, lds, 2, larger);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int e0 = place(i), n = p.K - e0;

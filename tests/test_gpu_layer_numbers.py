@@ -81,3 +81,15 @@ def test_8bit_rows_without_a_scale_of_their_own(dtype, K):
         assert (s[1::6] == 2.0 ** -100).all() and not q[1::6].any()
         for first in (2, 3, 4):
             assert s[first::6].isnan().all() and q[first::6].isnan().all()
+
+
+@pytest.mark.parametrize("K", [8, 300, 5000])
+@pytest.mark.parametrize("eps", [1e-3, 1.0, 2.0 ** 26, 2.0 ** 30, 1e20, 3e38])
+def test_norm_of_small_rows_under_a_large_eps(eps, K):
+    """Rows whose squares fp32 does not hold beside an eps that is all of the root: y = h / sqrt(eps), which bf16 holds."""
+    P = need_gpu()
+    gen = torch.Generator().manual_seed(K)
+    x = torch.stack([(torch.rand(K, generator=gen) + 0.4) * 2.0 ** e for e in (-60, -50, -47, -40, 0, 50, 62)]).bfloat16()
+    w = (torch.rand(K, generator=gen) + 0.5).bfloat16()
+    y = plain.norm(x, w, eps)[1]
+    rounded_once(P.rms_norm(x.cuda(), w.cuda(), eps), y, BF16, NORM_REL)

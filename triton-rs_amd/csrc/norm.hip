@@ -104,7 +104,8 @@ __global__ __launch_bounds__(TPR == WIDE ? 1024 : 256) void norm_kernel(NormPara
     sum = row_all<TPR>(sum, lds, 0, add);
     float eps = p.eps;
     // Squares that leave fp32: the row times a power of two (eps times its square), of its largest element where that
-    // is large, of 2^50 at most where there is an eps that counts beside them.
+    // is large, of 2^50 at most where there is an eps that counts beside them, less where that would take eps past fp32 (which then
+    // is all of the root).
     if (!(sum < 0x1p100f && sum > 0x1p-90f)) {
         float top = 0.f;
 #pragma unroll
@@ -112,7 +113,8 @@ __global__ __launch_bounds__(TPR == WIDE ? 1024 : 256) void norm_kernel(NormPara
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = larger(top, __builtin_fabsf(y[i][e]));
         top = row_all<TPR>(top, lds, 1, larger);
-        const int up = min(127 - (int)(__float_as_uint(top) >> 23), p.eps > 0.f ? 50 : 126);
+        const int most_up = p.eps > 0.f ? min(50, max(0, 126 - (int)(__float_as_uint(p.eps) >> 24))) : 126;
+        const int up = min(127 - (int)(__float_as_uint(top) >> 23), most_up);
         if (top > 0.f && top < INFINITY) {
             eps = __builtin_ldexpf(eps, 2 * up);
             sum = 0.f;

@@ -93,3 +93,36 @@ def test_norm_of_small_rows_under_a_large_eps(eps, K):
     w = (torch.rand(K, generator=gen) + 0.5).bfloat16()
     y = plain.norm(x, w, eps)[1]
     rounded_once(P.rms_norm(x.cuda(), w.cuda(), eps), y, BF16, NORM_REL)
+
+
+@TYPES
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("magnitude", [1.0, 1.5, -2.0, 1000.0, 3e38, 1e-3])
+def test_rope_of_the_largest_values(dtype, interleaved, magnitude):
+    """Pairs at the type's end, whose products with the magnitude pass fp32 and whose sums may be anything from 0 to beyond the
+    type: the formula's value, to the largest finite one beyond that, and never NaN."""
+    P = need_gpu()
+    T, H, D = 200, 2, 64
+    gen = torch.Generator().manual_seed(3)
+    most = torch.finfo(dtype).max
+    x = torch.where(torch.rand((T, H, D), generator=gen) < 0.5, -most, most)
+    x[:, 1] *= torch.rand((T, D), generator=gen)
+    x = x.to(dtype).clamp(-most, most)
+    positions = torch.randint(-3000, 3000, (T,), generator=gen).int()
+    r = P.Rope(D, 10000.0, interleaved=interleaved, magnitude=magnitude)
+    got = P.rope(x.cuda(), positions.cuda(), r, q_out=torch.empty_like(x.cuda())).double().cpu()
+    want, reach = plain.rotate(x.double().numpy(), positions.numpy(), r.inv_freq.cpu().numpy(), interleaved, float(np.float32(magnitude)))
+    # four fp32 roundings of |a| + |b|, and the angle's in fp64, 2^-50 of it; then one to the type, below its largest value
+    want, off = torch.from_numpy(want), torch.from_numpy(reach * (4 * 2.0 ** -24 + 3000 * 2.0 ** -50))
+    eps = torch.finfo(dtype).eps / 2
+    low, high = (want - off).clamp(-most, most), (want + off).clamp(-most, most)
+    tiny = 2.0 ** -25 if dtype == F16 else 2.0 ** -134
+    assert torch.isfinite(got).all()
+    assert (got >= low - low.abs() * eps - tiny).all() and (got <= high + high.abs() * eps + tiny).all()
+    # the same bits where rows are appended to a cache
+    cache, out = P.kv8_cache(T // 16 + 1, 1, D, 16), torch.empty_like(x.cuda())
+    k = torch.zeros((T, 1, D), dtype=dtype, device="cuda")
+    table = torch.arange(T // 16 + 1, dtype=torch.int32, device="cuda")[None]
+    P.kv8_write(k, k, cache, table, torch.tensor([T], dtype=torch.int32, device="cuda"), cu_q=torch.tensor([0, T], dtype=torch.int32, device="cuda"),
+                rope=r, positions=positions.cuda(), q=x.cuda(), q_out=out)
+    assert torch.equal(out.double().cpu(), got)

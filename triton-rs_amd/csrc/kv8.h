@@ -27,7 +27,8 @@ struct Kv8WriteParams {
     RopeRows q;                       // H = 0: none
     const int32_t* positions;         // [T], or null: a token's place in its sequence
     const double* inv_freq;           // null: no rotation
-    float magnitude;
+    float magnitude;                  // of keys,
+    Magnitude q_magnitude;            // and for queries
     int rot;
     bool interleaved;
     unsigned char* cache;

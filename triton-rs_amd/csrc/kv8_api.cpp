@@ -79,7 +79,7 @@ W4A16_API int w4a16_kv8_write(void* stream, int elem, const void* k, int32_t k_s
     Kv8WriteParams p{};
     p.k = k; p.v = v; p.k_st = k_stride_t; p.k_sh = k_stride_h; p.v_st = v_stride_t; p.v_sh = v_stride_h;
     p.q = {q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h, Hq};
-    p.positions = positions; p.inv_freq = inv_freq; p.magnitude = magnitude; p.rot = rot; p.interleaved = interleaved != 0;
+    p.positions = positions; p.inv_freq = inv_freq; p.magnitude = magnitude; p.q_magnitude = Magnitude::of(magnitude); p.rot = rot; p.interleaved = interleaved != 0;
     p.cache = static_cast<unsigned char*>(cache);
     p.table = page_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
     p.num_pages = num_pages; p.pages_per_seq = pages_per_seq; p.T = T; p.B = B; p.Hkv = Hkv;

@@ -115,10 +115,10 @@ __device__ __forceinline__ void turn_queries(const Kv8WriteParams& p, int D, int
             int position;
             if (p.positions) position = p.positions[t];
             else if (!place_of(p, t, position)) return;   // of no sequence: left as it is
-            for (int i = threadIdx.x; i < half; i += THREADS) turn[i] = angle(position, p.inv_freq[i], p.magnitude);
+            for (int i = threadIdx.x; i < half; i += THREADS) turn[i] = angle(position, p.inv_freq[i], p.q_magnitude.part);
             __syncthreads();
         }
-        if (e < all) store_turned<E, PAIRS>(v, x == o, o, turn, u, p.rot, D);
+        if (e < all) store_turned<E, PAIRS>(v, x == o, o, turn, p.q_magnitude.up, u, p.rot, D);
     }
 }
 

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <cmath>
+
 namespace w4a16 {
 
 constexpr int NORM_MAX_K = 65536;   // elements of a row: 1024 threads of 64
@@ -23,6 +25,18 @@ hipError_t launch_norm(bool bf16, const NormParams& p, hipStream_t st);
 
 constexpr int ROPE_MAX_D = 1024;
 
+// A rotation's factor as part 2^up, |part| <= 1: a pair of a type's largest values keeps its products within fp32, and what is
+// beyond the type is infinite only where 2^up takes it there.
+struct Magnitude {
+    float part;
+    int up;
+    static Magnitude of(float m) {
+        Magnitude r{m, 0};
+        if (std::fabs(m) > 1.f) r.part = std::frexp(m, &r.up);
+        return r;
+    }
+};
+
 struct RopeRows {
     const void* x;
     void* out;
@@ -32,7 +46,7 @@ struct RopeParams {
     RopeRows rows[2];         // queries, keys (H = 0: none)
     const int32_t* positions; // [T]
     const double* inv_freq;   // [rot / 2]
-    float magnitude;
+    Magnitude magnitude;
     int T, D, rot;
     bool interleaved;
 };

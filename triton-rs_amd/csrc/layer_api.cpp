@@ -117,7 +117,7 @@ W4A16_API int w4a16_rope(void* stream, int elem, const void* q, int32_t q_stride
     RopeParams p{};
     p.rows[0] = {q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h, Hq};
     p.rows[1] = {k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h, Hkv};
-    p.positions = positions; p.inv_freq = inv_freq; p.magnitude = magnitude;
+    p.positions = positions; p.inv_freq = inv_freq; p.magnitude = Magnitude::of(magnitude);
     p.T = T; p.D = D; p.rot = rot; p.interleaved = interleaved != 0;
     (void)hipGetLastError();
     const hipError_t e = launch_rope(elem == W4A16_BF16, p, static_cast<hipStream_t>(stream));

@@ -46,11 +46,11 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p, int tokens) {
         if (r0 == 0) {   // while the first rows are on their way
             for (int i = threadIdx.x; i < live * half; i += 256) {
                 const int t = i / half;
-                turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude);
+                turn[i] = angle(p.positions[t0 + t], p.inv_freq[i - t * half], p.magnitude.part);
             }
             __syncthreads();
         }
-        if (some) store_turned<E, PAIRS>(v, at.x == at.o, at.o, turn + t * half, u, p.rot, p.D);
+        if (some) store_turned<E, PAIRS>(v, at.x == at.o, at.o, turn + t * half, p.magnitude.up, u, p.rot, p.D);
     }
 }
 

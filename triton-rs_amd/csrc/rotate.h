@@ -38,12 +38,12 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float2 w) {
     a = x;
     b = y;
 }
-// the same, to the element type's largest finite value beyond that
+// the same times 2^up, to the element type's largest finite value beyond that
 template <typename E>
-__device__ __forceinline__ void rotate(float& a, float& b, float2 w) {
+__device__ __forceinline__ void rotate(float& a, float& b, float2 w, int up) {
     turn_pair(a, b, w);
-    a = saturate<E>(a);
-    b = saturate<E>(b);
+    a = saturate<E>(__builtin_ldexpf(a, up));
+    b = saturate<E>(__builtin_ldexpf(b, up));
 }
 
 // A row in units of its own order. PAIRS: unit u is elements 8 u ..; those beyond rot are copied. Halves: the first `turned` units
@@ -77,7 +77,7 @@ __device__ __forceinline__ Unit load_unit(const uint16_t* x, bool in_place, int 
 }
 // v of load_unit, to a row that is x (in_place) or overlaps none that is read
 template <typename E, bool PAIRS>
-__device__ __forceinline__ void store_turned(Unit v, bool in_place, uint16_t* o, const float2* angles, int u, int rot, int D) {
+__device__ __forceinline__ void store_turned(Unit v, bool in_place, uint16_t* o, const float2* angles, int up, int u, int rot, int D) {
     const UnitPlace p = unit_place<PAIRS>(u, rot, D, in_place);
     const int half = rot / 2;
     if (in_place && (PAIRS ? 8 * u >= rot : u >= turned_units(rot))) return;
@@ -85,7 +85,7 @@ __device__ __forceinline__ void store_turned(Unit v, bool in_place, uint16_t* o,
     to_f32<E>(v.a, f);
     if constexpr (PAIRS) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate<E>(f[2 * i], f[2 * i + 1], angles[min(4 * u + i, half - 1)]);
+        for (int i = 0; i < 4; ++i) rotate<E>(f[2 * i], f[2 * i + 1], angles[min(4 * u + i, half - 1)], up);
         const Elems8 to = from_f32<E>(f);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_turned(Unit v, bool in_place, uint16_t* o,
         float g[8];
         to_f32<E>(v.b, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rotate<E>(f[i], g[i], angles[min(p.a + i, half - 1)]);
+        for (int i = 0; i < 8; ++i) rotate<E>(f[i], g[i], angles[min(p.a + i, half - 1)], up);
         if (u < turned_units(rot)) {
             v.a = from_f32<E>(f);
             v.b = from_f32<E>(g);

@@ -850,7 +850,8 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table:
     pages that do not exist are passed over. Blocks of 16 tokens share a scale, which later rows may raise.
     max_q_len: a bound on the new tokens of a sequence (T unless given; a close one makes a smaller launch).
     rope: k is rotated first, in fp32, at positions (int32 [T]) or each token's place in its sequence, and q [T,
-    heads, D], where given, into q_out (in place unless given) in the same launch."""
+    heads, D], where given, into q_out (in place unless given) in the same launch. Rows of q outside every sequence are
+    left as they were; given positions, they are rotated too."""
     turn = (None, None, None) if rope is None else (rope.inv_freq, rope.magnitude, rope.interleaved)
     return (_calls or _load_calls()).kv8_write(k, v, cache, page_table, kv_lens, cu_q, max_q_len, *turn, positions, q, q_out)
 

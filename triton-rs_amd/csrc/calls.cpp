@@ -310,11 +310,11 @@ PyObject* kv8_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
             refuse("positions and q are for a rotation: give rope");
         }
         if (none(a[11]) && !none(a[12])) refuse("q_out without q");
-        if (T > 0 && t.B > 0) {
+        if (T > 0 && (t.B > 0 || (qr.p && positions))) {   // (without sequences queries are rotated at most)
             const int flag = elem_flag(k);
             call_on(c.device, [&](void* s) {
                 return w4a16_kv8_write(s, flag, kr.p, kr.st, kr.sh, vr.p, vr.st, vr.sh, qr.p, qr.st, qr.sh, qo.p, qo.st, qo.sh, positions, r.f, r.magnitude,
-                                       r.rot, r.interleaved, c.p, t.p, lens, cu, T, t.B, Hq, c.Hkv, c.D, c.pages, c.page, t.per, max_q);
+                                       r.rot, r.interleaved, c.p, t.p, lens, cu, T, t.B, Hq, c.Hkv, c.D, c.pages, c.page, t.B > 0 ? t.per : std::max(1, t.per), max_q);
             });
         }
         return given(a[2]);

@@ -65,8 +65,10 @@ W4A16_API int w4a16_kv8_write(void* stream, int elem, const void* k, int32_t k_s
         if (rot < 2 || rot % 2 || rot > D) return fail(W4A16_ERR_INVALID_ARG, "rot=%d: even, 2 to the head's %d dimensions", rot, D);
         if (!std::isfinite(magnitude)) return fail(W4A16_ERR_INVALID_ARG, "magnitude must be finite");
     }
-    if (T == 0 || B == 0) return W4A16_OK;
-    if (!cache || !page_table || !kv_lens) return fail(W4A16_ERR_INVALID_ARG, "null pointer argument (cache, page_table or kv_lens)");
+    // (without sequences there are queries at most, at positions of their own)
+    if (T == 0 || (B == 0 && (!q || !positions))) return W4A16_OK;
+    if (!cache || (B > 0 && (!page_table || !kv_lens)))
+        return fail(W4A16_ERR_INVALID_ARG, "null pointer argument (cache, page_table or kv_lens)");
     if (!aligned(cache, 16)) return fail(W4A16_ERR_INVALID_ARG, "cache must be 16-byte aligned");
     if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(cu_q, 4) || !aligned(positions, 4) || !aligned(inv_freq, 8))
         return fail(W4A16_ERR_INVALID_ARG, "page_table, kv_lens, cu_q and positions must be 4-byte aligned, inv_freq 8-byte");

@@ -29,3 +29,28 @@ def test_queries_at_given_positions_without_sequences(per):
     P.kv8_write(k, k, cache, table, lens, cu_q=i32([0]), rope=r, positions=pos)
     P.kv8_write(k, k, cache, table, lens)
     assert (out == 3).all() and torch.equal(cache, before)
+
+
+def test_memory_that_is_not_there():
+    """An output or workspace that cannot be had is torch's own error, so that a program that waits for it (to take a smaller
+    batch) sees it. (The process's share of the card is lowered: torch refuses before it asks the device.)"""
+    P = need_gpu()
+    one = torch.zeros((1, 1, 256), dtype=F16, device="cuda")
+    x, w = torch.zeros((1, 65536), dtype=F16, device="cuda"), torch.ones(65536, dtype=F16, device="cuda")
+    c4, c8, heads4, heads8 = (f(1, n, 256, 16) for n in (1, 128) for f in (P.kv4_cache, P.kv8_cache))
+    rows_ = x.expand(1 << 17, 65536)                        # 16 GiB of results, 8 in 8 bits
+    q = one.expand(1 << 22, 8, 256)                         # 16 GiB of results
+    many = one.expand(512, 1024, 256)                       # 1 GiB of workspace
+    table, lens = i32([[0]]), i32([1])
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (256 << 20)) / total)
+    try:
+        for call in (lambda: P.rms_norm(rows_, w), lambda: P.rms_norm_8bit(rows_, w),
+                     lambda: P.kv4_attention(q, c4, table, lens, cu_q=i32([0, 1]), max_q_len=1), lambda: P.kv8_attention(q, c8, table, lens, cu_q=i32([0, 1]), max_q_len=1),
+                     lambda: P.kv4_attention_workspace(many, heads4, 64, 8, 1 << 16), lambda: P.kv8_attention_workspace(many, heads8, 64, 8, 1 << 16)):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert not P.rms_norm(x, w).any()

@@ -5,6 +5,7 @@
 //
 // A module for CPython (built by build.py beside the library, imported by __init__.py): functions of positional
 // arguments, called by the functions of the same names there, which have the documentation.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -150,15 +151,15 @@ PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
         PyErr_Format(PyExc_TypeError, "%zd arguments, not %zd", want, n);
         return nullptr;
     }
+    HANDLE_TH_ERRORS   // torch's exceptions as torch's own functions raise them (memory that is not there: torch.OutOfMemoryError)
     try {
         return f();
     } catch (const Refused& e) {
         PyErr_SetString(invalid_argument, e.what.c_str());
     } catch (const PythonError&) {
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
     }
     return nullptr;
+    END_HANDLE_TH_ERRORS
 }
 PyObject* given(PyObject* o) {
     Py_INCREF(o);

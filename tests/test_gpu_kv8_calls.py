@@ -54,3 +54,12 @@ def test_memory_that_is_not_there():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert not P.rms_norm(x, w).any()
+
+
+def test_workspace_of_any_queries():
+    """Only the number of rows and heads counts: queries of either side of the bus, numpy's, or without a head dimension."""
+    P = need_gpu()
+    for cache, workspace in ((P.kv4_cache(2, 2, 64, 16), P.kv4_attention_workspace), (P.kv8_cache(2, 2, 64, 16), P.kv8_attention_workspace)):
+        want = workspace(torch.zeros((6, 4, 64), dtype=F16, device="cuda"), cache, 2, 3, 5000).numel()
+        for q in (torch.zeros((6, 4)), np.zeros((6, 4, 64)), torch.zeros((6, 4, 1, 64), device="cuda")):
+            assert workspace(q, cache, 2, 3, 5000).numel() == want

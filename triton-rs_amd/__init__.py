@@ -798,7 +798,7 @@ def kv4_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int,
     max_q_len and this max_kv_len or a smaller one. A call of another shape may need more, a smaller
     one too: a workspace for several is as large as the largest of theirs. Calls that may overlap in
     time need one each."""
-    return (_calls or _load_calls()).attention_workspace(4, q, cache, num_seqs, max_q_len, max_kv_len)
+    return (_calls or _load_calls()).attention_workspace(4, *q.shape[:2], cache, num_seqs, max_q_len, max_kv_len)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -873,7 +873,7 @@ def kv8_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
 def kv8_attention_workspace(q: torch.Tensor, cache: torch.Tensor, num_seqs: int, max_q_len: int,
                             max_kv_len: int) -> torch.Tensor:
     """A workspace for kv8_attention calls, as kv4_attention_workspace makes it."""
-    return (_calls or _load_calls()).attention_workspace(8, q, cache, num_seqs, max_q_len, max_kv_len)
+    return (_calls or _load_calls()).attention_workspace(8, *q.shape[:2], cache, num_seqs, max_q_len, max_kv_len)
 
 
 def kv8_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,

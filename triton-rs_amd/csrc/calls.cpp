@@ -366,14 +366,12 @@ at::Tensor new_workspace(const Format& f, const Cache& c, at::TensorOptions opti
 }
 static_assert(W4A16_KV4_COUNTER_BYTES == W4A16_KV8_COUNTER_BYTES, "one area of counters");
 
-// (bits, q, cache, num_seqs, max_q_len, max_kv_len)
+// (bits, rows of q, its heads, cache, num_seqs, max_q_len, max_kv_len)
 PyObject* attention_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 6, [&]() -> PyObject* {
+    return guarded(n, 7, [&]() -> PyObject* {
         const Format f = format_of(a[0]);
-        const at::Tensor& q = tensor(a[1], "q");
-        const Cache c = cache_of(a[2], f.bits);
-        if (q.dim() != 3) refuse("q must be [T, heads, D], not %s", text(q.sizes()).c_str());
-        return THPVariable_Wrap(new_workspace(f, c, tensor(a[2], "cache").options(), q.size(0), integer(a[3]), q.size(1), integer(a[4]), integer(a[5])));
+        const Cache c = cache_of(a[3], f.bits);
+        return THPVariable_Wrap(new_workspace(f, c, tensor(a[3], "cache").options(), integer(a[1]), integer(a[4]), integer(a[2]), integer(a[5]), integer(a[6])));
     });
 }
 

@@ -63,3 +63,16 @@ def test_workspace_of_any_queries():
         want = workspace(torch.zeros((6, 4, 64), dtype=F16, device="cuda"), cache, 2, 3, 5000).numel()
         for q in (torch.zeros((6, 4)), np.zeros((6, 4, 64)), torch.zeros((6, 4, 1, 64), device="cuda")):
             assert workspace(q, cache, 2, 3, 5000).numel() == want
+
+
+def test_sizes_below_32_bits():
+    """Python's integers beyond either end of 32 bits are refused, not cut."""
+    P = need_gpu()
+    q, table, lens = torch.zeros((1, 2, 64), dtype=F16, device="cuda"), i32([[0, 1]]), i32([1])
+    for cache, call, workspace in ((P.kv4_cache(2, 2, 64, 16), P.kv4_attention, P.kv4_attention_workspace), (P.kv8_cache(2, 2, 64, 16), P.kv8_attention, P.kv8_attention_workspace)):
+        for over in (dict(max_q_len=1 - 2 ** 32), dict(max_kv_len=16 - 2 ** 32), dict(window=-2 ** 32), dict(window=8 - 2 ** 32)):
+            with pytest.raises(P.InvalidArgument):
+                call(q, cache, table, lens, **over)
+        for a in ((1 - 2 ** 32, 1, 32), (1, 1 - 2 ** 32, 32), (1, 1, 32 - 2 ** 32)):
+            with pytest.raises(P.InvalidArgument):
+                workspace(q, cache, *a)

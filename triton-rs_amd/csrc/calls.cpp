@@ -352,7 +352,7 @@ Format format_of(PyObject* o) {
                            : Format{8, w4a16_kv8_attention_workspace_size, w4a16_kv8_attention};
 }
 at::Tensor new_workspace(const Format& f, const Cache& c, at::TensorOptions options, int64_t T, int64_t B, int64_t Hq, int64_t max_q, int64_t max_kv) {
-    if (std::max({T, B, Hq, max_q, max_kv}) > INT32_MAX)
+    if (std::max({T, B, Hq, max_q, max_kv}) > INT32_MAX || std::min({T, B, Hq, max_q, max_kv}) < INT32_MIN)
         refuse("sizes are 32-bit (%lld, %lld, %lld, %lld, %lld)", (long long)T, (long long)B, (long long)Hq, (long long)max_q, (long long)max_kv);
     const size_t need = f.workspace((int32_t)T, (int32_t)B, (int32_t)Hq, c.Hkv, c.D, (int32_t)max_q, (int32_t)max_kv);
     if (!need) {
@@ -395,7 +395,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             refuse("without cu_q every sequence has one query (%lld queries, %d sequences)", (long long)T, t.B);
         const int64_t max_q = none(a[6]) ? (cu ? std::max<int64_t>(1, T) : 1) : integer(a[6]);
         const int64_t max_kv = none(a[7]) ? (int64_t)t.per * c.page : integer(a[7]), window = integer(a[10]);
-        if (max_q > INT32_MAX || max_kv > INT32_MAX || window > INT32_MAX)
+        if (std::max({max_q, max_kv, window}) > INT32_MAX || std::min({max_q, max_kv, window}) < INT32_MIN)
             refuse("max_q_len, max_kv_len and window are 32-bit (%lld, %lld, %lld)", (long long)max_q, (long long)max_kv, (long long)window);
         const float scale = none(a[8]) ? (float)(1.0 / std::sqrt((double)c.D)) : (float)number(a[8]);
         const bool causal = truth(a[9]);
@@ -418,7 +418,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             const int flag = elem_flag(q);
             call_on(c.device, [&](void* s) {
                 return f.attention(s, flag, qr.p, qr.st, qr.sh, c.p, t.p, lens, cu, o.p, o.st, o.sh, lse, (int32_t)T, t.B, (int32_t)Hq, c.Hkv, c.D, c.pages,
-                                   c.page, t.per, (int32_t)max_q, (int32_t)max_kv, scale, causal, (int32_t)std::max<int64_t>(window, INT32_MIN), wp, bytes);
+                                   c.page, t.per, (int32_t)max_q, (int32_t)max_kv, scale, causal, (int32_t)window, wp, bytes);
             });
         }
         return none(a[11]) ? THPVariable_Wrap(made) : given(a[11]);

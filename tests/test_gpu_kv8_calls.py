@@ -76,3 +76,12 @@ def test_sizes_below_32_bits():
         for a in ((1 - 2 ** 32, 1, 32), (1, 1 - 2 ** 32, 32), (1, 1, 32 - 2 ** 32)):
             with pytest.raises(P.InvalidArgument):
                 workspace(q, cache, *a)
+
+
+def test_read_from_what_is_no_cache():
+    P = need_gpu()
+    slots = i32([0])
+    for bad in (torch.zeros((1, 1, 1, 8), dtype=torch.uint8, device="cuda"), torch.zeros((1, 1, 1, 100), dtype=torch.uint8, device="cuda"),
+                torch.zeros((1, 1, 1, 2064), dtype=torch.uint8), torch.zeros((1, 1, 2064), dtype=torch.uint8, device="cuda")):
+        with pytest.raises(P.InvalidArgument):
+            P.kv8_read(bad, slots)

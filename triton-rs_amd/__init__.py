@@ -865,7 +865,8 @@ def kv8_read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, k_ou
     if k_out is None:
         if not isinstance(cache, _Tensor) or not isinstance(slots, _Tensor) or cache.dim() != 4:
             raise InvalidArgument("cache and slots must be tensors, cache as kv8_cache makes it")
-        k_out, v_out = torch.zeros((2, slots.numel(), cache.shape[1], (cache.shape[3] - 16) // 32), dtype=dtype, device=cache.device)
+        head_dim = max(0, (cache.shape[3] - 16) // 32)   # (0: no cache, which the call says)
+        k_out, v_out = torch.zeros((2, slots.numel(), cache.shape[1], head_dim), dtype=dtype, device=cache.device)
     (_calls or _load_calls()).kv8_read(cache, slots, k_out, v_out)
     return k_out, v_out
 

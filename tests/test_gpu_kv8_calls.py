@@ -85,3 +85,84 @@ def test_read_from_what_is_no_cache():
                 torch.zeros((1, 1, 1, 2064), dtype=torch.uint8), torch.zeros((1, 1, 2064), dtype=torch.uint8, device="cuda")):
         with pytest.raises(P.InvalidArgument):
             P.kv8_read(bad, slots)
+
+
+# ------------------------------------------------------------------ gradients: there are none
+
+def calls_that_write(P):
+    """name -> (the call, tensors that it writes)"""
+    x, res, w = (torch.randn((4, 128), device="cuda").half() for _ in range(3))
+    w = w[0].contiguous()
+    q, k, v = (torch.randn((4, 2, 64), device="cuda").half() for _ in range(3))
+    cache, table, lens, r = P.kv8_cache(4, 2, 64, 16), i32([[0], [1], [2], [3]]), i32([1, 2, 3, 4]), P.Rope(64)
+    out, out8, scales = torch.empty_like(x), torch.empty((4, 128), dtype=P.E4M3, device="cuda"), torch.empty((4, 4), device="cuda")
+    total, qo, ko, lse = torch.empty_like(x), torch.empty_like(q), torch.empty_like(k), torch.empty((4, 2), device="cuda")
+    c4 = P.kv4_cache(4, 2, 64, 16)
+    return {
+        "norm": (lambda: P.rms_norm(x, w, residual=res, out=out), [res, out]),
+        "norm beside": (lambda: P.rms_norm(x, w, residual=res, residual_out=total), [total]),
+        "8 bits": (lambda: P.rms_norm_8bit(x, w, group=32, residual=res, out=out8, scales=scales), [res, out8, scales]),
+        "rope": (lambda: P.rope(q, lens, r, k=k), [q, k]),
+        "rope beside": (lambda: P.rope(q, lens, r, k=k, q_out=qo, k_out=ko), [qo, ko]),
+        "write": (lambda: P.kv8_write(k, v, cache, table, lens, rope=r, q=q), [cache, q]),
+        "write beside": (lambda: P.kv8_write(k, v, cache, table, lens, rope=r, q=q, q_out=qo), [cache, qo]),
+        "read": (lambda: P.kv8_read(cache, i32([0, 1, 2, 3]), k_out=ko, v_out=qo), [ko, qo]),
+        "attention": (lambda: P.kv8_attention(q, cache, table, lens, out=qo, lse=lse), [qo, lse]),
+        "4 bits": (lambda: P.kv4_attention(q, c4, table, lens, out=qo, lse=lse), [qo, lse]),
+    }, (x, res, w, q, k, v)
+
+
+def test_written_tensors_are_seen_as_changed():
+    """A backward pass that has saved a tensor which a call then writes raises torch's error; it does not run on the new values."""
+    P = need_gpu()
+    calls, _ = calls_that_write(P)
+    for name, (call, written) in calls.items():
+        for i, t in enumerate(written):
+            if not t.dtype.is_floating_point or t.dtype == P.E4M3:
+                before = t._version
+                call()
+                assert t._version > before, (name, i)
+                continue
+            leaf = torch.ones(t.shape, dtype=t.dtype, device="cuda", requires_grad=True)
+            y = (leaf * t.detach()).sum()     # saves t
+            call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+
+
+def test_inference_tensors_are_written_anywhere():
+    P = need_gpu()
+    with torch.inference_mode():
+        calls, _ = calls_that_write(P)
+        for call, _ in calls.values():
+            call()
+    for call, _ in calls.values():
+        call()
+
+
+def test_in_place_where_gradients_flow():
+    """The operators have no backward pass. In place on a tensor of a graph the rotation or the sum would be missing from the
+    gradients behind it, without an error: refused, as long as gradients are recorded. Out of place a result has no graph."""
+    P = need_gpu()
+    calls, (x, res, w, q, k, v) = calls_that_write(P)
+    for t in (res, q, k):
+        t.requires_grad_()
+    for name in ("norm", "8 bits", "rope", "write"):
+        with pytest.raises(P.InvalidArgument, match="no backward"):
+            calls[name][0]()
+        with torch.no_grad():
+            calls[name][0]()
+    for name in ("norm beside", "rope beside", "write beside", "attention", "4 bits"):
+        calls[name][0]()
+    for t in (x, w, v):
+        t.requires_grad_()
+    with torch.no_grad():
+        for t in (res, q, k):
+            t.requires_grad_(False)
+    assert not P.rms_norm(x, w, residual=res).requires_grad
+    for name in calls:
+        calls[name][0]()
+    # a tensor that is no leaf, as a projection's result is
+    h = (x[:, None] * 1.0).view(4, 2, 64)
+    with pytest.raises(P.InvalidArgument, match="no backward"):
+        P.rope(h, i32([0, 1, 2, 3]), P.Rope(64))

@@ -660,6 +660,8 @@ def _call_on(index: int, fn, *args) -> None:
 
 
 # ------------------------------------------------------------------ norm and rotary positions
+# (Neither these nor the caches' calls have a backward pass: results carry no graph, and to write to a tensor that requires grad while
+# gradients are recorded is refused.)
 
 E4M3 = torch.float8_e4m3fn
 

@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <cstdarg>
@@ -70,6 +71,22 @@ const at::Tensor& elements(PyObject* o, const char* name) {
     if (!is_elem(t.scalar_type())) refuse("%s has dtype %s, expected float16 or bfloat16", name, toString(t.scalar_type()));
     return t;
 }
+
+// Tensors that a call writes. There is no backward pass: written in place, a tensor of a graph that is being recorded would go
+// on without what was done to it. And whoever has saved one for a backward pass of its own is told by its version.
+struct Written {
+    const at::Tensor* t[4];
+    int n = 0;
+    void add(const at::Tensor& x, const char* name, bool any = false) {   // any: gradients or not
+        if (!any && x.requires_grad() && at::GradMode::is_enabled())
+            refuse("%s requires grad and would be written, and there is no backward pass: call under torch.no_grad(), or give a tensor of its own to write to", name);
+        t[n++] = &x;
+    }
+    void done() const {
+        for (int i = 0; i < n; ++i)
+            if (!t[i]->is_inference()) t[i]->unsafeGetTensorImpl()->bump_version();
+    }
+};
 
 int elem_flag(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? W4A16_BF16 : 0; }
 
@@ -179,9 +196,12 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (w.dim() != 1 || w.size(0) != K || !w.is_contiguous()) refuse("weight must be a contiguous [%d] tensor", K);
         const float eps = (float)number(a[2]);
         Rows r = NO_ROWS, ro = NO_ROWS;
+        Written written;
         if (!none(a[3])) {
-            r = rows(on(a[3], "residual", device, type), "residual", &shape, true);
-            ro = none(a[4]) ? r : rows(on(a[4], "residual_out", device, type), "residual_out", &shape, true);
+            const at::Tensor& residual = on(a[3], "residual", device, type);
+            r = ro = rows(residual, "residual", &shape, true);
+            if (!none(a[4])) ro = rows(on(a[4], "residual_out", device, type), "residual_out", &shape, true);
+            written.add(none(a[4]) ? residual : THPVariable_Unpack(a[4]), none(a[4]) ? "residual" : "residual_out");
         } else if (!none(a[4])) {
             refuse("residual_out without residual");
         }
@@ -191,12 +211,14 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (none(a[5])) made = at::empty(shape, x.options().dtype(out_type));
         const at::Tensor& out = none(a[5]) ? made : on(a[5], "out", device, out_type);
         const Rows o = rows(out, "out", &shape, true);
+        if (!none(a[5])) written.add(out, "out");
         const void* weight = w.data_ptr();
         const int flag = elem_flag(x);
         if (!bytes) {
             call_on(device, [&](void* s) {
                 return w4a16_rms_norm(s, flag, xr.p, xr.st, xr.sh, r.p, r.st, r.sh, ro.p, ro.st, ro.sh, weight, o.p, o.st, o.sh, T, H, K, eps);
             });
+            written.done();
             return none(a[5]) ? THPVariable_Wrap(made) : given(a[5]);
         }
         const int64_t group = integer(a[7]);
@@ -206,10 +228,12 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (none(a[6])) made_scales = at::empty(want, x.options().dtype(at::kFloat));
         const at::Tensor& scales = none(a[6]) ? made_scales : on(a[6], "scales", device, at::kFloat);
         if (scales.sizes() != at::IntArrayRef(want) || !scales.is_contiguous()) refuse("scales must be a contiguous %s tensor", text(want).c_str());
+        if (!none(a[6])) written.add(scales, "scales");
         float* sp = scales.data_ptr<float>();
         call_on(device, [&](void* s) {
             return w4a16_rms_norm_8bit(s, flag, xr.p, xr.st, xr.sh, r.p, r.st, r.sh, ro.p, ro.st, ro.sh, weight, o.p, o.st, o.sh, sp, T, H, K, (int32_t)group, eps);
         });
+        written.done();
         PyObject *po = none(a[5]) ? THPVariable_Wrap(made) : given(a[5]), *ps = none(a[6]) ? THPVariable_Wrap(made_scales) : given(a[6]);
         PyObject* both = po && ps ? PyTuple_Pack(2, po, ps) : nullptr;
         Py_XDECREF(po);
@@ -233,7 +257,10 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const auto type = q.scalar_type();
         const Rows qr = rows(q, "q", nullptr);
         const at::IntArrayRef shape = q.sizes();
-        const Rows qo = none(a[6]) ? qr : rows(on(a[6], "q_out", device, type), "q_out", &shape);
+        const at::Tensor& q_out = none(a[6]) ? q : on(a[6], "q_out", device, type);
+        const Rows qo = rows(q_out, "q_out", &shape);
+        Written written;
+        written.add(q_out, none(a[6]) ? "q" : "q_out");
         const int32_t T = (int32_t)shape[0], Hq = (int32_t)shape[1], D = (int32_t)shape[2];
         const int32_t* positions = indices(a[1], "positions", device, T);
         const Turn t = turn(a[2], a[3], a[4], device);
@@ -245,7 +272,9 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
             const at::IntArrayRef ks(want, 3);
             kr = rows(k, "k", &ks);
             Hkv = (int32_t)want[1];
-            ko = none(a[7]) ? kr : rows(on(a[7], "k_out", device, type), "k_out", &ks);
+            const at::Tensor& k_out = none(a[7]) ? k : on(a[7], "k_out", device, type);
+            ko = rows(k_out, "k_out", &ks);
+            written.add(k_out, none(a[7]) ? "k" : "k_out");
         } else if (!none(a[7])) {
             refuse("k_out without k");
         }
@@ -254,6 +283,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return w4a16_rope(s, flag, qr.p, qr.st, qr.sh, qo.p, qo.st, qo.sh, kr.p, kr.st, kr.sh, ko.p, ko.st, ko.sh, positions, t.f, t.magnitude, T, Hq,
                               Hkv, D, t.rot, t.interleaved);
         });
+        written.done();
         Py_RETURN_NONE;
     });
 }
@@ -296,6 +326,8 @@ PyObject* kv8_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t* positions = nullptr;
         Rows qr = NO_ROWS, qo = NO_ROWS;
         int32_t Hq = 0;
+        Written written;
+        written.add(THPVariable_Unpack(a[2]), "cache");
         if (!none(a[7])) {
             r = turn(a[7], a[8], a[9], c.device);
             if (!none(a[10])) positions = indices(a[10], "positions", c.device, T);
@@ -305,7 +337,9 @@ PyObject* kv8_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 const at::IntArrayRef qshape(qs, 3);
                 qr = rows(q, "q", &qshape);
                 Hq = (int32_t)qs[1];
-                qo = none(a[12]) ? qr : rows(on(a[12], "q_out", c.device, type), "q_out", &qshape);
+                const at::Tensor& q_out = none(a[12]) ? q : on(a[12], "q_out", c.device, type);
+                qo = rows(q_out, "q_out", &qshape);
+                written.add(q_out, none(a[12]) ? "q" : "q_out");
             }
         } else if (!none(a[10]) || !none(a[11])) {
             refuse("positions and q are for a rotation: give rope");
@@ -317,6 +351,7 @@ PyObject* kv8_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 return w4a16_kv8_write(s, flag, kr.p, kr.st, kr.sh, vr.p, vr.st, vr.sh, qr.p, qr.st, qr.sh, qo.p, qo.st, qo.sh, positions, r.f, r.magnitude,
                                        r.rot, r.interleaved, c.p, t.p, lens, cu, T, t.B, Hq, c.Hkv, c.D, c.pages, c.page, t.B > 0 ? t.per : std::max(1, t.per), max_q);
             });
+            written.done();
         }
         return given(a[2]);
     });
@@ -332,12 +367,17 @@ PyObject* kv8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::IntArrayRef shape(want, 3);
         const at::Tensor& k = elements(a[2], "k_out");
         on(a[2], "k_out", c.device, k.scalar_type());
-        const Rows kr = rows(k, "k_out", &shape), vr = rows(on(a[3], "v_out", c.device, k.scalar_type()), "v_out", &shape);
+        const at::Tensor& v = on(a[3], "v_out", c.device, k.scalar_type());
+        const Rows kr = rows(k, "k_out", &shape), vr = rows(v, "v_out", &shape);
+        Written written;
+        written.add(k, "k_out");
+        written.add(v, "v_out");
         const int32_t* sp = slots.data_ptr<int32_t>();
         const int flag = elem_flag(k);
         call_on(c.device, [&](void* s) {
             return w4a16_kv8_read(s, flag, c.p, sp, kr.p, kr.st, kr.sh, vr.p, vr.st, vr.sh, c.pages, (int32_t)want[0], c.Hkv, c.D, c.page);
         });
+        written.done();
         Py_RETURN_NONE;
     });
 }
@@ -403,10 +443,13 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (none(a[11])) made = cu ? at::zeros(shape, q.options()) : at::empty(shape, q.options());
         const at::Tensor& out = none(a[11]) ? made : on(a[11], "out", c.device, type);
         const Rows o = rows(out, "out", &shape);
+        Written written;
+        if (!none(a[11])) written.add(out, "out", f.bits == 4);   // (the 4-bit cache's calls have always taken one that requires grad)
         float* lse = nullptr;
         if (!none(a[12])) {
             const at::Tensor& l = on(a[12], "lse", c.device, at::kFloat);
             if (l.dim() != 2 || l.size(0) != T || l.size(1) != Hq || !l.is_contiguous()) refuse("lse must be a contiguous [%lld, %lld] tensor", (long long)T, (long long)Hq);
+            written.add(l, "lse", f.bits == 4);
             lse = l.data_ptr<float>();
         }
         if (T > 0 && t.B > 0) {
@@ -420,6 +463,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 return f.attention(s, flag, qr.p, qr.st, qr.sh, c.p, t.p, lens, cu, o.p, o.st, o.sh, lse, (int32_t)T, t.B, (int32_t)Hq, c.Hkv, c.D, c.pages,
                                    c.page, t.per, (int32_t)max_q, (int32_t)max_kv, scale, causal, (int32_t)window, wp, bytes);
             });
+            written.done();
         }
         return none(a[11]) ? THPVariable_Wrap(made) : given(a[11]);
     });

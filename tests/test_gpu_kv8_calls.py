@@ -31,6 +31,28 @@ def test_queries_at_given_positions_without_sequences(per):
     assert (out == 3).all() and torch.equal(cache, before)
 
 
+@TYPES
+@pytest.mark.parametrize("nq,L", [(3, 33), (5, 97), (5, 1601), (90, 129), (150, 401), (80, 2497)])
+def test_a_largest_row_that_others_do_not_see(dtype, nq, L):
+    """A block whose one token only the last query sees, its key, then its value, at the type's end: finite, so it counts for the
+    block's scale and reaches every product of its step, yet moves no bit of the other queries' results.
+    (The last query's own scale q . k may be more than fp32 holds.)"""
+    P = need_gpu()
+    assert L % 16 == 1
+    b = Batch8(P, [nq], [L], 4, 2, 64, 16, dtype, seed=6)
+    last = [torch.from_numpy(x[0][-1:]).to(dtype) for x in (b.k, b.v)]
+    out, lse = b.gpu(P)
+    most = torch.finfo(dtype).max
+    sign = torch.where(torch.rand((1, 2, 64), generator=torch.Generator().manual_seed(1)) < 0.5, -most, most).to(dtype)
+    for key, value in ((sign, last[1]), (last[0], sign), (sign, -sign)):
+        b.put(P, 0, L - 1, key, value)
+        out2, lse2 = b.gpu(P)
+        assert torch.equal(out[:-1], out2[:-1]) and torch.equal(lse[:-1], lse2[:-1])
+    b.put(P, 0, L - 1, *last)
+    out2, lse2 = b.gpu(P)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
 def test_memory_that_is_not_there():
     """An output or workspace that cannot be had is torch's own error, so that a program that waits for it (to take a smaller
     batch) sees it. (The process's share of the card is lowered: torch refuses before it asks the device.)"""

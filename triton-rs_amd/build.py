@@ -4,7 +4,10 @@ Outputs (next to this file):
   libw4a16.so         C ABI of include/w4a16.h (kernels embedded as a gfx950 fat binary)
   w4a16_typed.hsaco   code object with the reference-named kernels, for hiprt_module_load
   w4a16_typed.json    launch metadata for that code object
-  _calls.so           CPython module of the calls made once a layer and step (csrc/calls.cpp)
+  _calls.so           CPython module of the calls made once a layer and step (csrc/calls.cpp), bound to this
+                      interpreter and its torch; left out, with a message, where torch cannot be imported
+
+All but _calls.so need hipcc alone.
 
 Every HIP compile line carries `-Xclang -target-feature -Xclang -packed-fp32-ops`, which
 turns off packed-fp32 instruction selection on this target.
@@ -72,6 +75,14 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _has_torch() -> bool:
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False
+    return True
+
+
 def _compile_calls() -> str:
     """calls.cpp with torch's headers: the host compiler, as torch's own extensions are built."""
     import sysconfig
@@ -100,7 +111,7 @@ def build(verbose: bool = True) -> str:
         if f.endswith(".o") and os.path.join(BUILD, f) not in map(_obj, SOURCES):
             os.remove(os.path.join(BUILD, f))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        fut_calls = ex.submit(_compile_calls)
+        fut_calls = ex.submit(_compile_calls) if _has_torch() else None
         objs = list(ex.map(_compile, SOURCES))
         fut_hsaco = ex.submit(_run, [HIPCC, "-x", "hip", f"--offload-arch={ARCH}", *COMMON,
                                      "--genco", "--no-gpu-bundle-output", os.path.join(CSRC, "typed_module.hip"),
@@ -109,7 +120,6 @@ def build(verbose: bool = True) -> str:
     os.replace(HSACO + ".tmp", HSACO)
     _run([HIPCC, "-shared", "-fPIC", *objs, "-o", LIB + ".tmp"])
     os.replace(LIB + ".tmp", LIB)
-    _link_calls(fut_calls.result())
     meta = {
         "kernels": [
             {"name": name, "num_warps": 8, "threads_per_block": 256, "warp_size": 64,
@@ -123,15 +133,31 @@ def build(verbose: bool = True) -> str:
     with open(META, "w") as f:
         json.dump(meta, f, indent=2)
     if verbose:
-        print(f"built {LIB}, {HSACO} and {CALLS}")
+        print(f"built {LIB} and {HSACO}")
+    # the module last: what a program in C or Rust takes is whole without it
+    try:
+        if fut_calls is None:
+            print(f"{CALLS} is not built: torch cannot be imported by {sys.executable}; only the Python package needs it")
+            _remove(CALLS)
+        else:
+            _link_calls(fut_calls.result())
+            if verbose:
+                print(f"built {CALLS}")
+    except Exception:
+        _remove(CALLS)   # (an older one is of another library than the one beside it)
+        raise
     return LIB
+
+
+def _remove(path: str) -> None:
+    if os.path.exists(path):
+        os.remove(path)
 
 
 def clean() -> None:
     shutil.rmtree(BUILD, ignore_errors=True)
     for p in (LIB, HSACO, META, CALLS):
-        if os.path.exists(p):
-            os.remove(p)
+        _remove(p)
 
 
 if __name__ == "__main__":

@@ -496,11 +496,14 @@ W4A16_API int w4a16_kv4_attention(void* stream, int elem, const void* q, int32_t
  * 16 r + 4 e + i); from 32 D two fp32 scales, of the keys and of the values, powers of two; then a 32-bit word whose bit t
  * (16 + t) says that token t's keys (values) are not finite, and four bytes of zeros. A number n stands for n * scale.
  *
- * A block's scale is the smallest 2^e, e >= -60, of which 448 are no less than the largest magnitude that it holds;
- * x is held as x / scale rounded to nearest even. A row with an infinity or NaN is NaN throughout (and
- * does not count for the scale). Tokens are appended: a block that holds tokens of the sequence already keeps its
- * scale, or raises it to what the new rows need; the older numbers are then rounded at the new one, which leaves
- * them as they were except below 2^-6 scales. */
+ * A block's scale is the smallest 2^e, e >= -60, of which 448 are no less than the largest magnitude that was written to it
+ * since its first token was; x is held as x / scale rounded to nearest even. A row with an infinity or NaN is NaN
+ * throughout (and does not count for the scale). Tokens are appended: a block that holds tokens of the sequence already
+ * keeps its scale, or raises it to what the new rows need; the older numbers are then rounded at the new one, which
+ * leaves them as they were except below 2^-6 scales. That is not undone where a sequence goes back, as over drafts that
+ * were not accepted, and other tokens take their place: the block that they shared with older ones keeps a scale that they
+ * raised, under which the older numbers stay as they were rounded and newer ones are held at up to that much coarser steps
+ * below 2^-6 of it (a number above has its 2^-4 at any scale), until the block's first token is written anew. */
 
 /* Bytes of a cache (0: not supported). A cache needs no initialisation. */
 W4A16_API size_t w4a16_kv8_cache_bytes(int32_t num_pages, int32_t Hkv, int32_t D, int32_t page_size);

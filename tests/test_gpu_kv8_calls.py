@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import BF16, F16, need_gpu, rows
+from test_gpu_kv4 import F16, need_gpu, rows
 from test_gpu_kv8 import TYPES, Batch8, i32
 
 pytestmark = pytest.mark.gpu
@@ -107,6 +107,34 @@ def test_read_from_what_is_no_cache():
                 torch.zeros((1, 1, 1, 2064), dtype=torch.uint8), torch.zeros((1, 1, 2064), dtype=torch.uint8, device="cuda")):
         with pytest.raises(P.InvalidArgument):
             P.kv8_read(bad, slots)
+
+
+@TYPES
+def test_scale_stays_behind_drafts(dtype):
+    """A draft that raised its block's scale and is not accepted: the older rows stay as they were rounded for it, and what takes its
+    place is held at that scale; neither is further from its row than half a step there, 2^-4 of a number or 2^-10 scales."""
+    P = need_gpu()
+    H, D = 2, 64
+    gen = torch.Generator().manual_seed(12)
+    table, slots = i32([[0]]), i32(range(16))
+    k = [rows(gen, n, H, D, dtype) for n in (5, 3, 2)]
+    k[1] = (k[1].float() * 4096).to(dtype)
+    cache = P.kv8_cache(1, H, D, 16)
+    scales = []
+    for n, x in zip((5, 8, 7), k):
+        P.kv8_write(x.cuda(), x.cuda(), cache, table, i32([n]), cu_q=i32([0, len(x)]))
+        scales.append(cache[0, :, 0, 32 * D:32 * D + 8].contiguous().view(torch.float32).cpu())
+    assert (scales[1] > 256 * scales[0]).all() and torch.equal(scales[1], scales[2])
+    want = torch.cat((k[0], k[2])).double()
+    for which, got in enumerate(P.kv8_read(cache, slots, dtype)):
+        s = scales[2][:, which].double()[:, None]
+        err = (got[:7].double().cpu() - want).abs()
+        # (the older rows twice: at their own scale, then at this one)
+        step = torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10)
+        assert (err[5:] <= step[5:]).all() and (err[:5] <= step[:5] * (2 + 2.0 ** -4)).all()
+        assert (err > want.abs() * 2.0 ** -4).any()      # as said: coarser
+    P.kv8_write(k[0].cuda(), k[0].cuda(), cache, table, i32([5]), cu_q=i32([0, 5]))
+    assert torch.equal(cache[0, :, 0, 32 * D:32 * D + 8].contiguous().view(torch.float32).cpu(), scales[0])
 
 
 # ------------------------------------------------------------------ gradients: there are none

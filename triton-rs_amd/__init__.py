@@ -849,7 +849,8 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table:
     Rows cu_q[b] .. cu_q[b + 1] (int32 [B + 1]; None: one row each, T = B) are sequence b's newest tokens, the
     last of them at token kv_lens[b] - 1 (int32 [B]; lengths with the new tokens) of pages page_table[b] (int32
     [B, pages per sequence]). Rows outside every sequence (padding behind cu_q[B]), tokens beyond the table and
-    pages that do not exist are passed over. Blocks of 16 tokens share a scale, which later rows may raise.
+    pages that do not exist are passed over. Blocks of 16 tokens share a scale, which later rows may raise: also drafts that
+    are then not accepted (the sequence goes back, and other tokens are written in their place) do so for good.
     max_q_len: a bound on the new tokens of a sequence (T unless given; a close one makes a smaller launch).
     rope: k is rotated first, in fp32, at positions (int32 [T]) or each token's place in its sequence, and q [T,
     heads, D], where given, into q_out (in place unless given) in the same launch. Rows of q outside every sequence are

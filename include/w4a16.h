@@ -356,7 +356,7 @@ W4A16_API int w4a16_fused_moe_prepared(void* stream, const void* x, const float*
  * must not otherwise overlap an input. Nothing is allocated. At most 2^30 rows of a tensor in a call. */
 
 /* h = x + residual (nullable: h = x), y = h / sqrt(mean(h^2) + eps) * weight[K], in fp32 for each row of
- * K <= 65536 elements. residual_out takes h (both or neither; it may be residual itself), out takes y,
+ * K <= 65536 elements (the quotient ahead of the weight's product, both fp32). residual_out takes h (both or neither; it may be residual itself), out takes y,
  * each rounded once (beyond its type's range to infinity); y is made from the unrounded h. Squares that fp32 does not
  * hold are scaled: any finite h has its y. A row with a NaN is NaN throughout, one with infinities NaN
  * there and 0 elsewhere. */

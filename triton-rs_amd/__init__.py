@@ -722,14 +722,10 @@ def rope(q: torch.Tensor, positions: torch.Tensor, rope: Rope, k: torch.Tensor |
     return q_out if k is None else (q_out, k if k_out is None else k_out)
 
 
-# ------------------------------------------------------------------ attention over a paged cache
-
-KV_COUNTER_BYTES = KV4_COUNTER_BYTES = KV8_COUNTER_BYTES = 65536
+KV_COUNTER_BYTES = KV4_COUNTER_BYTES = KV8_COUNTER_BYTES = 65536   # of a workspace of attention over a paged cache
 
 
 # ------------------------------------------------------------------ key/value cache in 4 bits
-
-
 
 def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
               device="cuda") -> torch.Tensor:

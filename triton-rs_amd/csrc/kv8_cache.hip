@@ -10,7 +10,7 @@
 // a token, of values four tokens of four dimensions. Queries are rotated by workgroups of their own in the same launch (as
 // one of rope.hip's they took 4 to 10 us more, start and end).
 //
-// Measured, 8 heads of D = 128: 8192 tokens 15.0 us (50 MB, 3.3 TB/s), keys rotated on the way 21.0, and 32
+// Measured (rows from memory), 8 heads of D = 128: 8192 tokens 15.2 us (50 MB, 3.3 TB/s), keys rotated on the way 21.8, and 32
 // heads of queries 46 (184 MB, 4.0 TB/s); 48 tokens of 48 sequences 4.4
 // and 5.3; 8192 tokens read 11.6 (4.3 TB/s). What is left is registers: 77 and 91 of a thread leave six and five waves a SIMD (in 64
 // it spills: 28 us), the next head's rows on their way beside this one's cost a wave and 1 us.
@@ -334,8 +334,12 @@ static void write(const Kv8WriteParams& p, hipStream_t st) {
     const long long per = ((long long)(p.max_q < p.T ? p.max_q : p.T) + 30) / 16, all = (long long)p.T / 16 + 2 * (long long)p.B;
     const bool direct = per * p.B <= 2 * all;
     const int items = (int)(direct ? per * p.B : all);
-    // Heads of a workgroup: one where few blocks are there, so that they fill the device; more share the angles. Beside queries a half
-    // of it will do: 5424 tokens, 8 heads, 32 of queries 35.4 us in one head a workgroup, 33.1 in two; without queries 18.9 and 19.5.
+    // Heads of a workgroup: more share a token's angles, fewer fill the device, so twice as many as long as 2048 places for workgroups
+    // are left; 1024 beside queries, whose workgroups fill it, too. (Places: with max_q_len given, of sequences of all lengths, up to half of
+    // them are empty.) 8 heads of D = 128, us for 1, 2, 4, 8 a workgroup (captured, the same rows each time), * what the rule takes: 5 prompts
+    // of 60 to 2048 tokens with 32 heads of queries 31.6, 27.7, 24.8*, 26.8, without max_q_len 32.7, 28.2*, 25.5, 25.4, keys alone 19.9,
+    // 17.6*, 18.9, 24.5; 8192 tokens 43.6, 37.7, 34.5*, 35.2 and 25.5, 20.0*, 18.2, 23.2; 64 sequences of 64 25.4, 23.4*, 21.2, 24.4
+    // and 15.2*, 12.0, 14.8, 20.5; 2048 tokens 14.4*, 13.7, 14.7, 23.2 and 9.0*, 9.0, 12.0, 19.5.
     int heads = 1;
     while (heads < p.Hkv && (long long)items * ((p.Hkv + 2 * heads - 1) / (2 * heads)) >= (p.q.H ? 1024 : 2048)) heads *= 2;
     const int groups = (p.Hkv + heads - 1) / heads;

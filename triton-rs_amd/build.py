@@ -78,7 +78,7 @@ def _compile(src: str) -> str:
 def _has_torch() -> bool:
     try:
         import torch  # noqa: F401
-    except ImportError:
+    except (ImportError, OSError):   # (OSError: a library of it is missing)
         return False
     return True
 
